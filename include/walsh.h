@@ -428,6 +428,39 @@ int walsh_prefill_attention(const void *q, int64_t q_sb, int64_t q_sh, int64_t q
                             int64_t kv_sb, int64_t kv_sh, int64_t kv_st, int64_t B, int64_t H, int64_t T, int64_t D,
                             float scale, void *o, int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype, void *stream);
 
+/* ------------------------------------------------------------------ windowed attention
+ * No counterpart in the reference, whose attention is causal over everything
+ * (src/model/chassis.py:441-478): causal attention over the last `window` keys
+ * and the first `sinks` ones.  Query i of Tq stands at position
+ * p = i + Tk - Tq and sees key j iff j <= p and (j > p - window or j < sinks);
+ * window <= 0 is no window.  lengths (int32 [B] on the device, or null) are
+ * the sequences' keys, of Tk: a position at or past its sequence's length
+ * (padding) sees nothing and is seen by none.  Query head h of H reads key
+ * and value head h / (H / G) of G.
+ *   o = softmax(scale q k^T) v,  lse = log sum exp(scale q k^T)
+ * Rows that see nothing: o zeros, lse -inf.  dtype WALSH_F32 or WALSH_BF16;
+ * D in {16, 32, 64, 128}; element (b, h, t, d) of a tensor at
+ * b*sb + h*sh + t*st + d, strides multiples of 8, pointers 16-byte aligned;
+ * 0 < scale <= 1e6.  Scores, softmax and sums in float32; bf16 rounds the
+ * weights (and their gradients) to bf16 for the products with v (k and q).
+ *
+ * walsh_window_attention_fwd: lse [B, H, Tq] or null.
+ * walsh_window_attention_bwd: go the gradient of o, in o's dtype; dq dense
+ *   [B, H, Tq, D], dk and dv dense [B, G, Tk, D], overwritten (Tq, Tk >= 1).
+ *   Sums are formed in a fixed order: the same call gives the same bits. */
+int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k, const void *v,
+                               int64_t kv_sb, int64_t kv_sh, int64_t kv_st, int64_t B, int64_t H, int64_t G, int64_t Tq,
+                               int64_t Tk, int64_t D, int64_t window, int64_t sinks, const int *lengths, float scale,
+                               void *o, int64_t o_sb, int64_t o_sh, int64_t o_st, float *lse, int dtype, void *stream);
+int64_t walsh_window_attention_bwd_workspace_bytes(int64_t B, int64_t H, int64_t G, int64_t Tq, int64_t Tk, int64_t D,
+                                                   int64_t window, int64_t sinks, int dtype);
+int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k, const void *v,
+                               int64_t kv_sb, int64_t kv_sh, int64_t kv_st, const void *o, int64_t o_sb, int64_t o_sh,
+                               int64_t o_st, const void *go, int64_t go_sb, int64_t go_sh, int64_t go_st,
+                               const float *lse, int64_t B, int64_t H, int64_t G, int64_t Tq, int64_t Tk, int64_t D,
+                               int64_t window, int64_t sinks, const int *lengths, float scale, void *dq, void *dk,
+                               void *dv, int dtype, void *work, int64_t work_bytes, void *stream);
+
 /* ------------------------------------------------------------------ A14-A17
  * mHC residual streams.  Stream tensors are [M tokens][n streams][C] with row
  * stride ldx >= n*C (elements); n <= 4 and C % 4 == 0 in this build.

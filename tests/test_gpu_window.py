@@ -1,0 +1,254 @@
+"""Windowed attention and its gradients on the GPU against the float64 oracle
+on the same (rounded) inputs, element by element.
+
+Tolerances.  h is half a step of the tensors' type (2^-8 bf16, 2^-24
+float32): o is rounded once, and bf16 weights P and their gradients dS once
+for the products, so with a_x the sums of magnitudes of result x
+    |o - o*|   <= h |o*| + h a_o,          |dv - dv*| <= h |dv*| + h a_dv
+    |dq - dq*| <= h |dq*| + h a_dq + h e_dq  (e_dq: Delta from an o and a P
+                                              that are rounded), dk likewise.
+Everything else is float32: a score c q k is off by D 2^-24 c |q| |k|, which
+moves P by as much relatively; sums over n keys or queries are off by
+n 2^-24 of their magnitudes, exponentials by a few steps.  rho below adds
+these, and 2 rho a_x covers the two places (P, Delta) where it enters.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import attention as oatt
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+def make(B, H, G, Tq, Tk, D, dtype, seed, layout="bthd"):
+    g = torch.Generator().manual_seed(seed)
+
+    def mk(h, t):
+        if layout == "bthd":
+            return torch.randn(B, t, h, D, generator=g).to(dtype).cuda().transpose(1, 2)
+        return torch.randn(B, h, t, D, generator=g).to(dtype).cuda()
+    return mk(H, Tq), mk(G, Tk), mk(G, Tk), mk(H, Tq)
+
+
+def rho(q, k, Tq, Tk, scale):
+    D = q.shape[-1]
+    qa, ka = q.detach().double().abs().amax(dim=(0, 1, 2)), k.detach().double().abs().amax(dim=(0, 1, 2))
+    reach = float((qa * ka).sum()) * scale
+    return 2.0 ** -24 * (2 * D * reach + max(Tq, Tk) * (q.shape[1] // k.shape[1]) + 4 * D + 64)
+
+
+def check(name, got, want, tol):
+    got = got.double().cpu().numpy()
+    assert got.shape == want.shape and np.isfinite(got).all(), name
+    over = np.abs(got - want) / np.maximum(tol, 1e-30)
+    print(f"{name}: worst error / bound {over.max(initial=0):.3f}", flush=True)
+    assert (np.abs(got - want) <= tol).all(), (name, over.max())
+
+
+def check_all(q, k, v, go, o, grads, W, S, lengths, scale=None):
+    Tq, Tk, D = q.shape[2], k.shape[2], q.shape[3]
+    c = D ** -0.5 if scale is None else scale
+    h, p = HALF[q.dtype], rho(q, k, Tq, Tk, c)
+    ln = None if lengths is None else lengths.cpu().numpy()
+    r = oatt.window_attention_f64(*(t.detach().double().cpu().numpy() for t in (q, k, v)), W, S, ln, c,
+                                  None if go is None else go.double().cpu().numpy())
+    check("o", o.detach(), r["o"], h * np.abs(r["o"]) + (h + 2 * p) * r["a_o"])
+    if go is not None:
+        for n, t in zip(("dq", "dk", "dv"), grads):
+            tol = h * np.abs(r[n]) + (h + 2 * p) * r["a_" + n] + ((h + p) * r["e_" + n] if n != "dv" else 0)
+            check(n, t, r[n], tol)
+    return r
+
+
+# sizes on both sides of the tiles (32 queries a wavefront, 128 a workgroup, 64 keys a chunk), shared heads, windows
+# inside, at and past a tile, first tokens in and past the first chunk, rows that see nothing, padded sequences
+SHAPES = [
+    # B, H, G, Tq, Tk, D, W, S, lengths
+    (1, 1, 1, 1, 1, 16, 0, 0, None),
+    (2, 4, 2, 33, 33, 32, 8, 0, None),
+    (1, 2, 1, 130, 130, 64, 64, 4, None),
+    (2, 3, 3, 257, 257, 128, 100, 3, [257, 70]),
+    (1, 4, 1, 200, 331, 64, 63, 70, None),
+    (2, 2, 2, 129, 64, 16, 33, 1, None),          # more queries than keys: the first rows see nothing
+    (3, 2, 2, 96, 96, 16, 1, 0, [0, 1, 96]),
+    (1, 8, 8, 513, 513, 16, 0, 0, None),
+    (1, 2, 2, 64, 300, 128, 300, 2, [299]),
+    (1, 2, 1, 400, 400, 32, 17, 130, None),
+    (1, 1, 1, 700, 700, 128, 65, 1, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,G,Tq,Tk,D,W,S,lengths", SHAPES)
+def test_window_attention_and_gradients(B, H, G, Tq, Tk, D, W, S, lengths, dtype):
+    from src.model.attention import window_attention
+    print(f"case {B} {H}/{G} {Tq}/{Tk} {D} W={W} S={S} {lengths} {dtype}", flush=True)
+    q, k, v, go = make(B, H, G, Tq, Tk, D, dtype, Tq + 7 * D, "bthd" if W % 2 else "bhtd")
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        o0 = window_attention(q, k, v, W, S, ln)
+    torch.cuda.synchronize()
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    o = window_attention(q, k, v, W, S, ln)
+    grads = torch.autograd.grad(o, (q, k, v), go)
+    again = torch.autograd.grad(window_attention(q, k, v, W, S, ln), (q, k, v), go)
+    torch.cuda.synchronize()
+    assert torch.equal(o0, o.detach()) and all(torch.equal(a, b) for a, b in zip(grads, again))
+    check_all(q, k, v, go, o, grads, W, S, ln)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_window_attention_log_sums(dtype):
+    from src.model import kernels
+    q, k, v, _ = make(2, 4, 2, 90, 150, 64, dtype, 5)
+    ln = torch.tensor([150, 100], dtype=torch.int32, device="cuda")
+    _, lse = kernels.window_attention(q, k, v, 30, 2, ln, need_lse=True)
+    r = oatt.window_attention_f64(q.double().cpu(), k.double().cpu(), v.double().cpu(), 30, 2, [150, 100])["lse"]
+    lse = lse.double().cpu().numpy()
+    assert (np.isneginf(lse) == np.isneginf(r)).all()
+    ok = np.isfinite(r)
+    # a relative error of the sum is an absolute one of its logarithm
+    assert np.abs(lse[ok] - r[ok]).max() <= 2 * rho(q, k, 90, 150, 64 ** -0.5) + 2.0 ** -22 * np.abs(r[ok]).max()
+
+
+@pytest.mark.gpu
+def test_window_attention_layouts_and_partial_gradients():
+    """Rows at strides and offsets that the kernels do not read are copied;
+    only the gradients that are asked for come back; an expanded output
+    gradient is one tensor's worth of values."""
+    from src.model.attention import window_attention
+    B, H, G, T, D = 2, 4, 2, 70, 32
+    base, k, v, _ = make(B, H, G, T, T, D, torch.bfloat16, 9)
+    wide = torch.zeros(B, T, H, D + 3, dtype=torch.bfloat16, device="cuda")
+    wide[..., 1:D + 1] = base.transpose(1, 2)
+    odd = wide[..., 1:D + 1].transpose(1, 2)
+    want = window_attention(base, k, v, 20, 2)
+    assert torch.equal(window_attention(odd, k, v, 20, 2), want)
+    assert torch.equal(window_attention(base, k, v.contiguous(), 20, 2), want)
+    vr = v.detach().requires_grad_(True)
+    o = window_attention(base, k, vr, 20, 2)
+    (dv,) = torch.autograd.grad(o.sum(), (vr,))
+    check_all(base, k, vr, None, o, (), 20, 2, None)
+    r = oatt.window_attention_f64(*(t.detach().double().cpu().numpy() for t in (base, k, vr)), 20, 2,
+                                  go=np.ones((B, H, T, D)))
+    h, p = 2.0 ** -8, rho(base, k, T, T, D ** -0.5)
+    check("dv", dv, r["dv"], h * np.abs(r["dv"]) + (h + 2 * p) * r["a_dv"])
+
+
+@pytest.mark.gpu
+def test_window_attention_padding_may_hold_anything():
+    """Positions past a sequence's length hold no values: NaN and infinities
+    there reach neither outputs nor gradients of the others."""
+    from src.model.attention import window_attention
+    q, k, v, go = make(2, 2, 2, 150, 150, 64, torch.bfloat16, 3)
+    ln = torch.tensor([77, 150], dtype=torch.int32, device="cuda")
+    clean = [t.clone() for t in (q, k, v)]
+    dirty = [t.clone() for t in (q, k, v)]
+    for t in dirty:
+        t[0, :, 77:] = float("nan")
+        t[0, :, 100:] = float("inf")
+    god = go.clone()
+    god[0, :, 77:] = float("nan")
+    outs = []
+    for x, g in ((clean, go), (dirty, god)):
+        for t in x:
+            t.requires_grad_(True)
+        o = window_attention(*x, 40, 3, ln)
+        outs.append([o.detach()] + list(torch.autograd.grad(o, x, g)))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+        assert not a[0, :, 77:].any()
+
+
+@pytest.mark.gpu
+def test_window_attention_rows_before_the_first_key_may_hold_anything():
+    """More queries than keys: the first rows see nothing, and what they and
+    their output gradients hold reaches nothing."""
+    from src.model.attention import window_attention
+    q, k, v, go = make(1, 2, 1, 90, 50, 32, torch.float32, 4)
+    outs = []
+    for fill in (0.0, float("nan")):
+        q[:, :, :40] = go[:, :, :40] = fill
+        x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        o = window_attention(*x, 20, 1)
+        outs.append([o.detach()] + list(torch.autograd.grad(o, x, go)))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert not outs[0][0][:, :, :40].any() and not outs[0][1][:, :, :40].any()
+
+
+@pytest.mark.gpu
+def test_window_attention_in_a_graph():
+    """Forward and backward captured once and replayed on changing inputs,
+    with eager work between the replays."""
+    from src.model import kernels
+    q, k, v, go = make(1, 4, 2, 200, 200, 64, torch.bfloat16, 11, "bhtd")
+    args = (48, 2)
+
+    def step():
+        o, lse = kernels.window_attention(q, k, v, *args, need_lse=True)
+        return (o, lse) + kernels.window_attention_bwd(q, k, v, o, lse, go, *args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(4):
+        for t in (q, k, v, go):
+            t.copy_(torch.randn(t.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)))
+        want = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
+
+
+def test_window_attention_refusals():
+    """Checks made on the host, before the library is called."""
+    from src.model import kernels
+    q, k = torch.zeros(2, 4, 3, 16), torch.zeros(2, 2, 3, 16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        kernels.window_attention(q, k, k, 4)
+
+
+@pytest.mark.gpu
+def test_window_attention_refusals_on_the_gpu():
+    from src.model import _hip, kernels
+    from src.model.attention import window_attention
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, device="cuda", dtype=dt)  # noqa: E731
+    q, k = z(2, 4, 3, 16), z(2, 2, 3, 16)
+    with pytest.raises(AssertionError, match="evenly"):
+        kernels.window_attention(q, z(2, 3, 3, 16), z(2, 3, 3, 16), 4)
+    with pytest.raises(AssertionError, match="does not fit"):
+        kernels.window_attention(q, z(1, 2, 3, 16), z(1, 2, 3, 16), 4)
+    with pytest.raises(ValueError, match="head_dim 24"):
+        kernels.window_attention(z(1, 1, 2, 24), z(1, 1, 2, 24), z(1, 1, 2, 24), 4)
+    with pytest.raises(TypeError, match="one dtype"):
+        kernels.window_attention(q, k.bfloat16(), k.bfloat16(), 4)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        kernels.window_attention(q.half(), k.half(), k.half(), 4)
+    with pytest.raises(TypeError, match="int32"):
+        kernels.window_attention(q, k, k, 4, lengths=torch.ones(2, device="cuda", dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="tensors on"):
+        kernels.window_attention(q, k, k, 4, lengths=torch.ones(2, dtype=torch.int32))
+    for bad in (0.0, -1.0, float("nan"), 1e9):
+        with pytest.raises(_hip.WalshHipError, match="scale"):
+            kernels.window_attention(q, k, k, 4, scale=bad)
+    # nothing to do: no rows, no keys
+    assert window_attention(q[:, :, :0], k, k, 4).shape == (2, 4, 0, 16)
+    assert not window_attention(q, k[:, :, :0], k[:, :, :0], 4).any()
+    # the gradient of a gradient, and batched gradients, are refused
+    qr = q.clone().requires_grad_(True)
+    o = window_attention(qr, k, k, 4)
+    (g,) = torch.autograd.grad(o.sum(), (qr,), create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    o = window_attention(qr, k, k, 4)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(o, (qr,), torch.ones(2, *o.shape, device="cuda"), is_grads_batched=True)

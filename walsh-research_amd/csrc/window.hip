@@ -1,0 +1,807 @@
+// Attention over a sliding window and a few first tokens, forward and
+// backward.  Query i of Tq stands at position p = i + Tk - Tq of its sequence
+// and sees the keys
+//     j <= p  and  (j > p - W  or  j < S)
+// (W the window, S the number of first tokens that stay visible; W <= 0: no
+// window), and a position at or past the sequence's length sees nothing.
+//     o = softmax(c q K^T) V,      lse = log sum exp(c q K^T)
+// A row that sees nothing gives zeros and lse = -inf.  The backward rebuilds
+// P = exp(c q K^T - lse) tile by tile:
+//     Delta = rowsum(do o),  dV = P^T do,  dS = c P (do V^T - Delta),
+//     dQ = dS K,  dK = dS^T Q
+// with query heads h sharing the keys and values of head h / (H / G).
+//
+// Matrix layout.  Everything is a 32x32 product tile over 16 (bf16:
+// v_mfma_f32_32x32x16_bf16; float32: eight v_mfma_f32_32x32x2_f32), operands
+// eight consecutive elements per lane.  Scores are formed transposed to the
+// operand that stays in registers, so a lane holds 16 scores of ONE query
+// (forward, dQ) or ONE key (dK, dV) and the softmax weights are, as they come
+// out, the second operand of the next product.  A tile of 32-bit results has
+// its rows at 8 g + 4 hi + i (hi the lane's half), so product slot 8 hi + e
+// stands for row 16 t + 4 hi + e (e < 4) or 16 t + 8 + 4 hi + e - 4, and the
+// first operand is read in that order: bf16 with the transposing LDS load
+// (four rows of a column per lane), float32 with single loads.  One LDS copy
+// of a tile, row-major, so serves both the products over its columns and over
+// its rows.
+//
+// Roundings.  Scores, maxima, sums, lse, Delta and all accumulators are
+// float32.  bf16 tensors have their weights P and dS rounded to bf16 for the
+// second products (the matrix cores' operand type; relative 2^-9 each, the
+// size of the inputs' own rounding); the sum of weights that normalises a row
+// takes them unrounded.
+#include <type_traits>
+
+#include "common.h"
+
+namespace walsh {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kNoScore = -1e30f;  // running maximum of a row that has seen nothing: finite, so differences stay numbers
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---------------------------------------------------------------- operands
+// Eight elements of one row or column: a product operand.
+template <typename T> struct Frag;
+template <> struct Frag<uint16_t> { i16x8 v; };
+template <> struct Frag<float> { f32x8 v; };
+
+__device__ __forceinline__ void mma(f32x16 &c, const Frag<uint16_t> &a, const Frag<uint16_t> &b) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), c, 0,
+                                                0, 0);
+}
+__device__ __forceinline__ void mma(f32x16 &c, const Frag<float> &a, const Frag<float> &b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
+}
+// Result rows 16 t + (4 hi + 0..3, 8 + 4 hi + 0..3) as an operand.
+__device__ __forceinline__ void pack(Frag<uint16_t> &f, const float *p) {
+    const u32x4 u = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
+                     pack_bf16x2(p[6], p[7])};
+    f.v = __builtin_bit_cast(i16x8, u);
+}
+__device__ __forceinline__ void pack(Frag<float> &f, const float *p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = p[i];
+}
+__device__ __forceinline__ Frag<uint16_t> load_frag(const uint16_t *p) { return {*(const i16x8 *)p}; }
+__device__ __forceinline__ Frag<float> load_frag(const float *p) {
+    const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);
+    return {f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+__device__ __forceinline__ float dot(const Frag<float> &a, const Frag<float> &b) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += a.v[i] * b.v[i];
+    return s;
+}
+__device__ __forceinline__ float dot(const Frag<uint16_t> &a, const Frag<uint16_t> &b) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += bf16_to_f32((uint16_t)a.v[i]) * bf16_to_f32((uint16_t)b.v[i]);
+    return s;
+}
+
+// The value, newly computed as far as the compiler can see: what derives from
+// it is worked out again where it is used and holds no registers across a loop.
+__device__ __forceinline__ int fresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+__device__ __forceinline__ float other_half(float v) {   // the value of lane ^ 32
+    return __shfl_xor(v, 32, 64);
+}
+
+// ---------------------------------------------------------------- tiles in LDS
+// ROWS rows of D elements, row-major in 16-byte chunks; chunk c of row r lies
+// at position c ^ swz(r), so that the 16 rows of one chunk column fall on
+// distinct banks (row operands) and so do the four rows of a transposing load.
+template <typename T, int D, int ROWS> struct Tile {
+    static constexpr int NCH = D * (int)sizeof(T) / 16;       // chunks per row: 2 .. 32
+    static constexpr int ROWB = D * (int)sizeof(T);
+    static constexpr int BYTES = ROWS * ROWB;
+    static __device__ __forceinline__ int swz(int r) {
+        if (sizeof(T) == 4) return NCH >= 16 ? r & 15 : NCH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
+        if (NCH == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+        if (NCH == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+        return NCH == 4 ? (r >> 2) & 3 : (r >> 3) & 1;
+    }
+    // Rows r0 .. r0 + ROWS - 1 of a matrix with row stride st into LDS, by
+    // WAVES wavefronts, straight from memory (no registers); rows before lo
+    // and at or past n are zeros and are not read.
+    template <int WAVES>
+    static __device__ __forceinline__ void fetch(unsigned char *lds, const T *base, int64_t st, int r0, int lo, int n, int wave,
+                                                 int lane) {
+        const int rows = min(n - r0, ROWS);
+        const uint32_t span = rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * st + D) * (int)sizeof(T)) : 0u;
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (int64_t)r0 * st, span);
+        constexpr int N = BYTES / 1024;   // wavefront loads
+        static_assert(BYTES % 1024 == 0, "whole loads");
+#pragma unroll
+        for (int i = 0; i < (N + WAVES - 1) / WAVES; ++i) {
+            const int k = i * WAVES + __builtin_amdgcn_readfirstlane(wave);
+            if (N % WAVES && k >= N) break;
+            const int pos = k * 64 + lane, row = pos / NCH, c = (pos % NCH) ^ swz(row);
+            const uint32_t off = row < rows && row >= lo - r0 ? (uint32_t)row * (uint32_t)(st * (int)sizeof(T)) + 16 * c : kOOB;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(lds + k * 1024), 16,
+                                                     off, 0, 0, 0);
+        }
+    }
+    // Eight elements of row r from column 16 kk + 8 hi.
+    static __device__ __forceinline__ Frag<T> row(const unsigned char *lds, int r, int kk, int hi) {
+        const unsigned char *p = lds + r * ROWB;
+        const int s = swz(r);
+        if constexpr (sizeof(T) == 2) {
+            return {*(const i16x8 *)(p + (((2 * kk + hi) ^ s) << 4))};
+        } else {
+            const f32x4 a = *(const f32x4 *)(p + (((4 * kk + 2 * hi) ^ s) << 4));
+            const f32x4 b = *(const f32x4 *)(p + (((4 * kk + 2 * hi + 1) ^ s) << 4));
+            return {f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+        }
+    }
+    // Column 32 c + lane % 32 (modulo D) of rows r + 4 hi + 0..3 and r + 8 + 4 hi + 0..3.
+    static __device__ __forceinline__ Frag<T> col(const unsigned char *lds, int r, int c, int lane) {
+        const int hi = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            typedef short i16x4v __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) i16x4v *P;
+            const int l = lane & 15, half = D >= 32 ? (lane >> 4) & 1 : 0;
+            const int ch = 4 * c + 2 * half + ((l & 3) >> 1), byte = 8 * (l & 1);
+            const int ra = r + 4 * hi + (l >> 2), rb = ra + 8;
+            const i16x4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (P)(const_cast<unsigned char *>(lds) + ra * ROWB + ((ch ^ swz(ra)) << 4) + byte));
+            const i16x4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (P)(const_cast<unsigned char *>(lds) + rb * ROWB + ((ch ^ swz(rb)) << 4) + byte));
+            return {__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)};
+        } else {
+            const int d = (32 * c + (lane & 31)) % D;
+            f32x8 v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int rr = r + 4 * hi + (e & 3) + 8 * (e >> 2);
+                v[e] = *(const float *)(lds + rr * ROWB + (((d >> 2) ^ swz(rr)) << 4) + 4 * (d & 3));
+            }
+            return {v};
+        }
+    }
+};
+
+// All of this wavefront's loads into LDS have landed and its LDS reads are
+// done; then all wavefronts'.
+__device__ __forceinline__ void tiles_ready() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// ---------------------------------------------------------------- arguments
+struct WinTensor {
+    int64_t sb, sh, st;   // element (b, h, t, d) at b*sb + h*sh + t*st + d
+};
+struct WinArgs {
+    const void *q, *k, *v;
+    const int *lengths;   // [B] or null
+    void *o;
+    float *lse;           // [B, H, Tq]
+    WinTensor sq, skv, so;
+    int B, H, G, Tq, Tk, W, S;
+    float sl2;            // scale * log2(e)
+    // backward
+    const void *go;
+    void *dq, *dk, *dv;   // dense [B, H, Tq, D], [B, G, Tk, D]
+    WinTensor sgo;
+    float *delta;         // [B, H, Tq]
+    float scale;
+    float *part;          // partial dK, dV of key blocks whose queries are split
+    int nb, nsb, nn, ns;  // key blocks; those with first tokens; splits of the others' and of their queries
+};
+
+// Key positions of a sequence: all of Tk, or its length within it.
+__device__ __forceinline__ int win_len(const WinArgs &a, int b) {
+    return a.lengths ? max(0, min(a.lengths[b], a.Tk)) : a.Tk;
+}
+// The chunks of ROWS keys that positions p0 .. p1 see: n chunks, the first ns
+// of them the first tokens' (chunks 0 ..), the rest from chunk lo.
+struct Chunks {
+    int lo, ns, n;
+    __device__ __forceinline__ int at(int i) const { return i < ns ? i : lo + i - ns; }
+};
+template <int ROWS> __device__ __forceinline__ Chunks win_chunks(const WinArgs &a, int p0, int p1) {
+    Chunks c;
+    c.lo = a.W > 0 && p0 >= a.W ? (p0 - a.W + 1) / ROWS : 0;
+    c.ns = min((a.S + ROWS - 1) / ROWS, c.lo);
+    c.n = p1 < 0 ? 0 : c.ns + p1 / ROWS - c.lo + 1;
+    return c;
+}
+// How keys k0 .. k0 + n - 1 look to positions pa .. pb: 0 hidden from all, 2 seen by all, 1 mixed.
+__device__ __forceinline__ int win_kind(const WinArgs &a, int k0, int n, int pa, int pb) {
+    if (k0 > pb || (a.W > 0 && k0 + n <= pa - a.W + 1 && k0 >= a.S)) return 0;
+    return k0 + n - 1 <= pa && (a.W <= 0 || k0 > pb - a.W || k0 + n <= a.S) ? 2 : 1;
+}
+__device__ __forceinline__ bool win_sees(const WinArgs &a, int p, int j) {
+    return j <= p && (a.W <= 0 || j > p - a.W || j < a.S);
+}
+
+// Work item of this workgroup: workgroups go to the 8 XCDs in turn, so XCD x
+// takes items x n/8 ..: neighbouring items, which share keys, share an L2.
+// Returns -1 past the last one (the grid is a multiple of 8).
+__device__ __forceinline__ int xcd_item(int n) {
+    const int per = (n + 7) / 8, id = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+    return ((int)blockIdx.x >> 3) < per && id < n ? id : -1;
+}
+
+// ---------------------------------------------------------------- forward
+constexpr int kWinWaves = 4;
+constexpr int kWinQ = 32 * kWinWaves;   // queries (or keys, dK and dV) per workgroup
+template <typename T, int D> struct WinCfg {
+    static constexpr int KC = sizeof(T) == 4 && D == 128 ? 32 : 64;   // rows of a tile: four of them, 64 KB at most
+    static constexpr int NK = D / 16;                                 // products over D
+    static constexpr int ND = (D + 31) / 32;                          // 32-wide blocks of D
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_fwd_kernel(WinArgs a) {
+    constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
+    typedef Tile<T, D, KC> L;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const int nqt = (a.Tq + kWinQ - 1) / kWinQ;
+    const int id = xcd_item(nqt * a.H * a.B);
+    if (id < 0) return;
+    const int qt = nqt - 1 - id % nqt, h = id / nqt % a.H, b = id / nqt / a.H, g = h / (a.H / a.G);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    const int len = win_len(a, b), off = a.Tk - a.Tq;
+    const int qi = qt * kWinQ + 32 * wave + n, p = qi + off;   // this lane's query and its position
+    // positions of the workgroup and of the wavefront that have an output
+    const int wlo = max(0, qt * kWinQ + off), whi = min(min(qt * kWinQ + kWinQ, a.Tq) - 1 + off, len - 1);
+    const int pa = max(0, qt * kWinQ + 32 * wave + off), pb = min(qt * kWinQ + 32 * wave + 31 + off, len - 1);
+
+    const bool live = p >= 0 && p < len;
+
+    Frag<T> qf[NK];
+    {
+        const T *qp = (const T *)a.q + b * a.sq.sb + h * a.sq.sh + (int64_t)min(qi, a.Tq - 1) * a.sq.st;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) qf[kk] = load_frag(qp + 16 * kk + 8 * hi);
+    }
+    f32x16 acc[ND];
+#pragma unroll
+    for (int c = 0; c < ND; ++c) acc[c] = f32x16{};
+    float m = kNoScore, l = 0.f;
+
+    const T *kb = (const T *)a.k + b * a.skv.sb + g * a.skv.sh, *vb = (const T *)a.v + b * a.skv.sb + g * a.skv.sh;
+    const Chunks ch = wlo <= whi ? win_chunks<KC>(a, wlo, whi) : Chunks{0, 0, 0};
+    auto fetch = [&](int i) {
+        unsigned char *dst = smem + (i & 1) * 2 * L::BYTES;
+        L::template fetch<kWinWaves>(dst, kb, a.skv.st, ch.at(i) * KC, 0, len, wave, lane);
+        L::template fetch<kWinWaves>(dst + L::BYTES, vb, a.skv.st, ch.at(i) * KC, 0, len, wave, lane);
+    };
+    if (ch.n > 0) fetch(0);
+    for (int i = 0; i < ch.n; ++i) {
+        tiles_ready();
+        if (i + 1 < ch.n) fetch(i + 1);
+        const unsigned char *kl = smem + (i & 1) * 2 * L::BYTES, *vl = kl + L::BYTES;
+        const int k0 = ch.at(i) * KC;
+        const int kind = pa <= pb ? win_kind(a, k0, KC, pa, pb) : 0;
+        if (kind == 0) continue;
+        f32x16 s[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            s[j] = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) mma(s[j], L::row(kl, 32 * j + n, kk, hi), qf[kk]);
+        }
+        if (kind == 1) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3))) s[j][r] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
+        mx = fmaxf(mx, other_half(mx));
+        // the maximum moves only when some row of the wavefront would pass
+        // 2^8: weights and sums stay within float32 and the rescaling of the
+        // accumulators is rare
+        if (__any(live && (mx - m) * a.sl2 > 8.f)) {
+            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f((m - mn) * a.sl2);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int c = 0; c < ND; ++c) acc[c] *= al;
+        }
+        const float mo = -m * a.sl2;
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            float w[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], a.sl2, mo));
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                l0 += w[r];
+                l1 += w[r + 1];
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag<T> pf;
+                pack(pf, w + 8 * t);
+#pragma unroll
+                for (int c = 0; c < ND; ++c) mma(acc[c], L::col(vl, 32 * j + 16 * t, c, lane), pf);
+            }
+        }
+        l += l0 + l1;
+    }
+    l += other_half(l);
+    if (qi >= a.Tq) return;
+    const float inv = live && l > 0.f ? 1.f / l : 0.f;
+    T *op = (T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)qi * a.so.st;
+#pragma unroll
+    for (int c = 0; c < ND; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int d = 32 * c + 8 * t + 4 * hi;
+            if (D % 32 && d >= D) continue;
+            const f32x4 v = f32x4{acc[c][4 * t], acc[c][4 * t + 1], acc[c][4 * t + 2], acc[c][4 * t + 3]} * inv;
+            store4(op + d, live ? v : f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+    if (a.lse && hi == 0)
+        a.lse[((int64_t)b * a.H + h) * a.Tq + qi] = live ? (m * a.sl2 + log2f(l)) * (1.f / kLog2e) : -INFINITY;
+}
+
+// ---------------------------------------------------------------- backward: queries
+// dQ of 32 queries per wavefront, over the keys they see; also Delta, which
+// the keys' kernel reads.
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
+    constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
+    typedef Tile<T, D, KC> L;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const int nqt = (a.Tq + kWinQ - 1) / kWinQ;
+    const int id = xcd_item(nqt * a.H * a.B);
+    if (id < 0) return;
+    const int qt = nqt - 1 - id % nqt, h = id / nqt % a.H, b = id / nqt / a.H, g = h / (a.H / a.G);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    const int len = win_len(a, b), off = a.Tk - a.Tq;
+    const int qi = qt * kWinQ + 32 * wave + n, p = qi + off, qc = min(qi, a.Tq - 1);
+    const int wlo = max(0, qt * kWinQ + off), whi = min(min(qt * kWinQ + kWinQ, a.Tq) - 1 + off, len - 1);
+    const int pa = max(0, qt * kWinQ + 32 * wave + off), pb = min(qt * kWinQ + 32 * wave + 31 + off, len - 1);
+    const bool live = p >= 0 && p < len && qi < a.Tq;
+
+    Frag<T> qf[NK], gf[NK];
+    float delta = 0.f;
+    {
+        const T *qp = (const T *)a.q + b * a.sq.sb + h * a.sq.sh + (int64_t)qc * a.sq.st;
+        const T *gp = (const T *)a.go + b * a.sgo.sb + h * a.sgo.sh + (int64_t)qc * a.sgo.st;
+        const T *op = (const T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)qc * a.so.st;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+            qf[kk] = load_frag(qp + 16 * kk + 8 * hi);
+            gf[kk] = load_frag(gp + 16 * kk + 8 * hi);
+            delta += dot(gf[kk], load_frag(op + 16 * kk + 8 * hi));
+        }
+        delta += other_half(delta);
+    }
+    const int64_t row = ((int64_t)b * a.H + h) * a.Tq + qc;
+    if (hi == 0 && qi < a.Tq) a.delta[row] = live ? delta : 0.f;
+    const float lse2 = live ? a.lse[row] * kLog2e : INFINITY;   // a row that sees nothing has no weights
+    f32x16 acc[ND];
+#pragma unroll
+    for (int c = 0; c < ND; ++c) acc[c] = f32x16{};
+
+    const T *kb = (const T *)a.k + b * a.skv.sb + g * a.skv.sh, *vb = (const T *)a.v + b * a.skv.sb + g * a.skv.sh;
+    const Chunks ch = wlo <= whi ? win_chunks<KC>(a, wlo, whi) : Chunks{0, 0, 0};
+    auto fetch = [&](int i) {
+        unsigned char *dst = smem + (i & 1) * 2 * L::BYTES;
+        L::template fetch<kWinWaves>(dst, kb, a.skv.st, ch.at(i) * KC, 0, len, wave, lane);
+        L::template fetch<kWinWaves>(dst + L::BYTES, vb, a.skv.st, ch.at(i) * KC, 0, len, wave, lane);
+    };
+    if (ch.n > 0) fetch(0);
+    for (int i = 0; i < ch.n; ++i) {
+        tiles_ready();
+        if (i + 1 < ch.n) fetch(i + 1);
+        const unsigned char *kl = smem + (i & 1) * 2 * L::BYTES, *vl = kl + L::BYTES;
+        const int k0 = ch.at(i) * KC;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int kind = pa <= pb ? win_kind(a, k0 + 32 * j, 32, pa, pb) : 0;
+            if (kind == 0) continue;
+            f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                mma(s, L::row(kl, 32 * j + n, kk, hi), qf[kk]);
+                mma(dp, L::row(vl, 32 * j + n, kk, hi), gf[kk]);
+            }
+            if (kind == 1) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3))) s[r] = -INFINITY;
+            }
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse2)) * (dp[r] - delta);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag<T> f;
+                pack(f, ds + 8 * t);
+#pragma unroll
+                for (int c = 0; c < ND; ++c) mma(acc[c], L::col(kl, 32 * j + 16 * t, c, lane), f);
+            }
+        }
+    }
+    if (qi >= a.Tq) return;
+    T *dq = (T *)a.dq + (((int64_t)b * a.H + h) * a.Tq + qi) * D;
+#pragma unroll
+    for (int c = 0; c < ND; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int d = 32 * c + 8 * t + 4 * hi;
+            if (D % 32 && d >= D) continue;
+            const f32x4 v = f32x4{acc[c][4 * t], acc[c][4 * t + 1], acc[c][4 * t + 2], acc[c][4 * t + 3]} * a.scale;
+            store4(dq + d, live ? v : f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+}
+
+// ---------------------------------------------------------------- backward: keys
+// dK and dV of 32 keys per wavefront (a key block of 128 per workgroup) over
+// the queries that see them, of every query head that shares them.  The
+// (head, query tile) pairs of a block are cut into splits, each summed by a
+// workgroup of its own: blocks with first tokens, which every later query
+// sees, into ns, the others into nn.  A split block's parts go to `part` and
+// are summed in a fixed order; an unsplit block is stored at once.
+template <typename T, int D> struct WinBwdCfg {
+    static constexpr int QC = D == 128 && sizeof(T) == 4 ? 32 : 64;   // rows of a tile
+};
+// Tiles of QC queries (indexes from query 0) that see keys k0 .. k0 + 127.
+template <int QC> __device__ __forceinline__ void win_q_tiles(const WinArgs &a, int k0, int len, int *first, int *count) {
+    const int off = a.Tk - a.Tq;
+    const int lo = max(k0, off);                                     // first position that has a query
+    int end = min(len, a.Tk) - 1;
+    if (a.W > 0 && k0 >= a.S) end = (int)min((int64_t)end, (int64_t)k0 + kWinQ - 1 + a.W - 1);
+    *first = lo <= end ? (lo - off) / QC : 0;
+    *count = lo <= end ? (end - off) / QC - *first + 1 : 0;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWinWaves, D == 128 || (sizeof(T) == 4 && D == 64) ? 1 : 2) void window_bwd_kv_kernel(WinArgs a) {
+    constexpr int QC = WinBwdCfg<T, D>::QC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = QC / 32;
+    typedef Tile<T, D, QC> L;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ __align__(16) float stat[2][2][QC];   // [buffer][lse2, Delta]
+    const int per = a.nsb * a.ns + (a.nb - a.nsb) * a.nn;            // items per (sequence, kv head)
+    const int id = xcd_item(per * a.G * a.B);
+    if (id < 0) return;
+    const int it = id % per, g = id / per % a.G, b = id / per / a.G;
+    const bool sink = it < a.nsb * a.ns;
+    const int kblk = sink ? it / a.ns : a.nsb + (it - a.nsb * a.ns) / a.nn;
+    const int nsplit = sink ? a.ns : a.nn, split = sink ? it % a.ns : (it - a.nsb * a.ns) % a.nn;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    const int len = win_len(a, b), off = a.Tk - a.Tq, R = a.H / a.G;
+    const int k0 = kblk * kWinQ, kw = k0 + 32 * wave, key = kw + n;
+
+    Frag<T> kf[NK], vf[NK];
+    {
+        const int64_t at = b * a.skv.sb + g * a.skv.sh + (int64_t)min(key, a.Tk - 1) * a.skv.st;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+            kf[kk] = load_frag((const T *)a.k + at + 16 * kk + 8 * hi);
+            vf[kk] = load_frag((const T *)a.v + at + 16 * kk + 8 * hi);
+        }
+    }
+    f32x16 ak[ND], av[ND];
+#pragma unroll
+    for (int c = 0; c < ND; ++c) ak[c] = av[c] = f32x16{};
+    int t0, nt;
+    win_q_tiles<QC>(a, k0, len, &t0, &nt);
+    // this split's share of the R * nt (head, tile) pairs
+    const int total = R * nt, i0 = (int)((int64_t)total * split / nsplit), i1 = (int)((int64_t)total * (split + 1) / nsplit);
+    const int nq = max(0, min(a.Tq, len - off));                     // queries before the sequence's end
+    auto fetch = [&](int i) {
+        const int h = g * R + i / nt, q0 = (t0 + i % nt) * QC;
+        unsigned char *dst = smem + (i & 1) * 2 * L::BYTES;
+        L::template fetch<kWinWaves>(dst, (const T *)a.q + b * a.sq.sb + h * a.sq.sh, a.sq.st, q0, -off, nq, wave, lane);
+        L::template fetch<kWinWaves>(dst + L::BYTES, (const T *)a.go + b * a.sgo.sb + h * a.sgo.sh, a.sgo.st, q0, -off,
+                                     nq, wave, lane);
+    };
+    // lse and Delta of a tile travel through a register to LDS
+    const int sr = threadIdx.x % QC, sw = threadIdx.x / QC;
+    auto fetch_stat = [&](int i) {
+        const int h = g * R + i / nt, qi = (t0 + i % nt) * QC + sr;
+        float v = sw ? 0.f : INFINITY;
+        if (sw < 2 && qi < nq && qi + off >= 0) {
+            const int64_t row = ((int64_t)b * a.H + h) * a.Tq + qi;
+            v = sw ? a.delta[row] : a.lse[row] * kLog2e;
+        }
+        return v;
+    };
+    auto put_stat = [&](int i, float v) {
+        if (sw < 2) stat[i & 1][sw][sr] = v;
+    };
+    if (i0 < i1) {
+        fetch(i0);
+        put_stat(i0, fetch_stat(i0));
+    }
+    for (int i = i0; i < i1; ++i) {
+        tiles_ready();
+        float nextv = 0.f;
+        if (i + 1 < i1) {
+            nextv = fetch_stat(i + 1);
+            fetch(i + 1);
+        }
+        const unsigned char *ql = smem + (i & 1) * 2 * L::BYTES, *gl = ql + L::BYTES;
+        const int ln = fresh(lane), n = ln & 31, hi = ln >> 5;
+        const int pq = (t0 + i % nt) * QC + off;   // position of the tile's first query
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int pa = pq + 32 * j, pb = pa + 31;
+            const int kind = kw < len ? win_kind(a, kw, 32, pa, pb) : 0;
+            if (kind == 0) continue;
+            f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                mma(s, L::row(ql, 32 * j + n, kk, hi), kf[kk]);
+                mma(dp, L::row(gl, 32 * j + n, kk, hi), vf[kk]);
+            }
+            float w[16], ds[16];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const f32x4 ls = *(const f32x4 *)&stat[i & 1][0][32 * j + 8 * t + 4 * hi];
+                const f32x4 de = *(const f32x4 *)&stat[i & 1][1][32 * j + 8 * t + 4 * hi];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * t + e;
+                    float x = s[r];
+                    if (kind == 1 && !win_sees(a, pa + 8 * t + 4 * hi + e, key)) x = -INFINITY;
+                    w[r] = __builtin_amdgcn_exp2f(fmaf(x, a.sl2, -ls[e]));
+                    ds[r] = w[r] * (dp[r] - de[e]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag<T> pf, df;
+                pack(pf, w + 8 * t);
+                pack(df, ds + 8 * t);
+#pragma unroll
+                for (int c = 0; c < ND; ++c) {
+                    mma(av[c], L::col(gl, 32 * j + 16 * t, c, ln), pf);
+                    mma(ak[c], L::col(ql, 32 * j + 16 * t, c, ln), df);
+                }
+            }
+        }
+        if (i + 1 < i1) put_stat(i + 1, nextv);
+    }
+    // keys past the length (whatever they hold) have no gradient
+    if (key >= len) {
+#pragma unroll
+        for (int c = 0; c < ND; ++c) ak[c] = av[c] = f32x16{};
+    }
+    if (nsplit > 1) {
+        // partial rows, float32: [b, g][block's slot][split][dK, dV][128][D]
+        const int64_t slot = sink ? (int64_t)kblk * a.ns
+                                  : (a.ns > 1 ? (int64_t)a.nsb * a.ns : 0) + (int64_t)(kblk - a.nsb) * a.nn;
+        const int64_t slots = (a.ns > 1 ? (int64_t)a.nsb * a.ns : 0) + (a.nn > 1 ? (int64_t)(a.nb - a.nsb) * a.nn : 0);
+        float *pk = a.part + (((int64_t)b * a.G + g) * slots + slot + split) * 2 * kWinQ * D + (32 * wave + n) * D;
+#pragma unroll
+        for (int c = 0; c < ND; ++c)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int d = 32 * c + 8 * t + 4 * hi;
+                if (D % 32 && d >= D) continue;
+                store4(pk + d, f32x4{ak[c][4 * t], ak[c][4 * t + 1], ak[c][4 * t + 2], ak[c][4 * t + 3]} * a.scale);
+                store4(pk + kWinQ * D + d, f32x4{av[c][4 * t], av[c][4 * t + 1], av[c][4 * t + 2], av[c][4 * t + 3]});
+            }
+        return;
+    }
+    if (key >= a.Tk) return;
+    const int64_t at = (((int64_t)b * a.G + g) * a.Tk + key) * D;
+#pragma unroll
+    for (int c = 0; c < ND; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int d = 32 * c + 8 * t + 4 * hi;
+            if (D % 32 && d >= D) continue;
+            store4((T *)a.dk + at + d,
+                   f32x4{ak[c][4 * t], ak[c][4 * t + 1], ak[c][4 * t + 2], ak[c][4 * t + 3]} * a.scale);
+            store4((T *)a.dv + at + d, f32x4{av[c][4 * t], av[c][4 * t + 1], av[c][4 * t + 2], av[c][4 * t + 3]});
+        }
+}
+
+// dK and dV of the split key blocks: the splits' parts summed in order.
+template <typename T, int D> __global__ __launch_bounds__(256) void window_bwd_sum_kernel(WinArgs a) {
+    const int blk0 = a.ns > 1 ? 0 : a.nsb, blk1 = a.nn > 1 ? a.nb : a.nsb;   // split blocks (host: at least one)
+    const int kblk = blk0 + (int)blockIdx.x % (blk1 - blk0), bg = (int)blockIdx.x / (blk1 - blk0);
+    const bool sink = kblk < a.nsb;
+    const int nsplit = sink ? a.ns : a.nn;
+    const int64_t slot = sink ? (int64_t)kblk * a.ns
+                              : (a.ns > 1 ? (int64_t)a.nsb * a.ns : 0) + (int64_t)(kblk - a.nsb) * a.nn;
+    const int64_t slots = (a.ns > 1 ? (int64_t)a.nsb * a.ns : 0) + (a.nn > 1 ? (int64_t)(a.nb - a.nsb) * a.nn : 0);
+    const float *src = a.part + ((int64_t)bg * slots + slot) * 2 * kWinQ * D;
+    const int rows = min(kWinQ, a.Tk - kblk * kWinQ);
+    const int i = ((int)blockIdx.y * 256 + (int)threadIdx.x) * 4;            // element of [dK, dV][128][D]
+    const int which = i / (kWinQ * D), at = i % (kWinQ * D);
+    if (at / D >= rows) return;
+    f32x4 s = load4(src + i);
+    for (int k = 1; k < nsplit; ++k) s += load4(src + (int64_t)k * 2 * kWinQ * D + i);
+    store4((T *)(which ? a.dv : a.dk) + ((int64_t)bg * a.Tk + kblk * kWinQ) * D + at, s);
+}
+
+// ---------------------------------------------------------------- host
+// Splits of the key blocks' queries: blocks of first tokens are seen from
+// every later tile, the others from a window's; both are cut into splits of
+// about one window's tiles (or of what fills the chip, two workgroups per CU).
+static void win_splits(WinArgs &a, int QC) {
+    a.nb = (int)ceil_div(a.Tk, kWinQ);
+    a.nsb = a.W > 0 && a.W < a.Tk ? (int)ceil_div(a.S < a.Tk ? a.S : a.Tk, kWinQ) : 0;
+    const int64_t R = a.H / a.G, full = R * (ceil_div(a.Tk, QC) + 1);
+    int64_t near = a.W > 0 ? R * (ceil_div((int64_t)a.W + kWinQ, QC) + 1) : full;
+    if (near > full) near = full;
+    const int64_t groups = (int64_t)a.B * a.G * a.nb, fill = 2 * (int64_t)device_info().cu_count;
+    int64_t nn = groups >= fill ? 1 : ceil_div(fill, groups);
+    if (nn > ceil_div(near, 4)) nn = ceil_div(near, 4);   // four tiles at least
+    if (nn > 64) nn = 64;
+    const int64_t share = ceil_div(near, nn);
+    int64_t ns = ceil_div(full, share);
+    if (ns > 256) ns = 256;
+    a.nn = (int)nn;
+    a.ns = a.nsb ? (int)ns : 1;
+}
+
+static int64_t win_part_slots(const WinArgs &a) {
+    return (a.ns > 1 ? (int64_t)a.nsb * a.ns : 0) + (a.nn > 1 ? (int64_t)(a.nb - a.nsb) * a.nn : 0);
+}
+
+static int win_check(const char *fn, const WinArgs &a, int64_t B, int64_t H, int64_t G, int64_t Tq, int64_t Tk,
+                     int64_t D, int dtype) {
+    if (B < 0 || H < 1 || G < 1 || H % G || Tq < 0 || Tk < 0 || Tq > (1 << 24) || Tk > (1 << 24))
+        return set_error(WALSH_EINVAL, "%s: bad shape B=%lld H=%lld G=%lld Tq=%lld Tk=%lld", fn, (long long)B,
+                         (long long)H, (long long)G, (long long)Tq, (long long)Tk);
+    if (D != 16 && D != 32 && D != 64 && D != 128)
+        return set_error(WALSH_ENOTSUP, "%s: head_dim %lld (16, 32, 64 or 128)", fn, (long long)D);
+    if (dtype != WALSH_F32 && dtype != WALSH_BF16) return set_error(WALSH_ENOTSUP, "%s: dtype %d", fn, dtype);
+    if (!(a.scale > 0.f) || a.scale > 1e6f)
+        return set_error(WALSH_EINVAL, "%s: the scale must be positive and at most 1e6", fn);
+    if (B * H * ceil_div(Tq > Tk ? Tq : Tk, 32) > (1ll << 28))
+        return set_error(WALSH_ENOTSUP, "%s: B=%lld H=%lld T=%lld exceed the grid", fn, (long long)B, (long long)H,
+                         (long long)(Tq > Tk ? Tq : Tk));
+    return WALSH_OK;
+}
+
+// Rows are read in 16-byte pieces: strides multiples of 8 elements, rows that
+// do not overlap, and 64 of them within 2 GiB.
+static int win_check_tensor(const char *fn, const char *name, const void *p, const WinTensor &s, int64_t B, int64_t H,
+                            int64_t T, int64_t D) {
+    if (!p) return set_error(WALSH_EINVAL, "%s: null pointer (%s)", fn, name);
+    if ((uintptr_t)p % 16 || s.sb % 8 || s.sh % 8 || s.st % 8)
+        return set_error(WALSH_ENOTSUP, "%s: %s needs 16-byte alignment and strides that are multiples of 8", fn, name);
+    if ((T > 1 && s.st < D) || s.st < 0 || s.sb < 0 || s.sh < 0 || s.st > (1 << 22))
+        return set_error(WALSH_ENOTSUP, "%s: %s: row stride %lld (head_dim %lld to 2^22), no negative strides", fn, name,
+                         (long long)s.st, (long long)D);
+    return WALSH_OK;
+}
+
+}  // namespace walsh
+
+using namespace walsh;
+
+// Calls go(T(), integral constant D) for the dtype and head_dim at hand.
+template <typename F> static void win_dispatch(int dtype, int64_t D, F go) {
+    auto by_dim = [&](auto t) {
+        if (D == 16) go(t, std::integral_constant<int, 16>());
+        else if (D == 32) go(t, std::integral_constant<int, 32>());
+        else if (D == 64) go(t, std::integral_constant<int, 64>());
+        else go(t, std::integral_constant<int, 128>());
+    };
+    if (dtype == WALSH_BF16) by_dim(uint16_t(0));
+    else by_dim(float(0));
+}
+
+WALSH_EXPORT int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k,
+                                            const void *v, int64_t kv_sb, int64_t kv_sh, int64_t kv_st, int64_t B,
+                                            int64_t H, int64_t G, int64_t Tq, int64_t Tk, int64_t D, int64_t window,
+                                            int64_t sinks, const int *lengths, float scale, void *o, int64_t o_sb,
+                                            int64_t o_sh, int64_t o_st, float *lse, int dtype, void *stream) {
+    const char *fn = "walsh_window_attention_fwd";
+    WinArgs a{};
+    a.scale = scale;
+    int rc = win_check(fn, a, B, H, G, Tq, Tk, D, dtype);
+    if (rc) return rc;
+    if (B == 0 || Tq == 0) return WALSH_OK;
+    a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.o = o, a.lse = lse;
+    a.sq = {q_sb, q_sh, q_st}, a.skv = {kv_sb, kv_sh, kv_st}, a.so = {o_sb, o_sh, o_st};
+    rc = win_check_tensor(fn, "q", q, a.sq, B, H, Tq, D);
+    if (!rc && Tk) rc = win_check_tensor(fn, "k", k, a.skv, B, G, Tk, D);
+    if (!rc && Tk) rc = win_check_tensor(fn, "v", v, a.skv, B, G, Tk, D);
+    if (!rc) rc = win_check_tensor(fn, "o", o, a.so, B, H, Tq, D);
+    if (rc) return rc;
+    a.B = (int)B, a.H = (int)H, a.G = (int)G, a.Tq = (int)Tq, a.Tk = (int)Tk;
+    a.W = window > 0 && window < Tk ? (int)window : 0;
+    a.S = sinks < 0 ? 0 : (int)(sinks < Tk ? sinks : Tk);
+    a.sl2 = scale * kLog2e;
+    const int64_t n = ceil_div(Tq, kWinQ) * H * B;
+    win_dispatch(dtype, D, [&](auto t, auto d) {
+        typedef decltype(t) T;
+        constexpr int DD = decltype(d)::value;
+        launch(window_fwd_kernel<T, DD>, dim3((unsigned)(ceil_div(n, 8) * 8)), dim3(64 * kWinWaves),
+               (uint32_t)(4 * Tile<T, DD, WinCfg<T, DD>::KC>::BYTES), (hipStream_t)stream, a);
+    });
+    return check_hip(hipGetLastError(), fn);
+}
+
+static int win_bwd_qc(int64_t D, int dtype) { return D == 128 && dtype == WALSH_F32 ? 32 : 64; }
+
+static int64_t win_bwd_bytes(const WinArgs &a, int64_t D) {
+    const int64_t delta = ceil_div((int64_t)a.B * a.H * a.Tq * 4, 16) * 16;
+    return delta + (int64_t)a.B * a.G * win_part_slots(a) * 2 * kWinQ * D * 4;
+}
+
+WALSH_EXPORT int64_t walsh_window_attention_bwd_workspace_bytes(int64_t B, int64_t H, int64_t G, int64_t Tq, int64_t Tk,
+                                                                int64_t D, int64_t window, int64_t sinks, int dtype) {
+    if (B < 1 || H < 1 || G < 1 || H % G || Tq < 1 || Tk < 1 || D < 1 || Tq > (1 << 24) || Tk > (1 << 24)) return 0;
+    WinArgs a{};
+    a.B = (int)B, a.H = (int)H, a.G = (int)G, a.Tq = (int)Tq, a.Tk = (int)Tk;
+    a.W = window > 0 && window < Tk ? (int)window : 0;
+    a.S = sinks < 0 ? 0 : (int)(sinks < Tk ? sinks : Tk);
+    win_splits(a, win_bwd_qc(D, dtype));
+    return win_bwd_bytes(a, D);
+}
+
+WALSH_EXPORT int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k,
+                                            const void *v, int64_t kv_sb, int64_t kv_sh, int64_t kv_st, const void *o,
+                                            int64_t o_sb, int64_t o_sh, int64_t o_st, const void *go, int64_t go_sb,
+                                            int64_t go_sh, int64_t go_st, const float *lse, int64_t B, int64_t H,
+                                            int64_t G, int64_t Tq, int64_t Tk, int64_t D, int64_t window, int64_t sinks,
+                                            const int *lengths, float scale, void *dq, void *dk, void *dv, int dtype,
+                                            void *work, int64_t work_bytes, void *stream) {
+    const char *fn = "walsh_window_attention_bwd";
+    WinArgs a{};
+    a.scale = scale;
+    int rc = win_check(fn, a, B, H, G, Tq, Tk, D, dtype);
+    if (rc) return rc;
+    if (B == 0) return WALSH_OK;
+    if (Tq == 0 || Tk == 0) return set_error(WALSH_EINVAL, "%s: no queries or no keys: the gradients are zeros", fn);
+    a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.o = const_cast<void *>(o), a.lse = const_cast<float *>(lse);
+    a.go = go, a.dq = dq, a.dk = dk, a.dv = dv;
+    a.sq = {q_sb, q_sh, q_st}, a.skv = {kv_sb, kv_sh, kv_st}, a.so = {o_sb, o_sh, o_st}, a.sgo = {go_sb, go_sh, go_st};
+    rc = win_check_tensor(fn, "q", q, a.sq, B, H, Tq, D);
+    if (!rc) rc = win_check_tensor(fn, "k", k, a.skv, B, G, Tk, D);
+    if (!rc) rc = win_check_tensor(fn, "v", v, a.skv, B, G, Tk, D);
+    if (!rc) rc = win_check_tensor(fn, "o", o, a.so, B, H, Tq, D);
+    if (!rc) rc = win_check_tensor(fn, "go", go, a.sgo, B, H, Tq, D);
+    if (rc) return rc;
+    if (!lse || !dq || !dk || !dv || !work) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
+    if ((uintptr_t)dq % 16 || (uintptr_t)dk % 16 || (uintptr_t)dv % 16 || (uintptr_t)work % 16)
+        return set_error(WALSH_ENOTSUP, "%s: the gradients and the workspace must be 16-byte aligned", fn);
+    a.B = (int)B, a.H = (int)H, a.G = (int)G, a.Tq = (int)Tq, a.Tk = (int)Tk;
+    a.W = window > 0 && window < Tk ? (int)window : 0;
+    a.S = sinks < 0 ? 0 : (int)(sinks < Tk ? sinks : Tk);
+    a.sl2 = scale * kLog2e;
+    win_splits(a, win_bwd_qc(D, dtype));
+    if (work_bytes < win_bwd_bytes(a, D))
+        return set_error(WALSH_EINVAL, "%s: workspace of %lld bytes, needs %lld", fn, (long long)work_bytes,
+                         (long long)win_bwd_bytes(a, D));
+    a.delta = (float *)work;
+    a.part = (float *)((char *)work + ceil_div((int64_t)a.B * a.H * a.Tq * 4, 16) * 16);
+    hipStream_t s = (hipStream_t)stream;
+    const int64_t nq = ceil_div(Tq, kWinQ) * H * B;
+    const int64_t nk = ((int64_t)a.nsb * a.ns + (int64_t)(a.nb - a.nsb) * a.nn) * G * B;
+    if (nk > (1ll << 30)) return set_error(WALSH_ENOTSUP, "%s: %lld work items", fn, (long long)nk);
+    win_dispatch(dtype, D, [&](auto t, auto d) {
+        typedef decltype(t) T;
+        constexpr int DD = decltype(d)::value;
+        launch(window_bwd_q_kernel<T, DD>, dim3((unsigned)(ceil_div(nq, 8) * 8)), dim3(64 * kWinWaves),
+               (uint32_t)(4 * Tile<T, DD, WinCfg<T, DD>::KC>::BYTES), s, a);
+        launch(window_bwd_kv_kernel<T, DD>, dim3((unsigned)(ceil_div(nk, 8) * 8)), dim3(64 * kWinWaves),
+               (uint32_t)(4 * Tile<T, DD, WinBwdCfg<T, DD>::QC>::BYTES), s, a);
+        const int64_t blocks = (a.nn > 1 ? a.nb : a.nsb) - (a.ns > 1 ? 0 : a.nsb);
+        if (blocks > 0)
+            launch(window_bwd_sum_kernel<T, DD>, dim3((unsigned)(blocks * B * G), (unsigned)(2 * kWinQ * DD / 1024)),
+                   dim3(256), 0, s, a);
+    });
+    return check_hip(hipGetLastError(), fn);
+}

@@ -4,6 +4,7 @@ The library is loaded from ``walsh-research_amd/lib/`` (built in-tree by
 ``make -C walsh-research_amd``).  There is no fallback: if the library is
 missing or no GPU is present, every hot-path op raises.
 """
+import contextlib
 import ctypes
 import os
 import re
@@ -82,6 +83,12 @@ SIGNATURES = {
                                ctypes.c_float, _P, _I64, _P, _P, _I, _P, _I64, _P]),
     "walsh_prefill_attention": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                      ctypes.c_float, _P, _I64, _I64, _I64, _I, _P]),
+    "walsh_window_attention_fwd": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                        _I64, _I64, _I64, _P, _F, _P, _I64, _I64, _I64, _P, _I, _P]),
+    "walsh_window_attention_bwd_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I]),
+    "walsh_window_attention_bwd": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64,
+                                        _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _F, _P, _P,
+                                        _P, _I, _P, _I64, _P]),
     "walsh_linear_wgrad_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "walsh_linear_wgrad": (_I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "walsh_rmsnorm_fwd": (_I, [_P, _P, _I64, _I64, ctypes.c_float, _P, _P, _P]),
@@ -225,6 +232,30 @@ def call(name: str, *args, kernel: str = None, nbytes: int = 0, flops: int = 0) 
             lib().walsh_timing_tag(len(t.meta))
             t.meta.append((kernel, int(nbytes), int(flops)))
     check(getattr(lib(), name)(*args), name)
+
+
+def same_device(fn: str, first: torch.Tensor, *others) -> None:
+    """All tensors (None excepted) on the device of ``first``."""
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{fn}: tensors on {dev} and {t.device}")
+
+
+def device_of(device: torch.device):
+    """``device`` as the current one: what a launch on its streams, and the
+    library's own look at the device, need."""
+    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def call_on(device: torch.device, name: str, *args, **kw) -> None:
+    """``call`` with the device's current stream as the last argument, on
+    whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream(device), **kw)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream(device), **kw)
 
 
 def require_device(t: torch.Tensor, what: str = "tensor") -> None:

@@ -872,6 +872,102 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     return o
 
 
+# ------------------------------------------------------------------ windowed attention
+
+ATTENTION_HEAD_DIMS = (16, 32, 64, 128)
+
+
+def _attn_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [B, heads, T, D] as the attention kernels read it: unit inner
+    stride, the others multiples of 8, rows that do not overlap, 16-byte
+    aligned; itself or a copy."""
+    sb, sh, st, sd = t.stride()
+    if sd == 1 and not (sb | sh | st) & 7 and (st >= t.shape[3] or t.shape[2] == 1) and not t.data_ptr() & 15:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_window_attention(fn, q, k, v, lengths):
+    _hip.require_device(q, "query")
+    assert q.dim() == 4 and k.dim() == 4 and k.shape == v.shape, f"{fn}: q [B, H, Tq, D], k and v [B, G, Tk, D]"
+    B, H, Tq, D = q.shape
+    assert k.shape[0] == B and k.shape[3] == D, f"{fn}: k {tuple(k.shape)} does not fit q {tuple(q.shape)}"
+    assert k.shape[1] > 0 and H % k.shape[1] == 0, f"{fn}: {H} query heads do not share {k.shape[1]} key heads evenly"
+    if D not in ATTENTION_HEAD_DIMS:
+        raise ValueError(f"{fn}: head_dim {D} (one of {ATTENTION_HEAD_DIMS})")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{fn}: q, k, v of one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    _hip.same_device(fn, q, k, v, lengths)
+    if lengths is not None:
+        assert lengths.shape == (B,), f"{fn}: lengths [B]"
+        if lengths.dtype != torch.int32:
+            raise TypeError(f"{fn}: lengths are int32, got {lengths.dtype}")
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
+                     lengths: torch.Tensor = None, scale: float = None, need_lse: bool = False):
+    """Causal attention over the last ``window`` keys and the first ``sinks``
+    ones: q [B, H, Tq, D], k / v [B, G, Tk, D] (G dividing H) -> contiguous
+    [B, H, Tq, D], with ``need_lse`` also the rows' float32 log sum of
+    exponentials [B, H, Tq].  The queries are the last Tq of Tk positions;
+    ``window`` <= 0 is no window; ``lengths`` (int32 [B], on the device) are
+    the keys that each sequence has of Tk.  Rows that see no key are zeros
+    (lse -inf).  Values of keys within the lengths have to be finite, also
+    where the mask hides them from some rows.  Not differentiable by itself:
+    src.model.attention.window_attention is."""
+    _check_window_attention("window_attention", q, k, v, lengths)
+    q, k, v = _attn_rows(q), _attn_rows(k), _attn_rows(v)
+    if v.stride() != k.stride():
+        k, v = k.contiguous(), v.contiguous()
+    B, H, Tq, D = q.shape
+    G, Tk = k.shape[1], k.shape[2]
+    scale = D ** -0.5 if scale is None else float(scale)
+    lengths = None if lengths is None else lengths.contiguous()
+    o = torch.empty(B, H, Tq, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(B, H, Tq, device=q.device, dtype=torch.float32) if need_lse else None
+    span = min(Tk, window + sinks) if window > 0 else Tk
+    _hip.call_on(q.device, "walsh_window_attention_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
+                 *k.stride()[:3], B, H, G, Tq, Tk, D, int(window), int(sinks), _hip.ptr(lengths), scale, o.data_ptr(),
+                 *o.stride()[:3], _hip.ptr(lse), _hip.dtype_code(q.dtype),
+                 kernel="window_fwd_kernel", nbytes=2 * B * D * (H * Tq + G * Tk) * q.element_size(),
+                 flops=4 * B * H * Tq * span * D)
+    return (o, lse) if need_lse else o
+
+
+def window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                         go: torch.Tensor, window: int, sinks: int = 0, lengths: torch.Tensor = None,
+                         scale: float = None):
+    """(dq, dk, dv) of window_attention for the gradient ``go`` of its output:
+    contiguous, in the tensors' dtype.  The same call gives the same bits."""
+    _check_window_attention("window_attention_bwd", q, k, v, lengths)
+    assert go.shape == o.shape == q.shape and lse.shape == q.shape[:3], "window_attention_bwd: o, go as q, lse [B, H, Tq]"
+    if go.dtype != q.dtype or o.dtype != q.dtype or lse.dtype != torch.float32:
+        raise TypeError(f"window_attention_bwd: o, go in {q.dtype} and lse in float32")
+    _hip.same_device("window_attention_bwd", q, o, lse, go)
+    q, k, v, o, go = (_attn_rows(t) for t in (q, k, v, o, go))
+    if v.stride() != k.stride():
+        k, v = k.contiguous(), v.contiguous()
+    lse = lse.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    B, H, Tq, D = q.shape
+    G, Tk = k.shape[1], k.shape[2]
+    scale = D ** -0.5 if scale is None else float(scale)
+    if 0 in (B, Tq, Tk):
+        return tuple(torch.zeros(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+    dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+    dt = _hip.dtype_code(q.dtype)
+    with _hip.device_of(q.device):
+        nws = _hip.lib().walsh_window_attention_bwd_workspace_bytes(B, H, G, Tq, Tk, D, int(window), int(sinks), dt)
+    ws = torch.empty(nws, device=q.device, dtype=torch.uint8)
+    span = min(Tk, window + sinks) if window > 0 else Tk
+    _hip.call_on(q.device, "walsh_window_attention_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
+                 *k.stride()[:3], o.data_ptr(), *o.stride()[:3], go.data_ptr(), *go.stride()[:3], lse.data_ptr(), B, H, G,
+                 Tq, Tk, D, int(window), int(sinks), _hip.ptr(lengths), scale, dq.data_ptr(), dk.data_ptr(),
+                 dv.data_ptr(), dt, ws.data_ptr(), nws, kernel="window_bwd_kernels",
+                 nbytes=4 * B * D * (H * Tq + G * Tk) * q.element_size(), flops=14 * B * H * Tq * span * D)
+    return dq, dk, dv
+
+
 # ------------------------------------------------------------------ channel modulation
 
 def _groups(x: torch.Tensor) -> torch.Tensor:
