@@ -461,6 +461,58 @@ int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_
                                int64_t window, int64_t sinks, const int *lengths, float scale, void *dq, void *dk,
                                void *dv, int dtype, void *work, int64_t work_bytes, void *stream);
 
+/* ------------------------------------------------------------------ paged key-value cache
+ * No counterpart in the reference, whose cache is one dense tensor
+ * (src/model/chassis.py:262-330).  Row j of sequence b is row j % page of page
+ * table[b*table_sb + j / page] (int32); k_pages and v_pages hold n_pages pages
+ * [G][page][D], element (p, g, r, d) at p*sp + g*sg + r*sr + d of both.  page is
+ * a power of two from 16, or any size where pages_per_seq is 1; n_pages,
+ * strides multiples of 8, bases 16-byte aligned; pages_per_seq * page <= 2^30.
+ *
+ * walsh_paged_decode_attention: one new token per sequence, the last of its
+ *   lengths[b] rows (already written): q (b, h, d) at b*q_sb + h*q_sh + d, o
+ *   likewise, H a multiple of G, head h reading key head h / (H / G).  It sees
+ *   the last `window` rows and the first `sinks` ones (window <= 0: all).
+ *   o = softmax(scale q k^T) v; zeros for a length of 0.  A length past the
+ *   table, or a page number outside the pool among the rows seen, gives NaN
+ *   for that sequence and reads nothing outside.  Chunks of the rows are
+ *   joined from the workspace (walsh_paged_decode_workspace_bytes, 0 where one
+ *   chunk holds them all).
+ * walsh_paged_kv_write: k and v [B][T][G][D] (strides sb, st, sg of both) into
+ *   rows start[b] + t, t < count[b] (count null: all T); rows outside the
+ *   table or the pool are dropped.  The rows of one call must be distinct. */
+int64_t walsh_paged_decode_workspace_bytes(int64_t B, int64_t H, int64_t G, int64_t pages_per_seq, int64_t page,
+                                           int64_t D, int64_t window, int64_t sinks, int dtype);
+int walsh_paged_decode_attention(const void *q, int64_t q_sb, int64_t q_sh, const void *k_pages, const void *v_pages,
+                                 int64_t sp, int64_t sg, int64_t sr, int64_t n_pages, int64_t page, const int *table,
+                                 int64_t table_sb, int64_t pages_per_seq, const int *lengths, int64_t B, int64_t H,
+                                 int64_t G, int64_t D, int64_t window, int64_t sinks, float scale, void *o,
+                                 int64_t o_sb, int64_t o_sh, int dtype, void *work, int64_t work_bytes, void *stream);
+int walsh_paged_kv_write(const void *k, const void *v, int64_t sb, int64_t st, int64_t sg, int64_t B, int64_t T,
+                         int64_t G, int64_t D, void *k_pages, void *v_pages, int64_t sp, int64_t sgp, int64_t sr,
+                         int64_t n_pages, int64_t page, const int *table, int64_t table_sb, int64_t pages_per_seq,
+                         const int *start, const int *count, int dtype, void *stream);
+
+/* ------------------------------------------------------------------ sampling
+ * The reference samples by a sort and torch.multinomial on the softmax
+ * (src/model/mhc.py:754-772: temperature and top-k); here the random number is
+ * an input.  walsh_sample: out[b] = the token of row b of logits [B][V] (row
+ * stride ld, float32 or bf16, V <= 2^20) that u[b] in [0, 1) picks:
+ *   w = exp((l - max l) / temperature);  temperature <= 0: the largest logit
+ *   top_k    the k largest logits stay (of equal ones the lowest indexes);
+ *            k <= 0 or >= V: all
+ *   top_p    of these, in descending order, a token stays while the weight
+ *            before it is below top_p of their sum; >= 1: all
+ *   min_p    of these, those with w >= min_p stay
+ *   out      the first index whose running sum of what stays, in index order,
+ *            exceeds u times the whole sum
+ * NaN logits count as -inf; a row of nothing else, or one that min_p leaves
+ * empty, gives -1.  Each of temperature, top_k, top_p, min_p is an array [B] on
+ * the device, or null and the value behind it for every row. */
+int walsh_sample(const void *logits, int64_t ld, int64_t B, int64_t V, const float *u, const float *temperature,
+                 float temperature0, const int *top_k, int top_k0, const float *top_p, float top_p0, const float *min_p,
+                 float min_p0, int64_t *out, int dtype, void *stream);
+
 /* ------------------------------------------------------------------ A14-A17
  * mHC residual streams.  Stream tensors are [M tokens][n streams][C] with row
  * stride ldx >= n*C (elements); n <= 4 and C % 4 == 0 in this build.

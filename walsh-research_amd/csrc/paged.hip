@@ -1,0 +1,433 @@
+// A key-value cache in pages: writing new tokens, and the attention of one new
+// token per sequence over it.
+//
+// Token j of sequence b lies in row j % page of page table[b][j / page]; a
+// page holds [G key heads][page][D] (any strides).  The query of a sequence is
+// its last token, at position p = length - 1, and sees
+//     j > p - W  or  j < S     (W the window, S the first tokens; W <= 0: all)
+//     o = softmax(c q K^T) V
+//
+// Decode.  The visible keys t = 0 .. n - 1 (first tokens, then the window) are
+// cut into chunks; a workgroup takes one chunk of one (sequence, key head) for
+// all R = H / G query heads that share it, so the cache is read once.  Its
+// four wavefronts take every fourth block of keys, each with its own running
+// maximum, sum and accumulators, joined at the end in LDS, and chunks by a
+// second kernel.  Scores are S^T = K Q^T on 32x32 matrix-core tiles (key rows
+// come straight from memory in the operand's layout, 16 bytes a lane), so a
+// lane holds 16 scores of one head; O^T = V^T P^T takes V from LDS, read
+// transposed.  With R < 32 most of a tile is idle, which costs nothing: the
+// matrix cores could feed ten times what memory delivers, and the vector units
+// would be short at R >= 4.  Bound by memory: the next block's K (registers)
+// and V (straight into LDS) are on the way while one is used.
+//
+// Scores, maxima, sums and accumulators are float32; bf16 weights are rounded
+// to bf16 for the product with V (relative 2^-9, as the values' own rounding),
+// the sum takes them unrounded.
+#include "tiles.h"
+
+namespace walsh {
+
+constexpr int kPgWaves = 4;
+constexpr int kPgMaxChunk = 4096;                 // keys per workgroup
+constexpr int kPgMinPage = 16;                    // rows of a page, where a sequence has several
+constexpr int kPgEntries = kPgMaxChunk / kPgMinPage + 4;
+
+struct PgArgs {
+    const void *q;
+    int64_t q_sb, q_sh;                           // q[b][h][d]
+    const void *k, *v;
+    int64_t sp, sg, sr;                           // page, head and row strides of both
+    const int *table, *lengths;
+    int64_t table_sb;
+    int B, H, G, P, N, shift, W, S, chunk, ns;    // P pages in all, N per sequence of 2^shift rows; ns chunks
+    int64_t cap;                                  // rows that a sequence's table covers
+    float sl2;
+    void *o;
+    int64_t o_sb, o_sh;
+    float *part;                                  // [B][H][ns][D + 2]: acc, max, sum
+};
+
+// The visible keys of a sequence: n of them, the first s0 first tokens, key t
+// >= s0 at row t + skip.  bad: a length that the table does not cover.
+struct PgKeys {
+    int n, s0, skip;
+    bool bad;
+};
+__device__ __forceinline__ PgKeys pg_keys(const PgArgs &a, int b) {
+    const int len = a.lengths[b];
+    PgKeys r{max(len, 0), 0, 0, len > a.cap};
+    if (a.W > 0 && r.n > a.W) {
+        r.s0 = min(a.S, r.n - a.W);
+        r.skip = r.n - a.W - r.s0;
+        r.n = a.W + r.s0;
+    }
+    if (r.bad) r.n = 0;
+    return r;
+}
+
+template <typename T, int D> struct PgCfg {
+    // 32-key sub-blocks of a wavefront's step: 8 KB of K (bf16) whatever D
+    static constexpr int NB = sizeof(T) == 2 ? (D == 128 ? 1 : D == 64 ? 2 : 4) : (D >= 64 ? 1 : D == 32 ? 2 : 4);
+    static constexpr int VBYTES = NB * Tile<T, D, 32>::BYTES;
+    // two V buffers per wavefront; at the end 32 rows of D float32
+    static constexpr int WAVE = 2 * VBYTES > 32 * D * 4 ? 2 * VBYTES : 32 * D * 4;
+    static constexpr int LDS = kPgWaves * WAVE;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void paged_decode_kernel(PgArgs a) {
+    constexpr int NB = PgCfg<T, D>::NB, KB = 32 * NB, NK = D / 16, ND = (D + 31) / 32;
+    typedef Tile<T, D, 32> L;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ int pages[kPgEntries];
+    __shared__ float stat[kPgWaves][2][32];
+    __shared__ int any_bad;
+    const int R = a.H / a.G, nqt = (R + 31) / 32;
+    const int s = blockIdx.x, g = (int)blockIdx.y / nqt, r0 = (int)blockIdx.y % nqt * 32, b = blockIdx.z;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 31, hi = lane >> 5;
+    const int heads = min(32, R - r0), h0 = g * R + r0;
+    const PgKeys ks = pg_keys(a, b);
+    const int c0 = s * a.chunk, c1 = min(c0 + a.chunk, ks.n);
+    if (c0 >= c1 && s > 0) return;                // the combine looks at the chunks that exist
+
+    // the chunk's page numbers: of its first tokens, then of its window
+    const int mask = (int)((1u << a.shift) - 1);
+    const int ta = min(c1, ks.s0);                // first tokens c0 .. ta - 1
+    const int ea = c0 >> a.shift, na = c0 < ta ? ((ta - 1) >> a.shift) - ea + 1 : 0;
+    const int tb = max(c0, ks.s0);
+    const int eb = tb < c1 ? (tb + ks.skip) >> a.shift : 0, nb = tb < c1 ? ((c1 - 1 + ks.skip) >> a.shift) - eb + 1 : 0;
+    if (tid == 0) any_bad = ks.bad;
+    __syncthreads();
+    for (int i = tid; i < na + nb; i += 64 * kPgWaves) {
+        const int e = a.table[b * a.table_sb + (i < na ? ea + i : eb + i - na)];
+        const bool ok = (unsigned)e < (unsigned)a.P;
+        pages[i] = ok ? e : 0;
+        if (!ok) any_bad = 1;
+    }
+    __syncthreads();
+
+    Frag<T> qf[NK];
+    {
+        const T *qp = (const T *)a.q + b * a.q_sb + (h0 + min(n, heads - 1)) * a.q_sh;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) qf[kk] = load_frag(qp + 16 * kk + 8 * hi);
+    }
+    // element offset of visible key t (past the last one: the last, never counted)
+    auto at = [&](int t) {
+        t = min(t, c1 - 1);
+        const int j = t < ks.s0 ? t : t + ks.skip, e = t < ks.s0 ? (j >> a.shift) - ea : na + (j >> a.shift) - eb;
+        return pages[e] * a.sp + (j & mask) * a.sr;
+    };
+    const T *kb = (const T *)a.k + g * a.sg, *vb = (const T *)a.v + g * a.sg;
+    unsigned char *vl = smem + wave * PgCfg<T, D>::WAVE;
+    auto fetch_k = [&](Frag<T> (&kf)[NB][NK], int t0) {
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+            const T *p = kb + at(t0 + 32 * u + n) + 8 * hi;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) kf[u][kk] = load_frag(p + 16 * kk);
+        }
+    };
+    auto fetch_v = [&](unsigned char *dst, int t0) {
+        dst = (unsigned char *)__builtin_assume_aligned(dst, 16);
+#pragma unroll
+        for (int i = 0; i < NB * L::BYTES / 1024; ++i) {
+            const int pos = i * 64 + lane, row = pos / L::NCH, c = (pos % L::NCH) ^ L::swz(row & 31);
+            const T *p = vb + at(t0 + row) + c * (16 / (int)sizeof(T));
+            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)const_cast<T *>(p),
+                                             (__attribute__((address_space(3))) void *)(dst + i * 1024), 16, 0, 0);
+        }
+    };
+
+    f32x16 acc[ND];
+#pragma unroll
+    for (int c = 0; c < ND; ++c) acc[c] = f32x16{};
+    float m = kNoScore, l = 0.f;
+    const int stride = KB * kPgWaves;
+    int t0 = c0 + wave * KB, buf = 0;
+    Frag<T> kf[NB][NK];
+    if (t0 < c1) {
+        fetch_k(kf, t0);
+        fetch_v(vl, t0);
+    }
+    for (; t0 < c1; t0 += stride, buf ^= 1) {
+        const int tn = t0 + stride;
+        f32x16 sc[NB];
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+            sc[u] = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) mma(sc[u], kf[u][kk], qf[kk]);
+        }
+        // this block's V has landed (it was requested after this block's K)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (tn < c1) {
+            fetch_k(kf, tn);
+            fetch_v(vl + (buf ^ 1) * PgCfg<T, D>::VBYTES, tn);
+        }
+        if (t0 + KB > c1) {
+#pragma unroll
+            for (int u = 0; u < NB; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t0 + 32 * u + 8 * (r >> 2) + 4 * hi + (r & 3) >= c1) sc[u][r] = -INFINITY;
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
+        mx = fmaxf(mx, other_half(mx));
+        if (__any((mx - m) * a.sl2 > 8.f)) {      // as in the whole-sequence kernel: move the maximum rarely
+            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f((m - mn) * a.sl2);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int c = 0; c < ND; ++c) acc[c] *= al;
+        }
+        const float mo = -m * a.sl2;
+        const unsigned char *vt = vl + buf * PgCfg<T, D>::VBYTES;
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+            float w[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(fmaf(sc[u][r], a.sl2, mo));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) l += w[r];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag<T> pf;
+                pack(pf, w + 8 * t);
+#pragma unroll
+                for (int c = 0; c < ND; ++c) mma(acc[c], L::col(vt + u * L::BYTES, 16 * t, c, lane), pf);
+            }
+        }
+    }
+    l += other_half(l);
+
+    // the wavefronts' parts: o = sum_w acc_w e^(m_w - m) / sum_w l_w e^(m_w - m)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    float *av = (float *)vl;                      // [32 heads][D] of this wavefront (its V is used up)
+    if (n < heads) {
+#pragma unroll
+        for (int c = 0; c < ND; ++c)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int d = 32 * c + 8 * t + 4 * hi;
+                if (D % 32 && d >= D) continue;
+                store4(av + n * D + d, f32x4{acc[c][4 * t], acc[c][4 * t + 1], acc[c][4 * t + 2], acc[c][4 * t + 3]});
+            }
+        if (hi == 0) {
+            stat[wave][0][n] = m;
+            stat[wave][1][n] = l;
+        }
+    }
+    __syncthreads();
+    const bool bad = any_bad != 0;
+    for (int i = tid; i < heads * (D / 4); i += 64 * kPgWaves) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float mm = stat[0][0][r];
+#pragma unroll
+        for (int w = 1; w < kPgWaves; ++w) mm = fmaxf(mm, stat[w][0][r]);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        float ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < kPgWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f((stat[w][0][r] - mm) * a.sl2);
+            v += load4((const float *)(smem + w * PgCfg<T, D>::WAVE) + r * D + d) * f;
+            ll += stat[w][1][r] * f;
+        }
+        if (bad) ll = NAN;                        // a page or length outside the pool: not a number, never a stale value
+        if (a.ns == 1) {
+            store4((T *)a.o + b * a.o_sb + (h0 + r) * a.o_sh + d, bad ? v * ll : ll > 0.f ? v * (1.f / ll) : v * 0.f);
+        } else {
+            float *dst = a.part + (((int64_t)b * a.H + h0 + r) * a.ns + s) * (D + 2);
+            dst[d] = v.x, dst[d + 1] = v.y, dst[d + 2] = v.z, dst[d + 3] = v.w;
+            if (d == 0) dst[D] = mm, dst[D + 1] = ll;
+        }
+    }
+}
+
+// The chunks' parts of one (sequence, query head) joined.
+template <typename T, int D> __global__ __launch_bounds__(D) void paged_decode_join_kernel(PgArgs a) {
+    const int b = (int)blockIdx.x / a.H, h = (int)blockIdx.x % a.H, d = threadIdx.x;
+    const PgKeys ks = pg_keys(a, b);
+    const int ns = max(1, (ks.n + a.chunk - 1) / a.chunk);
+    const float *p = a.part + (int64_t)blockIdx.x * a.ns * (D + 2);
+    float mm = kNoScore;
+#pragma unroll 8
+    for (int s = 0; s < ns; ++s) mm = fmaxf(mm, p[s * (D + 2) + D]);
+    float num = 0.f, den = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < ns; ++s) {
+        const float f = __builtin_amdgcn_exp2f((p[s * (D + 2) + D] - mm) * a.sl2);
+        num += f * p[s * (D + 2) + d];
+        den += f * p[s * (D + 2) + D + 1];
+    }
+    Act<T>::store((T *)a.o + b * a.o_sb + h * a.o_sh + d, den == 0.f ? 0.f : num / den);
+}
+
+// ---------------------------------------------------------------- write
+// New tokens' k and v [B][T][G][D] into the rows start[b] + t of their
+// sequences, t < count[b]: 16 bytes of both per thread, neighbouring threads
+// in one row.  Rows that no page holds are dropped.  Bound by memory.
+struct PgWriteArgs {
+    const void *k, *v;
+    int64_t sb, st, sg;                           // new rows' strides (both)
+    void *kp, *vp;
+    int64_t pp, pg, pr;                           // page, head and row strides (both)
+    const int *table, *start, *count;
+    int64_t table_sb, total;                      // total: 16-byte pieces of k
+    int T, G, P, N, shift, nch;                   // nch: pieces of a row
+    int64_t cap;
+};
+template <typename T> __global__ __launch_bounds__(256) void paged_write_kernel(PgWriteArgs a) {
+    constexpr int E = 16 / (int)sizeof(T);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.total; i += (int64_t)gridDim.x * 256) {
+        const int c = (int)(i % a.nch);
+        const int64_t r = i / a.nch, bt = r / a.G;
+        const int g = (int)(r % a.G), t = (int)(bt % a.T), b = (int)(bt / a.T);
+        if (a.count && t >= a.count[b]) continue;
+        const int64_t j = (int64_t)a.start[b] + t;
+        if (j < 0 || j >= a.cap) continue;
+        const int e = a.table[b * a.table_sb + (j >> a.shift)];
+        if ((unsigned)e >= (unsigned)a.P) continue;
+        const int64_t src = b * a.sb + t * a.st + g * a.sg + c * E;
+        const int64_t dst = e * a.pp + g * a.pg + (j & ((1ll << a.shift) - 1)) * a.pr + c * E;
+        const uint4 kv = *(const uint4 *)((const T *)a.k + src), vv = *(const uint4 *)((const T *)a.v + src);
+        *(uint4 *)((T *)a.kp + dst) = kv;
+        *(uint4 *)((T *)a.vp + dst) = vv;
+    }
+}
+
+// ---------------------------------------------------------------- host
+// Rows of a page as a shift: powers of two from 16, or anything where one
+// page holds a whole sequence.
+static int pg_shift(int64_t N, int64_t page) {
+    if (N == 1) return page >= 1 && page <= (1 << 30) ? 30 : -1;
+    if (page < kPgMinPage || page > (1 << 20) || (page & (page - 1))) return -1;
+    int s = 0;
+    while ((1ll << s) < page) ++s;
+    return s;
+}
+
+static int pg_check(const char *fn, int64_t B, int64_t G, int64_t D, int64_t P, int64_t N, int64_t page, int64_t sp,
+                    int64_t sg, int64_t sr, const void *k, const void *v, const int *table, const int *lengths,
+                    int64_t table_sb, int dtype) {
+    if (B < 1 || B > 65535 || G < 1 || P < 1 || P > INT32_MAX || N < 1 || N > (1 << 24) || N * page > (1 << 30))
+        return set_error(WALSH_EINVAL, "%s: bad shape B=%lld G=%lld pages=%lld x %lld, %lld per sequence", fn,
+                         (long long)B, (long long)G, (long long)P, (long long)page, (long long)N);
+    if (D != 16 && D != 32 && D != 64 && D != 128)
+        return set_error(WALSH_ENOTSUP, "%s: head_dim %lld (16, 32, 64 or 128)", fn, (long long)D);
+    if (dtype != WALSH_F32 && dtype != WALSH_BF16) return set_error(WALSH_ENOTSUP, "%s: dtype %d", fn, dtype);
+    if (pg_shift(N, page) < 0)
+        return set_error(WALSH_ENOTSUP, "%s: pages of %lld rows (a power of two from %d, or one page per sequence)", fn,
+                         (long long)page, kPgMinPage);
+    if (!k || !v || !table || !lengths) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
+    if ((uintptr_t)k % 16 || (uintptr_t)v % 16 || sp % 8 || sg % 8 || sr % 8 || sr < D || sp < 0 || sg < 0 || table_sb < 0)
+        return set_error(WALSH_ENOTSUP, "%s: pages must be 16-byte aligned with strides multiples of 8", fn);
+    return WALSH_OK;
+}
+
+// Keys per workgroup.  As many as leave eight workgroups per slot (two per
+// CU): chunks of a batch of unequal lengths then end together; few sequences
+// are cut finer, down to a block per wavefront.
+static void pg_split(int64_t pairs, int64_t keys, int KB, int64_t *chunk, int64_t *ns) {
+    const int64_t slots = 2 * (int64_t)device_info().cu_count, step = KB * kPgWaves;
+    int64_t c = ceil_div(pairs * keys, 8 * slots);
+    const int64_t fill = ceil_div(pairs * keys, slots);   // what one round of workgroups would take
+    if (c < 512) c = fill < 512 ? fill : 512;             // finer only to fill the chip
+    c = ceil_div(c, step) * step;
+    *chunk = c < step ? step : c > kPgMaxChunk ? kPgMaxChunk : c;
+    *ns = ceil_div(keys, *chunk);
+    if (*ns < 1) *ns = 1;
+}
+static void pg_plan(int64_t B, int64_t H, int64_t G, int64_t cap, int64_t D, int64_t W, int64_t S, int dtype,
+                    int64_t *chunk, int64_t *ns) {
+    const int64_t keys = W > 0 && W + S < cap ? W + S : cap;
+    const int KB = 32 * (dtype == WALSH_BF16 ? (D == 128 ? 1 : D == 64 ? 2 : 4) : (D >= 64 ? 1 : D == 32 ? 2 : 4));
+    pg_split(B * G * ceil_div(H / G, 32), keys, KB, chunk, ns);
+}
+
+}  // namespace walsh
+
+using namespace walsh;
+
+WALSH_EXPORT int64_t walsh_paged_decode_workspace_bytes(int64_t B, int64_t H, int64_t G, int64_t pages_per_seq,
+                                                        int64_t page, int64_t D, int64_t window, int64_t sinks,
+                                                        int dtype) {
+    if (B < 1 || H < 1 || G < 1 || H % G || pages_per_seq < 1 || page < 1 || D < 1) return 0;
+    int64_t chunk, ns;
+    pg_plan(B, H, G, pages_per_seq * page, D, window, sinks < 0 ? 0 : sinks, dtype, &chunk, &ns);
+    return ns > 1 ? B * H * ns * (D + 2) * 4 : 0;
+}
+
+WALSH_EXPORT int walsh_paged_decode_attention(const void *q, int64_t q_sb, int64_t q_sh, const void *k_pages,
+                                              const void *v_pages, int64_t sp, int64_t sg, int64_t sr, int64_t n_pages,
+                                              int64_t page, const int *table, int64_t table_sb, int64_t pages_per_seq,
+                                              const int *lengths, int64_t B, int64_t H, int64_t G, int64_t D,
+                                              int64_t window, int64_t sinks, float scale, void *o, int64_t o_sb,
+                                              int64_t o_sh, int dtype, void *work, int64_t work_bytes, void *stream) {
+    const char *fn = "walsh_paged_decode_attention";
+    if (B == 0) return WALSH_OK;
+    int rc = pg_check(fn, B, G, D, n_pages, pages_per_seq, page, sp, sg, sr, k_pages, v_pages, table, lengths, table_sb,
+                      dtype);
+    if (rc) return rc;
+    if (H < 1 || H % G || H > 65535) return set_error(WALSH_EINVAL, "%s: H=%lld for G=%lld", fn, (long long)H, (long long)G);
+    if (!q || !o) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
+    if ((uintptr_t)q % 16 || (uintptr_t)o % 16 || q_sb % 8 || q_sh % 8 || o_sb % 8 || o_sh % 8)
+        return set_error(WALSH_ENOTSUP, "%s: q and o must be 16-byte aligned with strides multiples of 8", fn);
+    if (!(scale > 0.f) || scale > 1e6f)
+        return set_error(WALSH_EINVAL, "%s: the scale must be positive and at most 1e6", fn);
+    PgArgs a{};
+    a.q = q, a.q_sb = q_sb, a.q_sh = q_sh, a.k = k_pages, a.v = v_pages, a.sp = sp, a.sg = sg, a.sr = sr;
+    a.table = table, a.lengths = lengths, a.table_sb = table_sb;
+    a.B = (int)B, a.H = (int)H, a.G = (int)G, a.P = (int)n_pages, a.N = (int)pages_per_seq;
+    a.shift = pg_shift(pages_per_seq, page);
+    a.cap = pages_per_seq * page;
+    a.W = window > 0 && window < a.cap ? (int)window : 0;
+    a.S = sinks < 0 ? 0 : (int)(sinks < a.cap ? sinks : a.cap);
+    a.sl2 = scale * kLog2e;
+    a.o = o, a.o_sb = o_sb, a.o_sh = o_sh, a.part = (float *)work;
+    int64_t chunk, ns;
+    pg_plan(B, H, G, a.cap, D, a.W, a.S, dtype, &chunk, &ns);
+    a.chunk = (int)chunk, a.ns = (int)ns;
+    if (ns > 1 && (!work || work_bytes < B * H * ns * (D + 2) * 4 || (uintptr_t)work % 16))
+        return set_error(WALSH_EINVAL, "%s: workspace of %lld bytes, needs %lld (16-aligned)", fn, (long long)work_bytes,
+                         (long long)(B * H * ns * (D + 2) * 4));
+    const int64_t gy = G * ceil_div(H / G, 32);
+    if (gy > 65535 || B * H > INT32_MAX) return set_error(WALSH_ENOTSUP, "%s: H=%lld B=%lld", fn, (long long)H, (long long)B);
+    hipStream_t s = (hipStream_t)stream;
+    attn_dispatch(dtype, D, [&](auto t, auto d) {
+        typedef decltype(t) T;
+        constexpr int DD = decltype(d)::value;
+        launch(paged_decode_kernel<T, DD>, dim3((unsigned)ns, (unsigned)gy, (unsigned)B), dim3(64 * kPgWaves),
+               (uint32_t)PgCfg<T, DD>::LDS, s, a);
+        if (ns > 1) launch(paged_decode_join_kernel<T, DD>, dim3((unsigned)(B * H)), dim3(DD), 0, s, a);
+    });
+    return check_hip(hipGetLastError(), fn);
+}
+
+WALSH_EXPORT int walsh_paged_kv_write(const void *k, const void *v, int64_t sb, int64_t st, int64_t sg, int64_t B,
+                                      int64_t T, int64_t G, int64_t D, void *k_pages, void *v_pages, int64_t pp,
+                                      int64_t pg, int64_t pr, int64_t n_pages, int64_t page, const int *table,
+                                      int64_t table_sb, int64_t pages_per_seq, const int *start, const int *count,
+                                      int dtype, void *stream) {
+    const char *fn = "walsh_paged_kv_write";
+    if (B == 0 || T == 0) return WALSH_OK;
+    int rc = pg_check(fn, B, G, D, n_pages, pages_per_seq, page, pp, pg, pr, k_pages, v_pages, table, start, table_sb,
+                      dtype);
+    if (rc) return rc;
+    if (!k || !v || T < 0 || T > (1 << 24)) return set_error(WALSH_EINVAL, "%s: null pointer or T=%lld", fn, (long long)T);
+    if ((uintptr_t)k % 16 || (uintptr_t)v % 16 || sb % 8 || st % 8 || sg % 8)
+        return set_error(WALSH_ENOTSUP, "%s: k and v must be 16-byte aligned with strides multiples of 8", fn);
+    const int nch = (int)(D * (dtype == WALSH_BF16 ? 2 : 4) / 16);
+    PgWriteArgs a{k, v, sb, st, sg, k_pages, v_pages, pp, pg, pr, table, start, count, table_sb, B * T * G * nch,
+                  (int)T, (int)G, (int)n_pages, (int)pages_per_seq, pg_shift(pages_per_seq, page), nch,
+                  pages_per_seq * page};
+    const int64_t wgs = ceil_div(a.total, 256), most = 16 * (int64_t)device_info().cu_count;
+    const dim3 grid((unsigned)(wgs < most ? wgs : most));
+    if (dtype == WALSH_BF16) launch(paged_write_kernel<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    else launch(paged_write_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    return check_hip(hipGetLastError(), fn);
+}

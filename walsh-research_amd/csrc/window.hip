@@ -29,153 +29,9 @@
 // second products (the matrix cores' operand type; relative 2^-9 each, the
 // size of the inputs' own rounding); the sum of weights that normalises a row
 // takes them unrounded.
-#include <type_traits>
-
-#include "common.h"
+#include "tiles.h"
 
 namespace walsh {
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef short i16x8 __attribute__((ext_vector_type(8)));
-
-constexpr float kNoScore = -1e30f;  // running maximum of a row that has seen nothing: finite, so differences stay numbers
-constexpr float kLog2e = 1.4426950408889634f;
-
-// ---------------------------------------------------------------- operands
-// Eight elements of one row or column: a product operand.
-template <typename T> struct Frag;
-template <> struct Frag<uint16_t> { i16x8 v; };
-template <> struct Frag<float> { f32x8 v; };
-
-__device__ __forceinline__ void mma(f32x16 &c, const Frag<uint16_t> &a, const Frag<uint16_t> &b) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), c, 0,
-                                                0, 0);
-}
-__device__ __forceinline__ void mma(f32x16 &c, const Frag<float> &a, const Frag<float> &b) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
-}
-// Result rows 16 t + (4 hi + 0..3, 8 + 4 hi + 0..3) as an operand.
-__device__ __forceinline__ void pack(Frag<uint16_t> &f, const float *p) {
-    const u32x4 u = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
-                     pack_bf16x2(p[6], p[7])};
-    f.v = __builtin_bit_cast(i16x8, u);
-}
-__device__ __forceinline__ void pack(Frag<float> &f, const float *p) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f.v[i] = p[i];
-}
-__device__ __forceinline__ Frag<uint16_t> load_frag(const uint16_t *p) { return {*(const i16x8 *)p}; }
-__device__ __forceinline__ Frag<float> load_frag(const float *p) {
-    const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);
-    return {f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-}
-__device__ __forceinline__ float dot(const Frag<float> &a, const Frag<float> &b) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += a.v[i] * b.v[i];
-    return s;
-}
-__device__ __forceinline__ float dot(const Frag<uint16_t> &a, const Frag<uint16_t> &b) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += bf16_to_f32((uint16_t)a.v[i]) * bf16_to_f32((uint16_t)b.v[i]);
-    return s;
-}
-
-// The value, newly computed as far as the compiler can see: what derives from
-// it is worked out again where it is used and holds no registers across a loop.
-__device__ __forceinline__ int fresh(int v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
-__device__ __forceinline__ float other_half(float v) {   // the value of lane ^ 32
-    return __shfl_xor(v, 32, 64);
-}
-
-// ---------------------------------------------------------------- tiles in LDS
-// ROWS rows of D elements, row-major in 16-byte chunks; chunk c of row r lies
-// at position c ^ swz(r), so that the 16 rows of one chunk column fall on
-// distinct banks (row operands) and so do the four rows of a transposing load.
-template <typename T, int D, int ROWS> struct Tile {
-    static constexpr int NCH = D * (int)sizeof(T) / 16;       // chunks per row: 2 .. 32
-    static constexpr int ROWB = D * (int)sizeof(T);
-    static constexpr int BYTES = ROWS * ROWB;
-    static __device__ __forceinline__ int swz(int r) {
-        if (sizeof(T) == 4) return NCH >= 16 ? r & 15 : NCH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
-        if (NCH == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
-        if (NCH == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
-        return NCH == 4 ? (r >> 2) & 3 : (r >> 3) & 1;
-    }
-    // Rows r0 .. r0 + ROWS - 1 of a matrix with row stride st into LDS, by
-    // WAVES wavefronts, straight from memory (no registers); rows before lo
-    // and at or past n are zeros and are not read.
-    template <int WAVES>
-    static __device__ __forceinline__ void fetch(unsigned char *lds, const T *base, int64_t st, int r0, int lo, int n, int wave,
-                                                 int lane) {
-        const int rows = min(n - r0, ROWS);
-        const uint32_t span = rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * st + D) * (int)sizeof(T)) : 0u;
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (int64_t)r0 * st, span);
-        constexpr int N = BYTES / 1024;   // wavefront loads
-        static_assert(BYTES % 1024 == 0, "whole loads");
-#pragma unroll
-        for (int i = 0; i < (N + WAVES - 1) / WAVES; ++i) {
-            const int k = i * WAVES + __builtin_amdgcn_readfirstlane(wave);
-            if (N % WAVES && k >= N) break;
-            const int pos = k * 64 + lane, row = pos / NCH, c = (pos % NCH) ^ swz(row);
-            const uint32_t off = row < rows && row >= lo - r0 ? (uint32_t)row * (uint32_t)(st * (int)sizeof(T)) + 16 * c : kOOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(lds + k * 1024), 16,
-                                                     off, 0, 0, 0);
-        }
-    }
-    // Eight elements of row r from column 16 kk + 8 hi.
-    static __device__ __forceinline__ Frag<T> row(const unsigned char *lds, int r, int kk, int hi) {
-        const unsigned char *p = lds + r * ROWB;
-        const int s = swz(r);
-        if constexpr (sizeof(T) == 2) {
-            return {*(const i16x8 *)(p + (((2 * kk + hi) ^ s) << 4))};
-        } else {
-            const f32x4 a = *(const f32x4 *)(p + (((4 * kk + 2 * hi) ^ s) << 4));
-            const f32x4 b = *(const f32x4 *)(p + (((4 * kk + 2 * hi + 1) ^ s) << 4));
-            return {f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-        }
-    }
-    // Column 32 c + lane % 32 (modulo D) of rows r + 4 hi + 0..3 and r + 8 + 4 hi + 0..3.
-    static __device__ __forceinline__ Frag<T> col(const unsigned char *lds, int r, int c, int lane) {
-        const int hi = lane >> 5;
-        if constexpr (sizeof(T) == 2) {
-            typedef short i16x4v __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) i16x4v *P;
-            const int l = lane & 15, half = D >= 32 ? (lane >> 4) & 1 : 0;
-            const int ch = 4 * c + 2 * half + ((l & 3) >> 1), byte = 8 * (l & 1);
-            const int ra = r + 4 * hi + (l >> 2), rb = ra + 8;
-            const i16x4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (P)(const_cast<unsigned char *>(lds) + ra * ROWB + ((ch ^ swz(ra)) << 4) + byte));
-            const i16x4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (P)(const_cast<unsigned char *>(lds) + rb * ROWB + ((ch ^ swz(rb)) << 4) + byte));
-            return {__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)};
-        } else {
-            const int d = (32 * c + (lane & 31)) % D;
-            f32x8 v;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int rr = r + 4 * hi + (e & 3) + 8 * (e >> 2);
-                v[e] = *(const float *)(lds + rr * ROWB + (((d >> 2) ^ swz(rr)) << 4) + 4 * (d & 3));
-            }
-            return {v};
-        }
-    }
-};
-
-// All of this wavefront's loads into LDS have landed and its LDS reads are
-// done; then all wavefronts'.
-__device__ __forceinline__ void tiles_ready() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
 
 // ---------------------------------------------------------------- arguments
 struct WinTensor {
@@ -689,18 +545,6 @@ static int win_check_tensor(const char *fn, const char *name, const void *p, con
 
 using namespace walsh;
 
-// Calls go(T(), integral constant D) for the dtype and head_dim at hand.
-template <typename F> static void win_dispatch(int dtype, int64_t D, F go) {
-    auto by_dim = [&](auto t) {
-        if (D == 16) go(t, std::integral_constant<int, 16>());
-        else if (D == 32) go(t, std::integral_constant<int, 32>());
-        else if (D == 64) go(t, std::integral_constant<int, 64>());
-        else go(t, std::integral_constant<int, 128>());
-    };
-    if (dtype == WALSH_BF16) by_dim(uint16_t(0));
-    else by_dim(float(0));
-}
-
 WALSH_EXPORT int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k,
                                             const void *v, int64_t kv_sb, int64_t kv_sh, int64_t kv_st, int64_t B,
                                             int64_t H, int64_t G, int64_t Tq, int64_t Tk, int64_t D, int64_t window,
@@ -724,7 +568,7 @@ WALSH_EXPORT int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t
     a.S = sinks < 0 ? 0 : (int)(sinks < Tk ? sinks : Tk);
     a.sl2 = scale * kLog2e;
     const int64_t n = ceil_div(Tq, kWinQ) * H * B;
-    win_dispatch(dtype, D, [&](auto t, auto d) {
+    attn_dispatch(dtype, D, [&](auto t, auto d) {
         typedef decltype(t) T;
         constexpr int DD = decltype(d)::value;
         launch(window_fwd_kernel<T, DD>, dim3((unsigned)(ceil_div(n, 8) * 8)), dim3(64 * kWinWaves),
@@ -791,7 +635,7 @@ WALSH_EXPORT int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t
     const int64_t nq = ceil_div(Tq, kWinQ) * H * B;
     const int64_t nk = ((int64_t)a.nsb * a.ns + (int64_t)(a.nb - a.nsb) * a.nn) * G * B;
     if (nk > (1ll << 30)) return set_error(WALSH_ENOTSUP, "%s: %lld work items", fn, (long long)nk);
-    win_dispatch(dtype, D, [&](auto t, auto d) {
+    attn_dispatch(dtype, D, [&](auto t, auto d) {
         typedef decltype(t) T;
         constexpr int DD = decltype(d)::value;
         launch(window_bwd_q_kernel<T, DD>, dim3((unsigned)(ceil_div(nq, 8) * 8)), dim3(64 * kWinWaves),

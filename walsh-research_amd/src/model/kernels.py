@@ -968,6 +968,135 @@ def window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     return dq, dk, dv
 
 
+# ------------------------------------------------------------------ paged key-value cache
+
+def _check_pages(fn, k_pages, v_pages, table, rows, B, G, D, dtype):
+    """The checks that the host can make of a paged cache: pages
+    [P, G, page, D] and an int32 table [B, pages per sequence]."""
+    _hip.require_device(k_pages, "cache")
+    assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape, f"{fn}: k and v pages [P, G, page, D]"
+    assert k_pages.shape[1] == G and k_pages.shape[3] == D, \
+        f"{fn}: pages {tuple(k_pages.shape)} do not hold {G} heads of {D}"
+    assert table.dim() == 2 and table.shape[0] == B and rows.shape == (B,), f"{fn}: table [B, N] and lengths [B]"
+    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise TypeError(f"{fn}: pages in {dtype}, got {k_pages.dtype} and {v_pages.dtype}")
+    if table.dtype != torch.int32 or rows.dtype != torch.int32:
+        raise TypeError(f"{fn}: table and lengths are int32, got {table.dtype} and {rows.dtype}")
+    if D not in ATTENTION_HEAD_DIMS:
+        raise ValueError(f"{fn}: head_dim {D} (one of {ATTENTION_HEAD_DIMS})")
+    assert k_pages.stride() == v_pages.stride() and k_pages.stride(3) == 1, f"{fn}: pages of one layout, unit inner stride"
+    assert table.stride(1) == 1 or table.shape[1] == 1, f"{fn}: table rows are contiguous"
+
+
+def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                           lengths: torch.Tensor, window: int = 0, sinks: int = 0, scale: float = None) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged cache: q
+    [B, H, 1, D]; pages [P, G, page, D] (G dividing H); row j of sequence b in
+    page ``page_table[b, j // page]``; the query is the last of ``lengths[b]``
+    rows and sees the last ``window`` (<= 0: all) and the first ``sinks`` of
+    them -> [B, H, 1, D] in q.dtype, zeros for a length of 0, NaN where a
+    length or a page number lies outside the table or the pool (they are on
+    the device: nothing outside is read)."""
+    _hip.require_device(q, "query")
+    assert q.dim() == 4 and q.shape[2] == 1, "paged_decode_attention: q [B, H, 1, D]"
+    B, H, _, D = q.shape
+    _, G, page, _ = k_pages.shape
+    _check_pages("paged_decode_attention", k_pages, v_pages, page_table, lengths, B, G, D, q.dtype)
+    assert G > 0 and H % G == 0, f"paged_decode_attention: {H} query heads do not share {G} key heads evenly"
+    _hip.same_device("paged_decode_attention", q, k_pages, v_pages, page_table, lengths)
+    dt = _hip.dtype_code(q.dtype)
+    scale = D ** -0.5 if scale is None else float(scale)
+    q = _attn_rows(q)
+    lengths = lengths.contiguous()
+    o = torch.empty(B, H, 1, D, device=q.device, dtype=q.dtype)
+    N = page_table.shape[1]
+    with _hip.device_of(q.device):
+        nws = _hip.lib().walsh_paged_decode_workspace_bytes(B, H, G, N, page, D, int(window), int(sinks), dt)
+    ws = torch.empty(nws, device=q.device, dtype=torch.uint8) if nws else None
+    span = min(N * page, window + sinks) if window > 0 else N * page
+    _hip.call_on(q.device, "walsh_paged_decode_attention", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(),
+                 v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.shape[0], page, page_table.data_ptr(),
+                 page_table.stride(0), N, lengths.data_ptr(), B, H, G, D, int(window), int(sinks), scale, o.data_ptr(),
+                 o.stride(0), o.stride(1), dt, _hip.ptr(ws), nws, kernel="paged_decode_kernel",
+                 nbytes=2 * B * G * span * D * q.element_size(), flops=4 * B * H * span * D)
+    return o
+
+
+def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                   page_table: torch.Tensor, start: torch.Tensor, counts: torch.Tensor = None) -> None:
+    """Writes new tokens into a paged cache, in place: token t of sequence b
+    (k / v [B, T, G, D]) to row ``start[b] + t`` where t < ``counts[b]``
+    (None: all T).  Rows outside the table or the pool are dropped; two
+    sequences of one call must not share the rows they write."""
+    _hip.require_device(k, "keys")
+    assert k.dim() == 4 and k.shape == v.shape, "paged_kv_write: k and v [B, T, G, D]"
+    B, T, G, D = k.shape
+    _check_pages("paged_kv_write", k_pages, v_pages, page_table, start, B, G, D, k.dtype)
+    if v.dtype != k.dtype:
+        raise TypeError(f"paged_kv_write: k and v of one dtype, got {k.dtype} and {v.dtype}")
+    if counts is not None:
+        assert counts.shape == (B,), "paged_kv_write: counts [B]"
+        if counts.dtype != torch.int32:
+            raise TypeError(f"paged_kv_write: counts are int32, got {counts.dtype}")
+        counts = counts.contiguous()
+    _hip.same_device("paged_kv_write", k, v, k_pages, v_pages, page_table, start, counts)
+    k, v = _attn_rows(k), _attn_rows(v)
+    if k.stride() != v.stride():
+        k, v = k.contiguous(), v.contiguous()
+    start = start.contiguous()
+    _hip.call_on(k.device, "walsh_paged_kv_write", k.data_ptr(), v.data_ptr(), *k.stride()[:3], B, T, G, D,
+                 k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.shape[0], k_pages.shape[2],
+                 page_table.data_ptr(), page_table.stride(0), page_table.shape[1], start.data_ptr(), _hip.ptr(counts),
+                 _hip.dtype_code(k.dtype), kernel="paged_write_kernel", nbytes=4 * k.numel() * k.element_size())
+
+
+# ------------------------------------------------------------------ sampling
+
+def _row_setting(name, value, like, dtype):
+    """A setting of ``sample``: a value for all rows, or one per row."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    assert value.shape == like.shape[:1], f"sample: {name} is a number or [B]"
+    if value.dtype != dtype:
+        raise TypeError(f"sample: {name} is {dtype}, got {value.dtype}")
+    _hip.same_device("sample", like, value)
+    return value.contiguous(), 0
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
+    """Tokens [B] (int64) of logits [B, V] that the uniform numbers u [B]
+    (float32, in [0, 1)) pick: of the ``top_k`` largest (<= 0: all; of equal
+    ones the lowest indexes), those in descending order before which less than
+    ``top_p`` of the weight lies (>= 1: all), of these the ones with at least
+    ``min_p`` of the largest probability; the first token, in index order,
+    whose running probability exceeds u.  ``temperature`` <= 0 takes the
+    largest logit.  Each setting is a number or a tensor [B] (float32, top_k
+    int32).  A row with no finite logit gives -1."""
+    _hip.require_device(logits, "logits")
+    assert logits.dim() == 2 and u.shape == logits.shape[:1], "sample: logits [B, V] and u [B]"
+    if u.dtype != torch.float32:
+        raise TypeError(f"sample: u is float32, got {u.dtype}")
+    _hip.same_device("sample", logits, u)
+    if not isinstance(min_p, torch.Tensor) and not 0.0 <= min_p <= 1.0:
+        raise ValueError(f"sample: min_p {min_p} (0 to 1)")
+    if not isinstance(temperature, torch.Tensor) and temperature != temperature:
+        raise ValueError("sample: temperature is not a number")
+    B, V = logits.shape
+    dt = _hip.dtype_code(logits.dtype)
+    if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
+        logits = logits.contiguous()
+    tt, t0 = _row_setting("temperature", temperature, logits, torch.float32)
+    kt, k0 = _row_setting("top_k", top_k, logits, torch.int32)
+    pt, p0 = _row_setting("top_p", top_p, logits, torch.float32)
+    mt, m0 = _row_setting("min_p", min_p, logits, torch.float32)
+    u = u.contiguous()
+    out = torch.empty(B, device=logits.device, dtype=torch.int64)
+    _hip.call_on(logits.device, "walsh_sample", logits.data_ptr(), logits.stride(0), B, V, u.data_ptr(), _hip.ptr(tt), t0,
+                 _hip.ptr(kt), min(max(int(k0), 0), V), _hip.ptr(pt), p0, _hip.ptr(mt), m0, out.data_ptr(), dt,
+                 kernel="sample_kernel", nbytes=B * V * logits.element_size(), flops=4 * B * V)
+    return out
+
+
 # ------------------------------------------------------------------ channel modulation
 
 def _groups(x: torch.Tensor) -> torch.Tensor:
