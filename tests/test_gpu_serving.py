@@ -1,0 +1,279 @@
+"""The windowed attention, the paged cache and the sampling as a model uses
+them, together: cached against uncached, windowed against a masked attention,
+captured against eager.  Bars as of the other model tests: float32 within 1e-5
+relative, bf16 against the float32 forward within max(1e-2, 1.25 x the uncached
+bf16 forward's own distance)."""
+import pytest
+import torch
+from torch.nn.attention import SDPBackend, sdpa_kernel
+
+pytestmark = pytest.mark.gpu
+
+
+def rel(a, b):
+    a, b = a.double().cpu(), b.double().cpu()
+    return float((a - b).norm() / b.norm().clamp_min(1e-30))
+
+
+def make(C=512, n_layer=2, n_head=32, seed=0, cls="mHCWalsh", **kw):
+    import src.model as M
+    torch.manual_seed(seed)
+    args = dict(block_size=64, vocab_size=1000, n_layer=n_layer, n_head=n_head, n_embd=C, algebra="hadamard",
+                head_mixing=n_head % 32 == 0)
+    args.update(kw)
+    return getattr(M, cls)(M.WalshConfig(**args)).cuda().eval()
+
+
+def tokens(B, T, seed=1):
+    return torch.randint(0, 1000, (B, T), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def paged(model, batch, pages=64, dtype=torch.float32, page_size=16, max_seq_len=128):
+    from src.model import PagedKVCache
+    cfg = model.config
+    return PagedKVCache(cfg.n_layer, pages, cfg.n_head, cfg.n_embd // cfg.n_head, max_seq_len, "cuda", dtype, batch,
+                        page_size)
+
+
+@pytest.mark.parametrize("cls,kw", [("mHCWalsh", dict(attn_window=16, attn_sinks=2)), ("mHCWalsh", dict(attn_window=24)),
+                                    ("Walsh", dict(attn_window=16, attn_sinks=3, use_moe=True)),
+                                    ("mHCWalsh", dict(C=256, n_head=8, algebra="octonion", attn_window=9, attn_sinks=1))])
+def test_windowed_model_against_masked_attention(cls, kw, monkeypatch):
+    """Logits and gradients with the window on the kernels equal those with
+    the mask given to torch's attention (float32)."""
+    from src.model import kernels
+    model = make(cls=cls, **kw)
+    idx, tgt = tokens(2, 60), tokens(2, 60, 2)
+
+    def step():
+        model.train()
+        model.zero_grad()
+        with sdpa_kernel(SDPBackend.MATH):      # float32 products throughout
+            logits, loss = model(idx, targets=tgt)
+            loss.backward()
+        model.eval()
+        return [logits.detach()] + [p.grad.clone() for p in model.parameters() if p.grad is not None]
+    own = step()
+    monkeypatch.setattr(kernels, "window_attention_supported", lambda q: False)
+    ref = step()
+    # gradients that all but cancel (the stream mappings': their inputs are
+    # equal streams at the start) hold little but rounding: they are left out
+    most = max(g.norm() for g in ref[1:])
+    full = [rel(a, b) for a, b in zip(own, ref) if b.norm() > 1e-3 * most]
+    print(f"{cls} {kw}: logits {full[0]:.2e}, worst of {len(full) - 1} gradients {max(full[1:]):.2e}")
+    # the octonion layers compute with bf16 operands whatever the model's type:
+    # a difference of one float32 step may move a rounding, as in a bf16 model
+    own_bf16 = kw.get("algebra") == "octonion"
+    assert full[0] <= (1e-2 if own_bf16 else 1e-5) and max(full[1:]) <= (2e-2 if own_bf16 else 1e-4)
+    monkeypatch.undo()
+    model.layers[0].attention.window = 0
+    assert rel(step()[0], ref[0]) > 1e-3    # the window matters at this length
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kw", [dict(), dict(attn_window=16, attn_sinks=2), dict(attn_window=8, attn_sinks=0)])
+def test_dense_cache_decode_matches_uncached(kw, dtype):
+    from src.model import KVCache
+    model = make(**kw)
+    B, T0, steps = 3, 30, 6
+    idx = tokens(B, T0 + steps)
+    kv = KVCache(2, 64, 32, 16, torch.device("cuda"), dtype=dtype, batch=B)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+        for a, e in [(0, 20), (20, T0)] + [(T0 + s, T0 + s + 1) for s in range(steps)]:
+            lg, _ = model(idx[:, a:e], kv_cache=kv, start_pos=a)
+            kv.increment(e - a)
+            compare(model, idx[:, :e], lg, dtype, f"{kw} to {e}")
+
+
+def compare(model, idx, got, dtype, what):
+    ref, _ = model(idx)
+    if dtype == torch.float32:
+        r = rel(got, ref)
+        print(f"{what}: {r:.2e}")
+        assert r <= (1e-2 if model.config.algebra == "octonion" else 1e-5)   # octonion layers: bf16 operands
+        return
+    with torch.autocast("cuda", enabled=False):
+        ref32, _ = model(idx)
+    own, unc = rel(got, ref32), rel(ref, ref32)
+    print(f"{what}: cached {own:.2e}, uncached {unc:.2e} from float32")
+    assert own <= max(1e-2, 1.25 * unc)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kw", [dict(), dict(attn_window=16, attn_sinks=2), dict(C=256, n_head=8, use_moe=True),
+                                dict(C=256, n_head=8, algebra="octonion", attn_window=20, attn_sinks=1),
+                                dict(cls="Walsh", attn_window=8)])
+def test_paged_cache_matches_uncached_sequences(kw, dtype):
+    """Prompts of unequal lengths, padded, then one token at a time; one
+    sequence ends and its pages go to another; every step's logits equal the
+    uncached forward of that sequence alone."""
+    model = make(**kw)
+    B, T0 = 3, 30
+    lens = [30, 7, 18]
+    idx = tokens(B, 60)
+    kv = paged(model, B, pages=8, dtype=dtype, max_seq_len=60)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+        kv.reserve(lens)
+        lg, _ = model(idx[:, :T0], kv_cache=kv)
+        kv.increment()
+        at = list(lens)
+        seqs = [idx[b:b + 1] for b in range(B)]
+        for s in range(8):
+            for b in range(B):
+                if at[b]:
+                    compare(model, seqs[b][:, :at[b]], lg[b:b + 1], dtype, f"{kw} step {s} row {b}")
+            if s == 3:
+                kv.release(1)
+                at[1] = 0
+                seqs[1] = tokens(1, 60, 5)
+            take = [1, 0 if s == 5 else 1, 1]
+            kv.reserve(take)
+            lg, _ = model(torch.cat([q[:, n:n + 1] for q, n in zip(seqs, at)]), kv_cache=kv)
+            kv.increment()
+            lg = lg.clone()
+            at = [n + c for n, c in zip(at, take)]
+            if s == 5:
+                lg[1] = model(seqs[1][:, :at[1]])[0]      # took no token: nothing to compare
+    assert kv.seq_lens == at
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(attn_window=16, attn_sinks=2)])
+def test_prompts_in_parts(kw):
+    """A second part of several tokens behind cached ones, of two of three
+    sequences."""
+    model = make(**kw)
+    idx = tokens(3, 50)
+    kv = paged(model, 3)
+    with torch.no_grad():
+        kv.reserve([20, 20, 5])
+        model(idx[:, :20], kv_cache=kv)
+        kv.increment()
+        kv.reserve([30, 11, 0])
+        lg, _ = model(idx[:, 20:50], kv_cache=kv)
+        kv.increment()
+        for b, n in ((0, 50), (1, 31)):
+            compare(model, idx[b:b + 1, :n], lg[b:b + 1], torch.float32, f"{kw} part two, row {b}")
+        kv.reserve([0, 0, 1])
+        lg, _ = model(idx[:, 5:6], kv_cache=kv)
+        kv.increment()
+        compare(model, idx[2:, :6], lg[2:], torch.float32, f"{kw} row 2")
+
+
+def test_generate_with_the_paged_cache():
+    """The largest logit each time: the same tokens as without a cache, for
+    prompts alone and padded together; and drawn ones from the same random
+    numbers as the sampling called by hand."""
+    from src.model import kernels
+    model = make(attn_window=16, attn_sinks=2)
+    idx = tokens(3, 20)
+    want = idx.clone()
+    with torch.no_grad():
+        for _ in range(12):
+            want = torch.cat([want, model(want)[0][:, -1].argmax(-1, keepdim=True)], 1)
+    got = model.generate(idx, 12, temperature=0.0, kv_cache=paged(model, 3))
+    assert torch.equal(got, want)
+    lens = [20, 4, 11]
+    got = model.generate(idx, 6, temperature=0.0, kv_cache=paged(model, 3), lengths=lens)
+    for b, n in enumerate(lens):
+        w = idx[b:b + 1, :n]
+        with torch.no_grad():
+            for _ in range(6):
+                w = torch.cat([w, model(w)[0][:, -1].argmax(-1, keepdim=True)], 1)
+        assert torch.equal(got[b, 20:], w[0, n:]), b
+    settings = dict(temperature=0.9, top_k=50, top_p=0.9, min_p=0.01)
+    torch.manual_seed(3)
+    got = model.generate(idx, 5, kv_cache=paged(model, 3), **settings)
+    torch.manual_seed(3)
+    w = idx
+    with torch.no_grad():
+        for _ in range(5):
+            t = kernels.sample(model(w)[0][:, -1], torch.rand(3, device="cuda"), **settings)
+            w = torch.cat([w, t[:, None]], 1)
+    assert torch.equal(got, w)
+    torch.manual_seed(3)
+    assert torch.equal(model.generate(idx, 5, **settings), w)
+
+
+def test_generate_without_new_arguments_is_the_old_loop():
+    model = make()
+    idx = tokens(2, 10)
+    torch.manual_seed(5)
+    got = model.generate(idx, 4, temperature=0.8, top_k=20)
+    torch.manual_seed(5)
+    with torch.no_grad():
+        for _ in range(4):
+            z = model(idx)[0][:, -1].float() / 0.8
+            z[z < torch.topk(z, 20)[0][:, [-1]]] = -float("inf")
+            idx = torch.cat([idx, torch.multinomial(torch.softmax(z, -1), 1)], 1)
+    assert torch.equal(got, idx)
+
+
+def test_captured_decode_step_with_sampling():
+    """Model, cache and sampling of one token captured once and replayed as
+    the sequences grow, with eager work in between, against eager steps."""
+    from src.model import kernels
+    model = make(attn_window=24, attn_sinks=2)
+    B, lens, steps = 3, [20, 3, 11], 10
+    idx = tokens(B, 20)
+    g = torch.Generator().manual_seed(0)
+    us = torch.rand(steps, B, generator=g).cuda()
+    runs = []
+    for captured in (False, True):
+        kv = paged(model, B, dtype=torch.bfloat16)
+        u, tok = us[0].clone(), torch.zeros(B, 1, dtype=torch.int64, device="cuda")
+
+        def step():
+            with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+                lg, _ = model(tok, kv_cache=kv)
+            return kernels.sample(lg[:, -1], u, 0.9, 100, 0.95)
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+            kv.reserve(lens)
+            lg, _ = model(idx, kv_cache=kv)
+            kv.increment()
+        tok.copy_(lg[:, -1].argmax(-1, keepdim=True))
+        graph, out = None, []
+        for s in range(steps):
+            u.copy_(us[s])
+            kv.reserve(1)
+            if captured and graph is None:
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    step()
+                torch.cuda.current_stream().wait_stream(side)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    new = step()
+            if captured:
+                graph.replay()
+                torch.randn(256, 256, device="cuda").sum().item()
+            else:
+                new = step()
+            kv.increment()
+            tok.copy_(new[:, None])
+            out.append(new.clone())
+        runs.append(torch.stack(out))
+    assert torch.equal(*runs)
+
+
+def test_paged_cache_refusals_in_a_model():
+    model = make()
+    idx = tokens(2, 5)
+    kv = paged(model, 2)
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="reserved"):
+            model(idx, kv_cache=kv)
+        kv.reserve([5, 5])
+        with pytest.raises(AssertionError, match="2 sequences"):
+            model(idx[:1], kv_cache=kv)
+        with pytest.raises(ValueError, match="rotary"):
+            model(idx, kv_cache=paged(model, 2, max_seq_len=1000))
+        kv.reset()
+        with pytest.raises(ValueError, match="lengths"):
+            model.generate(idx, 2, kv_cache=kv, lengths=[6, 1])
+        with pytest.raises(ValueError, match="kv_cache"):
+            model.generate(idx, 2, lengths=[5, 1])
+        kv.reserve(1)
+        kv.increment()
+        with pytest.raises(ValueError, match="not empty"):
+            model.generate(idx, 2, kv_cache=kv)

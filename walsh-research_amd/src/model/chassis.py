@@ -23,6 +23,7 @@ from .hadamard import HadamardHeadMixer, HadamardHeadMixerFused
 from .octonion import OctonionHeadMixerFused, OctonionTernaryLinear
 from . import kernels
 from ._common import WeightCache, act_dtype, cached_linear, first_order, plain_eager
+from .attention import PagedKVCache, window_attention, window_mask
 
 _HADAMARD_AVAILABLE = True
 _HADAMARD_HEAD_MIXER_AVAILABLE = True
@@ -30,7 +31,7 @@ _HADAMARD_HEAD_MIXER_AVAILABLE = True
 
 @dataclass
 class WalshConfig:
-    """chassis.py:33-51 (fields and defaults unchanged)."""
+    """chassis.py:33-51 (its fields and defaults unchanged, two added)."""
     block_size: int = 256
     vocab_size: int = 65
     n_layer: int = 6
@@ -46,6 +47,10 @@ class WalshConfig:
     moe_min_experts: int = 1
     moe_max_experts: int = 4
     use_channel_mod: bool = False
+    # no counterpart in the reference: attention over the last attn_window
+    # positions and the first attn_sinks ones (0: over all of them)
+    attn_window: int = 0
+    attn_sinks: int = 0
 
 
 def get_linear_layer(config: WalshConfig):
@@ -181,6 +186,28 @@ class KVCache:
         self.cached_len = 0
 
 
+def cache_freqs(freqs_cis, T, start_pos, kv_cache):
+    """Rotary rows of a forward: positions start_pos .. start_pos + T - 1, or
+    where a paged cache stands: one position per sequence for a single token,
+    the sequences' common one for several."""
+    if not isinstance(kv_cache, PagedKVCache):
+        return freqs_cis[start_pos:start_pos + T]
+    if kv_cache.max_seq_len > freqs_cis.shape[0]:
+        raise ValueError(f"paged cache of {kv_cache.max_seq_len} positions for {freqs_cis.shape[0]} rotary rows")
+    if T > 1:
+        return freqs_cis[kv_cache.cached_len:kv_cache.cached_len + T]
+    return freqs_cis.index_select(0, kv_cache.lengths.clamp(0, freqs_cis.shape[0] - 1))
+
+
+def last_rows(h, kv_cache):
+    """[B, 1, C]: the last token of every row of h [B, T, C] (of a padded
+    prompt going into a paged cache: the last that counts)."""
+    if not isinstance(kv_cache, PagedKVCache) or h.size(1) == 1:
+        return h[:, -1:, :]
+    at = (kv_cache.counts.long() - 1).clamp_min(0)
+    return h.gather(1, at[:, None, None].expand(-1, 1, h.size(2)))
+
+
 def precompute_freqs_cis(dim: int, end: int, theta: float = 10000.0):
     """RoPE table (chassis.py:332-337)."""
     freqs = 1.0 / (theta ** (torch.arange(0, dim, 2)[: (dim // 2)].float() / dim))
@@ -249,6 +276,8 @@ class CausalSelfAttention(nn.Module):
         self.wv = LinearLayer(config.n_embd, config.n_embd)
         self.wo = LinearLayer(config.n_embd, config.n_embd)
         self.dropout = config.dropout
+        self.window = getattr(config, 'attn_window', 0)
+        self.sinks = getattr(config, 'attn_sinks', 0)
         self.head_mixer = get_head_mixer(config, self.head_dim)
 
     def _qkv_multi(self, x, freqs_cis, T, outs=None):
@@ -280,13 +309,14 @@ class CausalSelfAttention(nn.Module):
         return kernels.head_mixer_proj(x, self.head_mixer._kweight(torch.bfloat16), self.head_mixer.beta, kw,
                                        wo.alpha, wo.beta)
 
-    def forward(self, x, freqs_cis, kv_cache: Optional[KVCache] = None, layer_idx: int = 0):
+    def _qkv(self, x, freqs_cis, kv_cache, layer_idx):
+        """q, k (roped) and v [B, T, n_head, head_dim] of x [B, T, C], and
+        whether k and v already lie in the dense cache's slot."""
         B, T, C = x.size()
-        dt = act_dtype(x)
-        x = x.to(dt)
-        q = k = None
+        dt = x.dtype
         fused, in_cache = None, False
-        if (kv_cache is not None and T == 1 and B <= kv_cache.batch and self.n_head == 32
+        if (kv_cache is not None and not isinstance(kv_cache, PagedKVCache) and T == 1 and B <= kv_cache.batch
+                and self.n_head == 32
                 and kv_cache.cached_len < kv_cache.max_seq_len and kv_cache.k_cache[layer_idx].dtype == dt):
             # decode: k and v go straight into the cache slot (no copy kernels)
             fused = self._qkv_multi(x, freqs_cis, T, outs=(None,) + kv_cache.slot(layer_idx, B))
@@ -294,14 +324,13 @@ class CausalSelfAttention(nn.Module):
         if fused is None:
             fused = self._qkv_multi(x, freqs_cis, T)
         if fused is not None:
-            q, k, v = (t.view(B, T, self.n_head, self.head_dim) for t in fused)
-        elif hasattr(self.wq, "forward_full_rope") and freqs_cis.shape[0] >= T:
+            return tuple(t.view(B, T, self.n_head, self.head_dim) for t in fused) + (in_cache,)
+        q = k = None
+        if hasattr(self.wq, "forward_full_rope") and freqs_cis.shape[0] >= T:
             # the rotary embedding rides on the q and k projections' stores
             q = self.wq.forward_full_rope(x, freqs_cis, self.head_dim)
             k = self.wk.forward_full_rope(x, freqs_cis, self.head_dim) if q is not None else None
-        if fused is not None:
-            pass
-        elif q is not None and k is not None:
+        if q is not None and k is not None:
             q = q.view(B, T, self.n_head, self.head_dim)
             k = k.view(B, T, self.n_head, self.head_dim)
             v = _full(self.wv, x).view(B, T, self.n_head, self.head_dim)
@@ -310,8 +339,48 @@ class CausalSelfAttention(nn.Module):
             k = _full(self.wk, x).view(B, T, self.n_head, self.head_dim)
             v = _full(self.wv, x).view(B, T, self.n_head, self.head_dim)
             q, k = apply_rotary_emb(q, k, freqs_cis)
-        if kv_cache is not None:
+        return q, k, v, False
+
+    def _windowed(self, q, k, v, drop, dense_cache):
+        """Attention of the last T of the keys' positions over a window and
+        the first tokens: on the HIP kernels, or masked SDPA for dropout and
+        for head sizes that they do not take."""
+        T, total = q.size(2), k.size(2)
+        if drop == 0 and kernels.window_attention_supported(q):
+            if T == 1 and dense_cache and not (torch.is_grad_enabled() and q.requires_grad):
+                # one row over the cache, read in place as one page per
+                # sequence: split over its length
+                table = torch.arange(q.size(0), device=q.device, dtype=torch.int32)[:, None]
+                n = torch.full((q.size(0),), total, device=q.device, dtype=torch.int32)
+                return kernels.paged_decode_attention(q, k, v, table, n, self.window, self.sinks)
+            return window_attention(q, k, v, self.window, self.sinks)
+        mask = window_mask(T, total, self.window, self.sinks, q.device)
+        return F.scaled_dot_product_attention(q, k, v, attn_mask=mask, dropout_p=drop)
+
+    def forward(self, x, freqs_cis, kv_cache: Optional[KVCache] = None, layer_idx: int = 0):
+        B, T, C = x.size()
+        dt = act_dtype(x)
+        x = x.to(dt)
+        paged = isinstance(kv_cache, PagedKVCache)
+        if paged and T == 1:
+            # every sequence's token has a position of its own, so the batch
+            # is the axis along which freqs_cis runs
+            q, k, v, _ = self._qkv(x.transpose(0, 1), freqs_cis, kv_cache, layer_idx)
+            q, k, v = (t.transpose(0, 1) for t in (q, k, v))
+            in_cache = False
+        else:
+            q, k, v, in_cache = self._qkv(x, freqs_cis, kv_cache, layer_idx)
+        if paged:
+            kv_cache.write(layer_idx, k, v)
+            past = 0 if T == 1 else kv_cache.cached_len
+            if past > 0:
+                pk, pv = kv_cache.rows(layer_idx, past)
+                k, v = torch.cat([pk.to(k.dtype), k], dim=1), torch.cat([pv.to(v.dtype), v], dim=1)
+        elif kv_cache is not None:
+            past = kv_cache.cached_len
             k, v = kv_cache.filled(layer_idx, B) if in_cache else kv_cache.update(layer_idx, k, v)
+        else:
+            past = 0
         q = q.transpose(1, 2)
         k = k.transpose(1, 2).to(q.dtype)
         v = v.transpose(1, 2).to(q.dtype)
@@ -319,14 +388,18 @@ class CausalSelfAttention(nn.Module):
         tracked = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
         drop = self.dropout if self.training else 0
         with _attention_backends(tracked and q.is_cuda and q.dtype != torch.float32):
-            if kv_cache is not None and kv_cache.cached_len > 0 and T == 1:
+            if paged and T == 1:
+                y = kv_cache.attend(layer_idx, q, self.window, self.sinks)
+            elif 0 < self.window < k.size(2):
+                y = self._windowed(q, k, v, drop, kv_cache is not None and not paged)
+            elif past > 0 and T == 1:
                 # one new position attends to every cached one: no mask needed;
                 # the split-K decode kernel reads the cache in place
                 if not tracked and drop == 0 and kernels.decode_attention_supported(q, k, v):
                     y = kernels.decode_attention(q, k, v)
                 else:
                     y = F.scaled_dot_product_attention(q, k, v, dropout_p=drop)
-            elif kv_cache is not None and kv_cache.cached_len > 0:
+            elif past > 0:
                 total = k.size(2)
                 mask = torch.ones(T, total, dtype=torch.bool, device=q.device).tril(diagonal=total - T)
                 y = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, dropout_p=drop)
@@ -453,7 +526,7 @@ class Walsh(nn.Module):
                 return_hidden: bool = False):
         B, T = idx.shape
         h = self.tok_embeddings(idx)
-        freqs_cis = self.freqs_cis[start_pos:start_pos + T]
+        freqs_cis = cache_freqs(self.freqs_cis, T, start_pos, kv_cache)
         for layer_idx, layer in enumerate(self.layers):
             if self.training and torch.is_grad_enabled():
                 # every layer checkpointed in training (chassis.py:570-572)
@@ -465,7 +538,7 @@ class Walsh(nn.Module):
             logits = cached_linear(self.output, h, self._output_cast)
             loss = F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1))
         else:
-            logits = cached_linear(self.output, h[:, [-1], :], self._output_cast)
+            logits = cached_linear(self.output, last_rows(h, kv_cache), self._output_cast)
             loss = None
         if return_hidden:
             return logits, loss, h

@@ -877,6 +877,11 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
 ATTENTION_HEAD_DIMS = (16, 32, 64, 128)
 
 
+def window_attention_supported(q: torch.Tensor) -> bool:
+    """Whether window_attention takes a query of this device, type and head size."""
+    return q.is_cuda and q.dtype in (torch.float32, torch.bfloat16) and q.shape[-1] in ATTENTION_HEAD_DIMS
+
+
 def _attn_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [B, heads, T, D] as the attention kernels read it: unit inner
     stride, the others multiples of 8, rows that do not overlap, 16-byte

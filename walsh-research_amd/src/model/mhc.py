@@ -457,12 +457,13 @@ class mHCWalsh(nn.Module):
             torch.nn.init.normal_(module.weight, mean=0.0, std=0.02)
 
     def forward(self, idx, targets=None, kv_cache=None, start_pos=0, return_hidden=False):
+        from .chassis import cache_freqs, last_rows
         B, T = idx.shape
         h = self.tok_embeddings(idx)
         h = cached_linear(self.stream_proj, h, self._casts["proj"])
         dt = act_dtype(h)
         h = h.to(dt).view(B, T, self.n_streams, self.config.n_embd)
-        freqs_cis = self.freqs_cis[start_pos:start_pos + T]
+        freqs_cis = cache_freqs(self.freqs_cis, T, start_pos, kv_cache)
         checkpointed = self.gradient_checkpointing and self.training and torch.is_grad_enabled()
         for layer_idx, layer in enumerate(self.layers):
             if checkpointed:
@@ -480,7 +481,7 @@ class mHCWalsh(nn.Module):
             logits = cached_linear(self.output, h_out, self._casts["output"])
             loss = F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1), ignore_index=-1)
         else:
-            logits = cached_linear(self.output, h_out[:, -1:, :], self._casts["output"])
+            logits = cached_linear(self.output, last_rows(h_out, kv_cache), self._casts["output"])
             loss = None
         if return_hidden:
             return logits, loss, h_out
@@ -528,15 +529,48 @@ class mHCWalsh(nn.Module):
         return {k: sum(s[k] for s in stats) / len(stats) for k in ('scale_mean', 'scale_std', 'shift_mean')}
 
     @torch.no_grad()
-    def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None):
-        """Sampling loop without a cache, as in the reference (mhc.py:754-772)."""
-        for _ in range(max_new_tokens):
-            idx_cond = idx if idx.size(1) <= self.config.block_size else idx[:, -self.config.block_size:]
-            logits, _ = self(idx_cond)
-            logits = logits[:, -1, :].float() / temperature
-            if top_k is not None and top_k > 0:
-                v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
-                logits[logits < v[:, [-1]]] = -float('Inf')
-            probs = F.softmax(logits, dim=-1)
-            idx = torch.cat((idx, torch.multinomial(probs, num_samples=1)), dim=1)
+    def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None, top_p=None, min_p=None, kv_cache=None,
+                 lengths=None):
+        """``idx`` [B, T] with ``max_new_tokens`` sampled tokens behind it.
+
+        Without the last four arguments the reference's loop (mhc.py:754-772):
+        no cache, torch.multinomial.  ``top_p`` or ``min_p`` draws each token
+        with kernels.sample (its filters) from torch's uniform numbers.
+        ``kv_cache``, an empty PagedKVCache for B sequences of at least T +
+        max_new_tokens positions, keeps the keys and values; the prompts may
+        then be padded on the right to T, ``lengths`` (B whole numbers) of
+        them each."""
+        if top_p is None and min_p is None and kv_cache is None:
+            if lengths is not None:
+                raise ValueError("generate: prompts of unequal lengths need a kv_cache")
+            for _ in range(max_new_tokens):
+                idx_cond = idx if idx.size(1) <= self.config.block_size else idx[:, -self.config.block_size:]
+                logits, _ = self(idx_cond)
+                logits = logits[:, -1, :].float() / temperature
+                if top_k is not None and top_k > 0:
+                    v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
+                    logits[logits < v[:, [-1]]] = -float('Inf')
+                probs = F.softmax(logits, dim=-1)
+                idx = torch.cat((idx, torch.multinomial(probs, num_samples=1)), dim=1)
+            return idx
+        if kv_cache is None and lengths is not None:
+            raise ValueError("generate: prompts of unequal lengths need a kv_cache")
+        if lengths is not None and (len(lengths) != idx.size(0) or min(lengths) < 1 or max(lengths) > idx.size(1)):
+            raise ValueError(f"generate: lengths {list(lengths)} of prompts {tuple(idx.shape)}")
+        if kv_cache is not None and any(kv_cache.seq_lens):
+            raise ValueError("generate: the kv_cache is not empty")
+        for step in range(max_new_tokens):
+            if kv_cache is None:
+                logits, _ = self(idx[:, -self.config.block_size:])
+            elif step == 0:
+                kv_cache.reserve(idx.size(1) if lengths is None else lengths)
+                logits, _ = self(idx, kv_cache=kv_cache)
+                kv_cache.increment()
+            else:
+                kv_cache.reserve(1)
+                logits, _ = self(idx[:, -1:], kv_cache=kv_cache)
+                kv_cache.increment()
+            token = kernels.sample(logits[:, -1, :], torch.rand(idx.size(0), device=idx.device), temperature, top_k or 0,
+                                   1.0 if top_p is None else top_p, 0.0 if min_p is None else min_p)
+            idx = torch.cat((idx, token[:, None]), dim=1)
         return idx
