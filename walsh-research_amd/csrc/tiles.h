@@ -84,22 +84,25 @@ template <typename T, int D, int ROWS> struct Tile {
         return NCH == 4 ? (r >> 2) & 3 : (r >> 3) & 1;
     }
     // Rows r0 .. r0 + ROWS - 1 of a matrix with row stride st into LDS, by
-    // WAVES wavefronts, straight from memory (no registers); rows before lo
-    // and at or past n are zeros and are not read.
+    // WAVES wavefronts (wave: a scalar), straight from memory (no registers);
+    // rows before lo and at or past n are zeros and are not read.
     template <int WAVES>
     static __device__ __forceinline__ void fetch(unsigned char *lds, const T *base, int64_t st, int r0, int lo, int n, int wave,
                                                  int lane) {
         const int rows = min(n - r0, ROWS);
         const uint32_t span = rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * st + D) * (int)sizeof(T)) : 0u;
         const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (int64_t)r0 * st, span);
-        constexpr int N = BYTES / 1024;   // wavefront loads
+        constexpr int N = BYTES / 1024, STEP = 64 * WAVES / NCH;   // wavefront loads; rows that one of each cover
         static_assert(BYTES % 1024 == 0, "whole loads");
+        const uint32_t rowb = (uint32_t)(st * (int)sizeof(T)), pos0 = (uint32_t)(wave * 64 + lane);
+        const int row0 = (int)(pos0 / NCH);
+        uint32_t c = (pos0 % NCH) ^ swz(row0);
 #pragma unroll
         for (int i = 0; i < (N + WAVES - 1) / WAVES; ++i) {
-            const int k = i * WAVES + __builtin_amdgcn_readfirstlane(wave);
+            const int k = i * WAVES + wave, row = row0 + i * STEP;
             if (N % WAVES && k >= N) break;
-            const int pos = k * 64 + lane, row = pos / NCH, c = (pos % NCH) ^ swz(row);
-            const uint32_t off = row < rows && row >= lo - r0 ? (uint32_t)row * (uint32_t)(st * (int)sizeof(T)) + 16 * c : kOOB;
+            if (STEP % 16) c = (pos0 % NCH) ^ swz(row);            // (else the swizzle, of period 16, is the same)
+            const uint32_t off = row < rows && row >= lo - r0 ? (uint32_t)row * rowb + 16 * c : kOOB;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(lds + k * 1024), 16,
                                                      off, 0, 0, 0);
         }

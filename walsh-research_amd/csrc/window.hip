@@ -49,15 +49,19 @@ struct WinArgs {
     const void *go;
     void *dq, *dk, *dv;   // dense [B, H, Tq, D], [B, G, Tk, D]
     WinTensor sgo;
-    float *delta;         // [B, H, Tq]
+    float *stat;          // [2][B, H, Tq]: lse * log2(e) (inf for rows that see nothing), Delta
     float scale;
     float *part;          // partial dK, dV of key blocks whose queries are split
     int nb, nsb, nn, ns;  // key blocks; those with first tokens; splits of the others' and of their queries
 };
 
+// A value that is the same in every lane, as a scalar: quotients and loads
+// leave such values in vector registers, and their users with them.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Key positions of a sequence: all of Tk, or its length within it.
 __device__ __forceinline__ int win_len(const WinArgs &a, int b) {
-    return a.lengths ? max(0, min(a.lengths[b], a.Tk)) : a.Tk;
+    return a.lengths ? uniform(max(0, min(a.lengths[b], a.Tk))) : a.Tk;
 }
 // The chunks of ROWS keys that positions p0 .. p1 see: n chunks, the first ns
 // of them the first tokens' (chunks 0 ..), the rest from chunk lo.
@@ -77,8 +81,10 @@ __device__ __forceinline__ int win_kind(const WinArgs &a, int k0, int n, int pa,
     if (k0 > pb || (a.W > 0 && k0 + n <= pa - a.W + 1 && k0 >= a.S)) return 0;
     return k0 + n - 1 <= pa && (a.W <= 0 || k0 > pb - a.W || k0 + n <= a.S) ? 2 : 1;
 }
+// (no branches: a tile of mixed keys asks for every element)
 __device__ __forceinline__ bool win_sees(const WinArgs &a, int p, int j) {
-    return j <= p && (a.W <= 0 || j > p - a.W || j < a.S);
+    const uint32_t near = a.W > 0 ? (uint32_t)a.W : 0x7fffffffu;
+    return ((uint32_t)(p - j) < near) | ((j < a.S) & (j <= p));
 }
 
 // Work item of this workgroup: workgroups go to the 8 XCDs in turn, so XCD x
@@ -106,8 +112,9 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     const int nqt = (a.Tq + kWinQ - 1) / kWinQ;
     const int id = xcd_item(nqt * a.H * a.B);
     if (id < 0) return;
-    const int qt = nqt - 1 - id % nqt, h = id / nqt % a.H, b = id / nqt / a.H, g = h / (a.H / a.G);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    const int bh = uniform(id / nqt), qt = nqt - 1 - (id - bh * nqt);
+    const int b = uniform(bh / a.H), h = bh - b * a.H, g = uniform(h / (a.H / a.G));
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
     const int len = win_len(a, b), off = a.Tk - a.Tq;
     const int qi = qt * kWinQ + 32 * wave + n, p = qi + off;   // this lane's query and its position
     // positions of the workgroup and of the wavefront that have an output
@@ -154,7 +161,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3))) s[j][r] = -INFINITY;
+                    s[j][r] = win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3)) ? s[j][r] : -INFINITY;
         }
         float mx = s[0][0];
 #pragma unroll
@@ -212,8 +219,8 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 }
 
 // ---------------------------------------------------------------- backward: queries
-// dQ of 32 queries per wavefront, over the keys they see; also Delta, which
-// the keys' kernel reads.
+// dQ of 32 queries per wavefront, over the keys they see; also the rows' lse
+// and Delta as the keys' kernel reads them.
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
@@ -222,8 +229,9 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     const int nqt = (a.Tq + kWinQ - 1) / kWinQ;
     const int id = xcd_item(nqt * a.H * a.B);
     if (id < 0) return;
-    const int qt = nqt - 1 - id % nqt, h = id / nqt % a.H, b = id / nqt / a.H, g = h / (a.H / a.G);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    const int bh = uniform(id / nqt), qt = nqt - 1 - (id - bh * nqt);
+    const int b = uniform(bh / a.H), h = bh - b * a.H, g = uniform(h / (a.H / a.G));
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
     const int len = win_len(a, b), off = a.Tk - a.Tq;
     const int qi = qt * kWinQ + 32 * wave + n, p = qi + off, qc = min(qi, a.Tq - 1);
     const int wlo = max(0, qt * kWinQ + off), whi = min(min(qt * kWinQ + kWinQ, a.Tq) - 1 + off, len - 1);
@@ -245,8 +253,11 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
         delta += other_half(delta);
     }
     const int64_t row = ((int64_t)b * a.H + h) * a.Tq + qc;
-    if (hi == 0 && qi < a.Tq) a.delta[row] = live ? delta : 0.f;
     const float lse2 = live ? a.lse[row] * kLog2e : INFINITY;   // a row that sees nothing has no weights
+    if (hi == 0 && qi < a.Tq) {
+        a.stat[row] = lse2;
+        a.stat[(int64_t)a.B * a.H * a.Tq + row] = live ? delta : 0.f;
+    }
     f32x16 acc[ND];
 #pragma unroll
     for (int c = 0; c < ND; ++c) acc[c] = f32x16{};
@@ -277,7 +288,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             if (kind == 1) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3))) s[r] = -INFINITY;
+                    s[r] = win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3)) ? s[r] : -INFINITY;
             }
             float ds[16];
 #pragma unroll
@@ -312,6 +323,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // sees, into ns, the others into nn.  A split block's parts go to `part` and
 // are summed in a fixed order; an unsplit block is stored at once.
 template <typename T, int D> struct WinBwdCfg {
+    static constexpr int KL = D == 128 && sizeof(T) == 2 ? 2 : 0;     // K operands kept in LDS
     static constexpr int QC = D == 128 && sizeof(T) == 4 ? 32 : 64;   // rows of a tile
 };
 // Tiles of QC queries (indexes from query 0) that see keys k0 .. k0 + 127.
@@ -325,28 +337,34 @@ template <int QC> __device__ __forceinline__ void win_q_tiles(const WinArgs &a, 
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWinWaves, D == 128 || (sizeof(T) == 4 && D == 64) ? 1 : 2) void window_bwd_kv_kernel(WinArgs a) {
+__global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) void window_bwd_kv_kernel(WinArgs a) {
     constexpr int QC = WinBwdCfg<T, D>::QC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = QC / 32;
     typedef Tile<T, D, QC> L;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ __align__(16) float stat[2][2][QC];   // [buffer][lse2, Delta]
+    __shared__ __align__(16) float stat[2][2][64];   // [buffer][lse * log2(e), Delta]
+    // the last K operands of each lane wait in LDS where the registers of two
+    // wavefronts per SIMD do not hold them all beside the accumulators
+    constexpr int KL = WinBwdCfg<T, D>::KL, KR = NK - KL;
+    __shared__ Frag<T> klast[KL ? KL : 1][KL ? 64 * kWinWaves : 1];
     const int per = a.nsb * a.ns + (a.nb - a.nsb) * a.nn;            // items per (sequence, kv head)
     const int id = xcd_item(per * a.G * a.B);
     if (id < 0) return;
-    const int it = id % per, g = id / per % a.G, b = id / per / a.G;
+    const int bg = uniform(id / per), it = id - bg * per, b = uniform(bg / a.G), g = bg - b * a.G;
     const bool sink = it < a.nsb * a.ns;
-    const int kblk = sink ? it / a.ns : a.nsb + (it - a.nsb * a.ns) / a.nn;
-    const int nsplit = sink ? a.ns : a.nn, split = sink ? it % a.ns : (it - a.nsb * a.ns) % a.nn;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
-    const int len = win_len(a, b), off = a.Tk - a.Tq, R = a.H / a.G;
+    const int nsplit = sink ? a.ns : a.nn, rel = sink ? it : it - a.nsb * a.ns, blk = uniform(rel / nsplit);
+    const int kblk = sink ? blk : a.nsb + blk, split = rel - blk * nsplit;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    const int len = win_len(a, b), off = a.Tk - a.Tq, R = uniform(a.H / a.G);
     const int k0 = kblk * kWinQ, kw = k0 + 32 * wave, key = kw + n;
 
-    Frag<T> kf[NK], vf[NK];
+    Frag<T> kf[KR], vf[NK];
     {
         const int64_t at = b * a.skv.sb + g * a.skv.sh + (int64_t)min(key, a.Tk - 1) * a.skv.st;
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
-            kf[kk] = load_frag((const T *)a.k + at + 16 * kk + 8 * hi);
+            const Frag<T> f = load_frag((const T *)a.k + at + 16 * kk + 8 * hi);
+            if (kk < KR) kf[kk] = f;
+            else klast[kk - KR][threadIdx.x] = f;      // read by this lane only
             vf[kk] = load_frag((const T *)a.v + at + 16 * kk + 8 * hi);
         }
     }
@@ -356,81 +374,81 @@ __global__ __launch_bounds__(64 * kWinWaves, D == 128 || (sizeof(T) == 4 && D ==
     int t0, nt;
     win_q_tiles<QC>(a, k0, len, &t0, &nt);
     // this split's share of the R * nt (head, tile) pairs
-    const int total = R * nt, i0 = (int)((int64_t)total * split / nsplit), i1 = (int)((int64_t)total * (split + 1) / nsplit);
+    const int total = R * nt, i0 = uniform((int)((int64_t)total * split / nsplit));
+    const int i1 = uniform((int)((int64_t)total * (split + 1) / nsplit));
     const int nq = max(0, min(a.Tq, len - off));                     // queries before the sequence's end
-    auto fetch = [&](int i) {
-        const int h = g * R + i / nt, q0 = (t0 + i % nt) * QC;
+    auto fetch = [&](int i, int hr, int tile) {                      // pair i: head hr of the group, tile t0 + tile
+        const int h = g * R + hr, q0 = (t0 + tile) * QC, lane = fresh(threadIdx.x & 63);
         unsigned char *dst = smem + (i & 1) * 2 * L::BYTES;
         L::template fetch<kWinWaves>(dst, (const T *)a.q + b * a.sq.sb + h * a.sq.sh, a.sq.st, q0, -off, nq, wave, lane);
         L::template fetch<kWinWaves>(dst + L::BYTES, (const T *)a.go + b * a.sgo.sb + h * a.sgo.sh, a.sgo.st, q0, -off,
                                      nq, wave, lane);
-    };
-    // lse and Delta of a tile travel through a register to LDS
-    const int sr = threadIdx.x % QC, sw = threadIdx.x / QC;
-    auto fetch_stat = [&](int i) {
-        const int h = g * R + i / nt, qi = (t0 + i % nt) * QC + sr;
-        float v = sw ? 0.f : INFINITY;
-        if (sw < 2 && qi < nq && qi + off >= 0) {
-            const int64_t row = ((int64_t)b * a.H + h) * a.Tq + qi;
-            v = sw ? a.delta[row] : a.lse[row] * kLog2e;
+        // one wavefront the tile's lse, another its Delta; rows past the last
+        // one are zeros, as their q and do are: weights of 1 times nothing
+        const int w = __builtin_amdgcn_readfirstlane(wave);
+        if (w < 2) {
+            const float *sp = a.stat + ((int64_t)w * a.B * a.H + (int64_t)b * a.H + h) * a.Tq + q0;
+            const __amdgpu_buffer_rsrc_t rs = make_rsrc(sp, (uint32_t)(4 * min(QC, nq - q0)));
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)&stat[i & 1][w][0], 4,
+                                                     4 * lane, 0, 0, 0);
         }
-        return v;
     };
-    auto put_stat = [&](int i, float v) {
-        if (sw < 2) stat[i & 1][sw][sr] = v;
-    };
-    if (i0 < i1) {
-        fetch(i0);
-        put_stat(i0, fetch_stat(i0));
-    }
+    int hr = nt ? uniform(i0 / nt) : 0, tile = i0 - hr * nt;
+    if (i0 < i1) fetch(i0, hr, tile);
     for (int i = i0; i < i1; ++i) {
         tiles_ready();
-        float nextv = 0.f;
-        if (i + 1 < i1) {
-            nextv = fetch_stat(i + 1);
-            fetch(i + 1);
-        }
+        const int pq = (t0 + tile) * QC + off;                       // position of the tile's first query
+        if (++tile == nt) tile = 0, ++hr;
+        if (i + 1 < i1) fetch(i + 1, hr, tile);
         const unsigned char *ql = smem + (i & 1) * 2 * L::BYTES, *gl = ql + L::BYTES;
-        const int ln = fresh(lane), n = ln & 31, hi = ln >> 5;
-        const int pq = (t0 + i % nt) * QC + off;   // position of the tile's first query
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < NJ; ++j) {
+            const int ln = fresh(lane), n = ln & 31, hi = ln >> 5;
             const int pa = pq + 32 * j, pb = pa + 31;
             const int kind = kw < len ? win_kind(a, kw, 32, pa, pb) : 0;
             if (kind == 0) continue;
-            f32x16 s = f32x16{}, dp = f32x16{};
+            // scores, weights, dV; then do V^T, dS, dK: one after the other, so
+            // that 32 results at a time are live beside the accumulators
+            f32x16 s = f32x16{};
 #pragma unroll
-            for (int kk = 0; kk < NK; ++kk) {
-                mma(s, L::row(ql, 32 * j + n, kk, hi), kf[kk]);
-                mma(dp, L::row(gl, 32 * j + n, kk, hi), vf[kk]);
+            for (int kk = 0; kk < NK; ++kk)
+                mma(s, L::row(ql, 32 * j + n, kk, hi), kk < KR ? kf[kk < KR ? kk : 0] : klast[kk < KR ? 0 : kk - KR][threadIdx.x]);
+            if (kind == 1) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[r] = win_sees(a, pa + 8 * (r >> 2) + 4 * hi + (r & 3), kw + n) ? s[r] : -INFINITY;
             }
-            float w[16], ds[16];
+            float w[16];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 const f32x4 ls = *(const f32x4 *)&stat[i & 1][0][32 * j + 8 * t + 4 * hi];
-                const f32x4 de = *(const f32x4 *)&stat[i & 1][1][32 * j + 8 * t + 4 * hi];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * t + e;
-                    float x = s[r];
-                    if (kind == 1 && !win_sees(a, pa + 8 * t + 4 * hi + e, key)) x = -INFINITY;
-                    w[r] = __builtin_amdgcn_exp2f(fmaf(x, a.sl2, -ls[e]));
-                    ds[r] = w[r] * (dp[r] - de[e]);
-                }
+                for (int e = 0; e < 4; ++e) w[4 * t + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * t + e], a.sl2, -ls[e]));
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                Frag<T> pf, df;
-                pack(pf, w + 8 * t);
-                pack(df, ds + 8 * t);
+                Frag<T> f;
+                pack(f, w + 8 * t);
 #pragma unroll
-                for (int c = 0; c < ND; ++c) {
-                    mma(av[c], L::col(gl, 32 * j + 16 * t, c, ln), pf);
-                    mma(ak[c], L::col(ql, 32 * j + 16 * t, c, ln), df);
-                }
+                for (int c = 0; c < ND; ++c) mma(av[c], L::col(gl, 32 * j + 16 * t, c, ln), f);
+            }
+            f32x16 dp = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) mma(dp, L::row(gl, 32 * j + n, kk, hi), vf[kk]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const f32x4 de = *(const f32x4 *)&stat[i & 1][1][32 * j + 8 * t + 4 * hi];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * t + e] *= dp[4 * t + e] - de[e];
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag<T> f;
+                pack(f, w + 8 * t);
+#pragma unroll
+                for (int c = 0; c < ND; ++c) mma(ak[c], L::col(ql, 32 * j + 16 * t, c, ln), f);
             }
         }
-        if (i + 1 < i1) put_stat(i + 1, nextv);
     }
     // keys past the length (whatever they hold) have no gradient
     if (key >= len) {
@@ -579,9 +597,9 @@ WALSH_EXPORT int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t
 
 static int win_bwd_qc(int64_t D, int dtype) { return D == 128 && dtype == WALSH_F32 ? 32 : 64; }
 
+static int64_t win_stat_bytes(const WinArgs &a) { return ceil_div((int64_t)a.B * a.H * a.Tq * 8, 16) * 16; }
 static int64_t win_bwd_bytes(const WinArgs &a, int64_t D) {
-    const int64_t delta = ceil_div((int64_t)a.B * a.H * a.Tq * 4, 16) * 16;
-    return delta + (int64_t)a.B * a.G * win_part_slots(a) * 2 * kWinQ * D * 4;
+    return win_stat_bytes(a) + (int64_t)a.B * a.G * win_part_slots(a) * 2 * kWinQ * D * 4;
 }
 
 WALSH_EXPORT int64_t walsh_window_attention_bwd_workspace_bytes(int64_t B, int64_t H, int64_t G, int64_t Tq, int64_t Tk,
@@ -629,8 +647,8 @@ WALSH_EXPORT int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t
     if (work_bytes < win_bwd_bytes(a, D))
         return set_error(WALSH_EINVAL, "%s: workspace of %lld bytes, needs %lld", fn, (long long)work_bytes,
                          (long long)win_bwd_bytes(a, D));
-    a.delta = (float *)work;
-    a.part = (float *)((char *)work + ceil_div((int64_t)a.B * a.H * a.Tq * 4, 16) * 16);
+    a.stat = (float *)work;
+    a.part = (float *)((char *)work + win_stat_bytes(a));
     hipStream_t s = (hipStream_t)stream;
     const int64_t nq = ceil_div(Tq, kWinQ) * H * B;
     const int64_t nk = ((int64_t)a.nsb * a.ns + (int64_t)(a.nb - a.nsb) * a.nn) * G * B;
