@@ -76,6 +76,11 @@ SHAPES = [
     (1, 2, 2, 64, 300, 128, 300, 2, [299]),
     (1, 2, 1, 400, 400, 32, 17, 130, None),
     (1, 1, 1, 700, 700, 128, 65, 1, None),
+    # enough rows that a workgroup takes 128 queries instead of 32
+    (3, 32, 8, 300, 333, 16, 70, 5, [333, 100, 1]),
+    (2, 33, 11, 520, 520, 32, 130, 0, None),
+    (3, 32, 32, 300, 300, 64, 0, 0, [17, 300, 299]),
+    (2, 48, 6, 400, 390, 128, 150, 66, None),
 ]
 
 

@@ -177,7 +177,7 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
         for (int u = 0; u < NB; ++u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
-        mx = fmaxf(mx, other_half(mx));
+        mx = half_max(mx);
         if (__any((mx - m) * a.sl2 > 8.f)) {      // as in the whole-sequence kernel: move the maximum rarely
             const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f((m - mn) * a.sl2);
             m = mn;
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
             }
         }
     }
-    l += other_half(l);
+    l = half_sum(l);
 
     // the wavefronts' parts: o = sum_w acc_w e^(m_w - m) / sum_w l_w e^(m_w - m)
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -65,8 +65,47 @@ __device__ __forceinline__ int fresh(int v) {
     return v;
 }
 
-__device__ __forceinline__ float other_half(float v) {   // the value of lane ^ 32
-    return __shfl_xor(v, 32, 64);
+// Sum and maximum of a lane's value and that of lane ^ 32, by the exchange of
+// the wavefront's halves (vector unit; no LDS round trip as a shuffle has).
+__device__ __forceinline__ float half_sum(float v) {
+    const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
+                                                                              false, false));
+    return __uint_as_float(u.x) + __uint_as_float(u.y);
+}
+__device__ __forceinline__ float half_max(float v) {
+    const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
+                                                                              false, false));
+    return fmaxf(__uint_as_float(u.x), __uint_as_float(u.y));
+}
+
+// ---------------------------------------------------------------- loads into LDS
+// 16 (4) bytes per lane from a buffer at byte offset off (past its size:
+// zeros) to 64 consecutive slots at the LDS byte address lds; both scalar but
+// off.  Written out, because the compiler makes every LDS read through the
+// transposing load wait for all such loads of its own that are on their way,
+// next tile's included.  Nothing comes back in registers; the caller waits
+// (tiles_ready) before it reads.  (M0, the LDS address of such a load, has no
+// other user in kernels that call this.)
+__device__ __forceinline__ u32x4 lds_load_rsrc(const void *p, uint32_t bytes) {
+    const uint64_t a = (uint64_t)p;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu)),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+template <int BYTES> __device__ __forceinline__ void lds_load(u32x4 rsrc, uint32_t off, uint32_t lds) {
+    static_assert(BYTES == 16 || BYTES == 4, "sizes in use");
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    if (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                     ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+}
+// The LDS byte address of a shared variable, as a scalar.
+__device__ __forceinline__ uint32_t lds_addr(const void *p) {
+    return (uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p);
 }
 
 // ---------------------------------------------------------------- tiles in LDS
@@ -91,7 +130,8 @@ template <typename T, int D, int ROWS> struct Tile {
                                                  int lane) {
         const int rows = min(n - r0, ROWS);
         const uint32_t span = rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * st + D) * (int)sizeof(T)) : 0u;
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (int64_t)r0 * st, span);
+        const u32x4 rs = lds_load_rsrc(base + (int64_t)r0 * st, span);
+        const uint32_t dst = lds_addr(lds);
         constexpr int N = BYTES / 1024, STEP = 64 * WAVES / NCH;   // wavefront loads; rows that one of each cover
         static_assert(BYTES % 1024 == 0, "whole loads");
         const uint32_t rowb = (uint32_t)(st * (int)sizeof(T)), pos0 = (uint32_t)(wave * 64 + lane);
@@ -103,8 +143,7 @@ template <typename T, int D, int ROWS> struct Tile {
             if (N % WAVES && k >= N) break;
             if (STEP % 16) c = (pos0 % NCH) ^ swz(row);            // (else the swizzle, of period 16, is the same)
             const uint32_t off = row < rows && row >= lo - r0 ? (uint32_t)row * rowb + 16 * c : kOOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(lds + k * 1024), 16,
-                                                     off, 0, 0, 0);
+            lds_load<16>(rs, off, dst + k * 1024);
         }
     }
     // Eight elements of row r from column 16 kk + 8 hi.
@@ -146,12 +185,32 @@ template <typename T, int D, int ROWS> struct Tile {
     }
 };
 
-// All of this wavefront's loads into LDS have landed and its LDS reads are
-// done; then all wavefronts'.
+// All loads of this wavefront have landed and its LDS reads are done: vmcnt(0)
+// lgkmcnt(0), as the builtin that the compiler's own count of loads follows.
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    asm volatile("" ::: "memory");
+}
+// The same of all wavefronts: tiles requested before are there.
 __device__ __forceinline__ void tiles_ready() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    wait_loads();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+}
+
+// Order of the LDS reads and products before this call, in its basic block: N
+// products of READS reads each, the reads of DEPTH products ahead.  Left to
+// itself the compiler, short of registers, puts each read right before its
+// product, which then waits out the LDS latency, four times its own length.
+template <int READS, int N, int DEPTH> __device__ __forceinline__ void pace() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * DEPTH, 0);
+#pragma unroll
+    for (int i = 0; i < N - DEPTH; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, DEPTH, 0);
 }
 
 // Calls go(T(), integral constant D) for the dtype and head_dim at hand.

@@ -147,50 +147,43 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
         if (i + 1 < ch.n) fetch(i + 1);
         const unsigned char *kl = smem + (i & 1) * 2 * L::BYTES, *vl = kl + L::BYTES;
         const int k0 = ch.at(i) * KC;
-        const int kind = pa <= pb ? win_kind(a, k0, KC, pa, pb) : 0;
-        if (kind == 0) continue;
-        f32x16 s[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            s[j] = f32x16{};
+            const int kind = pa <= pb ? win_kind(a, k0 + 32 * j, 32, pa, pb) : 0;
+            if (kind == 0) continue;
+            f32x16 s = f32x16{};
 #pragma unroll
-            for (int kk = 0; kk < NK; ++kk) mma(s[j], L::row(kl, 32 * j + n, kk, hi), qf[kk]);
-        }
-        if (kind == 1) {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
+            for (int kk = 0; kk < NK; ++kk) mma(s, L::row(kl, 32 * j + n, kk, hi), qf[kk]);
+            if constexpr (sizeof(T) == 2 && NK > 4) pace<1, NK, 4>();
+            if (kind == 1) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[j][r] = win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3)) ? s[j][r] : -INFINITY;
-        }
-        float mx = s[0][0];
+                    s[r] = win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3)) ? s[r] : -INFINITY;
+            }
+            float mx = s[0];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+            mx = half_max(mx);
+            // the maximum moves only when some row of the wavefront would pass
+            // 2^8: weights and sums stay within float32 and the rescaling of the
+            // accumulators is rare
+            if (__any(live && (mx - m) * a.sl2 > 8.f)) {
+                const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f((m - mn) * a.sl2);
+                m = mn;
+                l *= al;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
-        mx = fmaxf(mx, other_half(mx));
-        // the maximum moves only when some row of the wavefront would pass
-        // 2^8: weights and sums stay within float32 and the rescaling of the
-        // accumulators is rare
-        if (__any(live && (mx - m) * a.sl2 > 8.f)) {
-            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f((m - mn) * a.sl2);
-            m = mn;
-            l *= al;
+                for (int c = 0; c < ND; ++c) acc[c] *= al;
+            }
+            const float mo = -m * a.sl2;
+            float w[16], l0 = 0.f, l1 = 0.f;
 #pragma unroll
-            for (int c = 0; c < ND; ++c) acc[c] *= al;
-        }
-        const float mo = -m * a.sl2;
-        float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            float w[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], a.sl2, mo));
+            for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, mo));
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
                 l0 += w[r];
                 l1 += w[r + 1];
             }
+            l += l0 + l1;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 Frag<T> pf;
@@ -199,9 +192,8 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
                 for (int c = 0; c < ND; ++c) mma(acc[c], L::col(vl, 32 * j + 16 * t, c, lane), pf);
             }
         }
-        l += l0 + l1;
     }
-    l += other_half(l);
+    l = half_sum(l);
     if (qi >= a.Tq) return;
     const float inv = live && l > 0.f ? 1.f / l : 0.f;
     T *op = (T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)qi * a.so.st;
@@ -216,6 +208,128 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
         }
     if (a.lse && hi == 0)
         a.lse[((int64_t)b * a.H + h) * a.Tq + qi] = live ? (m * a.sl2 + log2f(l)) * (1.f / kLog2e) : -INFINITY;
+}
+
+// The same for grids that would leave most of the chip idle (a short part of a
+// prompt, few heads): 32 queries per workgroup, whose four wavefronts take
+// every fourth block of 32 keys, each with its own maximum, sum and
+// accumulators, joined at the end.  Nothing is shared on the way: a wavefront
+// reads its K rows straight into operands and V into LDS of its own, the next
+// block's while it works on one.  777 queries of 8 heads of 64 in float32 on
+// 1,301 keys, window 256: 41 us by four times 32 queries, 15 us so.
+template <typename T, int D> struct WinSplitCfg {
+    static constexpr int VB = Tile<T, D, 32>::BYTES;
+    static constexpr int WAVE = 2 * VB > 32 * D * 4 ? 2 * VB : 32 * D * 4;   // two V tiles; at the end 32 rows of D
+};
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_fwd_split_kernel(WinArgs a) {
+    constexpr int NK = D / 16, ND = (D + 31) / 32;
+    typedef Tile<T, D, 32> L;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ float stat[kWinWaves][2][32];
+    const int nqt = (a.Tq + 31) / 32;
+    const int id = xcd_item(nqt * a.H * a.B);
+    if (id < 0) return;
+    const int bh = uniform(id / nqt), qt = nqt - 1 - (id - bh * nqt);
+    const int b = uniform(bh / a.H), h = bh - b * a.H, g = uniform(h / (a.H / a.G));
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    const int len = win_len(a, b), off = a.Tk - a.Tq;
+    const int qi = qt * 32 + n, p = qi + off;
+    const int pa = max(0, qt * 32 + off), pb = min(min(qt * 32 + 32, a.Tq) - 1 + off, len - 1);
+
+    Frag<T> qf[NK], kf[NK];
+    {
+        const T *qp = (const T *)a.q + b * a.sq.sb + h * a.sq.sh + (int64_t)min(qi, a.Tq - 1) * a.sq.st;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) qf[kk] = load_frag(qp + 16 * kk + 8 * hi);
+    }
+    f32x16 acc[ND];
+#pragma unroll
+    for (int c = 0; c < ND; ++c) acc[c] = f32x16{};
+    float m = kNoScore, l = 0.f;
+    const T *kb = (const T *)a.k + b * a.skv.sb + g * a.skv.sh, *vb = (const T *)a.v + b * a.skv.sb + g * a.skv.sh;
+    const Chunks ch = pa <= pb ? win_chunks<32>(a, pa, pb) : Chunks{0, 0, 0};
+    unsigned char *vl = smem + wave * WinSplitCfg<T, D>::WAVE;
+    auto fetch = [&](int i, int buf) {
+        const int k0 = ch.at(i) * 32;
+        const T *kp = kb + (int64_t)min(k0 + n, len - 1) * a.skv.st + 8 * hi;   // (past the end: a row that is masked)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) kf[kk] = load_frag(kp + 16 * kk);
+        L::template fetch<1>(vl + buf * WinSplitCfg<T, D>::VB, vb, a.skv.st, k0, 0, len, 0, lane);
+    };
+    int i = wave, buf = 0;
+    if (i < ch.n) fetch(i, 0);
+    for (; i < ch.n; i += kWinWaves, buf ^= 1) {
+        const int k0 = ch.at(i) * 32;
+        wait_loads();
+        f32x16 s = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) mma(s, kf[kk], qf[kk]);
+        if (i + kWinWaves < ch.n) fetch(i + kWinWaves, buf ^ 1);
+        if (win_kind(a, k0, 32, pa, pb) != 2) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[r] = win_sees(a, p, k0 + 8 * (r >> 2) + 4 * hi + (r & 3)) ? s[r] : -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        mx = half_max(mx);
+        if (__any(p >= 0 && p < len && (mx - m) * a.sl2 > 8.f)) {
+            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f((m - mn) * a.sl2);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int c = 0; c < ND; ++c) acc[c] *= al;
+        }
+        const float mo = -m * a.sl2;
+        float w[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, mo));
+            l += w[r];
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            Frag<T> pf;
+            pack(pf, w + 8 * t);
+#pragma unroll
+            for (int c = 0; c < ND; ++c) mma(acc[c], L::col(vl + buf * WinSplitCfg<T, D>::VB, 16 * t, c, lane), pf);
+        }
+    }
+    l = half_sum(l);
+    // the wavefronts' parts: o = sum_w acc_w e^(m_w - m) / sum_w l_w e^(m_w - m)
+    wait_loads();
+    float *av = (float *)vl;   // [32 queries][D] of this wavefront (its V is used up)
+#pragma unroll
+    for (int c = 0; c < ND; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int d = 32 * c + 8 * t + 4 * hi;
+            if (D % 32 && d >= D) continue;
+            store4(av + n * D + d, f32x4{acc[c][4 * t], acc[c][4 * t + 1], acc[c][4 * t + 2], acc[c][4 * t + 3]});
+        }
+    if (hi == 0) stat[wave][0][n] = m, stat[wave][1][n] = l;
+    __syncthreads();
+    for (int e = threadIdx.x; e < 32 * (D / 4); e += 64 * kWinWaves) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4, q = qt * 32 + r, pos = q + off;
+        if (q >= a.Tq) break;
+        const bool live = pos >= 0 && pos < len;
+        float mm = stat[0][0][r], ll = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWinWaves; ++w) mm = fmaxf(mm, stat[w][0][r]);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWinWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f((stat[w][0][r] - mm) * a.sl2);
+            v += load4((const float *)(smem + w * WinSplitCfg<T, D>::WAVE) + r * D + d) * f;
+            ll += stat[w][1][r] * f;
+        }
+        store4((T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)q * a.so.st + d,
+               live ? v * (1.f / ll) : f32x4{0.f, 0.f, 0.f, 0.f});
+        if (a.lse && d == 0)
+            a.lse[((int64_t)b * a.H + h) * a.Tq + q] = live ? (mm * a.sl2 + log2f(ll)) * (1.f / kLog2e) : -INFINITY;
+    }
 }
 
 // ---------------------------------------------------------------- backward: queries
@@ -250,7 +364,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             gf[kk] = load_frag(gp + 16 * kk + 8 * hi);
             delta += dot(gf[kk], load_frag(op + 16 * kk + 8 * hi));
         }
-        delta += other_half(delta);
+        delta = half_sum(delta);
     }
     const int64_t row = ((int64_t)b * a.H + h) * a.Tq + qc;
     const float lse2 = live ? a.lse[row] * kLog2e : INFINITY;   // a row that sees nothing has no weights
@@ -285,6 +399,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
                 mma(s, L::row(kl, 32 * j + n, kk, hi), qf[kk]);
                 mma(dp, L::row(vl, 32 * j + n, kk, hi), gf[kk]);
             }
+            if constexpr (sizeof(T) == 2 && NK > 1) pace<1, 2 * NK, 4>();
             if (kind == 1) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -388,9 +503,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) 
         const int w = __builtin_amdgcn_readfirstlane(wave);
         if (w < 2) {
             const float *sp = a.stat + ((int64_t)w * a.B * a.H + (int64_t)b * a.H + h) * a.Tq + q0;
-            const __amdgpu_buffer_rsrc_t rs = make_rsrc(sp, (uint32_t)(4 * min(QC, nq - q0)));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)&stat[i & 1][w][0], 4,
-                                                     4 * lane, 0, 0, 0);
+            lds_load<4>(lds_load_rsrc(sp, (uint32_t)(4 * min(QC, nq - q0))), 4 * lane, lds_addr(&stat[i & 1][w][0]));
         }
     };
     int hr = nt ? uniform(i0 / nt) : 0, tile = i0 - hr * nt;
@@ -413,6 +526,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) 
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
                 mma(s, L::row(ql, 32 * j + n, kk, hi), kk < KR ? kf[kk < KR ? kk : 0] : klast[kk < KR ? 0 : kk - KR][threadIdx.x]);
+            if constexpr (sizeof(T) == 2 && NK > 3) pace<1, NK, 3>();
             if (kind == 1) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -435,6 +549,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) 
             f32x16 dp = f32x16{};
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk) mma(dp, L::row(gl, 32 * j + n, kk, hi), vf[kk]);
+            if constexpr (sizeof(T) == 2 && NK > 3) pace<1, NK, 3>();
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 const f32x4 de = *(const f32x4 *)&stat[i & 1][1][32 * j + 8 * t + 4 * hi];
@@ -585,12 +700,17 @@ WALSH_EXPORT int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t
     a.W = window > 0 && window < Tk ? (int)window : 0;
     a.S = sinks < 0 ? 0 : (int)(sinks < Tk ? sinks : Tk);
     a.sl2 = scale * kLog2e;
-    const int64_t n = ceil_div(Tq, kWinQ) * H * B;
+    const int64_t n = ceil_div(Tq, kWinQ) * H * B, n32 = ceil_div(Tq, 32) * H * B;
+    const bool split = n < device_info().cu_count;   // a wavefront per SIMD and less: cut the keys, too
     attn_dispatch(dtype, D, [&](auto t, auto d) {
         typedef decltype(t) T;
         constexpr int DD = decltype(d)::value;
-        launch(window_fwd_kernel<T, DD>, dim3((unsigned)(ceil_div(n, 8) * 8)), dim3(64 * kWinWaves),
-               (uint32_t)(4 * Tile<T, DD, WinCfg<T, DD>::KC>::BYTES), (hipStream_t)stream, a);
+        if (split)
+            launch(window_fwd_split_kernel<T, DD>, dim3((unsigned)(ceil_div(n32, 8) * 8)), dim3(64 * kWinWaves),
+                   (uint32_t)(kWinWaves * WinSplitCfg<T, DD>::WAVE), (hipStream_t)stream, a);
+        else
+            launch(window_fwd_kernel<T, DD>, dim3((unsigned)(ceil_div(n, 8) * 8)), dim3(64 * kWinWaves),
+                   (uint32_t)(4 * Tile<T, DD, WinCfg<T, DD>::KC>::BYTES), (hipStream_t)stream, a);
     });
     return check_hip(hipGetLastError(), fn);
 }
