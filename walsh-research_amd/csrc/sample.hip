@@ -21,11 +21,11 @@
 // arithmetic up to the weights' own rounding.
 //
 // One workgroup of 16 wavefronts per row; wavefront w walks the indexes from
-// w * ceil(V / 1024) * 64 on, 64 at a time.  The row is read for its maximum,
-// for the histogram, and once more to keep the tokens that the histogram
-// leaves in question, each wavefront's in a list in LDS; what follows works on
-// the lists, or, where one overflows (nothing filtered, or thousands kept), on
-// the row again, out of the L2.
+// w * ceil(V / 1024) * 64 on, 64 at a time, held in registers up to 65,536
+// tokens.  Three walks over the row: its maximum, the histogram, and the
+// tokens that the histogram leaves in question, each wavefront's into a list
+// in LDS; what follows works on the lists, or, where one overflows (nothing
+// filtered, or thousands kept), on the row again, out of the L2.
 #include "common.h"
 
 namespace walsh {
@@ -34,8 +34,11 @@ constexpr int kSmWaves = 16;
 constexpr int kSmThreads = 64 * kSmWaves;
 constexpr int kSmBins = 2048, kSmList = 2048;
 constexpr int kSmKept = 512;                    // tokens of a wavefront's list
-constexpr int kSmParts = 8;                     // parts of a wavefront's walk with sums of their own
+constexpr int kSmStep = 8;                      // steps of a walk between its marks
+constexpr int kSmParts = 16;                    // parts of a wavefront's walk with sums of their own
 constexpr float kSmBinsPer2 = 64.f;             // bins to a factor of two
+
+typedef unsigned long long u64;
 
 struct SampleArgs {
     const void *logits;
@@ -47,101 +50,115 @@ struct SampleArgs {
     int64_t *out;
 };
 
-// Order-preserving integer of a float (no NaN); -0 counts as 0.
+// Order-preserving integer of a float (no NaN; -0 counts as 0), and back.
 __device__ __forceinline__ uint32_t sm_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-
-struct SmShared {
-    unsigned long long mass[kSmBins];
-    uint32_t count[kSmBins];
-    uint32_t list[kSmList];                     // keys of a bin
-    uint2 kept[kSmWaves][kSmKept];              // (key, index) of the tokens in question, by wavefront
-    unsigned long long wsum[kSmWaves], part[kSmWaves][kSmParts];
-    uint32_t wcnt[kSmWaves];
-    float wmax[kSmWaves];
-    // results of a search
-    uint32_t n, kmin, kmax, before;
-    unsigned long long mbefore;
-    int bin, over;
-};
-
-__device__ __forceinline__ unsigned long long shfl64(unsigned long long v, int src) {
-    return ((unsigned long long)(uint32_t)__shfl((int)(v >> 32), src) << 32) | (uint32_t)__shfl((int)(uint32_t)v, src);
-}
-// Inclusive sums over the wavefront's lanes.
-__device__ __forceinline__ void wave_scan(uint32_t &c, unsigned long long &m, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t oc = (uint32_t)__shfl_up((int)c, o);
-        const unsigned long long om = ((unsigned long long)(uint32_t)__shfl_up((int)(m >> 32), o) << 32) |
-                                      (uint32_t)__shfl_up((int)(uint32_t)m, o);
-        if (lane >= o) c += oc, m += om;
-    }
-}
-__device__ __forceinline__ unsigned long long wave_sum64(unsigned long long v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        v += ((unsigned long long)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32) |
-             (uint32_t)__shfl_xor((int)(uint32_t)v, o);
-    return v;
-}
-
 __device__ __forceinline__ float sm_value(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+struct SmShared {
+    u64 mass[kSmBins];
+    uint32_t count[kSmBins];
+    uint32_t list[kSmList];                     // keys of a bin
+    uint2 kept[kSmWaves][kSmKept];              // (key, index) of the tokens in question, by wavefront
+    u64 wsum[kSmWaves], part[kSmWaves][kSmParts];
+    uint32_t wcnt[kSmWaves];
+    float wmax[kSmWaves];
+    // results of a search
+    uint32_t n, kmin, kmax, before;
+    u64 mbefore;
+    int bin, over, edge;
+};
+
+__device__ __forceinline__ u64 shfl64(u64 v, int src) {
+    return ((u64)(uint32_t)__shfl((int)(v >> 32), src) << 32) | (uint32_t)__shfl((int)(uint32_t)v, src);
+}
+__device__ __forceinline__ u64 xor64(u64 v, int o) {
+    return ((u64)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, o);
+}
+// Inclusive sums over the wavefront's lanes.
+__device__ __forceinline__ void wave_scan(uint32_t &c, u64 &m, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t oc = (uint32_t)__shfl_up((int)c, o);
+        const u64 om = ((u64)(uint32_t)__shfl_up((int)(m >> 32), o) << 32) | (uint32_t)__shfl_up((int)(uint32_t)m, o);
+        if (lane >= o) c += oc, m += om;
+    }
+}
+__device__ __forceinline__ u64 wave_sum64(u64 v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += xor64(v, o);
+    return v;
+}
+// What the wavefronts left in wcnt / wsum: before this one, and in all.
+__device__ __forceinline__ void waves_before(const SmShared &sh, int wave, int lane, uint32_t &c, u64 &m, u64 &all) {
+    const int w = lane & (kSmWaves - 1);
+    uint32_t ci = w < wave ? sh.wcnt[w] : 0;
+    u64 ms = sh.wsum[w], mi = w < wave ? ms : 0;
+#pragma unroll
+    for (int o = 1; o < kSmWaves; o <<= 1) ci += (uint32_t)__shfl_xor((int)ci, o), mi += xor64(mi, o), ms += xor64(ms, o);
+    c = ci, m = mi, all = ms;
+}
+
 // The row's weights.
 struct SmWeights {
-    float m, chi, clo;     // log2(e) / T in two parts
-    bool one;              // only the maximum counts (T <= 0 or tiny, or an infinite maximum)
-    __device__ __forceinline__ float log2_of(float x) const {       // -inf .. 0
+    float m, chi, clo;     // the maximum (finite); log2(e) / T in two parts
+    __device__ __forceinline__ float of(float x) const {            // 0 .. 1
         const float s = x - m;
-        return fmaf(s, chi, s * clo);
-    }
-    __device__ __forceinline__ float of(float x) const {
-        return one ? (x == m ? 1.f : 0.f) : x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(log2_of(x));
+        return x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(s, chi, s * clo));
     }
     // of() in units of 2^-44, by the addition of 1.5 * 2^8: 44 fraction bits are left below it
-    static __device__ __forceinline__ unsigned long long fixed(float w) {
-        return (unsigned long long)__double_as_longlong((double)w + 384.0) - 0x4078000000000000ull;
+    static __device__ __forceinline__ u64 fixed(float w) {
+        return (u64)__double_as_longlong((double)w + 384.0) - 0x4078000000000000ull;
     }
-    __device__ __forceinline__ unsigned long long mass(float x) const { return fixed(of(x)); }
-    __device__ __forceinline__ int bin(float x) const {             // monotone in x
-        if (one) return x == m ? 0 : kSmBins - 1;
-        const float y = (x - m) * chi * -kSmBinsPer2;
+    __device__ __forceinline__ u64 mass(float x) const { return fixed(of(x)); }
+    __device__ __forceinline__ int bin(float x) const {             // monotone in x; what is no number (0 times -inf): last
+        const float y = (x - m) * (chi * -kSmBinsPer2);
         return y < (float)(kSmBins - 1) ? (int)y : kSmBins - 1;
+    }
+    // a value that every token of bins 0 .. q lies at or above
+    __device__ __forceinline__ float floor_of(int q) const {
+        const float r = ((float)q + 1.5f) / (chi * kSmBinsPer2);
+        return q >= kSmBins - 1 ? -INFINITY : m - r - 1e-5f * (r + fabsf(m));
     }
 };
 
-// The tokens that a wavefront walks, 64 at a time and in index order:
-// each(f) calls f(step, there, value) with every lane.
+// The tokens that a wavefront walks, 64 at a time and in index order.
+// each(f, mark): f(step, there, value) with every lane, mark(steps done) after
+// every kSmStep steps and the last.  A value that is no number is not there.
 template <typename T> struct SmRow {
     const T *p;
     int base, n, end;      // first index of the lane, steps, past the last index
+    bool inf;              // the maximum is infinite: it counts as 0, the rest as -inf
     __device__ __forceinline__ SmRow(const T *row, int V, int wave, int lane) {
         n = (V + kSmThreads - 1) / kSmThreads;
         p = row;
         base = wave * n * 64 + lane;
         end = min(V, (wave + 1) * n * 64);
+        inf = false;
     }
     __device__ __forceinline__ int index(int i) const { return base + 64 * i; }
-    template <typename F> __device__ __forceinline__ void each(int i0, int i1, F f) const {
-        constexpr int U = 8;                                        // loads on their way together
+    __device__ __forceinline__ float value(float v) const { return inf && v == v ? (v == INFINITY ? 0.f : -INFINITY) : v; }
+    // some element of the row, whether or not step i has one: no branch around the load
+    __device__ __forceinline__ float some(int i) const { return Act<T>::load(p + max(0, min(index(i), end - 1))); }
+    template <typename F, typename M> __device__ __forceinline__ void each(int i0, int i1, F f, M mark) const {
+        constexpr int U = 16;                                       // loads on their way together
+        static_assert(U % kSmStep == 0, "marks inside a batch");
         for (int i = i0; i < i1; i += U) {
             float v[U];
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const int at = index(i + j);
-                v[j] = i + j < i1 && at < end ? Act<T>::load(p + at) : -INFINITY;
-            }
+            for (int j = 0; j < U; ++j) v[j] = some(i + j);
 #pragma unroll
-            for (int j = 0; j < U; ++j)
-                if (i + j < i1) f(i + j, index(i + j) < end, v[j] == v[j] ? v[j] : -INFINITY);
+            for (int j = 0; j < U; ++j) {
+                const float x = index(i + j) < end ? value(v[j]) : NAN;
+                if (i + j < i1) f(i + j, x == x, x);
+                if ((j + 1) % kSmStep == 0 && i + j + 1 - kSmStep < i1) mark(min(i + j + 1, i1));
+            }
         }
     }
-    template <typename F> __device__ __forceinline__ void each(F f) const { each(0, n, f); }
 };
 struct SmKeptRow {
     const uint2 *p;
@@ -150,52 +167,47 @@ struct SmKeptRow {
         p = list, lane = lane_, end = count, n = (count + 63) / 64;
     }
     __device__ __forceinline__ int index(int i) const { return (int)p[lane + 64 * i].y; }
-    template <typename F> __device__ __forceinline__ void each(int i0, int i1, F f) const {
+    template <typename F, typename M> __device__ __forceinline__ void each(int i0, int i1, F f, M mark) const {
         for (int i = i0; i < i1; ++i) {
             const bool there = lane + 64 * i < end;
-            f(i, there, there ? sm_value(p[lane + 64 * i].x) : -INFINITY);
+            f(i, there, there ? sm_value(p[lane + 64 * i].x) : NAN);
         }
+        mark(i1);
     }
-    template <typename F> __device__ __forceinline__ void each(F f) const { each(0, n, f); }
 };
 
-// A threshold: tokens with a larger key stay, and the first `ties` of those
-// with this key.
+// A threshold: tokens with a larger key stay, and the first `ties` of the
+// `equal` ones with this key.
 struct SmCut {
-    uint32_t key, ties;
+    uint32_t key, ties, equal;
 };
-// What a search looks for: the place where the count (or, by_mass, the
-// weight) before a token, in descending order, reaches `need`.
-__device__ __forceinline__ uint32_t sm_ties(bool by_mass, uint32_t need, uint32_t before, unsigned long long mneed,
-                                            unsigned long long mbefore, unsigned long long w) {
-    if (!by_mass) return need - before;
-    const unsigned long long left = mneed - mbefore;                // > 0; w > 0, or nothing would be left to reach
-    return w ? (uint32_t)((left + w - 1) / w) : 1u;
-}
 
 // The first bin, in order from the maximum, at whose end the running count or
-// weight reaches the need; with what lies before it.  All threads.
-__device__ __forceinline__ void sm_find_bin(SmShared &sh, int nbins, bool by_mass, uint32_t need,
-                                            unsigned long long mneed) {
+// weight reaches the need; with what lies before it.  by_mass with share >= 0:
+// the need is that share of the whole.  Returns the need.  All threads.
+__device__ __forceinline__ u64 sm_find_bin(SmShared &sh, int nbins, bool by_mass, uint32_t need, u64 mneed, float share) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = nbins / kSmThreads > 0 ? nbins / kSmThreads : 1;   // 2 for the histogram, 1 for 256 digits
+    const int per = nbins > kSmThreads ? nbins / kSmThreads : 1;
     uint32_t c = 0;
-    unsigned long long m = 0;
+    u64 m = 0;
     const bool mine = tid * per < nbins;
     if (mine)
         for (int i = 0; i < per; ++i) c += sh.count[tid * per + i], m += sh.mass[tid * per + i];
-    uint32_t ci = c;
-    unsigned long long mi = m;
+    uint32_t ci = c, c0;
+    u64 mi = m, m0, all;
     wave_scan(ci, mi, lane);
     if (lane == 63) sh.wcnt[wave] = ci, sh.wsum[wave] = mi;
     __syncthreads();
-    uint32_t c0 = ci - c;
-    unsigned long long m0 = mi - m;
-    for (int w = 0; w < wave; ++w) c0 += sh.wcnt[w], m0 += sh.wsum[w];
+    waves_before(sh, wave, lane, c0, m0, all);
+    if (by_mass && share >= 0.f) {
+        const double t = ceil((double)share * (double)all);
+        mneed = t >= (double)all ? all : t > 1. ? (u64)t : 1ull;
+    }
+    c0 += ci - c, m0 += mi - m;
     if (mine && (by_mass ? m0 < mneed && mneed <= m0 + m : c0 < need && need <= c0 + c)) {   // one thread
         for (int i = 0; i < per; ++i) {
             const uint32_t cb = sh.count[tid * per + i];
-            const unsigned long long mb = sh.mass[tid * per + i];
+            const u64 mb = sh.mass[tid * per + i];
             if (by_mass ? mneed <= m0 + mb : need <= c0 + cb) {
                 sh.bin = tid * per + i, sh.before = c0, sh.mbefore = m0;
                 break;
@@ -204,32 +216,32 @@ __device__ __forceinline__ void sm_find_bin(SmShared &sh, int nbins, bool by_mas
         }
     }
     __syncthreads();
+    return mneed;
 }
 
-// The cut within bin `sh.bin`, among the tokens of it that `in` admits.  All threads.
-template <typename Row, typename In>
+// The tokens of the search's bin: their number, range and, as far as they fit,
+// a list of their keys.  sm_open before, by all threads; then sm_put of each.
+__device__ __forceinline__ void sm_open(SmShared &sh) {
+    if (threadIdx.x == 0) sh.n = 0, sh.kmin = 0xffffffffu, sh.kmax = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ void sm_put(SmShared &sh, uint32_t key) {
+    const uint32_t at = atomicAdd(&sh.n, 1u);
+    if (at < kSmList) sh.list[at] = key;
+    atomicMin(&sh.kmin, key);
+    atomicMax(&sh.kmax, key);
+}
+
+// The cut within bin `sh.bin`, among the tokens put (where they overflow the
+// list, again those of the bin from key `least` on).  All threads.
+template <typename Row>
 __device__ __forceinline__ SmCut sm_select(SmShared &sh, const Row &row, const SmWeights &wt, bool by_mass, uint32_t need,
-                                           unsigned long long mneed, In in) {
+                                           u64 mneed, uint32_t least) {
     const int tid = threadIdx.x, bin = sh.bin;
     uint32_t before = sh.before;
-    unsigned long long mbefore = sh.mbefore;
-    __syncthreads();
-    if (tid == 0) sh.n = 0, sh.kmin = 0xffffffffu, sh.kmax = 0;
-    __syncthreads();
-    row.each([&](int, bool there, float x) {
-        if (there && wt.bin(x) == bin) {
-            const uint32_t k = sm_key(x);
-            if (in(k)) {
-                const uint32_t at = atomicAdd(&sh.n, 1u);
-                if (at < kSmList) sh.list[at] = k;
-                atomicMin(&sh.kmin, k);
-                atomicMax(&sh.kmax, k);
-            }
-        }
-    });
-    __syncthreads();
+    u64 mbefore = sh.mbefore;
     const uint32_t n = sh.n;
-    uint32_t lo = sh.kmin;                                          // the cut's key lies in lo .. lo + 2^bits - 1
+    uint32_t lo = sh.kmin, equal = n;                               // the cut's key lies in lo .. lo + 2^bits - 1
     int bits = lo == sh.kmax ? 0 : 32 - __clz((int)(sh.kmax - lo));
     while (bits > 0) {
         const int d = bits < 8 ? bits : 8, sft = bits - d;          // the next digit, its largest value first
@@ -246,205 +258,270 @@ __device__ __forceinline__ SmCut sm_select(SmShared &sh, const Row &row, const S
         if (n <= kSmList) {
             for (uint32_t i = tid; i < n; i += kSmThreads) put(sh.list[i]);
         } else {
-            row.each([&](int, bool there, float x) {
-                if (there && wt.bin(x) == bin) {
-                    const uint32_t k = sm_key(x);
-                    if (in(k)) put(k);
-                }
-            });
+            row.each(0, row.n, [&](int, bool there, float x) {
+                if (there && wt.bin(x) == bin && sm_key(x) >= least) put(sm_key(x));
+            }, [](int) {});
         }
         __syncthreads();
-        sm_find_bin(sh, 256, by_mass, need - before, mneed - mbefore);
+        sm_find_bin(sh, 256, by_mass, need - before, mneed - mbefore, -1.f);
         before += sh.before, mbefore += sh.mbefore;
         lo += (uint32_t)(((1u << d) - 1) - sh.bin) << sft;
+        equal = sh.count[sh.bin];
         bits = sft;
     }
-    return SmCut{lo, sm_ties(by_mass, need, before, mneed, mbefore, wt.mass(sm_value(lo)))};
+    // equal ones before the need is reached (w > 0, or nothing would be left to reach)
+    const u64 w = wt.mass(sm_value(lo)), left = mneed - mbefore;
+    const uint32_t ties = by_mass ? (w ? (uint32_t)((left + w - 1) / w) : 1u) : need - before;
+    return SmCut{lo, ties, equal};
 }
 
-// The sum of the histogram's weights.  All threads.
-__device__ __forceinline__ unsigned long long sm_total(SmShared &sh) {
-    const int tid = threadIdx.x;
-    unsigned long long s = 0, total = 0;
-    for (int i = tid; i < kSmBins; i += kSmThreads) s += sh.mass[i];
-    s = wave_sum64(s);
-    if ((tid & 63) == 0) sh.wsum[tid >> 6] = s;
-    __syncthreads();
-    for (int w = 0; w < kSmWaves; ++w) total += sh.wsum[w];
-    __syncthreads();
-    return total;
-}
-// The weight that top-p asks for.
-__device__ __forceinline__ unsigned long long sm_share(float p, unsigned long long total) {
-    const double t = ceil((double)p * (double)total);
-    return t >= (double)total ? total : t > 1. ? (unsigned long long)t : 1ull;
-}
-
-// From the first search's bin (sh.bin, sh.before, sh.mbefore) to the token, on
-// the whole row or on the lists.
-template <typename Row>
-__device__ __forceinline__ void sm_finish(SmShared &sh, const Row &row, const SmWeights &wt, bool by_k, bool by_p,
-                                          uint32_t k, float top_p, unsigned long long need, float min_p, float u,
-                                          int64_t *out) {
+// From the first search's bin (sh.bin, sh.before, sh.mbefore) to the token.
+// walk: row.each of everything, or the same out of registers.
+template <typename Row, typename Walk>
+__device__ __forceinline__ void sm_finish(SmShared &sh, const Row &row, Walk walk, const SmWeights &wt, bool by_k, bool by_p,
+                                          uint32_t k, float top_p, u64 need, float min_p, float u, int64_t *out) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    SmCut cut{0u, 0u};
+    auto nothing = [](int) {};
+    // the keys of the search's bin from `least` on
+    auto collect = [&](uint32_t least) {
+        const int bin = sh.bin;
+        const float lo = wt.floor_of(bin);
+        sm_open(sh);
+        row.each(0, row.n, [&](int, bool there, float x) {
+            if (!__any(x >= lo)) return;
+            if (there && wt.bin(x) == bin && sm_key(x) >= least) sm_put(sh, sm_key(x));
+        }, nothing);
+        __syncthreads();
+    };
+    SmCut cut{0u, 0u, 0u};
+    if (by_k || by_p) collect(0u);
     if (by_k) {
-        cut = sm_select(sh, row, wt, false, k, 0ull, [](uint32_t) { return true; });
+        cut = sm_select(sh, row, wt, false, k, 0ull, 0u);
         if (by_p) {
             // the histogram of what top-k keeps; the ties at its cut weigh the
             // same, so any of them stand for the first ones
             __syncthreads();
             for (int i = tid; i < kSmBins; i += kSmThreads) sh.count[i] = 0, sh.mass[i] = 0;
             __syncthreads();
-            row.each([&](int, bool there, float x) {
+            row.each(0, row.n, [&](int, bool there, float x) {
                 if (there && sm_key(x) > cut.key) atomicAdd(&sh.mass[wt.bin(x)], wt.mass(x));
-            });
+            }, nothing);
             if (tid == 0) {
                 const float x = sm_value(cut.key);
                 atomicAdd(&sh.mass[wt.bin(x)], wt.mass(x) * cut.ties);
             }
             __syncthreads();
-            need = sm_share(top_p, sm_total(sh));
-            sm_find_bin(sh, kSmBins, true, 0u, need);
+            need = sm_find_bin(sh, kSmBins, true, 0u, 0ull, top_p);
+            collect(cut.key);
         }
     }
     if (by_p) {
-        const uint32_t least = cut.key;
-        const SmCut c = sm_select(sh, row, wt, true, 0u, need, [&](uint32_t q) { return q >= least; });
+        const SmCut c = sm_select(sh, row, wt, true, 0u, need, cut.key);
         if (!by_k || c.key > cut.key) cut = c;
         else cut.ties = min(cut.ties, c.ties);
     }
-    const bool cutting = by_k || by_p;
-    uint32_t tie = 0;                                               // ties at the cut before this wavefront
-    __syncthreads();
-    if (cutting) {
-        uint32_t t = 0;
-        row.each([&](int, bool there, float x) { t += __popcll(__ballot(there && sm_key(x) == cut.key)); });
-        if (lane == 0) sh.wcnt[wave] = t;
+    // What stays: values above xc, and those equal to it below index `edge`.
+    const bool all_stay = !by_k && !by_p;
+    const float xc = all_stay ? -INFINITY : sm_value(cut.key);
+    int edge = 0x7fffffff;
+    if (!all_stay && cut.ties < cut.equal) {
+        // the index of the first equal one that goes
+        uint32_t t = 0, before;
+        walk([&](int, bool there, float x) { t += __popcll(__ballot(there && x == xc)); }, nothing);
         __syncthreads();
-        for (int w = 0; w < wave; ++w) tie += sh.wcnt[w];
-    }
-    // the weight that a token keeps (0: it is gone); `seen` counts the ties on
-    auto rest = [&](bool there, float x, uint32_t &seen) {
-        if (cutting) {
-            const uint32_t q = sm_key(x);
-            const unsigned long long eq = __ballot(there && q == cut.key);
-            const uint32_t r = seen + __popcll(eq & ((1ull << lane) - 1));
-            there = there && (q > cut.key || (q == cut.key && r < cut.ties));
-            seen += __popcll(eq);
+        if (lane == 0) sh.wcnt[wave] = t, sh.wsum[wave] = 0;
+        __syncthreads();
+        u64 m0, m1;
+        waves_before(sh, wave, lane, before, m0, m1);
+        if (before <= cut.ties && cut.ties < before + t) {          // one wavefront's
+            row.each(0, row.n, [&](int i, bool there, float x) {
+                const u64 eq = __ballot(there && x == xc);
+                const uint32_t here = __popcll(eq & ((1ull << lane) - 1));
+                if (there && x == xc && before + here == cut.ties) sh.edge = row.index(i);
+                before += __popcll(eq);
+            }, nothing);
         }
+        __syncthreads();
+        edge = sh.edge;
+    }
+    auto rest = [&](int i, bool there, float x) {
         const float w = wt.of(x);
-        return there && w >= min_p ? SmWeights::fixed(w) : 0ull;
+        const bool stay = there && (x > xc || (x == xc && (edge == 0x7fffffff || row.index(i) < edge))) && w >= min_p;
+        return stay ? SmWeights::fixed(w) : 0ull;
     };
     // sums of the parts of the walk, then of wavefronts
-    const int step = (row.n + kSmParts - 1) / kSmParts;
-    unsigned long long mine = 0;
-    uint32_t seen = tie;
-    for (int j = 0; j < kSmParts; ++j) {
-        unsigned long long s = 0;
-        if (j * step < row.n) {
-            if (lane == 0) sh.part[wave][j] = 0;
-            const uint32_t at = seen;
-            row.each(j * step, min(row.n, (j + 1) * step), [&](int, bool there, float x) { s += rest(there, x, seen); });
-            s = wave_sum64(s);
-            if (lane == 0) sh.part[wave][j] = s;
-            if (lane == 0) sh.list[wave * kSmParts + j] = at;       // ties before the part
-        }
-        mine += s;
-    }
+    const int step = kSmStep * ((row.n + kSmStep * kSmParts - 1) / (kSmStep * kSmParts));
+    u64 mine = 0, s = 0;
+    walk([&](int i, bool there, float x) { s += rest(i, there, x); },
+         [&](int done) {
+             if (done % step && done < row.n) return;
+             s = wave_sum64(s);
+             if (lane == 0) sh.part[wave][(done - 1) / step] = s;
+             mine += s;
+             s = 0;
+         });
+    __syncthreads();
     if (lane == 0) sh.wsum[wave] = mine;
     __syncthreads();
-    unsigned long long all = 0, run = 0;
-    for (int w = 0; w < kSmWaves; ++w) {
-        if (w == wave) run = all;
-        all += sh.wsum[w];
-    }
+    uint32_t c0;
+    u64 run, all;
+    waves_before(sh, wave, lane, c0, run, all);
     if (all == 0) {                                                 // min_p above 1, or not a number
         if (tid == 0) *out = -1;
         return;
     }
     const double ut = (double)(u > 0.f ? u : 0.f) * (double)all;
-    unsigned long long thr = ut < (double)all ? (unsigned long long)ut : all - 1;   // the first running sum above this
+    u64 thr = ut < (double)all ? (u64)ut : all - 1;                 // the first running sum above this
     if (thr >= all) thr = all - 1;
     if (thr < run || thr >= run + mine) return;                     // another wavefront's
     int j = 0;
     while (run + sh.part[wave][j] <= thr) run += sh.part[wave][j++];
-    seen = sh.list[wave * kSmParts + j];
     bool found = false;
     row.each(j * step, min(row.n, (j + 1) * step), [&](int i, bool there, float x) {
-        unsigned long long s = rest(there, x, seen);
-        if (found || !__any(s != 0)) return;
+        if (found) return;
+        u64 v = rest(i, there, x);
+        if (!__any(v != 0)) return;
         uint32_t none = 0;
-        wave_scan(none, s, lane);
-        const unsigned long long hit = __ballot(run + s > thr);
+        wave_scan(none, v, lane);
+        const u64 hit = __ballot(run + v > thr);
         if (hit) {
             if (lane == (int)__ffsll((long long)hit) - 1) *out = row.index(i);
             found = true;
         }
-        run += shfl64(s, 63);
-    });
+        run += shfl64(v, 63);
+    }, nothing);
 }
 
-template <typename T> __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
+// NPT: values that a lane holds in registers (V <= NPT * 1024), or 0.
+template <typename T, int NPT> __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
     extern __shared__ __align__(16) unsigned char sm_smem[];
     SmShared &sh = *(SmShared *)sm_smem;
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    SmRow<T> row((const T *)a.logits + b * a.ld, (int)a.V, wave, lane);
+    float v[NPT ? NPT : 1];
+    if constexpr (NPT > 0) {
+#pragma unroll
+        for (int i = 0; i < NPT; ++i) {
+            v[i] = row.some(i);
+            if (i % kSmStep == kSmStep - 1) __builtin_amdgcn_sched_barrier(0);   // (addresses one after the other)
+        }
+    }
     const float temp = a.temperature ? a.temperature[b] : a.temperature0;
     const float top_p = a.top_p ? a.top_p[b] : a.top_p0, min_p = a.min_p ? a.min_p[b] : a.min_p0;
     const int top_k = a.top_k ? a.top_k[b] : a.top_k0;
     const float u = a.u[b];
-    const SmRow<T> row((const T *)a.logits + b * a.ld, (int)a.V, wave, lane);
+    for (int i = tid; i < kSmBins; i += kSmThreads) sh.count[i] = 0, sh.mass[i] = 0;
+    if (tid == 0) sh.over = 0;
+    auto walk = [&](auto f, auto mark) {
+        if constexpr (NPT > 0) {
+#pragma unroll
+            for (int g = 0; g < NPT; g += kSmStep) {
+                if (g < row.n) {                                    // the last steps may lie past the row
+#pragma unroll
+                    for (int j = 0; j < kSmStep; ++j) {
+                        float x = v[g + j];
+                        asm volatile("" : "+v"(x));                 // (whether it is there is found anew, not kept)
+                        f(g + j, x == x, x);
+                    }
+                    mark(min(g + kSmStep, row.n));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            row.each(0, row.n, f, mark);
+        }
+    };
+    auto nothing = [](int) {};
 
     float m = -INFINITY;
-    row.each([&](int, bool, float x) { m = fmaxf(m, x); });
+    if constexpr (NPT > 0) {
+        // from here on what lies past the row is no number
+        int base = row.base;
+        asm volatile("" : "+v"(base));                              // (the addresses are not kept for this)
+#pragma unroll
+        for (int i = 0; i < NPT; ++i) {
+            v[i] = i < row.n && base + 64 * i < row.end ? v[i] : NAN;
+            m = fmaxf(m, v[i]);
+            if (i % kSmStep == kSmStep - 1) __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+        walk([&](int, bool, float x) { m = fmaxf(m, x); }, nothing);
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     if (lane == 0) sh.wmax[wave] = m;
-    for (int i = tid; i < kSmBins; i += kSmThreads) sh.count[i] = 0, sh.mass[i] = 0;
-    if (tid == 0) sh.over = 0;
     __syncthreads();
-    m = sh.wmax[0];
-    for (int w = 1; w < kSmWaves; ++w) m = fmaxf(m, sh.wmax[w]);
+    m = sh.wmax[lane & (kSmWaves - 1)];
+#pragma unroll
+    for (int o = 1; o < kSmWaves; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
     if (m == -INFINITY) {
         if (tid == 0) a.out[b] = -1;
         return;
     }
+    if (m == INFINITY) {                                            // the infinite ones share the weight
+        row.inf = true;
+        m = 0.f;
+        if constexpr (NPT > 0) {
+#pragma unroll
+            for (int i = 0; i < NPT; ++i) v[i] = row.value(v[i]);
+        }
+    }
     const bool greedy = !(temp > 0.f);
-    const double c = greedy ? 0. : 1.4426950408889634074 / (double)temp;
-    const SmWeights wt{m, (float)c, (float)(c - (double)(float)c), greedy || m == INFINITY || !(c < 1e30)};
+    const double c = greedy ? 1. : fmin(1.4426950408889634074 / (double)temp, 1e30);   // (1e30: only the maximum counts)
+    const SmWeights wt{m, (float)c, (float)(c - (double)(float)c)};
     const bool by_k = greedy || (top_k > 0 && top_k < a.V), by_p = !greedy && top_p < 1.f;
     const uint32_t k = greedy ? 1u : (uint32_t)top_k;
-    unsigned long long need = 0;
+    u64 need = 0;
+    float least = -INFINITY;                                        // no token that may stay lies below
     if (by_k || by_p) {
-        row.each([&](int, bool there, float x) {
-            if (there) {
-                const int q = wt.bin(x);
-                if (by_k) atomicAdd(&sh.count[q], 1u);
-                else atomicAdd(&sh.mass[q], wt.mass(x));
-            }
-        });
+        if (by_k)
+            walk([&](int, bool there, float x) {
+                if (there) atomicAdd(&sh.count[wt.bin(x)], 1u);
+            }, nothing);
+        else
+            walk([&](int, bool there, float x) {
+                if (there) atomicAdd(&sh.mass[wt.bin(x)], wt.mass(x));
+            }, nothing);
         __syncthreads();
-        if (!by_k) need = sm_share(top_p, sm_total(sh));
-        sm_find_bin(sh, kSmBins, !by_k, k, need);
+        need = sm_find_bin(sh, kSmBins, !by_k, k, 0ull, top_p);
+        least = wt.floor_of(sh.bin);
+    } else if (min_p > 0.f) {
+        least = wt.floor_of((int)fminf(ceilf(-log2f(min_p) * kSmBinsPer2), (float)(kSmBins - 1)));
     }
-    // the tokens still in question: down to the search's bin, or to min_p
-    const int last = by_k || by_p ? sh.bin : kSmBins;
+    // the tokens still in question
     int kept = 0;
-    if (last < kSmBins || min_p > 0.f) {
-        row.each([&](int i, bool there, float x) {
-            const bool in = there && (last < kSmBins ? wt.bin(x) <= last : wt.of(x) >= min_p);
-            const unsigned long long who = __ballot(in);
+    if (least > -INFINITY) {
+        walk([&](int i, bool, float x) {
+            const u64 who = __ballot(x >= least);
+            if (!who) return;
+            int index = row.base;
+            asm volatile("" : "+v"(index));                         // (not kept from the loads)
             const int at = kept + __popcll(who & ((1ull << lane) - 1));
-            if (in && at < kSmKept) sh.kept[wave][at] = make_uint2(sm_key(x), (uint32_t)row.index(i));
+            if (x >= least && at < kSmKept) sh.kept[wave][at] = make_uint2(sm_key(x), (uint32_t)(index + 64 * i));
             kept += __popcll(who);
-        });
-        if (kept > kSmKept && lane == 0) sh.over = 1;
-    } else if (tid == 0) {
-        sh.over = 1;
+        }, nothing);
+    } else {
+        kept = kSmKept + 1;
     }
+    if (kept > kSmKept && lane == 0) sh.over = 1;
     __syncthreads();
-    if (sh.over) sm_finish(sh, row, wt, by_k, by_p, k, top_p, need, min_p, u, a.out + b);
-    else sm_finish(sh, SmKeptRow(sh.kept[wave], kept, lane), wt, by_k, by_p, k, top_p, need, min_p, u, a.out + b);
+    if (sh.over) {
+        sm_finish(sh, row, [&](auto f, auto mark) { row.each(0, row.n, f, mark); }, wt, by_k, by_p, k, top_p, need, min_p, u, a.out + b);
+    } else {
+        const SmKeptRow mine(sh.kept[wave], kept, lane);
+        sm_finish(sh, mine, [&](auto f, auto mark) { mine.each(0, mine.n, f, mark); }, wt, by_k, by_p, k, top_p, need,
+                  min_p, u, a.out + b);
+    }
+}
+
+template <typename T> static void sample_launch(const SampleArgs &a, unsigned rows, hipStream_t s) {
+    const dim3 G(rows), N(kSmThreads);
+    const uint32_t lds = (uint32_t)sizeof(SmShared);
+    // registers for as many values as leave 16 wavefronts on a CU
+    if (a.V <= 16 * kSmThreads) launch(sample_kernel<T, 16>, G, N, lds, s, a);
+    else if (a.V <= 64 * kSmThreads) launch(sample_kernel<T, 64>, G, N, lds, s, a);
+    else launch(sample_kernel<T, 0>, G, N, lds, s, a);
 }
 
 }  // namespace walsh
@@ -463,10 +540,7 @@ WALSH_EXPORT int walsh_sample(const void *logits, int64_t ld, int64_t B, int64_t
     if (!logits || !u || !out) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
     if (B > 1 && ld < V) return set_error(WALSH_EINVAL, "%s: row stride %lld for %lld logits", fn, (long long)ld, (long long)V);
     const SampleArgs a{logits, ld, V, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, out};
-    const dim3 G((unsigned)B), N(kSmThreads);
-    hipStream_t s = (hipStream_t)stream;
-    const uint32_t lds = (uint32_t)sizeof(SmShared);
-    if (dtype == WALSH_BF16) launch(sample_kernel<uint16_t>, G, N, lds, s, a);
-    else launch(sample_kernel<float>, G, N, lds, s, a);
+    if (dtype == WALSH_BF16) sample_launch<uint16_t>(a, (unsigned)B, (hipStream_t)stream);
+    else sample_launch<float>(a, (unsigned)B, (hipStream_t)stream);
     return check_hip(hipGetLastError(), fn);
 }
