@@ -21,7 +21,7 @@
 // arithmetic up to the weights' own rounding.
 //
 // One workgroup of 16 wavefronts per row; wavefront w walks the indexes from
-// w * ceil(V / 1024) * 64 on, 64 at a time, held in registers up to 65,536
+// w * ceil(V / 1024) * 64 on, 64 at a time, held in registers up to 57,344
 // tokens.  Three walks over the row: its maximum, the histogram, and the
 // tokens that the histogram leaves in question, each wavefront's into a list
 // in LDS; what follows works on the lists, or, where one overflows (nothing
@@ -70,7 +70,7 @@ struct SmShared {
     // results of a search
     uint32_t n, kmin, kmax, before;
     u64 mbefore;
-    int bin, over, edge;
+    int bin, over[2], edge;
 };
 
 __device__ __forceinline__ u64 shfl64(u64 v, int src) {
@@ -124,12 +124,17 @@ struct SmWeights {
         const float r = ((float)q + 1.5f) / (chi * kSmBinsPer2);
         return q >= kSmBins - 1 ? -INFINITY : m - r - 1e-5f * (r + fabsf(m));
     }
+    // and one that no token of bin q lies above
+    __device__ __forceinline__ float ceiling_of(int q) const {
+        const float r = fmaxf((float)q - 0.5f, 0.f) / (chi * kSmBinsPer2);
+        return q == 0 ? INFINITY : m - r + 1e-5f * (r + fabsf(m));
+    }
 };
 
 // The tokens that a wavefront walks, 64 at a time and in index order.
 // each(f, mark): f(step, there, value) with every lane, mark(steps done) after
 // every kSmStep steps and the last.  A value that is no number is not there.
-template <typename T> struct SmRow {
+template <typename T, int U> struct SmRow {                          // U: loads on their way together
     const T *p;
     int base, n, end;      // first index of the lane, steps, past the last index
     bool inf;              // the maximum is infinite: it counts as 0, the rest as -inf
@@ -141,12 +146,15 @@ template <typename T> struct SmRow {
         inf = false;
     }
     __device__ __forceinline__ int index(int i) const { return base + 64 * i; }
+    __device__ __forceinline__ int index_anew(int i) const {        // not kept in a register from an earlier use
+        int at = base;
+        asm volatile("" : "+v"(at));
+        return at + 64 * i;
+    }
     __device__ __forceinline__ float value(float v) const { return inf && v == v ? (v == INFINITY ? 0.f : -INFINITY) : v; }
     // some element of the row, whether or not step i has one: no branch around the load
     __device__ __forceinline__ float some(int i) const { return Act<T>::load(p + max(0, min(index(i), end - 1))); }
     template <typename F, typename M> __device__ __forceinline__ void each(int i0, int i1, F f, M mark) const {
-        constexpr int U = 16;                                       // loads on their way together
-        static_assert(U % kSmStep == 0, "marks inside a batch");
         for (int i = i0; i < i1; i += U) {
             float v[U];
 #pragma unroll
@@ -155,7 +163,7 @@ template <typename T> struct SmRow {
             for (int j = 0; j < U; ++j) {
                 const float x = index(i + j) < end ? value(v[j]) : NAN;
                 if (i + j < i1) f(i + j, x == x, x);
-                if ((j + 1) % kSmStep == 0 && i + j + 1 - kSmStep < i1) mark(min(i + j + 1, i1));
+                if (i + j < i1 && ((i + j + 1) % kSmStep == 0 || i + j + 1 == i1)) mark(i + j + 1);
             }
         }
     }
@@ -166,7 +174,8 @@ struct SmKeptRow {
     __device__ __forceinline__ SmKeptRow(const uint2 *list, int count, int lane_) {
         p = list, lane = lane_, end = count, n = (count + 63) / 64;
     }
-    __device__ __forceinline__ int index(int i) const { return (int)p[lane + 64 * i].y; }
+    __device__ __forceinline__ int index(int i) const { return lane + 64 * i < end ? (int)p[lane + 64 * i].y : 0; }
+    __device__ __forceinline__ int index_anew(int i) const { return index(i); }
     template <typename F, typename M> __device__ __forceinline__ void each(int i0, int i1, F f, M mark) const {
         for (int i = i0; i < i1; ++i) {
             const bool there = lane + 64 * i < end;
@@ -276,25 +285,30 @@ __device__ __forceinline__ SmCut sm_select(SmShared &sh, const Row &row, const S
 }
 
 // From the first search's bin (sh.bin, sh.before, sh.mbefore) to the token.
-// walk: row.each of everything, or the same out of registers.
+// walk: row.each of everything, or the same out of registers; listed: tokens
+// that hold all of the first search's bin, if so_listed.
 template <typename Row, typename Walk>
-__device__ __forceinline__ void sm_finish(SmShared &sh, const Row &row, Walk walk, const SmWeights &wt, bool by_k, bool by_p,
-                                          uint32_t k, float top_p, u64 need, float min_p, float u, int64_t *out) {
+__device__ __forceinline__ void sm_finish(SmShared &sh, const Row &row, Walk walk, const SmKeptRow &listed,
+                                          bool so_listed, const SmWeights &wt, bool by_k, bool by_p, uint32_t k, float top_p, u64 need,
+                                          float min_p, float u, int64_t *out) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     auto nothing = [](int) {};
     // the keys of the search's bin from `least` on
-    auto collect = [&](uint32_t least) {
+    auto collect = [&](const auto &from, uint32_t least) {
         const int bin = sh.bin;
         const float lo = wt.floor_of(bin);
         sm_open(sh);
-        row.each(0, row.n, [&](int, bool there, float x) {
+        from.each(0, from.n, [&](int, bool there, float x) {
             if (!__any(x >= lo)) return;
             if (there && wt.bin(x) == bin && sm_key(x) >= least) sm_put(sh, sm_key(x));
         }, nothing);
         __syncthreads();
     };
     SmCut cut{0u, 0u, 0u};
-    if (by_k || by_p) collect(0u);
+    if (by_k || by_p) {
+        if (so_listed) collect(listed, 0u);
+        else collect(row, 0u);
+    }
     if (by_k) {
         cut = sm_select(sh, row, wt, false, k, 0ull, 0u);
         if (by_p) {
@@ -312,7 +326,7 @@ __device__ __forceinline__ void sm_finish(SmShared &sh, const Row &row, Walk wal
             }
             __syncthreads();
             need = sm_find_bin(sh, kSmBins, true, 0u, 0ull, top_p);
-            collect(cut.key);
+            collect(row, cut.key);
         }
     }
     if (by_p) {
@@ -346,7 +360,8 @@ __device__ __forceinline__ void sm_finish(SmShared &sh, const Row &row, Walk wal
     }
     auto rest = [&](int i, bool there, float x) {
         const float w = wt.of(x);
-        const bool stay = there && (x > xc || (x == xc && (edge == 0x7fffffff || row.index(i) < edge))) && w >= min_p;
+        bool stay = there && x >= xc && w >= min_p;
+        if (edge != 0x7fffffff) stay = stay && (x > xc || row.index_anew(i) < edge);
         return stay ? SmWeights::fixed(w) : 0ull;
     };
     // sums of the parts of the walk, then of wavefronts
@@ -398,7 +413,7 @@ template <typename T, int NPT> __global__ __launch_bounds__(kSmThreads) void sam
     SmShared &sh = *(SmShared *)sm_smem;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    SmRow<T> row((const T *)a.logits + b * a.ld, (int)a.V, wave, lane);
+    SmRow<T, NPT ? 4 : 16> row((const T *)a.logits + b * a.ld, (int)a.V, wave, lane);
     float v[NPT ? NPT : 1];
     if constexpr (NPT > 0) {
 #pragma unroll
@@ -412,7 +427,7 @@ template <typename T, int NPT> __global__ __launch_bounds__(kSmThreads) void sam
     const int top_k = a.top_k ? a.top_k[b] : a.top_k0;
     const float u = a.u[b];
     for (int i = tid; i < kSmBins; i += kSmThreads) sh.count[i] = 0, sh.mass[i] = 0;
-    if (tid == 0) sh.over = 0;
+    if (tid == 0) sh.over[0] = sh.over[1] = 0;
     auto walk = [&](auto f, auto mark) {
         if constexpr (NPT > 0) {
 #pragma unroll
@@ -489,30 +504,32 @@ template <typename T, int NPT> __global__ __launch_bounds__(kSmThreads) void sam
     } else if (min_p > 0.f) {
         least = wt.floor_of((int)fminf(ceilf(-log2f(min_p) * kSmBinsPer2), (float)(kSmBins - 1)));
     }
-    // the tokens still in question
-    int kept = 0;
-    if (least > -INFINITY) {
+    // the tokens still in question into the wavefronts' lists; where a list
+    // overflows, those of the search's bin alone
+    float most = INFINITY;
+    int kept = 0, pass = 0;
+    for (; pass < 2 && least > -INFINITY; ++pass) {
+        kept = 0;
         walk([&](int i, bool, float x) {
-            const u64 who = __ballot(x >= least);
+            const u64 who = __ballot(x >= least && x <= most);
             if (!who) return;
-            int index = row.base;
-            asm volatile("" : "+v"(index));                         // (not kept from the loads)
             const int at = kept + __popcll(who & ((1ull << lane) - 1));
-            if (x >= least && at < kSmKept) sh.kept[wave][at] = make_uint2(sm_key(x), (uint32_t)(index + 64 * i));
+            if (x >= least && x <= most && at < kSmKept) sh.kept[wave][at] = make_uint2(sm_key(x), (uint32_t)row.index_anew(i));
             kept += __popcll(who);
         }, nothing);
-    } else {
-        kept = kSmKept + 1;
+        if (kept > kSmKept && lane == 0) sh.over[pass] = 1;
+        __syncthreads();
+        if (!sh.over[pass]) break;
+        if (!by_k && !by_p) pass = 1;
+        else if (pass == 0) least = wt.floor_of(sh.bin), most = wt.ceiling_of(sh.bin);
     }
-    if (kept > kSmKept && lane == 0) sh.over = 1;
-    __syncthreads();
-    if (sh.over) {
-        sm_finish(sh, row, [&](auto f, auto mark) { row.each(0, row.n, f, mark); }, wt, by_k, by_p, k, top_p, need, min_p, u, a.out + b);
-    } else {
-        const SmKeptRow mine(sh.kept[wave], kept, lane);
-        sm_finish(sh, mine, [&](auto f, auto mark) { mine.each(0, mine.n, f, mark); }, wt, by_k, by_p, k, top_p, need,
-                  min_p, u, a.out + b);
-    }
+    const SmKeptRow mine(sh.kept[wave], min(kept, kSmKept), lane);
+    const bool listed = pass < 2 && least > -INFINITY;
+    if (listed && pass == 0)
+        sm_finish(sh, mine, [&](auto f, auto mark) { mine.each(0, mine.n, f, mark); }, mine, true, wt, by_k, by_p, k, top_p,
+                  need, min_p, u, a.out + b);
+    else
+        sm_finish(sh, row, walk, mine, listed, wt, by_k, by_p, k, top_p, need, min_p, u, a.out + b);
 }
 
 template <typename T> static void sample_launch(const SampleArgs &a, unsigned rows, hipStream_t s) {
@@ -520,7 +537,7 @@ template <typename T> static void sample_launch(const SampleArgs &a, unsigned ro
     const uint32_t lds = (uint32_t)sizeof(SmShared);
     // registers for as many values as leave 16 wavefronts on a CU
     if (a.V <= 16 * kSmThreads) launch(sample_kernel<T, 16>, G, N, lds, s, a);
-    else if (a.V <= 64 * kSmThreads) launch(sample_kernel<T, 64>, G, N, lds, s, a);
+    else if (a.V <= 56 * kSmThreads) launch(sample_kernel<T, 56>, G, N, lds, s, a);
     else launch(sample_kernel<T, 0>, G, N, lds, s, a);
 }
 
