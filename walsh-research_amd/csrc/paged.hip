@@ -28,7 +28,7 @@
 namespace walsh {
 
 constexpr int kPgWaves = 4;
-constexpr int kPgMaxChunk = 4096;                 // keys per workgroup
+constexpr int kPgMaxChunk = 1024;                 // keys per workgroup
 constexpr int kPgMinPage = 16;                    // rows of a page, where a sequence has several
 constexpr int kPgEntries = kPgMaxChunk / kPgMinPage + 4;
 
@@ -44,7 +44,7 @@ struct PgArgs {
     float sl2;
     void *o;
     int64_t o_sb, o_sh;
-    float *part;                                  // [B][H][ns][D + 2]: acc, max, sum
+    float *part;                                  // [B][H][ns][D] accumulators, then [B][H][ns] (max, sum)
 };
 
 // The visible keys of a sequence: n of them, the first s0 first tokens, key t
@@ -82,9 +82,11 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
     __shared__ int pages[kPgEntries];
     __shared__ float stat[kPgWaves][2][32];
     __shared__ int any_bad;
-    const int R = a.H / a.G, nqt = (R + 31) / 32;
-    const int s = blockIdx.x, g = (int)blockIdx.y / nqt, r0 = (int)blockIdx.y % nqt * 32, b = blockIdx.z;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 31, hi = lane >> 5;
+    const int R = uniform(a.H / a.G), nqt = (R + 31) / 32;
+    // the heads of a chunk side by side: their rows share pages
+    const int gy = a.G * nqt, s = uniform((int)blockIdx.x / gy), gq = (int)blockIdx.x - s * gy, b = blockIdx.y;
+    const int g = uniform(gq / nqt), r0 = (gq - g * nqt) * 32;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, hi = lane >> 5;
     const int heads = min(32, R - r0), h0 = g * R + r0;
     const PgKeys ks = pg_keys(a, b);
     const int c0 = s * a.chunk, c1 = min(c0 + a.chunk, ks.n);
@@ -128,14 +130,12 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
             for (int kk = 0; kk < NK; ++kk) kf[u][kk] = load_frag(p + 16 * kk);
         }
     };
-    auto fetch_v = [&](unsigned char *dst, int t0) {
-        dst = (unsigned char *)__builtin_assume_aligned(dst, 16);
+    auto fetch_v = [&](int buf, int t0) {
+        const uint32_t dst = lds_addr(vl) + buf * PgCfg<T, D>::VBYTES;
 #pragma unroll
         for (int i = 0; i < NB * L::BYTES / 1024; ++i) {
             const int pos = i * 64 + lane, row = pos / L::NCH, c = (pos % L::NCH) ^ L::swz(row & 31);
-            const T *p = vb + at(t0 + row) + c * (16 / (int)sizeof(T));
-            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)const_cast<T *>(p),
-                                             (__attribute__((address_space(3))) void *)(dst + i * 1024), 16, 0, 0);
+            lds_gather(vb + at(t0 + row) + c * (16 / (int)sizeof(T)), dst + i * 1024);
         }
     };
 
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
     Frag<T> kf[NB][NK];
     if (t0 < c1) {
         fetch_k(kf, t0);
-        fetch_v(vl, t0);
+        fetch_v(0, t0);
     }
     for (; t0 < c1; t0 += stride, buf ^= 1) {
         const int tn = t0 + stride;
@@ -160,10 +160,10 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
             for (int kk = 0; kk < NK; ++kk) mma(sc[u], kf[u][kk], qf[kk]);
         }
         // this block's V has landed (it was requested after this block's K)
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        wait_loads();
         if (tn < c1) {
             fetch_k(kf, tn);
-            fetch_v(vl + (buf ^ 1) * PgCfg<T, D>::VBYTES, tn);
+            fetch_v(buf ^ 1, tn);
         }
         if (t0 + KB > c1) {
 #pragma unroll
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
     l = half_sum(l);
 
     // the wavefronts' parts: o = sum_w acc_w e^(m_w - m) / sum_w l_w e^(m_w - m)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    wait_loads();
     float *av = (float *)vl;                      // [32 heads][D] of this wavefront (its V is used up)
     if (n < heads) {
 #pragma unroll
@@ -241,29 +241,43 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
         if (a.ns == 1) {
             store4((T *)a.o + b * a.o_sb + (h0 + r) * a.o_sh + d, bad ? v * ll : ll > 0.f ? v * (1.f / ll) : v * 0.f);
         } else {
-            float *dst = a.part + (((int64_t)b * a.H + h0 + r) * a.ns + s) * (D + 2);
-            dst[d] = v.x, dst[d + 1] = v.y, dst[d + 2] = v.z, dst[d + 3] = v.w;
-            if (d == 0) dst[D] = mm, dst[D + 1] = ll;
+            const int64_t at = ((int64_t)b * a.H + h0 + r) * a.ns + s;
+            store4(a.part + at * D + d, v);
+            if (d == 0) ((float2 *)(a.part + (int64_t)a.B * a.H * a.ns * D))[at] = make_float2(mm, ll);
         }
     }
 }
 
-// The chunks' parts of one (sequence, query head) joined.
-template <typename T, int D> __global__ __launch_bounds__(D) void paged_decode_join_kernel(PgArgs a) {
-    const int b = (int)blockIdx.x / a.H, h = (int)blockIdx.x % a.H, d = threadIdx.x;
+// The chunks' parts of one (sequence, query head) joined: blockDim.x / D groups
+// of D threads take every so many parts each.
+template <typename T, int D> __global__ __launch_bounds__(1024) void paged_decode_join_kernel(PgArgs a) {
+    __shared__ float num_l[1024], den_l[1024 / D], max_l[16];
+    const int b = (int)blockIdx.x / a.H, h = (int)blockIdx.x % a.H, tid = threadIdx.x, d = tid % D, grp = tid / D;
+    const int groups = (int)blockDim.x / D;
     const PgKeys ks = pg_keys(a, b);
     const int ns = max(1, (ks.n + a.chunk - 1) / a.chunk);
-    const float *p = a.part + (int64_t)blockIdx.x * a.ns * (D + 2);
+    const float *acc = a.part + (int64_t)blockIdx.x * a.ns * D + d;
+    const float2 *st = (const float2 *)(a.part + (int64_t)a.B * a.H * a.ns * D) + (int64_t)blockIdx.x * a.ns;   // (max, sum)
     float mm = kNoScore;
-#pragma unroll 8
-    for (int s = 0; s < ns; ++s) mm = fmaxf(mm, p[s * (D + 2) + D]);
+    for (int s = tid; s < ns; s += (int)blockDim.x) mm = fmaxf(mm, st[s].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+    if ((tid & 63) == 0) max_l[tid >> 6] = mm;
+    __syncthreads();
+    for (int w = 0; w < ((int)blockDim.x + 63) / 64; ++w) mm = fmaxf(mm, max_l[w]);
     float num = 0.f, den = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < ns; ++s) {
-        const float f = __builtin_amdgcn_exp2f((p[s * (D + 2) + D] - mm) * a.sl2);
-        num += f * p[s * (D + 2) + d];
-        den += f * p[s * (D + 2) + D + 1];
+    for (int s = grp; s < ns; s += groups) {
+        const float2 v = st[s];
+        const float f = __builtin_amdgcn_exp2f((v.x - mm) * a.sl2);
+        num += f * acc[(int64_t)s * D];
+        den += f * v.y;
     }
+    num_l[tid] = num;
+    if (d == 0) den_l[grp] = den;
+    __syncthreads();
+    if (grp > 0) return;
+    for (int g = 1; g < groups; ++g) num += num_l[g * D + d], den += den_l[g];
     Act<T>::store((T *)a.o + b * a.o_sb + h * a.o_sh + d, den == 0.f ? 0.f : num / den);
 }
 
@@ -329,15 +343,13 @@ static int pg_check(const char *fn, int64_t B, int64_t G, int64_t D, int64_t P, 
     return WALSH_OK;
 }
 
-// Keys per workgroup.  As many as leave eight workgroups per slot (two per
-// CU): chunks of a batch of unequal lengths then end together; few sequences
-// are cut finer, down to a block per wavefront.
+// Keys per workgroup: 1,024, so that a batch of unequal lengths ends together
+// (64 sequences of up to 4,096, 32 heads of 128 in bf16: 375 us with 512 or
+// 1,024, 384 with 2,048, 404 with 4,096); fewer where that would not fill the
+// chip (two workgroups per CU), down to a block per wavefront.
 static void pg_split(int64_t pairs, int64_t keys, int KB, int64_t *chunk, int64_t *ns) {
     const int64_t slots = 2 * (int64_t)device_info().cu_count, step = KB * kPgWaves;
-    int64_t c = ceil_div(pairs * keys, 8 * slots);
-    const int64_t fill = ceil_div(pairs * keys, slots);   // what one round of workgroups would take
-    if (c < 512) c = fill < 512 ? fill : 512;             // finer only to fill the chip
-    c = ceil_div(c, step) * step;
+    int64_t c = ceil_div(ceil_div(pairs * keys, slots), step) * step;   // what one round of workgroups would take
     *chunk = c < step ? step : c > kPgMaxChunk ? kPgMaxChunk : c;
     *ns = ceil_div(keys, *chunk);
     if (*ns < 1) *ns = 1;
@@ -396,14 +408,19 @@ WALSH_EXPORT int walsh_paged_decode_attention(const void *q, int64_t q_sb, int64
         return set_error(WALSH_EINVAL, "%s: workspace of %lld bytes, needs %lld (16-aligned)", fn, (long long)work_bytes,
                          (long long)(B * H * ns * (D + 2) * 4));
     const int64_t gy = G * ceil_div(H / G, 32);
-    if (gy > 65535 || B * H > INT32_MAX) return set_error(WALSH_ENOTSUP, "%s: H=%lld B=%lld", fn, (long long)H, (long long)B);
+    if (gy > 65535 || B * H > INT32_MAX || ns * gy > INT32_MAX) return set_error(WALSH_ENOTSUP, "%s: H=%lld B=%lld", fn, (long long)H, (long long)B);
     hipStream_t s = (hipStream_t)stream;
     attn_dispatch(dtype, D, [&](auto t, auto d) {
         typedef decltype(t) T;
         constexpr int DD = decltype(d)::value;
-        launch(paged_decode_kernel<T, DD>, dim3((unsigned)ns, (unsigned)gy, (unsigned)B), dim3(64 * kPgWaves),
+        launch(paged_decode_kernel<T, DD>, dim3((unsigned)(ns * gy), (unsigned)B), dim3(64 * kPgWaves),
                (uint32_t)PgCfg<T, DD>::LDS, s, a);
-        if (ns > 1) launch(paged_decode_join_kernel<T, DD>, dim3((unsigned)(B * H)), dim3(DD), 0, s, a);
+        // about four parts per group of threads, a wavefront at least
+        int64_t groups = ceil_div(ns, 4);
+        if (groups > 1024 / DD) groups = 1024 / DD;
+        if (groups * DD < 64) groups = 64 / DD;
+        if (ns > 1)
+            launch(paged_decode_join_kernel<T, DD>, dim3((unsigned)(B * H)), dim3((unsigned)(groups * DD)), 0, s, a);
     });
     return check_hip(hipGetLastError(), fn);
 }

@@ -58,6 +58,10 @@ __device__ __forceinline__ float dot(const Frag<uint16_t> &a, const Frag<uint16_
     return s;
 }
 
+// A value that is the same in every lane, as a scalar: quotients and loads
+// leave such values in vector registers, and their users with them.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // The value, newly computed as far as the compiler can see: what derives from
 // it is worked out again where it is used and holds no registers across a loop.
 __device__ __forceinline__ int fresh(int v) {
@@ -101,6 +105,11 @@ template <int BYTES> __device__ __forceinline__ void lds_load(u32x4 rsrc, uint32
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                      ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+}
+// 16 bytes per lane from each lane's own address, likewise.
+__device__ __forceinline__ void lds_gather(const void *p, uint32_t lds) {
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
 }
 // The LDS byte address of a shared variable, as a scalar.
 __device__ __forceinline__ uint32_t lds_addr(const void *p) {

@@ -55,10 +55,6 @@ struct WinArgs {
     int nb, nsb, nn, ns;  // key blocks; those with first tokens; splits of the others' and of their queries
 };
 
-// A value that is the same in every lane, as a scalar: quotients and loads
-// leave such values in vector registers, and their users with them.
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
 // Key positions of a sequence: all of Tk, or its length within it.
 __device__ __forceinline__ int win_len(const WinArgs &a, int b) {
     return a.lengths ? uniform(max(0, min(a.lengths[b], a.Tk))) : a.Tk;
