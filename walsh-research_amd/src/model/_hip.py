@@ -4,7 +4,6 @@ The library is loaded from ``walsh-research_amd/lib/`` (built in-tree by
 ``make -C walsh-research_amd``).  There is no fallback: if the library is
 missing or no GPU is present, every hot-path op raises.
 """
-import contextlib
 import ctypes
 import os
 import re
@@ -242,26 +241,29 @@ def call(name: str, *args, kernel: str = None, nbytes: int = 0, flops: int = 0) 
 
 def same_device(fn: str, first: torch.Tensor, *others) -> None:
     """All tensors (None excepted) on the device of ``first``."""
-    dev = first.device
+    dev = first.get_device()
     for t in others:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{fn}: tensors on {dev} and {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"{fn}: tensors on {first.device} and {t.device}")
 
 
-def device_of(device: torch.device):
-    """``device`` as the current one: what a launch on its streams, and the
-    library's own look at the device, need."""
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+def on_device(index: int, fn, *args):
+    """``fn(*args)`` with device ``index`` current: what a launch on its
+    streams, and the library's own look at the device, need."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
 
 
-def call_on(device: torch.device, name: str, *args, **kw) -> None:
-    """``call`` with the device's current stream as the last argument, on
-    whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream(device), **kw)
+def call_on(index: int, name: str, *args, **kw) -> None:
+    """``call`` with the current stream of device ``index`` as the last
+    argument, on whichever device is current."""
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index), **kw)
     else:
-        with torch.cuda.device(device):
-            call(name, *args, stream(device), **kw)
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index), **kw)
 
 
 def require_device(t: torch.Tensor, what: str = "tensor") -> None:

@@ -5,6 +5,8 @@ allocates its outputs with the torch caching allocator, validates shapes with
 the exception types the reference uses (AssertionError for shape contracts,
 TypeError/RuntimeError otherwise) and never falls back to a CPU path.
 """
+import functools
+
 import torch
 
 from . import _hip
@@ -877,6 +879,13 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
 ATTENTION_HEAD_DIMS = (16, 32, 64, 128)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace(name: str, device: int, *sizes) -> int:
+    """Workspace bytes that the library asks for on a device (a function of
+    the sizes alone)."""
+    return _hip.on_device(device, getattr(_hip.lib(), name), *sizes)
+
+
 def window_attention_supported(q: torch.Tensor) -> bool:
     """Whether window_attention takes a query of this device, type and head size."""
     return q.is_cuda and q.dtype in (torch.float32, torch.bfloat16) and q.shape[-1] in ATTENTION_HEAD_DIMS
@@ -931,7 +940,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     o = torch.empty(B, H, Tq, D, device=q.device, dtype=q.dtype)
     lse = torch.empty(B, H, Tq, device=q.device, dtype=torch.float32) if need_lse else None
     span = min(Tk, window + sinks) if window > 0 else Tk
-    _hip.call_on(q.device, "walsh_window_attention_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
+    _hip.call_on(q.get_device(), "walsh_window_attention_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
                  *k.stride()[:3], B, H, G, Tq, Tk, D, int(window), int(sinks), _hip.ptr(lengths), scale, o.data_ptr(),
                  *o.stride()[:3], _hip.ptr(lse), _hip.dtype_code(q.dtype),
                  kernel="window_fwd_kernel", nbytes=2 * B * D * (H * Tq + G * Tk) * q.element_size(),
@@ -961,11 +970,11 @@ def window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
         return tuple(torch.zeros(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
     dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
     dt = _hip.dtype_code(q.dtype)
-    with _hip.device_of(q.device):
-        nws = _hip.lib().walsh_window_attention_bwd_workspace_bytes(B, H, G, Tq, Tk, D, int(window), int(sinks), dt)
+    nws = _workspace("walsh_window_attention_bwd_workspace_bytes", q.get_device(), B, H, G, Tq, Tk, D, int(window),
+                     int(sinks), dt)
     ws = torch.empty(nws, device=q.device, dtype=torch.uint8)
     span = min(Tk, window + sinks) if window > 0 else Tk
-    _hip.call_on(q.device, "walsh_window_attention_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
+    _hip.call_on(q.get_device(), "walsh_window_attention_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
                  *k.stride()[:3], o.data_ptr(), *o.stride()[:3], go.data_ptr(), *go.stride()[:3], lse.data_ptr(), B, H, G,
                  Tq, Tk, D, int(window), int(sinks), _hip.ptr(lengths), scale, dq.data_ptr(), dk.data_ptr(),
                  dv.data_ptr(), dt, ws.data_ptr(), nws, kernel="window_bwd_kernels",
@@ -1015,11 +1024,10 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     lengths = lengths.contiguous()
     o = torch.empty(B, H, 1, D, device=q.device, dtype=q.dtype)
     N = page_table.shape[1]
-    with _hip.device_of(q.device):
-        nws = _hip.lib().walsh_paged_decode_workspace_bytes(B, H, G, N, page, D, int(window), int(sinks), dt)
+    nws = _workspace("walsh_paged_decode_workspace_bytes", q.get_device(), B, H, G, N, page, D, int(window), int(sinks), dt)
     ws = torch.empty(nws, device=q.device, dtype=torch.uint8) if nws else None
     span = min(N * page, window + sinks) if window > 0 else N * page
-    _hip.call_on(q.device, "walsh_paged_decode_attention", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(),
+    _hip.call_on(q.get_device(), "walsh_paged_decode_attention", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(),
                  v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.shape[0], page, page_table.data_ptr(),
                  page_table.stride(0), N, lengths.data_ptr(), B, H, G, D, int(window), int(sinks), scale, o.data_ptr(),
                  o.stride(0), o.stride(1), dt, _hip.ptr(ws), nws, kernel="paged_decode_kernel",
@@ -1049,7 +1057,7 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     if k.stride() != v.stride():
         k, v = k.contiguous(), v.contiguous()
     start = start.contiguous()
-    _hip.call_on(k.device, "walsh_paged_kv_write", k.data_ptr(), v.data_ptr(), *k.stride()[:3], B, T, G, D,
+    _hip.call_on(k.get_device(), "walsh_paged_kv_write", k.data_ptr(), v.data_ptr(), *k.stride()[:3], B, T, G, D,
                  k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.shape[0], k_pages.shape[2],
                  page_table.data_ptr(), page_table.stride(0), page_table.shape[1], start.data_ptr(), _hip.ptr(counts),
                  _hip.dtype_code(k.dtype), kernel="paged_write_kernel", nbytes=4 * k.numel() * k.element_size())
@@ -1096,7 +1104,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     mt, m0 = _row_setting("min_p", min_p, logits, torch.float32)
     u = u.contiguous()
     out = torch.empty(B, device=logits.device, dtype=torch.int64)
-    _hip.call_on(logits.device, "walsh_sample", logits.data_ptr(), logits.stride(0), B, V, u.data_ptr(), _hip.ptr(tt), t0,
+    _hip.call_on(logits.get_device(), "walsh_sample", logits.data_ptr(), logits.stride(0), B, V, u.data_ptr(), _hip.ptr(tt), t0,
                  _hip.ptr(kt), min(max(int(k0), 0), V), _hip.ptr(pt), p0, _hip.ptr(mt), m0, out.data_ptr(), dt,
                  kernel="sample_kernel", nbytes=B * V * logits.element_size(), flops=4 * B * V)
     return out
