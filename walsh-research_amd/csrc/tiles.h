@@ -40,6 +40,15 @@ __device__ __forceinline__ void pack(Frag<float> &f, const float *p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f.v[i] = p[i];
 }
+// What pack rounded away, as an operand of its own.
+__device__ __forceinline__ void pack_rest(Frag<uint16_t> &f, const float *p, const Frag<uint16_t> &packed) {
+    const u32x4 u = __builtin_bit_cast(u32x4, packed.v);
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = pack_bf16x2(p[2 * i] - __uint_as_float(u[i] << 16), p[2 * i + 1] - __uint_as_float(u[i] & 0xffff0000u));
+    f.v = __builtin_bit_cast(i16x8, r);
+}
 __device__ __forceinline__ Frag<uint16_t> load_frag(const uint16_t *p) { return {*(const i16x8 *)p}; }
 __device__ __forceinline__ Frag<float> load_frag(const float *p) {
     const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);

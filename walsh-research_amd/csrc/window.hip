@@ -28,7 +28,7 @@
 // float32.  bf16 tensors have their weights P and dS rounded to bf16 for the
 // second products (the matrix cores' operand type; relative 2^-9 each, the
 // size of the inputs' own rounding); the sum of weights that normalises a row
-// takes them unrounded.
+// takes them unrounded, and dQ at D <= 32 dS in two parts.
 #include "tiles.h"
 
 namespace walsh {
@@ -408,8 +408,19 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             for (int t = 0; t < 2; ++t) {
                 Frag<T> f;
                 pack(f, ds + 8 * t);
+                if constexpr (sizeof(T) == 2 && ND == 1) {
+                    // one product a block: dS goes in two parts, its rounding
+                    // with it (relative error of dQ at D = 16, its own
+                    // rounding in it: 2.6e-3 without, 1.8e-3 so)
+                    const Frag<T> kc = L::col(kl, 32 * j + 16 * t, 0, lane);
+                    Frag<T> rest;
+                    pack_rest(rest, ds + 8 * t, f);
+                    mma(acc[0], kc, f);
+                    mma(acc[0], kc, rest);
+                } else {
 #pragma unroll
-                for (int c = 0; c < ND; ++c) mma(acc[c], L::col(kl, 32 * j + 16 * t, c, lane), f);
+                    for (int c = 0; c < ND; ++c) mma(acc[c], L::col(kl, 32 * j + 16 * t, c, lane), f);
+                }
             }
         }
     }
