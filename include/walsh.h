@@ -467,7 +467,8 @@ int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_
  * table[b*table_sb + j / page] (int32); k_pages and v_pages hold n_pages pages
  * [G][page][D], element (p, g, r, d) at p*sp + g*sg + r*sr + d of both.  page is
  * a power of two from 16, or any size where pages_per_seq is 1; n_pages,
- * strides multiples of 8, bases 16-byte aligned; pages_per_seq * page <= 2^30.
+ * strides multiples of 8, bases 16-byte aligned; pages_per_seq * page <= 2^30;
+ * B <= 65535.
  *
  * walsh_paged_decode_attention: one new token per sequence, the last of its
  *   lengths[b] rows (already written): q (b, h, d) at b*q_sb + h*q_sh + d, o
@@ -497,7 +498,7 @@ int walsh_paged_kv_write(const void *k, const void *v, int64_t sb, int64_t st, i
  * The reference samples by a sort and torch.multinomial on the softmax
  * (src/model/mhc.py:754-772: temperature and top-k); here the random number is
  * an input.  walsh_sample: out[b] = the token of row b of logits [B][V] (row
- * stride ld, float32 or bf16, V <= 2^20) that u[b] in [0, 1) picks:
+ * stride ld, float32 or bf16, V < 2^20) that u[b] in [0, 1) picks:
  *   w = exp((l - max l) / temperature);  temperature <= 0: the largest logit
  *   top_k    the k largest logits stay (of equal ones the lowest indexes);
  *            k <= 0 or >= V: all

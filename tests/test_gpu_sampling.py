@@ -178,4 +178,8 @@ def test_sample_refusals():
         kernels.sample(z, u.cpu())
     with pytest.raises(_hip.WalshHipError, match="V="):
         kernels.sample(z[:, :0], u)
+    with pytest.raises(_hip.WalshHipError, match="V="):
+        kernels.sample(torch.zeros(2, 1 << 20, device="cuda"), u)
+    # the most that are taken: equal ones, whose sum stays within 64 bits
+    assert kernels.sample(torch.zeros(1, (1 << 20) - 1, device="cuda"), u[:1] + 0.5).item() == ((1 << 20) - 1) // 2
     assert kernels.sample(z[:0], u[:0]).shape == (0,)

@@ -273,7 +273,30 @@ def test_paged_cache_refusals_in_a_model():
             model.generate(idx, 2, kv_cache=kv, lengths=[6, 1])
         with pytest.raises(ValueError, match="kv_cache"):
             model.generate(idx, 2, lengths=[5, 1])
+        with pytest.raises(ValueError, match="positions"):
+            model.generate(idx, 125, kv_cache=kv)
         kv.reserve(1)
         kv.increment()
         with pytest.raises(ValueError, match="not empty"):
             model.generate(idx, 2, kv_cache=kv)
+    kv.reset()
+    kv.reserve(5)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        model(idx, kv_cache=kv)
+
+
+def test_generate_survives_logits_that_are_no_numbers():
+    """Such a row has no token; what follows it is some token of the
+    vocabulary, and the other rows are as they were."""
+    model = make()
+    idx = tokens(2, 6)
+    want = model.generate(idx, 4, temperature=0.0, top_p=1.0)
+    with torch.no_grad():
+        old = model.output.weight[int(idx[1, -1])].clone()
+        bad = idx.clone()
+        bad[1, :] = 999
+        model.output.weight[999] = float("nan")
+        model.invalidate_weight_caches()
+        got = model.generate(bad, 4, temperature=0.0, top_p=1.0)
+        assert int(got.min()) >= 0 and int(got.max()) < 1000
+        assert old.isfinite().all() and want.shape == got.shape

@@ -134,6 +134,19 @@ def test_window_attention_layouts_and_partial_gradients():
     want = window_attention(base, k, v, 20, 2)
     assert torch.equal(window_attention(odd, k, v, 20, 2), want)
     assert torch.equal(window_attention(base, k, v.contiguous(), 20, 2), want)
+    # one head's and one sequence's keys for all (expanded), and rows far apart
+    ke, ve = k[:1, :1].expand(B, G, T, D), v[:1, :1].expand(B, G, T, D)
+    assert torch.equal(window_attention(base, ke, ve, 20, 2), window_attention(base, ke.contiguous(), ve.contiguous(), 20, 2))
+    kr = k[:1, :1].detach().clone().requires_grad_(True)
+    (dk,) = torch.autograd.grad(window_attention(base, kr.expand(B, G, T, D), ve, 20, 2).sum(), (kr,))
+    kx = kr.detach().expand(B, G, T, D).contiguous().requires_grad_(True)
+    (dx,) = torch.autograd.grad(window_attention(base, kx, ve.contiguous(), 20, 2).sum(), (kx,))
+    assert torch.equal(dk, dx.sum((0, 1), keepdim=True))
+    far = torch.zeros(T, (1 << 22) + 8, dtype=torch.bfloat16, device="cuda")
+    far = far.as_strided((1, 1, T, D), (0, 0, (1 << 22) + 8, 1))
+    far.copy_(k[:1, :1])
+    assert torch.equal(window_attention(base[:1, :2], far, v[:1, :1], 20, 2),
+                       window_attention(base[:1, :2], k[:1, :1], v[:1, :1], 20, 2))
     vr = v.detach().requires_grad_(True)
     o = window_attention(base, k, vr, 20, 2)
     (dv,) = torch.autograd.grad(o.sum(), (vr,))

@@ -550,8 +550,8 @@ WALSH_EXPORT int walsh_sample(const void *logits, int64_t ld, int64_t B, int64_t
                               const float *top_p, float top_p0, const float *min_p, float min_p0, int64_t *out, int dtype,
                               void *stream) {
     const char *fn = "walsh_sample";
-    if (B < 0 || B > INT32_MAX || V < 1 || V > (1 << 20))
-        return set_error(WALSH_EINVAL, "%s: bad shape B=%lld V=%lld (1 to 2^20)", fn, (long long)B, (long long)V);
+    if (B < 0 || B > INT32_MAX || V < 1 || V >= (1 << 20))   // (2^20 weights of 2^44 would pass 64 bits)
+        return set_error(WALSH_EINVAL, "%s: bad shape B=%lld V=%lld (1 to 2^20 - 1)", fn, (long long)B, (long long)V);
     if (dtype != WALSH_F32 && dtype != WALSH_BF16) return set_error(WALSH_ENOTSUP, "%s: dtype %d", fn, dtype);
     if (B == 0) return WALSH_OK;
     if (!logits || !u || !out) return set_error(WALSH_EINVAL, "%s: null pointer", fn);

@@ -5,6 +5,7 @@ The reference's attention is causal over everything (chassis.py:441-478) and
 its cache one dense tensor (:262-330); here a query may see the last
 ``window`` keys and the first ``sinks`` ones, and the cache may lie in pages.
 """
+import numbers
 from typing import List, Sequence, Union
 
 import torch
@@ -107,7 +108,7 @@ class PagedKVCache:
         """Room for the next ``counts`` tokens (one number, or one per
         sequence) of the coming forward; nothing is taken if any does not
         fit."""
-        counts = [int(counts)] * self.batch if isinstance(counts, int) else [int(c) for c in counts]
+        counts = [int(counts)] * self.batch if isinstance(counts, numbers.Integral) else [int(c) for c in counts]
         if len(counts) != self.batch or min(counts) < 0:
             raise ValueError(f"PagedKVCache: counts for {self.batch} sequences, got {counts}")
         ends = [n + c for n, c in zip(self.seq_lens, counts)]

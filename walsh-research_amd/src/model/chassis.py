@@ -371,6 +371,8 @@ class CausalSelfAttention(nn.Module):
         else:
             q, k, v, in_cache = self._qkv(x, freqs_cis, kv_cache, layer_idx)
         if paged:
+            if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+                raise RuntimeError("a paged cache holds no gradients: run the model under torch.no_grad()")
             kv_cache.write(layer_idx, k, v)
             past = 0 if T == 1 else kv_cache.cached_len
             if past > 0:

@@ -893,10 +893,11 @@ def window_attention_supported(q: torch.Tensor) -> bool:
 
 def _attn_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [B, heads, T, D] as the attention kernels read it: unit inner
-    stride, the others multiples of 8, rows that do not overlap, 16-byte
-    aligned; itself or a copy."""
+    stride, the others multiples of 8, rows that do not overlap and lie at
+    most 2^22 elements apart, 16-byte aligned; itself or a copy."""
     sb, sh, st, sd = t.stride()
-    if sd == 1 and not (sb | sh | st) & 7 and (st >= t.shape[3] or t.shape[2] == 1) and not t.data_ptr() & 15:
+    if (sd == 1 and not (sb | sh | st) & 7 and (t.shape[3] <= st or t.shape[2] == 1) and st <= 1 << 22
+            and not t.data_ptr() & 15):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

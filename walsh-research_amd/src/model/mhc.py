@@ -557,8 +557,12 @@ class mHCWalsh(nn.Module):
             raise ValueError("generate: prompts of unequal lengths need a kv_cache")
         if lengths is not None and (len(lengths) != idx.size(0) or min(lengths) < 1 or max(lengths) > idx.size(1)):
             raise ValueError(f"generate: lengths {list(lengths)} of prompts {tuple(idx.shape)}")
-        if kv_cache is not None and any(kv_cache.seq_lens):
-            raise ValueError("generate: the kv_cache is not empty")
+        if kv_cache is not None:
+            if any(kv_cache.seq_lens):
+                raise ValueError("generate: the kv_cache is not empty")
+            if max(lengths or [idx.size(1)]) + max_new_tokens - 1 > kv_cache.max_seq_len:
+                raise ValueError(f"generate: {max_new_tokens} tokens behind {idx.size(1)} of at most "
+                                 f"{kv_cache.max_seq_len} positions")
         for step in range(max_new_tokens):
             if kv_cache is None:
                 logits, _ = self(idx[:, -self.config.block_size:])
@@ -572,5 +576,6 @@ class mHCWalsh(nn.Module):
                 kv_cache.increment()
             token = kernels.sample(logits[:, -1, :], torch.rand(idx.size(0), device=idx.device), temperature, top_k or 0,
                                    1.0 if top_p is None else top_p, 0.0 if min_p is None else min_p)
+            token.clamp_(min=0)     # a row of logits that are no numbers has no token: an index that is one
             idx = torch.cat((idx, token[:, None]), dim=1)
         return idx
