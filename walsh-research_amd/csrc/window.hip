@@ -628,24 +628,32 @@ template <typename T, int D> __global__ __launch_bounds__(256) void window_bwd_s
 }
 
 // ---------------------------------------------------------------- host
-// Splits of the key blocks' queries: blocks of first tokens are seen from
-// every later tile, the others from a window's; both are cut into splits of
-// about one window's tiles (or of what fills the chip, two workgroups per CU).
+// Splits of the key blocks' queries.  A split costs its partial sums, about
+// five tiles' time written and read back, so blocks of a window, all of a
+// length, are split only where they do not fill the chip (two workgroups per
+// CU).  Without a window the first block is seen by every query and the last
+// by few: a split then takes at most three quarters of an even part of the
+// whole, or 24 tiles (32 heads on 8 of 64, 2 x 4,096 causal: dK, dV 665 us in
+// one piece, 387 in three).  Blocks of first tokens, which every later tile
+// sees, are split into parts as long as the others'.
 static void win_splits(WinArgs &a, int QC) {
     a.nb = (int)ceil_div(a.Tk, kWinQ);
     a.nsb = a.W > 0 && a.W < a.Tk ? (int)ceil_div(a.S < a.Tk ? a.S : a.Tk, kWinQ) : 0;
     const int64_t R = a.H / a.G, full = R * (ceil_div(a.Tk, QC) + 1);
     int64_t near = a.W > 0 ? R * (ceil_div((int64_t)a.W + kWinQ, QC) + 1) : full;
     if (near > full) near = full;
-    const int64_t groups = (int64_t)a.B * a.G * a.nb, fill = 2 * (int64_t)device_info().cu_count;
-    int64_t nn = groups >= fill ? 1 : ceil_div(fill, groups);
+    const int64_t blocks = (int64_t)a.B * a.G * a.nb, slots = 2 * (int64_t)device_info().cu_count;
+    int64_t nn = blocks < slots ? ceil_div(slots, blocks) : 1;
     if (nn > ceil_div(near, 4)) nn = ceil_div(near, 4);   // four tiles at least
+    if (a.W <= 0) {
+        int64_t share = ceil_div(blocks * full / 2 * 3, slots * 4);
+        if (share < 24) share = 24;
+        if (nn < ceil_div(full, share)) nn = ceil_div(full, share);
+    }
     if (nn > 64) nn = 64;
-    const int64_t share = ceil_div(near, nn);
-    int64_t ns = ceil_div(full, share);
-    if (ns > 256) ns = 256;
+    const int64_t ns = ceil_div(full, ceil_div(near, nn));
     a.nn = (int)nn;
-    a.ns = a.nsb ? (int)ns : 1;
+    a.ns = a.nsb ? (int)(ns > 256 ? 256 : ns) : 1;
 }
 
 static int64_t win_part_slots(const WinArgs &a) {
