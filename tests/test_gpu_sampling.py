@@ -125,6 +125,37 @@ def test_sample_odd_values():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [40, 3000, 20000, 60000])
+def test_sample_more_asked_for_than_there_are_numbers(V):
+    """top-k above the number of logits that are numbers: NaN counts as -inf,
+    so the others stay, all of them."""
+    z, u = rows(4, V, torch.float32, V)
+    keep = torch.rand(4, V, generator=torch.Generator().manual_seed(V)) < 0.2
+    keep[:, 7] = True
+    z[~keep] = float("nan")
+    for args in ((1.0, V // 2, 1.0, 0.0), (0.8, V // 2, 0.9, 0.0), (1.0, V - 1, 0.95, 0.01), (1.0, 0, 0.9, 0.0)):
+        # (how many rows lie too close to a border depends on the rows and settings alone)
+        print(args, check(z, u, *args, run(z, u, *args)), "undecided", flush=True)
+    assert torch.equal(run(z, u, 1.0, V // 2), run(z, u))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sample_masks_of_the_lowest_value_at_any_temperature(dtype):
+    """Logits masked with the type's lowest value have no weight, at
+    temperatures where their distance passes float32, too."""
+    V = 2000
+    z, u = rows(3, V, dtype, 5)
+    z[:, ::3] = torch.finfo(dtype).min
+    for T in (1.0, 1e-3, 1e-10, 3e-30, 1e-38):
+        for k, p, m in ((0, 1.0, 0.0), (300, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.02)):
+            got = run(z, u, T, k, p, m)
+            print(T, k, p, m, check(z, u, T, k, p, m, got), "undecided", flush=True)
+            if T < 1e-6:
+                assert torch.equal(z.gather(1, got[:, None])[:, 0], z.amax(-1))
+
+
+@pytest.mark.gpu
 def test_sample_strides_streams_and_graph():
     from src.model import kernels
     z, u = rows(4, 5000, torch.bfloat16, 3)

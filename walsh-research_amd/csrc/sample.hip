@@ -108,7 +108,8 @@ struct SmWeights {
     float m, chi, clo;     // the maximum (finite); log2(e) / T in two parts
     __device__ __forceinline__ float of(float x) const {            // 0 .. 1
         const float s = x - m;
-        return x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(s, chi, s * clo));
+        // (far below what counts the two parts might pass float32 with opposite signs)
+        return s * chi > -150.f ? __builtin_amdgcn_exp2f(fmaf(s, chi, s * clo)) : 0.f;
     }
     // of() in units of 2^-44, by the addition of 1.5 * 2^8: 44 fraction bits are left below it
     static __device__ __forceinline__ u64 fixed(float w) {
@@ -133,7 +134,7 @@ struct SmWeights {
 
 // The tokens that a wavefront walks, 64 at a time and in index order.
 // each(f, mark): f(step, there, value) with every lane, mark(steps done) after
-// every kSmStep steps and the last.  A value that is no number is not there.
+// every kSmStep steps and the last.  What is not there has no number as value.
 template <typename T, int U> struct SmRow {                          // U: loads on their way together
     const T *p;
     int base, n, end;      // first index of the lane, steps, past the last index
@@ -151,7 +152,10 @@ template <typename T, int U> struct SmRow {                          // U: loads
         asm volatile("" : "+v"(at));
         return at + 64 * i;
     }
-    __device__ __forceinline__ float value(float v) const { return inf && v == v ? (v == INFINITY ? 0.f : -INFINITY) : v; }
+    __device__ __forceinline__ float value(float v) const {          // what is no number counts as -inf
+        v = fmaxf(v, -INFINITY);
+        return inf ? (v == INFINITY ? 0.f : -INFINITY) : v;
+    }
     // some element of the row, whether or not step i has one: no branch around the load
     __device__ __forceinline__ float some(int i) const { return Act<T>::load(p + max(0, min(index(i), end - 1))); }
     template <typename F, typename M> __device__ __forceinline__ void each(int i0, int i1, F f, M mark) const {
@@ -181,7 +185,7 @@ struct SmKeptRow {
             const bool there = lane + 64 * i < end;
             f(i, there, there ? sm_value(p[lane + 64 * i].x) : NAN);
         }
-        mark(i1);
+        if (i1 > i0) mark(i1);
     }
 };
 
@@ -456,7 +460,7 @@ template <typename T, int NPT> __global__ __launch_bounds__(kSmThreads) void sam
         asm volatile("" : "+v"(base));                              // (the addresses are not kept for this)
 #pragma unroll
         for (int i = 0; i < NPT; ++i) {
-            v[i] = i < row.n && base + 64 * i < row.end ? v[i] : NAN;
+            v[i] = i < row.n && base + 64 * i < row.end ? row.value(v[i]) : NAN;
             m = fmaxf(m, v[i]);
             if (i % kSmStep == kSmStep - 1) __builtin_amdgcn_sched_barrier(0);
         }
@@ -479,7 +483,7 @@ template <typename T, int NPT> __global__ __launch_bounds__(kSmThreads) void sam
         m = 0.f;
         if constexpr (NPT > 0) {
 #pragma unroll
-            for (int i = 0; i < NPT; ++i) v[i] = row.value(v[i]);
+            for (int i = 0; i < NPT; ++i) v[i] = v[i] == v[i] ? row.value(v[i]) : v[i];
         }
     }
     const bool greedy = !(temp > 0.f);
@@ -550,8 +554,8 @@ WALSH_EXPORT int walsh_sample(const void *logits, int64_t ld, int64_t B, int64_t
                               const float *top_p, float top_p0, const float *min_p, float min_p0, int64_t *out, int dtype,
                               void *stream) {
     const char *fn = "walsh_sample";
-    if (B < 0 || B > INT32_MAX || V < 1 || V >= (1 << 20))   // (2^20 weights of 2^44 would pass 64 bits)
-        return set_error(WALSH_EINVAL, "%s: bad shape B=%lld V=%lld (1 to 2^20 - 1)", fn, (long long)B, (long long)V);
+    if (B < 0 || B >= (1 << 22) || V < 1 || V >= (1 << 20))   // (2^20 weights of 2^44 would pass 64 bits)
+        return set_error(WALSH_EINVAL, "%s: bad shape B=%lld (below 2^22) V=%lld (1 to 2^20 - 1)", fn, (long long)B, (long long)V);
     if (dtype != WALSH_F32 && dtype != WALSH_BF16) return set_error(WALSH_ENOTSUP, "%s: dtype %d", fn, dtype);
     if (B == 0) return WALSH_OK;
     if (!logits || !u || !out) return set_error(WALSH_EINVAL, "%s: null pointer", fn);

@@ -1085,7 +1085,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     ``min_p`` of the largest probability; the first token, in index order,
     whose running probability exceeds u.  ``temperature`` <= 0 takes the
     largest logit.  Each setting is a number or a tensor [B] (float32, top_k
-    int32).  A row with no finite logit gives -1."""
+    int32).  NaN counts as -inf, and a row of nothing else gives -1; infinite
+    logits share all the weight."""
     _hip.require_device(logits, "logits")
     assert logits.dim() == 2 and u.shape == logits.shape[:1], "sample: logits [B, V] and u [B]"
     if u.dtype != torch.float32:
