@@ -13,6 +13,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import kernels
+from .attention import PagedKVCache
 from .linear import FewRowsLinear
 from ._common import WeightCache, act_dtype, cached_linear, invalidate_weight_caches
 
@@ -555,9 +556,13 @@ class mHCWalsh(nn.Module):
             return idx
         if kv_cache is None and lengths is not None:
             raise ValueError("generate: prompts of unequal lengths need a kv_cache")
-        if lengths is not None and (len(lengths) != idx.size(0) or min(lengths) < 1 or max(lengths) > idx.size(1)):
-            raise ValueError(f"generate: lengths {list(lengths)} of prompts {tuple(idx.shape)}")
+        if lengths is not None:
+            lengths = [int(n) for n in lengths]
+            if len(lengths) != idx.size(0) or min(lengths) < 1 or max(lengths) > idx.size(1):
+                raise ValueError(f"generate: lengths {lengths} of prompts {tuple(idx.shape)}")
         if kv_cache is not None:
+            if not isinstance(kv_cache, PagedKVCache):
+                raise TypeError("generate: kv_cache is a PagedKVCache")
             if any(kv_cache.seq_lens):
                 raise ValueError("generate: the kv_cache is not empty")
             if max(lengths or [idx.size(1)]) + max_new_tokens - 1 > kv_cache.max_seq_len:
