@@ -441,8 +441,11 @@ int walsh_prefill_attention(const void *q, int64_t q_sb, int64_t q_sh, int64_t q
  * Rows that see nothing: o zeros, lse -inf.  dtype WALSH_F32 or WALSH_BF16;
  * D in {16, 32, 64, 128}; element (b, h, t, d) of a tensor at
  * b*sb + h*sh + t*st + d, strides multiples of 8, pointers 16-byte aligned;
- * 0 < scale <= 1e6.  Scores, softmax and sums in float32; bf16 rounds the
- * weights (and their gradients) to bf16 for the products with v (k and q).
+ * 0 < scale <= 1e6; B * H * ceil(max(Tq, Tk) / 128) < 2^24 - 7.  Scores,
+ * softmax and sums in float32 (a visible q k^T below -1e30 has no weight);
+ * bf16 rounds the weights (and their gradients) to bf16 for the products with
+ * v (k and q).  k and v within the lengths must be finite: what the mask hides
+ * from a row enters its sums with a weight of 0.
  *
  * walsh_window_attention_fwd: lse [B, H, Tq] or null.
  * walsh_window_attention_bwd: go the gradient of o, in o's dtype; dq dense
@@ -468,7 +471,7 @@ int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_
  * [G][page][D], element (p, g, r, d) at p*sp + g*sg + r*sr + d of both.  page is
  * a power of two from 16, or any size where pages_per_seq is 1; n_pages,
  * strides multiples of 8, bases 16-byte aligned; pages_per_seq * page <= 2^30;
- * B <= 65535.
+ * B <= 65535, B * H < 2^22.
  *
  * walsh_paged_decode_attention: one new token per sequence, the last of its
  *   lengths[b] rows (already written): q (b, h, d) at b*q_sb + h*q_sh + d, o
@@ -498,7 +501,7 @@ int walsh_paged_kv_write(const void *k, const void *v, int64_t sb, int64_t st, i
  * The reference samples by a sort and torch.multinomial on the softmax
  * (src/model/mhc.py:754-772: temperature and top-k); here the random number is
  * an input.  walsh_sample: out[b] = the token of row b of logits [B][V] (row
- * stride ld, float32 or bf16, V < 2^20) that u[b] in [0, 1) picks:
+ * stride ld, float32 or bf16, B < 2^22, V < 2^20) that u[b] in [0, 1) picks:
  *   w = exp((l - max l) / temperature);  temperature <= 0: the largest logit
  *   top_k    the k largest logits stay (of equal ones the lowest indexes);
  *            k <= 0 or >= V: all
@@ -507,8 +510,8 @@ int walsh_paged_kv_write(const void *k, const void *v, int64_t sb, int64_t st, i
  *   min_p    of these, those with w >= min_p stay
  *   out      the first index whose running sum of what stays, in index order,
  *            exceeds u times the whole sum
- * NaN logits count as -inf; a row of nothing else, or one that min_p leaves
- * empty, gives -1.  Each of temperature, top_k, top_p, min_p is an array [B] on
+ * NaN logits count as -inf; a row of nothing but -inf, or one that min_p
+ * leaves empty, gives -1; infinite logits share all the weight.  Each of temperature, top_k, top_p, min_p is an array [B] on
  * the device, or null and the value behind it for every row. */
 int walsh_sample(const void *logits, int64_t ld, int64_t B, int64_t V, const float *u, const float *temperature,
                  float temperature0, const int *top_k, int top_k0, const float *top_p, float top_p0, const float *min_p,

@@ -248,7 +248,8 @@ def test_paged_entry_points_check_before_they_launch():
                                               G, D, 0, 0, scale, p, 256, 64, dtype, p, work, None)
     for kw, rc in ((dict(page=48), -2), (dict(page=8), -2), (dict(D=24), -2), (dict(H=3), -1), (dict(P=0), -1),
                    (dict(sr=60), -2), (dict(q=p + 2), -2), (dict(scale=0.0), -1), (dict(dtype=7), -2),
-                   (dict(N=1 << 24, page=1 << 10), -1), (dict(N=4096, work=16), -1), (dict(B=-1), -1)):
+                   (dict(N=1 << 24, page=1 << 10), -1), (dict(N=4096, work=16), -1), (dict(B=-1), -1),
+                   (dict(B=65535, H=128), -2)):
         assert call(**kw) == rc, kw
         assert L.walsh_last_error()
     assert call(B=0) == 0

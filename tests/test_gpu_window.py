@@ -235,6 +235,35 @@ def test_window_attention_refusals():
         kernels.window_attention(q, k, k, 4)
 
 
+def test_window_entry_points_check_before_they_launch():
+    """Sizes that a launch does not hold, strides and workspaces are refused
+    by the library itself (no pointer is followed)."""
+    import os
+    from src.model import _hip
+    if not os.path.exists(_hip.LIB_PATH):
+        pytest.skip("library not built")
+    L = _hip.lib()
+    p = 4096
+
+    def fwd(B=1, H=2, G=1, Tq=8, Tk=8, D=64, st=64, q=p, scale=0.1, dtype=1):
+        return L.walsh_window_attention_fwd(q, 1 << 20, 1 << 16, st, p, p, 1 << 20, 1 << 16, 64, B, H, G, Tq, Tk, D, 4,
+                                            1, None, scale, p, 1 << 20, 1 << 16, 64, p, dtype, None)
+
+    def bwd(Tq=8, Tk=8, work=1 << 30, dq=p):
+        return L.walsh_window_attention_bwd(p, 1 << 20, 1 << 16, 64, p, p, 1 << 20, 1 << 16, 64, p, 1 << 20, 1 << 16, 64,
+                                            p, 1 << 20, 1 << 16, 64, p, 1, 2, 1, Tq, Tk, 64, 4, 1, None, 0.1, dq, p, p,
+                                            1, p, work, None)
+    for kw, rc in ((dict(H=3, G=2), -1), (dict(Tq=(1 << 24) + 1), -1), (dict(D=24), -2), (dict(st=60), -2),
+                   (dict(st=1 << 23), -2), (dict(q=p + 8), -2), (dict(scale=0.0), -1), (dict(dtype=5), -2),
+                   (dict(B=1 << 14, H=1 << 10, Tq=128), -2), (dict(B=1 << 60, H=1 << 30), -2),
+                   (dict(B=4, H=32, Tq=1 << 24, Tk=1 << 24), -2)):
+        assert fwd(**kw) == rc, kw
+        assert L.walsh_last_error()
+    assert fwd(B=0) == fwd(Tq=0) == 0
+    assert bwd(Tq=0) == bwd(Tk=0) == bwd(work=16) == -1
+    assert bwd(dq=p + 4) == -2
+
+
 @pytest.mark.gpu
 def test_window_attention_refusals_on_the_gpu():
     from src.model import _hip, kernels

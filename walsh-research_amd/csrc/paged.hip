@@ -239,7 +239,7 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
         }
         if (bad) ll = NAN;                        // a page or length outside the pool: not a number, never a stale value
         if (a.ns == 1) {
-            store4((T *)a.o + b * a.o_sb + (h0 + r) * a.o_sh + d, bad ? v * ll : ll > 0.f ? v * (1.f / ll) : v * 0.f);
+            store4((T *)a.o + b * a.o_sb + (h0 + r) * a.o_sh + d, ks.n > 0 || bad ? v * (1.f / ll) : f32x4{0.f, 0.f, 0.f, 0.f});
         } else {
             const int64_t at = ((int64_t)b * a.H + h0 + r) * a.ns + s;
             store4(a.part + at * D + d, v);
@@ -278,7 +278,7 @@ template <typename T, int D> __global__ __launch_bounds__(1024) void paged_decod
     __syncthreads();
     if (grp > 0) return;
     for (int g = 1; g < groups; ++g) num += num_l[g * D + d], den += den_l[g];
-    Act<T>::store((T *)a.o + b * a.o_sb + h * a.o_sh + d, den == 0.f ? 0.f : num / den);
+    Act<T>::store((T *)a.o + b * a.o_sb + h * a.o_sh + d, ks.n > 0 || ks.bad ? num / den : 0.f);
 }
 
 // ---------------------------------------------------------------- write
@@ -408,7 +408,8 @@ WALSH_EXPORT int walsh_paged_decode_attention(const void *q, int64_t q_sb, int64
         return set_error(WALSH_EINVAL, "%s: workspace of %lld bytes, needs %lld (16-aligned)", fn, (long long)work_bytes,
                          (long long)(B * H * ns * (D + 2) * 4));
     const int64_t gy = G * ceil_div(H / G, 32);
-    if (gy > 65535 || B * H > INT32_MAX || ns * gy > INT32_MAX) return set_error(WALSH_ENOTSUP, "%s: H=%lld B=%lld", fn, (long long)H, (long long)B);
+    // (a launch counts its threads along an axis in 32 bits)
+    if (B * H >= (1 << 22) || ns * gy >= (1 << 24)) return set_error(WALSH_ENOTSUP, "%s: H=%lld B=%lld", fn, (long long)H, (long long)B);
     hipStream_t s = (hipStream_t)stream;
     attn_dispatch(dtype, D, [&](auto t, auto d) {
         typedef decltype(t) T;

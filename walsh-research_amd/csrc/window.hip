@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     }
     l = half_sum(l);
     if (qi >= a.Tq) return;
-    const float inv = live && l > 0.f ? 1.f / l : 0.f;
+    const float inv = 1.f / l;                    // (no row that sees a key has none but infinite scores' l = 0)
     T *op = (T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)qi * a.so.st;
 #pragma unroll
     for (int c = 0; c < ND; ++c)
@@ -670,7 +670,8 @@ static int win_check(const char *fn, const WinArgs &a, int64_t B, int64_t H, int
     if (dtype != WALSH_F32 && dtype != WALSH_BF16) return set_error(WALSH_ENOTSUP, "%s: dtype %d", fn, dtype);
     if (!(a.scale > 0.f) || a.scale > 1e6f)
         return set_error(WALSH_EINVAL, "%s: the scale must be positive and at most 1e6", fn);
-    if (B * H * ceil_div(Tq > Tk ? Tq : Tk, 32) > (1ll << 28))
+    // work items of 128 positions, whose threads a launch counts in 32 bits
+    if (B > (1 << 24) || H > (1 << 24) || B * H > ((1 << 24) - 8) / ceil_div(Tq > Tk ? Tq : Tk > 0 ? Tk : 1, kWinQ))
         return set_error(WALSH_ENOTSUP, "%s: B=%lld H=%lld T=%lld exceed the grid", fn, (long long)B, (long long)H,
                          (long long)(Tq > Tk ? Tq : Tk));
     return WALSH_OK;
@@ -787,7 +788,7 @@ WALSH_EXPORT int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t
     hipStream_t s = (hipStream_t)stream;
     const int64_t nq = ceil_div(Tq, kWinQ) * H * B;
     const int64_t nk = ((int64_t)a.nsb * a.ns + (int64_t)(a.nb - a.nsb) * a.nn) * G * B;
-    if (nk > (1ll << 30)) return set_error(WALSH_ENOTSUP, "%s: %lld work items", fn, (long long)nk);
+    if (nk >= (1ll << 24) - 8) return set_error(WALSH_ENOTSUP, "%s: %lld work items", fn, (long long)nk);
     attn_dispatch(dtype, D, [&](auto t, auto d) {
         typedef decltype(t) T;
         constexpr int DD = decltype(d)::value;
