@@ -84,6 +84,34 @@ def test_paged_decode_against_oracle(H, G, D, page, lengths, W, S, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,G,D,page,lengths,W,S", [
+    # 3, 4, 5 and 8 query heads on a key head, lengths about a wavefront's step and a chunk
+    (9, 3, 128, 16, [1, 7, 8, 9, 33], 0, 0), (6, 2, 16, 32, [63, 64, 65, 1023, 1025], 0, 0),
+    (8, 2, 128, 64, [1024, 2049], 0, 0), (4, 1, 16, 64, [5000, 3], 0, 0), (4, 1, 64, 16, [90, 1700], 300, 9),
+    (12, 3, 32, 16, [257, 0, 31], 0, 0), (5, 1, 64, 16, [400, 2], 0, 0), (16, 2, 128, 64, [3000, 64], 1000, 70),
+])
+def test_paged_decode_shared_heads(H, G, D, page, lengths, W, S, dtype):
+    q, kp, vp, table, n = make(len(lengths), H, G, D, page, lengths, dtype, D + H)
+    check(decode(q, kp, vp, table, n, W, S), q, kp, vp, table, n, W, S)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,n", [(1, 40), (5, 40), (1, 3000), (5, 3000)])
+def test_paged_decode_of_infinite_scores_is_no_number(H, n, dtype):
+    """Scores of -inf alone leave no weight, as in the formula: not a number,
+    and not the zeros of an empty sequence; other sequences are as without."""
+    q, kp, vp, table, lens = make(2, H, 1, 64, 16, [n, 50], dtype, 5)
+    want = decode(q, kp, vp, table, lens)
+    mine = table[0][table[0] >= 0].long()
+    q[0] = 1.0
+    kp[mine] = float("-inf")
+    got = decode(q, kp, vp, table, lens)
+    assert got[0].isnan().all() and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
 def test_paged_decode_takes_a_dense_cache_as_one_page_per_sequence():
     """[B, H, Lmax, D] storage of any length is B pages; the result equals the
     dense decode attention's up to the order of sums."""

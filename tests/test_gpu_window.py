@@ -200,6 +200,23 @@ def test_window_attention_rows_before_the_first_key_may_hold_anything():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B", [1, 80])
+def test_window_attention_of_infinite_scores_is_no_number(B, dtype):
+    """Rows that see scores of -inf alone have no weights: not a number, in
+    few and in many work items; rows that see others are as without."""
+    from src.model.attention import window_attention
+    q, k, v, _ = make(B, 4, 2, 40, 40, 32, dtype, 8)
+    q = q.abs()
+    k2 = k.clone()
+    k2[:, :, :10] = float("-inf")
+    o = window_attention(q, k2, v, 6)
+    assert o[:, :, :10].isnan().all()
+    want = window_attention(q, k, v, 6)
+    assert torch.equal(o[:, :, 15:], want[:, :, 15:])
+
+
+@pytest.mark.gpu
 def test_window_attention_in_a_graph():
     """Forward and backward captured once and replayed on changing inputs,
     with eager work between the replays."""

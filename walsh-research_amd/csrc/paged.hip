@@ -15,10 +15,13 @@
 // second kernel.  Scores are S^T = K Q^T on 32x32 matrix-core tiles (key rows
 // come straight from memory in the operand's layout, 16 bytes a lane), so a
 // lane holds 16 scores of one head; O^T = V^T P^T takes V from LDS, read
-// transposed.  With R < 32 most of a tile is idle, which costs nothing: the
-// matrix cores could feed ten times what memory delivers, and the vector units
-// would be short at R >= 4.  Bound by memory: the next block's K (registers)
-// and V (straight into LDS) are on the way while one is used.
+// transposed.  With R < 32 most of a tile is idle, which costs nothing in bf16:
+// the matrix cores could feed ten times what memory delivers, and the vector
+// units would be short at R >= 2.  Bound by memory: the next block's K
+// (registers) and V (straight into LDS) are on the way while one is used; 64
+// sequences of up to 4,096, 32 heads of 128: 376 us, 5.9 TB/s.  float32 takes
+// the vector units up to R = 4 (paged_decode_rows_kernel), and reaches 2 to 3
+// TB/s by products above.
 //
 // Scores, maxima, sums and accumulators are float32; bf16 weights are rounded
 // to bf16 for the product with V (relative 2^-9, as the values' own rounding),
@@ -65,6 +68,66 @@ __device__ __forceinline__ PgKeys pg_keys(const PgArgs &a, int b) {
     return r;
 }
 
+// Visible keys c0 .. c1 - 1 of a sequence and the entries of its page table
+// that they need, read once into LDS.
+struct PgChunk {
+    PgKeys ks;
+    int c0, c1;
+    int ea, na, eb;      // first entry and number of the first tokens' entries; first of the window's, behind them
+    __device__ __forceinline__ void open(const PgArgs &a, int b, int *pages, int *any_bad) {
+        const int ta = min(c1, ks.s0);                // first tokens c0 .. ta - 1
+        ea = c0 >> a.shift, na = c0 < ta ? ((ta - 1) >> a.shift) - ea + 1 : 0;
+        const int tb = max(c0, ks.s0);
+        eb = tb < c1 ? (tb + ks.skip) >> a.shift : 0;
+        const int nb = tb < c1 ? ((c1 - 1 + ks.skip) >> a.shift) - eb + 1 : 0;
+        if (threadIdx.x == 0) *any_bad = ks.bad;
+        __syncthreads();
+        for (int i = threadIdx.x; i < na + nb; i += 64 * kPgWaves) {
+            const int e = a.table[b * a.table_sb + (i < na ? ea + i : eb + i - na)];
+            const bool ok = (unsigned)e < (unsigned)a.P;
+            pages[i] = ok ? e : 0;
+            if (!ok) *any_bad = 1;
+        }
+        __syncthreads();
+    }
+    // element offset of visible key t (past the last one: the last, never counted)
+    __device__ __forceinline__ int64_t at(const PgArgs &a, const int *pages, int t) const {
+        t = min(t, c1 - 1);
+        const int j = t < ks.s0 ? t : t + ks.skip, e = t < ks.s0 ? (j >> a.shift) - ea : na + (j >> a.shift) - eb;
+        return pages[e] * a.sp + (j & ((1 << a.shift) - 1)) * a.sr;
+    }
+};
+
+// The wavefronts' parts of `heads` query heads from h0 on, joined:
+//     o = sum_w acc_w e^(m_w - m) / sum_w l_w e^(m_w - m)
+// to the output, or where a sequence has several chunks to the workspace.
+// stat(w, 0, r) and stat(w, 1, r): maximum and sum, acc(w, r): D accumulators.
+template <typename T, int D, typename S, typename A>
+__device__ __forceinline__ void pg_join(const PgArgs &a, int b, int h0, int heads, int s, bool some, bool bad, S stat, A acc) {
+    for (int i = threadIdx.x; i < heads * (D / 4); i += 64 * kPgWaves) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float mm = stat(0, 0, r);
+#pragma unroll
+        for (int w = 1; w < kPgWaves; ++w) mm = fmaxf(mm, stat(w, 0, r));
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        float ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < kPgWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f((stat(w, 0, r) - mm) * a.sl2);
+            v += load4(acc(w, r) + d) * f;
+            ll += stat(w, 1, r) * f;
+        }
+        if (bad) ll = NAN;                        // a page or length outside the pool: not a number, never a stale value
+        if (a.ns == 1) {
+            store4((T *)a.o + b * a.o_sb + (h0 + r) * a.o_sh + d, some || bad ? v * (1.f / ll) : f32x4{0.f, 0.f, 0.f, 0.f});
+        } else {
+            const int64_t at = ((int64_t)b * a.H + h0 + r) * a.ns + s;
+            store4(a.part + at * D + d, v);
+            if (d == 0) ((float2 *)(a.part + (int64_t)a.B * a.H * a.ns * D))[at] = make_float2(mm, ll);
+        }
+    }
+}
+
 template <typename T, int D> struct PgCfg {
     // 32-key sub-blocks of a wavefront's step: 8 KB of K (bf16) whatever D
     static constexpr int NB = sizeof(T) == 2 ? (D == 128 ? 1 : D == 64 ? 2 : 4) : (D >= 64 ? 1 : D == 32 ? 2 : 4);
@@ -92,21 +155,8 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
     const int c0 = s * a.chunk, c1 = min(c0 + a.chunk, ks.n);
     if (c0 >= c1 && s > 0) return;                // the combine looks at the chunks that exist
 
-    // the chunk's page numbers: of its first tokens, then of its window
-    const int mask = (int)((1u << a.shift) - 1);
-    const int ta = min(c1, ks.s0);                // first tokens c0 .. ta - 1
-    const int ea = c0 >> a.shift, na = c0 < ta ? ((ta - 1) >> a.shift) - ea + 1 : 0;
-    const int tb = max(c0, ks.s0);
-    const int eb = tb < c1 ? (tb + ks.skip) >> a.shift : 0, nb = tb < c1 ? ((c1 - 1 + ks.skip) >> a.shift) - eb + 1 : 0;
-    if (tid == 0) any_bad = ks.bad;
-    __syncthreads();
-    for (int i = tid; i < na + nb; i += 64 * kPgWaves) {
-        const int e = a.table[b * a.table_sb + (i < na ? ea + i : eb + i - na)];
-        const bool ok = (unsigned)e < (unsigned)a.P;
-        pages[i] = ok ? e : 0;
-        if (!ok) any_bad = 1;
-    }
-    __syncthreads();
+    PgChunk ck{ks, c0, c1};
+    ck.open(a, b, pages, &any_bad);
 
     Frag<T> qf[NK];
     {
@@ -114,12 +164,7 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) qf[kk] = load_frag(qp + 16 * kk + 8 * hi);
     }
-    // element offset of visible key t (past the last one: the last, never counted)
-    auto at = [&](int t) {
-        t = min(t, c1 - 1);
-        const int j = t < ks.s0 ? t : t + ks.skip, e = t < ks.s0 ? (j >> a.shift) - ea : na + (j >> a.shift) - eb;
-        return pages[e] * a.sp + (j & mask) * a.sr;
-    };
+    auto at = [&](int t) { return ck.at(a, pages, t); };
     const T *kb = (const T *)a.k + g * a.sg, *vb = (const T *)a.v + g * a.sg;
     unsigned char *vl = smem + wave * PgCfg<T, D>::WAVE;
     auto fetch_k = [&](Frag<T> (&kf)[NB][NK], int t0) {
@@ -223,29 +268,131 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
         }
     }
     __syncthreads();
-    const bool bad = any_bad != 0;
-    for (int i = tid; i < heads * (D / 4); i += 64 * kPgWaves) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float mm = stat[0][0][r];
+    pg_join<T, D>(a, b, h0, heads, s, ks.n > 0, any_bad != 0, [&](int w, int i, int r) { return stat[w][i][r]; },
+                  [&](int w, int r) { return (const float *)(smem + w * PgCfg<T, D>::WAVE) + r * D; });
+}
+
+// Up to four heads on a key head in float32, where the matrix cores would be
+// the bound (a 32x32 product costs 16 times a bf16 one, most of it for idle
+// columns): the same chunks on the vector units.  D / 4 lanes hold one key's
+// row, 16 bytes each, so a wavefront reads 1 KB of whole rows at a time, four
+// of K and four of V on their way together, and with 60 to 122 registers four
+// to eight wavefronts per SIMD are there to ask.  A dot product is summed over
+// its row's lanes (a vector move per factor of two); every such group of lanes
+// keeps a maximum, sum and accumulators of its own, joined at the end.
+//   32 heads of 128, 16 sequences of up to 4,096:   312 us by products, 203 so (5.3 TB/s)
+//   32 heads of 16, 64 sequences of up to 8,192:    349 us, 192 (5.6 TB/s)
+//   32 heads of 128 on 8, 32 of up to 8,192:        370 us, 225 (4.8 TB/s)
+// With eight heads the sums over lanes are the bound (240 us by either for 32
+// heads of 128 on 4, 277 against 200 at 64), and bf16, whose products are 16
+// times cheaper and values dearer to unpack, gains nothing with one head and
+// loses with two (130 us against 102).
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+// v combined over N >= 4 neighbouring lanes (all hold the result).
+template <int N, typename F> __device__ __forceinline__ float over_lanes(float v, F f) {
+    v = f(v, dpp<0xB1>(v));                       // lane ^ 1
+    v = f(v, dpp<0x4E>(v));                       // lane ^ 2
+    if (N >= 8) v = f(v, dpp<0x141>(v));          // 7 - lane: the other four
+    if (N >= 16) v = f(v, dpp<0x140>(v));         // 15 - lane: the other eight
+    if (N >= 32) {
+        const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+        v = f(__uint_as_float(u.x), __uint_as_float(u.y));
+    }
+    return v;
+}
+// v combined over lanes N apart (N >= 4).
+template <int N, typename F> __device__ __forceinline__ float over_groups(float v, F f) {
+    if (N <= 4) v = f(v, dpp<0x124>(v));          // rotations of the row by 4 and 8
+    if (N <= 8) v = f(v, dpp<0x128>(v));
+    if (N <= 16) {
+        const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+        v = f(__uint_as_float(u.x), __uint_as_float(u.y));
+    }
+    const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return f(__uint_as_float(u.x), __uint_as_float(u.y));
+}
+
+template <int D, int R> __global__ __launch_bounds__(64 * kPgWaves) void paged_decode_rows_kernel(PgArgs a) {
+    constexpr int E = 4, LPR = D / E, KPL = 64 / LPR, U = 4, KB = U * KPL;
+    __shared__ int pages[kPgEntries];
+    __shared__ float stat[kPgWaves][2][R];
+    __shared__ __align__(16) float part[kPgWaves][R][D];
+    __shared__ int any_bad;
+    const int s = uniform((int)blockIdx.x / a.G), g = (int)blockIdx.x - s * a.G, b = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), grp = lane / LPR, col = lane % LPR * E;
+    const int heads = a.H / a.G, h0 = g * heads;  // at most R
+    const PgKeys ks = pg_keys(a, b);
+    const int c0 = s * a.chunk, c1 = min(c0 + a.chunk, ks.n);
+    if (c0 >= c1 && s > 0) return;
+    PgChunk ck{ks, c0, c1};
+    ck.open(a, b, pages, &any_bad);
+
+    f32x4 q[R], acc[R];
+    float m[R], l[R];
 #pragma unroll
-        for (int w = 1; w < kPgWaves; ++w) mm = fmaxf(mm, stat[w][0][r]);
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        float ll = 0.f;
+    for (int r = 0; r < R; ++r) {
+        q[r] = load4((const float *)a.q + b * a.q_sb + (h0 + min(r, heads - 1)) * a.q_sh + col);
+        acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m[r] = kNoScore, l[r] = 0.f;
+    }
+    const float *kb = (const float *)a.k + g * a.sg + col, *vb = (const float *)a.v + g * a.sg + col;
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
+    auto sum = [](float x, float y) { return x + y; };
+    for (int t0 = c0 + wave * KB; t0 < c1; t0 += KB * kPgWaves) {
+        f32x4 k[U], v[U];
 #pragma unroll
-        for (int w = 0; w < kPgWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f((stat[w][0][r] - mm) * a.sl2);
-            v += load4((const float *)(smem + w * PgCfg<T, D>::WAVE) + r * D + d) * f;
-            ll += stat[w][1][r] * f;
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = ck.at(a, pages, t0 + u * KPL + grp);
+            k[u] = load4(kb + at);
+            v[u] = load4(vb + at);
         }
-        if (bad) ll = NAN;                        // a page or length outside the pool: not a number, never a stale value
-        if (a.ns == 1) {
-            store4((T *)a.o + b * a.o_sb + (h0 + r) * a.o_sh + d, ks.n > 0 || bad ? v * (1.f / ll) : f32x4{0.f, 0.f, 0.f, 0.f});
-        } else {
-            const int64_t at = ((int64_t)b * a.H + h0 + r) * a.ns + s;
-            store4(a.part + at * D + d, v);
-            if (d == 0) ((float2 *)(a.part + (int64_t)a.B * a.H * a.ns * D))[at] = make_float2(mm, ll);
+        float w[U][R];
+        bool up = false;                          // as above: move the maxima rarely
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float d = over_lanes<LPR>(q[r].x * k[u].x + q[r].y * k[u].y + q[r].z * k[u].z + q[r].w * k[u].w, sum);
+                w[u][r] = t0 + u * KPL + grp < c1 ? d : -INFINITY;
+                up |= (w[u][r] - m[r]) * a.sl2 > 8.f;
+            }
+        }
+        if (__any(up)) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float mn = m[r];
+#pragma unroll
+                for (int u = 0; u < U; ++u) mn = fmaxf(mn, w[u][r]);
+                const float al = __builtin_amdgcn_exp2f((m[r] - mn) * a.sl2);
+                m[r] = mn;
+                l[r] *= al;
+                acc[r] *= al;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(w[u][r], a.sl2, -m[r] * a.sl2));
+                l[r] += p;
+                acc[r] += p * v[u];
+            }
         }
     }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float mm = over_groups<LPR>(m[r], larger), f = __builtin_amdgcn_exp2f((m[r] - mm) * a.sl2);
+        const float ll = over_groups<LPR>(l[r] * f, sum);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[r][e] = over_groups<LPR>(acc[r][e] * f, sum);
+        if (grp == 0) store4(&part[wave][r][col], acc[r]);
+        if (lane == 0) stat[wave][0][r] = mm, stat[wave][1][r] = ll;
+    }
+    __syncthreads();
+    pg_join<float, D>(a, b, h0, heads, s, ks.n > 0, any_bad != 0, [&](int w, int i, int r) { return stat[w][i][r]; },
+                  [&](int w, int r) { return part[w][r]; });
 }
 
 // The chunks' parts of one (sequence, query head) joined: blockDim.x / D groups
@@ -414,8 +561,15 @@ WALSH_EXPORT int walsh_paged_decode_attention(const void *q, int64_t q_sb, int64
     attn_dispatch(dtype, D, [&](auto t, auto d) {
         typedef decltype(t) T;
         constexpr int DD = decltype(d)::value;
-        launch(paged_decode_kernel<T, DD>, dim3((unsigned)(ns * gy), (unsigned)B), dim3(64 * kPgWaves),
-               (uint32_t)PgCfg<T, DD>::LDS, s, a);
+        const dim3 grid((unsigned)(ns * gy), (unsigned)B), threads(64 * kPgWaves);
+        const int64_t R = H / G;
+        if constexpr (sizeof(T) == 4) {
+            if (R == 1) launch(paged_decode_rows_kernel<DD, 1>, grid, threads, 0, s, a);
+            else if (R == 2) launch(paged_decode_rows_kernel<DD, 2>, grid, threads, 0, s, a);
+            else if (R <= 4) launch(paged_decode_rows_kernel<DD, 4>, grid, threads, 0, s, a);
+        }
+        if (sizeof(T) == 2 || R > 4)
+            launch(paged_decode_kernel<T, DD>, grid, threads, (uint32_t)PgCfg<T, DD>::LDS, s, a);
         // about four parts per group of threads, a wavefront at least
         int64_t groups = ceil_div(ns, 4);
         if (groups > 1024 / DD) groups = 1024 / DD;
