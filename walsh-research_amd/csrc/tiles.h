@@ -164,6 +164,31 @@ template <typename T, int D, int ROWS> struct Tile {
             lds_load<16>(rs, off, dst + k * 1024);
         }
     }
+    // The same of many tiles of one stride (st >= D), what depends on the lane
+    // alone worked out once: rows past the last one lie past the buffer.
+    template <int WAVES> struct Loads {
+        static constexpr int N = BYTES / 1024, PER = (N + WAVES - 1) / WAVES;
+        uint32_t off[PER];
+        __device__ __forceinline__ Loads(int64_t st, int wave, int lane) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const uint32_t pos = (uint32_t)((i * WAVES + wave) * 64 + lane);
+                const int row = (int)(pos / NCH);
+                off[i] = (uint32_t)row * (uint32_t)(st * (int)sizeof(T)) + 16 * ((pos % NCH) ^ swz(row));
+            }
+        }
+        __device__ __forceinline__ void go(unsigned char *lds, const T *base, int64_t st, int r0, int n, int wave) const {
+            const int rows = min(n - r0, ROWS);
+            const uint32_t span = rows > 0 ? (uint32_t)(((rows - 1) * (int)st + D) * (int)sizeof(T)) : 0u;
+            const u32x4 rs = lds_load_rsrc(base + r0 * st, span);
+            const uint32_t dst = lds_addr(lds) + wave * 1024;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                if (N % WAVES && i * WAVES + wave >= N) break;
+                lds_load<16>(rs, off[i], dst + i * WAVES * 1024);
+            }
+        }
+    };
     // Eight elements of row r from column 16 kk + 8 hi.
     static __device__ __forceinline__ Frag<T> row(const unsigned char *lds, int r, int kk, int hi) {
         const unsigned char *p = lds + r * ROWB;

@@ -132,20 +132,22 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 
     const T *kb = (const T *)a.k + b * a.skv.sb + g * a.skv.sh, *vb = (const T *)a.v + b * a.skv.sb + g * a.skv.sh;
     const Chunks ch = wlo <= whi ? win_chunks<KC>(a, wlo, whi) : Chunks{0, 0, 0};
-    auto fetch = [&](int i) {
-        unsigned char *dst = smem + (i & 1) * 2 * L::BYTES;
-        L::template fetch<kWinWaves>(dst, kb, a.skv.st, ch.at(i) * KC, 0, len, wave, lane);
-        L::template fetch<kWinWaves>(dst + L::BYTES, vb, a.skv.st, ch.at(i) * KC, 0, len, wave, lane);
-    };
-    if (ch.n > 0) fetch(0);
+    const typename L::template Loads<kWinWaves> loads(a.skv.st, wave, lane);
+    auto fetch_k = [&](int i) { loads.go(smem + (i & 1) * 2 * L::BYTES, kb, a.skv.st, ch.at(i) * KC, len, wave); };
+    auto fetch_v = [&](int i) { loads.go(smem + (i & 1) * 2 * L::BYTES + L::BYTES, vb, a.skv.st, ch.at(i) * KC, len, wave); };
+    if (ch.n > 0) fetch_k(0), fetch_v(0);
     for (int i = 0; i < ch.n; ++i) {
         tiles_ready();
-        if (i + 1 < ch.n) fetch(i + 1);
         const unsigned char *kl = smem + (i & 1) * 2 * L::BYTES, *vl = kl + L::BYTES;
         const int k0 = ch.at(i) * KC;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int kind = pa <= pb ? win_kind(a, k0 + 32 * j, 32, pa, pb) : 0;
+            // the next tile's loads in two bursts, each behind a product's
+            if (i + 1 < ch.n) {
+                if (j == 0) fetch_k(i + 1);
+                if (j == NJ - 1) fetch_v(i + 1);
+            }
             if (kind == 0) continue;
             f32x16 s = f32x16{};
 #pragma unroll
@@ -374,20 +376,22 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 
     const T *kb = (const T *)a.k + b * a.skv.sb + g * a.skv.sh, *vb = (const T *)a.v + b * a.skv.sb + g * a.skv.sh;
     const Chunks ch = wlo <= whi ? win_chunks<KC>(a, wlo, whi) : Chunks{0, 0, 0};
-    auto fetch = [&](int i) {
-        unsigned char *dst = smem + (i & 1) * 2 * L::BYTES;
-        L::template fetch<kWinWaves>(dst, kb, a.skv.st, ch.at(i) * KC, 0, len, wave, lane);
-        L::template fetch<kWinWaves>(dst + L::BYTES, vb, a.skv.st, ch.at(i) * KC, 0, len, wave, lane);
-    };
-    if (ch.n > 0) fetch(0);
+    const typename L::template Loads<kWinWaves> loads(a.skv.st, wave, lane);
+    auto fetch_k = [&](int i) { loads.go(smem + (i & 1) * 2 * L::BYTES, kb, a.skv.st, ch.at(i) * KC, len, wave); };
+    auto fetch_v = [&](int i) { loads.go(smem + (i & 1) * 2 * L::BYTES + L::BYTES, vb, a.skv.st, ch.at(i) * KC, len, wave); };
+    if (ch.n > 0) fetch_k(0), fetch_v(0);
     for (int i = 0; i < ch.n; ++i) {
         tiles_ready();
-        if (i + 1 < ch.n) fetch(i + 1);
         const unsigned char *kl = smem + (i & 1) * 2 * L::BYTES, *vl = kl + L::BYTES;
         const int k0 = ch.at(i) * KC;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int kind = pa <= pb ? win_kind(a, k0 + 32 * j, 32, pa, pb) : 0;
+            // the next tile's loads in two bursts, each behind a product's
+            if (i + 1 < ch.n) {
+                if (j == 0) fetch_k(i + 1);
+                if (j == NJ - 1) fetch_v(i + 1);
+            }
             if (kind == 0) continue;
             f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
@@ -716,6 +720,7 @@ WALSH_EXPORT int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t
     a.W = window > 0 && window < Tk ? (int)window : 0;
     a.S = sinks < 0 ? 0 : (int)(sinks < Tk ? sinks : Tk);
     a.sl2 = scale * kLog2e;
+    if (Tk == 1) a.skv.st = D;                    // (the tiles' loads count rows by it)
     const int64_t n = ceil_div(Tq, kWinQ) * H * B, n32 = ceil_div(Tq, 32) * H * B;
     const bool split = n < device_info().cu_count;   // a wavefront per SIMD and less: cut the keys, too
     attn_dispatch(dtype, D, [&](auto t, auto d) {
@@ -779,6 +784,7 @@ WALSH_EXPORT int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t
     a.W = window > 0 && window < Tk ? (int)window : 0;
     a.S = sinks < 0 ? 0 : (int)(sinks < Tk ? sinks : Tk);
     a.sl2 = scale * kLog2e;
+    if (Tk == 1) a.skv.st = D;                    // (the tiles' loads count rows by it)
     win_splits(a, win_bwd_qc(D, dtype));
     if (work_bytes < win_bwd_bytes(a, D))
         return set_error(WALSH_EINVAL, "%s: workspace of %lld bytes, needs %lld", fn, (long long)work_bytes,
