@@ -26,6 +26,10 @@
 // tokens that the histogram leaves in question, each wavefront's into a list
 // in LDS; what follows works on the lists, or, where one overflows (nothing
 // filtered, or thousands kept), on the row again, out of the L2.
+// Bound by that chain, not by memory: 50,257 logits in bf16 with top-k 50 and
+// top-p 0.95 take 22 us for one row (load and maximum 5, histogram 5, search 2,
+// the rest lists, cut and draw) and 53 us for 256 rows of float32 with every
+// filter, one row to a CU.
 #include "common.h"
 
 namespace walsh {
