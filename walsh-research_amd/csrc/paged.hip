@@ -164,23 +164,24 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) qf[kk] = load_frag(qp + 16 * kk + 8 * hi);
     }
-    auto at = [&](int t) { return ck.at(a, pages, t); };
     const T *kb = (const T *)a.k + g * a.sg, *vb = (const T *)a.v + g * a.sg;
     unsigned char *vl = smem + wave * PgCfg<T, D>::WAVE;
-    auto fetch_k = [&](Frag<T> (&kf)[NB][NK], int t0) {
-#pragma unroll
-        for (int u = 0; u < NB; ++u) {
-            const T *p = kb + at(t0 + 32 * u + n) + 8 * hi;
-#pragma unroll
-            for (int kk = 0; kk < NK; ++kk) kf[u][kk] = load_frag(p + 16 * kk);
-        }
-    };
-    auto fetch_v = [&](int buf, int t0) {
+    // K of the keys from t0 on into operands, V into a buffer; a V row's offset
+    // comes from the lane that has that row of K
+    auto fetch = [&](Frag<T> (&kf)[NB][NK], int buf, int t0) {
         const uint32_t dst = lds_addr(vl) + buf * PgCfg<T, D>::VBYTES;
 #pragma unroll
-        for (int i = 0; i < NB * L::BYTES / 1024; ++i) {
-            const int pos = i * 64 + lane, row = pos / L::NCH, c = (pos % L::NCH) ^ L::swz(row & 31);
-            lds_gather(vb + at(t0 + row) + c * (16 / (int)sizeof(T)), dst + i * 1024);
+        for (int u = 0; u < NB; ++u) {
+            const int64_t at = ck.at(a, pages, t0 + 32 * u + n);
+            const T *p = kb + at + 8 * hi;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) kf[u][kk] = load_frag(p + 16 * kk);
+#pragma unroll
+            for (int i = 0; i < L::BYTES / 1024; ++i) {
+                const int pos = i * 64 + lane, row = pos / L::NCH, c = (pos % L::NCH) ^ L::swz(row);
+                const int64_t from = ((int64_t)__shfl((int)(at >> 32), row) << 32) | (uint32_t)__shfl((int)at, row);
+                lds_gather(vb + from + c * (16 / (int)sizeof(T)), dst + u * L::BYTES + i * 1024);
+            }
         }
     };
 
@@ -191,10 +192,7 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
     const int stride = KB * kPgWaves;
     int t0 = c0 + wave * KB, buf = 0;
     Frag<T> kf[NB][NK];
-    if (t0 < c1) {
-        fetch_k(kf, t0);
-        fetch_v(0, t0);
-    }
+    if (t0 < c1) fetch(kf, 0, t0);
     for (; t0 < c1; t0 += stride, buf ^= 1) {
         const int tn = t0 + stride;
         f32x16 sc[NB];
@@ -206,10 +204,7 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
         }
         // this block's V has landed (it was requested after this block's K)
         wait_loads();
-        if (tn < c1) {
-            fetch_k(kf, tn);
-            fetch_v(buf ^ 1, tn);
-        }
+        if (tn < c1) fetch(kf, buf ^ 1, tn);
         if (t0 + KB > c1) {
 #pragma unroll
             for (int u = 0; u < NB; ++u)
@@ -493,13 +488,20 @@ static int pg_check(const char *fn, int64_t B, int64_t G, int64_t D, int64_t P, 
 }
 
 // Keys per workgroup: 1,024, so that a batch of unequal lengths ends together
-// (64 sequences of up to 4,096, 32 heads of 128 in bf16: 375 us with 512 or
-// 1,024, 384 with 2,048, 404 with 4,096); fewer where that would not fill the
-// chip (two workgroups per CU), down to a block per wavefront.
-static void pg_split(int64_t pairs, int64_t keys, int KB, int64_t *chunk, int64_t *ns) {
+// (64 sequences of up to 4,096, 32 heads of 128 in bf16: 375 us with 1,024, 384
+// with 2,048, 404 with 4,096); 512 where 1,024 would leave few workgroups to
+// even out the lengths and a chunk's end costs little against its rows, with
+// rows of 128 bytes and up to eight heads (32 of up to 8,192, 32 heads of 128
+// on 4 in bf16: 59 us with 1,024, 51 with 512; but 4 of up to 131,072: 252 and
+// 258, heads of 16: 98 and 113, and 16 heads of 64 on a key head: 31 and 33);
+// fewer where that would not fill the chip (two workgroups per CU), down to a
+// block per wavefront.
+static void pg_split(int64_t pairs, int64_t keys, int64_t R, int64_t row_bytes, int KB, int64_t *chunk, int64_t *ns) {
     const int64_t slots = 2 * (int64_t)device_info().cu_count, step = KB * kPgWaves;
+    const bool few = pairs * ceil_div(keys, kPgMaxChunk) < 8 * slots;
+    const int64_t most = few && R <= 8 && row_bytes >= 128 ? kPgMaxChunk / 2 : kPgMaxChunk;
     int64_t c = ceil_div(ceil_div(pairs * keys, slots), step) * step;   // what one round of workgroups would take
-    *chunk = c < step ? step : c > kPgMaxChunk ? kPgMaxChunk : c;
+    *chunk = c < step ? step : c > most ? most : c;
     *ns = ceil_div(keys, *chunk);
     if (*ns < 1) *ns = 1;
 }
@@ -507,7 +509,7 @@ static void pg_plan(int64_t B, int64_t H, int64_t G, int64_t cap, int64_t D, int
                     int64_t *chunk, int64_t *ns) {
     const int64_t keys = W > 0 && W + S < cap ? W + S : cap;
     const int KB = 32 * (dtype == WALSH_BF16 ? (D == 128 ? 1 : D == 64 ? 2 : 4) : (D >= 64 ? 1 : D == 32 ? 2 : 4));
-    pg_split(B * G * ceil_div(H / G, 32), keys, KB, chunk, ns);
+    pg_split(B * G * ceil_div(H / G, 32), keys, H / G, D * (dtype == WALSH_BF16 ? 2 : 4), KB, chunk, ns);
 }
 
 }  // namespace walsh
