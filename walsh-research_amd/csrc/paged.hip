@@ -19,7 +19,7 @@
 // the matrix cores could feed ten times what memory delivers, and the vector
 // units would be short at R >= 2.  Bound by memory: the next block's K
 // (registers) and V (straight into LDS) are on the way while one is used; 64
-// sequences of up to 4,096, 32 heads of 128: 376 us, 5.9 TB/s.  float32 takes
+// sequences of up to 4,096, 32 heads of 128: 370 us, 6.0 TB/s.  float32 takes
 // the vector units up to R = 4 (paged_decode_rows_kernel), and reaches 2 to 3
 // TB/s by products above.
 //
@@ -275,13 +275,13 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
 // to eight wavefronts per SIMD are there to ask.  A dot product is summed over
 // its row's lanes (a vector move per factor of two); every such group of lanes
 // keeps a maximum, sum and accumulators of its own, joined at the end.
-//   32 heads of 128, 16 sequences of up to 4,096:   312 us by products, 203 so (5.3 TB/s)
+//   32 heads of 128, 16 sequences of up to 4,096:   312 us by products, 191 so (5.6 TB/s)
 //   32 heads of 16, 64 sequences of up to 8,192:    349 us, 192 (5.6 TB/s)
 //   32 heads of 128 on 8, 32 of up to 8,192:        370 us, 225 (4.8 TB/s)
-// With eight heads the sums over lanes are the bound (240 us by either for 32
-// heads of 128 on 4, 277 against 200 at 64), and bf16, whose products are 16
-// times cheaper and values dearer to unpack, gains nothing with one head and
-// loses with two (130 us against 102).
+// With eight heads the sums over lanes are the bound (158 us by products, 219 so
+// for 32 heads of 64 on 4; 204 and 189 at 128; 88 and 113 at 32), and bf16,
+// whose products are 16 times cheaper and values dearer to unpack, gains nothing
+// with one head and loses with two (102 us by products, 130 so).
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
 }
