@@ -189,42 +189,58 @@ template <typename T, int D, int ROWS> struct Tile {
             }
         }
     };
-    // Eight elements of row r from column 16 kk + 8 hi.
-    static __device__ __forceinline__ Frag<T> row(const unsigned char *lds, int r, int kk, int hi) {
-        const unsigned char *p = lds + r * ROWB;
-        const int s = swz(r);
+    // Eight elements of row r from column 16 kk + 8 hi, and of column
+    // 32 c + lane % 32 (modulo D) the rows r + 4 hi + 0..3 and r + 8 + 4 hi +
+    // 0..3 (r a multiple of 16).  A swizzle's bits are bits of the row, so an
+    // operand's address is that of the first one, worked out once, with an
+    // exclusive or and an offset that the instruction holds (tiles lie at
+    // multiples of 1,024 bytes).
+    static __device__ __forceinline__ uint32_t row_base(const unsigned char *lds, int r, int hi) {
+        return lds_addr(lds) + r * ROWB + ((((int)sizeof(T) / 2 * hi) ^ swz(r)) << 4);
+    }
+    static __device__ __forceinline__ uint32_t row_step(int kk) { return (uint32_t)kk * 16 * sizeof(T); }
+    static __device__ __forceinline__ Frag<T> row_from(uint32_t base, int kk) {
+        base ^= row_step(kk);
         if constexpr (sizeof(T) == 2) {
-            return {*(const i16x8 *)(p + (((2 * kk + hi) ^ s) << 4))};
+            return {*lds_at<i16x8>(base)};
         } else {
-            const f32x4 a = *(const f32x4 *)(p + (((4 * kk + 2 * hi) ^ s) << 4));
-            const f32x4 b = *(const f32x4 *)(p + (((4 * kk + 2 * hi + 1) ^ s) << 4));
+            const f32x4 a = *lds_at<f32x4>(base), b = *lds_at<f32x4>(base ^ 16);
             return {f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
         }
     }
-    // Column 32 c + lane % 32 (modulo D) of rows r + 4 hi + 0..3 and r + 8 + 4 hi + 0..3.
-    static __device__ __forceinline__ Frag<T> col(const unsigned char *lds, int r, int c, int lane) {
+    static __device__ __forceinline__ uint32_t col_base(const unsigned char *lds, int lane) {
         const int hi = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            const int l = lane & 15, half = D >= 32 ? (lane >> 4) & 1 : 0, r = 4 * hi + (l >> 2);
+            return lds_addr(lds) + r * ROWB + (((2 * half + ((l & 3) >> 1)) ^ swz(r)) << 4) + 8 * (l & 1);
+        } else {
+            const int d = (lane & 31) % D;
+            return lds_addr(lds) + 4 * hi * ROWB + (((d >> 2) ^ swz(4 * hi)) << 4) + 4 * (d & 3);
+        }
+    }
+    static __device__ __forceinline__ Frag<T> col_from(uint32_t base, int r, int c) {
         if constexpr (sizeof(T) == 2) {
             typedef short i16x4v __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) i16x4v *P;
-            const int l = lane & 15, half = D >= 32 ? (lane >> 4) & 1 : 0;
-            const int ch = 4 * c + 2 * half + ((l & 3) >> 1), byte = 8 * (l & 1);
-            const int ra = r + 4 * hi + (l >> 2), rb = ra + 8;
-            const i16x4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (P)(const_cast<unsigned char *>(lds) + ra * ROWB + ((ch ^ swz(ra)) << 4) + byte));
-            const i16x4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (P)(const_cast<unsigned char *>(lds) + rb * ROWB + ((ch ^ swz(rb)) << 4) + byte));
-            return {__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)};
+            const uint32_t a = base ^ (c << 6), b = a ^ (swz(8) << 4);
+            const i16x4v u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)(a + r * ROWB));
+            const i16x4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)(b + (r + 8) * ROWB));
+            return {__builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7)};
         } else {
-            const int d = (32 * c + (lane & 31)) % D;
             f32x8 v;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int rr = r + 4 * hi + (e & 3) + 8 * (e >> 2);
-                v[e] = *(const float *)(lds + rr * ROWB + (((d >> 2) ^ swz(rr)) << 4) + 4 * (d & 3));
+                const int k = (e & 3) + 8 * (e >> 2);
+                v[e] = *lds_at<float>((base ^ (c << 7) ^ (swz(k) << 4)) + (r + k) * ROWB);
             }
             return {v};
         }
+    }
+    template <typename V> static __device__ __forceinline__ __attribute__((address_space(3))) const V *lds_at(uint32_t at) {
+        return (__attribute__((address_space(3))) const V *)(uintptr_t)at;
+    }
+    static __device__ __forceinline__ Frag<T> col(const unsigned char *lds, int r, int c, int lane) {
+        return col_from(col_base(lds, lane), r, c);
     }
 };
 

@@ -97,7 +97,7 @@ __device__ __forceinline__ int xcd_item(int n) {
 // 32 keys that none of a wavefront's queries sees are passed over, and only
 // those seen in part are masked.  Bound by the matrix products and the
 // softmax's vector instructions, which two wavefronts per SIMD overlap in part:
-// 2 x 32 heads of 128, 8,192 tokens, window 1,024, bf16: 351 us, 740 TFLOP/s of
+// 2 x 32 heads of 128, 8,192 tokens, window 1,024, bf16: 352 us, 735 TFLOP/s of
 // what is visible (a large product reaches 1,210).  Of 362 us without the
 // loads' present order, 51 went without the softmax, 54 without the tiles'
 // loads.  256 queries on a tile took 394 us, 64 queries per wavefront (each
@@ -147,10 +147,13 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     const typename L::template Loads<kWinWaves> loads(a.skv.st, wave, lane);
     auto fetch_k = [&](int i) { loads.go(smem + (i & 1) * 2 * L::BYTES, kb, a.skv.st, ch.at(i) * KC, len, wave); };
     auto fetch_v = [&](int i) { loads.go(smem + (i & 1) * 2 * L::BYTES + L::BYTES, vb, a.skv.st, ch.at(i) * KC, len, wave); };
+    // a row's operands' addresses, held: worked out between the paced reads they cost a tenth of the time
+    uint32_t ka[NK], va = L::col_base(smem + L::BYTES, lane);
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) ka[kk] = L::row_base(smem, n, hi) ^ L::row_step(kk);
     if (ch.n > 0) fetch_k(0), fetch_v(0);
     for (int i = 0; i < ch.n; ++i) {
         tiles_ready();
-        const unsigned char *kl = smem + (i & 1) * 2 * L::BYTES, *vl = kl + L::BYTES;
         const int k0 = ch.at(i) * KC;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             if (kind == 0) continue;
             f32x16 s = f32x16{};
 #pragma unroll
-            for (int kk = 0; kk < NK; ++kk) mma(s, L::row(kl, 32 * j + n, kk, hi), qf[kk]);
+            for (int kk = 0; kk < NK; ++kk) mma(s, L::row_from(ka[kk] + 32 * j * L::ROWB, 0), qf[kk]);
             if constexpr (sizeof(T) == 2 && NK > 4) pace<1, NK, 4>();
             if (kind == 1) {
 #pragma unroll
@@ -199,9 +202,13 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
                 Frag<T> pf;
                 pack(pf, w + 8 * t);
 #pragma unroll
-                for (int c = 0; c < ND; ++c) mma(acc[c], L::col(vl, 32 * j + 16 * t, c, lane), pf);
+                for (int c = 0; c < ND; ++c) mma(acc[c], L::col_from(va, 32 * j + 16 * t, c), pf);
             }
         }
+        const int other = i & 1 ? -2 * L::BYTES : 2 * L::BYTES;          // the next tile's buffer
+        va += other;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) ka[kk] += other;
     }
     l = half_sum(l);
     if (qi >= a.Tq) return;
@@ -347,7 +354,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // and Delta as the keys' kernel reads them.  Delta is formed from the stored,
 // rounded output.  Tiles and bounds as in the forward, three products where
 // that has two: 32 heads on 8 of 128, 2 x 4,096 padded tokens, window 1,024,
-// 16 first tokens, bf16: 203 us (the forward 155).
+// 16 first tokens, bf16: 205 us (the forward 156).
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
@@ -394,10 +401,12 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     const typename L::template Loads<kWinWaves> loads(a.skv.st, wave, lane);
     auto fetch_k = [&](int i) { loads.go(smem + (i & 1) * 2 * L::BYTES, kb, a.skv.st, ch.at(i) * KC, len, wave); };
     auto fetch_v = [&](int i) { loads.go(smem + (i & 1) * 2 * L::BYTES + L::BYTES, vb, a.skv.st, ch.at(i) * KC, len, wave); };
+    uint32_t ka[NK], kc = L::col_base(smem, lane);
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) ka[kk] = L::row_base(smem, n, hi) ^ L::row_step(kk);
     if (ch.n > 0) fetch_k(0), fetch_v(0);
     for (int i = 0; i < ch.n; ++i) {
         tiles_ready();
-        const unsigned char *kl = smem + (i & 1) * 2 * L::BYTES, *vl = kl + L::BYTES;
         const int k0 = ch.at(i) * KC;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -411,8 +420,8 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk) {
-                mma(s, L::row(kl, 32 * j + n, kk, hi), qf[kk]);
-                mma(dp, L::row(vl, 32 * j + n, kk, hi), gf[kk]);
+                mma(s, L::row_from(ka[kk] + 32 * j * L::ROWB, 0), qf[kk]);
+                mma(dp, L::row_from(ka[kk] + L::BYTES + 32 * j * L::ROWB, 0), gf[kk]);
             }
             if constexpr (sizeof(T) == 2 && NK > 1) pace<1, 2 * NK, 4>();
             if (kind == 1) {
@@ -431,17 +440,21 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
                     // one product a block: dS goes in two parts, its rounding
                     // with it (relative error of dQ at D = 16, its own
                     // rounding in it: 2.6e-3 without, 1.8e-3 so)
-                    const Frag<T> kc = L::col(kl, 32 * j + 16 * t, 0, lane);
+                    const Frag<T> k0c = L::col_from(kc, 32 * j + 16 * t, 0);
                     Frag<T> rest;
                     pack_rest(rest, ds + 8 * t, f);
-                    mma(acc[0], kc, f);
-                    mma(acc[0], kc, rest);
+                    mma(acc[0], k0c, f);
+                    mma(acc[0], k0c, rest);
                 } else {
 #pragma unroll
-                    for (int c = 0; c < ND; ++c) mma(acc[c], L::col(kl, 32 * j + 16 * t, c, lane), f);
+                    for (int c = 0; c < ND; ++c) mma(acc[c], L::col_from(kc, 32 * j + 16 * t, c), f);
                 }
             }
         }
+        const int other = i & 1 ? -2 * L::BYTES : 2 * L::BYTES;          // the next tile's buffer
+        kc += other;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) ka[kk] += other;
     }
     if (qi >= a.Tq) return;
     T *dq = (T *)a.dq + (((int64_t)b * a.H + h) * a.Tq + qi) * D;
@@ -465,8 +478,9 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // are summed in a fixed order; an unsplit block is stored at once.  Keys stay
 // in registers and queries pass by, so shared heads' gradients need no sum
 // afterwards.  Four products, and registers for no more than one of the score
-// tiles at a time: 296 us for the case above (its loads in two bursts, as in
-// the other kernels, took 330).
+// tiles at a time: 283 us for the case above (loads in two bursts, as in the
+// other kernels, took 12% more).  float32 at D = 64 runs two wavefronts per SIMD
+// (332 us for 32 heads on 8, 2,048 tokens, causal; 368 with one).
 template <typename T, int D> struct WinBwdCfg {
     static constexpr int KL = D == 128 && sizeof(T) == 2 ? 2 : 0;     // K operands kept in LDS
     static constexpr int QC = D == 128 && sizeof(T) == 4 ? 32 : 64;   // rows of a tile
@@ -482,7 +496,7 @@ template <int QC> __device__ __forceinline__ void win_q_tiles(const WinArgs &a, 
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) void window_bwd_kv_kernel(WinArgs a) {
+__global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_kv_kernel(WinArgs a) {
     constexpr int QC = WinBwdCfg<T, D>::QC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = QC / 32;
     typedef Tile<T, D, QC> L;
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -543,7 +557,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) 
         const int pq = (t0 + tile) * QC + off;                       // position of the tile's first query
         if (++tile == nt) tile = 0, ++hr;
         if (i + 1 < i1) fetch(i + 1, hr, tile);
-        const unsigned char *ql = smem + (i & 1) * 2 * L::BYTES, *gl = ql + L::BYTES;
+        const unsigned char *ql = smem + (i & 1) * 2 * L::BYTES;   // then the tile of do
 #pragma unroll 1
         for (int j = 0; j < NJ; ++j) {
             const int ln = fresh(lane), n = ln & 31, hi = ln >> 5;
@@ -552,10 +566,11 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) 
             if (kind == 0) continue;
             // scores, weights, dV; then do V^T, dS, dK: one after the other, so
             // that 32 results at a time are live beside the accumulators
+            const uint32_t rows = L::row_base(ql + 32 * j * L::ROWB, n, hi), cols = L::col_base(ql + 32 * j * L::ROWB, ln);
             f32x16 s = f32x16{};
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
-                mma(s, L::row(ql, 32 * j + n, kk, hi), kk < KR ? kf[kk < KR ? kk : 0] : klast[kk < KR ? 0 : kk - KR][threadIdx.x]);
+                mma(s, L::row_from(rows, kk), kk < KR ? kf[kk < KR ? kk : 0] : klast[kk < KR ? 0 : kk - KR][threadIdx.x]);
             if constexpr (sizeof(T) == 2 && NK > 3) pace<1, NK, 3>();
             if (kind == 1) {
 #pragma unroll
@@ -574,11 +589,11 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) 
                 Frag<T> f;
                 pack(f, w + 8 * t);
 #pragma unroll
-                for (int c = 0; c < ND; ++c) mma(av[c], L::col(gl, 32 * j + 16 * t, c, ln), f);
+                for (int c = 0; c < ND; ++c) mma(av[c], L::col_from(cols + L::BYTES, 16 * t, c), f);
             }
             f32x16 dp = f32x16{};
 #pragma unroll
-            for (int kk = 0; kk < NK; ++kk) mma(dp, L::row(gl, 32 * j + n, kk, hi), vf[kk]);
+            for (int kk = 0; kk < NK; ++kk) mma(dp, L::row_from(rows + L::BYTES, kk), vf[kk]);
             if constexpr (sizeof(T) == 2 && NK > 3) pace<1, NK, 3>();
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -591,7 +606,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D >= 64 ? 1 : 2) 
                 Frag<T> f;
                 pack(f, w + 8 * t);
 #pragma unroll
-                for (int c = 0; c < ND; ++c) mma(ak[c], L::col(ql, 32 * j + 16 * t, c, ln), f);
+                for (int c = 0; c < ND; ++c) mma(ak[c], L::col_from(cols, 16 * t, c), f);
             }
         }
     }
