@@ -77,10 +77,26 @@ __device__ __forceinline__ int win_kind(const WinArgs &a, int k0, int n, int pa,
     if (k0 > pb || (a.W > 0 && k0 + n <= pa - a.W + 1 && k0 >= a.S)) return 0;
     return k0 + n - 1 <= pa && (a.W <= 0 || k0 > pb - a.W || k0 + n <= a.S) ? 2 : 1;
 }
-// (no branches: a tile of mixed keys asks for every element)
-__device__ __forceinline__ bool win_sees(const WinArgs &a, int p, int j) {
-    const uint32_t near = a.W > 0 ? (uint32_t)a.W : 0x7fffffffu;
-    return ((uint32_t)(p - j) < near) | ((j < a.S) & (j <= p));
+// Of 32 consecutive keys from k0 the ones that position p sees, and of 32
+// consecutive positions from p0 the ones that see key j, as bits; and scores
+// by such bits: row 8 (r / 4) + 4 hi + r % 4 of a result is bit 8 (r / 4) + r % 4
+// of bits >> 4 hi.  (Two instructions a score; comparing positions took eight.)
+__device__ __forceinline__ uint32_t bits_below(int n) { return (uint32_t)((1ull << max(0, min(n, 32))) - 1); }
+__device__ __forceinline__ uint32_t win_keys(const WinArgs &a, int p, int k0) {
+    const int n = p - k0 + 1, W = a.W > 0 ? a.W : 1 << 29;
+    return (bits_below(n) & ~bits_below(n - W)) | bits_below(min(n, a.S - k0));
+}
+__device__ __forceinline__ uint32_t win_rows(const WinArgs &a, int p0, int j) {
+    const int n = j - p0, W = a.W > 0 ? a.W : 1 << 29;
+    return ~bits_below(n) & (j < a.S ? ~0u : bits_below(n + W));
+}
+__device__ __forceinline__ void win_hide(f32x16 &s, uint32_t seen, int hi) {
+    const uint32_t hidden = ~seen >> (4 * hi);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const uint32_t all = (uint32_t)((int)(hidden << (31 - 8 * (r >> 2) - (r & 3))) >> 31);   // the bit, 32 times
+        s[r] = __uint_as_float((all & 0xff800000u) | (~all & __float_as_uint(s[r])));
+    }
 }
 
 // Work item of this workgroup: workgroups go to the 8 XCDs in turn, so XCD x
@@ -97,12 +113,12 @@ __device__ __forceinline__ int xcd_item(int n) {
 // 32 keys that none of a wavefront's queries sees are passed over, and only
 // those seen in part are masked.  Bound by the matrix products and the
 // softmax's vector instructions, which two wavefronts per SIMD overlap in part:
-// 2 x 32 heads of 128, 8,192 tokens, window 1,024, bf16: 352 us, 735 TFLOP/s of
+// 2 x 32 heads of 128, 8,192 tokens, window 1,024, bf16: 340 us, 760 TFLOP/s of
 // what is visible (a large product reaches 1,210).  Of 362 us without the
 // loads' present order, 51 went without the softmax, 54 without the tiles'
 // loads.  256 queries on a tile took 394 us, 64 queries per wavefront (each
 // LDS operand used twice, at twice the accumulators) 680, three to four tiles
-// on their way 440.  Heads of 16: 33 us for 8 x 32 heads, 1,024 tokens, window
+// on their way 440.  Heads of 16: 28 us for 8 x 32 heads, 1,024 tokens, window
 // 256, the exponentials and masks of short products.
 constexpr int kWinWaves = 4;
 constexpr int kWinQ = 32 * kWinWaves;   // queries (or keys, dK and dV) per workgroup
@@ -168,11 +184,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk) mma(s, L::row_from(ka[kk] + 32 * j * L::ROWB, 0), qf[kk]);
             if constexpr (sizeof(T) == 2 && NK > 4) pace<1, NK, 4>();
-            if (kind == 1) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[r] = win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3)) ? s[r] : -INFINITY;
-            }
+            if (kind == 1) win_hide(s, win_keys(a, p, k0 + 32 * j), hi);
             float mx = s[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -283,11 +295,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) mma(s, kf[kk], qf[kk]);
         if (i + kWinWaves < ch.n) fetch(i + kWinWaves, buf ^ 1);
-        if (win_kind(a, k0, 32, pa, pb) != 2) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                s[r] = win_sees(a, p, k0 + 8 * (r >> 2) + 4 * hi + (r & 3)) ? s[r] : -INFINITY;
-        }
+        if (win_kind(a, k0, 32, pa, pb) != 2) win_hide(s, win_keys(a, p, k0), hi);
         float mx = s[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -354,7 +362,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // and Delta as the keys' kernel reads them.  Delta is formed from the stored,
 // rounded output.  Tiles and bounds as in the forward, three products where
 // that has two: 32 heads on 8 of 128, 2 x 4,096 padded tokens, window 1,024,
-// 16 first tokens, bf16: 205 us (the forward 156).
+// 16 first tokens, bf16: 199 us (the forward 151).
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
@@ -424,11 +432,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
                 mma(dp, L::row_from(ka[kk] + L::BYTES + 32 * j * L::ROWB, 0), gf[kk]);
             }
             if constexpr (sizeof(T) == 2 && NK > 1) pace<1, 2 * NK, 4>();
-            if (kind == 1) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[r] = win_sees(a, p, k0 + 32 * j + 8 * (r >> 2) + 4 * hi + (r & 3)) ? s[r] : -INFINITY;
-            }
+            if (kind == 1) win_hide(s, win_keys(a, p, k0 + 32 * j), hi);
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, -lse2)) * (dp[r] - delta);
@@ -478,7 +482,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // are summed in a fixed order; an unsplit block is stored at once.  Keys stay
 // in registers and queries pass by, so shared heads' gradients need no sum
 // afterwards.  Four products, and registers for no more than one of the score
-// tiles at a time: 283 us for the case above (loads in two bursts, as in the
+// tiles at a time: 273 us for the case above (loads in two bursts, as in the
 // other kernels, took 12% more).  float32 at D = 64 runs two wavefronts per SIMD
 // (332 us for 32 heads on 8, 2,048 tokens, causal; 368 with one).
 template <typename T, int D> struct WinBwdCfg {
@@ -572,11 +576,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             for (int kk = 0; kk < NK; ++kk)
                 mma(s, L::row_from(rows, kk), kk < KR ? kf[kk < KR ? kk : 0] : klast[kk < KR ? 0 : kk - KR][threadIdx.x]);
             if constexpr (sizeof(T) == 2 && NK > 3) pace<1, NK, 3>();
-            if (kind == 1) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[r] = win_sees(a, pa + 8 * (r >> 2) + 4 * hi + (r & 3), kw + n) ? s[r] : -INFINITY;
-            }
+            if (kind == 1) win_hide(s, win_rows(a, pa, kw + n), hi);
             float w[16];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
