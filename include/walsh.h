@@ -447,20 +447,24 @@ int walsh_prefill_attention(const void *q, int64_t q_sb, int64_t q_sh, int64_t q
  * v (k and q).  k and v within the lengths must be finite: what the mask hides
  * from a row enters its sums with a weight of 0.
  *
- * walsh_window_attention_fwd: lse [B, H, Tq] or null.
- * walsh_window_attention_bwd: go the gradient of o, in o's dtype; dq dense
+ * walsh_window_attention_fwd: lse [B, H, Tq] or null; rest, bf16, dense
+ *   [B, H, Tq, D] or null, takes what rounding took from o.
+ * walsh_window_attention_bwd: rest as the forward left it, or null (the
+ *   gradients a little less exact); go the gradient of o, in o's dtype; dq dense
  *   [B, H, Tq, D], dk and dv dense [B, G, Tk, D], overwritten (Tq, Tk >= 1).
  *   Sums are formed in a fixed order: the same call gives the same bits. */
 int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k, const void *v,
                                int64_t kv_sb, int64_t kv_sh, int64_t kv_st, int64_t B, int64_t H, int64_t G, int64_t Tq,
                                int64_t Tk, int64_t D, int64_t window, int64_t sinks, const int *lengths, float scale,
-                               void *o, int64_t o_sb, int64_t o_sh, int64_t o_st, float *lse, int dtype, void *stream);
+                               void *o, int64_t o_sb, int64_t o_sh, int64_t o_st, float *lse, void *rest, int dtype,
+                               void *stream);
 int64_t walsh_window_attention_bwd_workspace_bytes(int64_t B, int64_t H, int64_t G, int64_t Tq, int64_t Tk, int64_t D,
                                                    int64_t window, int64_t sinks, int dtype);
 int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k, const void *v,
                                int64_t kv_sb, int64_t kv_sh, int64_t kv_st, const void *o, int64_t o_sb, int64_t o_sh,
                                int64_t o_st, const void *go, int64_t go_sb, int64_t go_sh, int64_t go_st,
-                               const float *lse, int64_t B, int64_t H, int64_t G, int64_t Tq, int64_t Tk, int64_t D,
+                               const float *lse, const void *rest, int64_t B, int64_t H, int64_t G, int64_t Tq,
+                               int64_t Tk, int64_t D,
                                int64_t window, int64_t sinks, const int *lengths, float scale, void *dq, void *dk,
                                void *dv, int dtype, void *work, int64_t work_bytes, void *stream);
 

@@ -158,6 +158,32 @@ def test_window_attention_layouts_and_partial_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,D", [(1, 150, 64), (80, 130, 32)])
+def test_window_attention_rest_of_the_output(B, T, D):
+    """What rounding took from the output: at most half a step of it, nothing
+    in rows that see nothing; the backward's row sums come closer with it."""
+    from src.model import kernels
+    q, k, v, go = make(B, 4, 2, T, T, D, torch.bfloat16, 12)
+    ln = torch.full((B,), T - 7, dtype=torch.int32, device="cuda")
+    o, lse, rest = kernels.window_attention(q, k, v, 50, 3, ln, need_rest=True)
+    assert torch.equal(o, kernels.window_attention(q, k, v, 50, 3, ln)) and rest.shape == o.shape
+    assert (rest.float().abs() <= 2.0 ** -8 * o.float().abs()).all() and rest.any() and not rest[:, :, T - 7:].any()
+    r = oatt.window_attention_f64(*(t.detach().double().cpu().numpy() for t in (q[:2], k[:2], v[:2])), 50, 3,
+                                  ln[:2].cpu().numpy(), go=go[:2].double().cpu().numpy())
+    err = []
+    for x in (rest, None):
+        dq, dk, dv = kernels.window_attention_bwd(q, k, v, o, lse, go, 50, 3, ln, rest=x)
+        err.append([float(np.linalg.norm(a[:2].double().cpu().numpy() - r[n]) / np.linalg.norm(r[n]))
+                    for a, n in ((dq, "dq"), (dk, "dk"), (dv, "dv"))])
+    print(err, flush=True)
+    assert err[0][0] < err[1][0] and err[0][1] < err[1][1] and err[0][2] == err[1][2]
+    o32, lse, rest = kernels.window_attention(q.float(), k.float(), v.float(), 50, 3, need_rest=True)
+    assert rest is None and lse is not None
+    with pytest.raises(AssertionError, match="rest"):
+        kernels.window_attention_bwd(q, k, v, o, lse, go, 50, 3, ln, rest=o[:, :, 1:])
+
+
+@pytest.mark.gpu
 def test_window_attention_padding_may_hold_anything():
     """Positions past a sequence's length hold no values: NaN and infinities
     there reach neither outputs nor gradients of the others."""
@@ -262,16 +288,16 @@ def test_window_entry_points_check_before_they_launch():
     L = _hip.lib()
     p = 4096
 
-    def fwd(B=1, H=2, G=1, Tq=8, Tk=8, D=64, st=64, q=p, scale=0.1, dtype=1):
+    def fwd(B=1, H=2, G=1, Tq=8, Tk=8, D=64, st=64, q=p, scale=0.1, dtype=1, rest=None):
         return L.walsh_window_attention_fwd(q, 1 << 20, 1 << 16, st, p, p, 1 << 20, 1 << 16, 64, B, H, G, Tq, Tk, D, 4,
-                                            1, None, scale, p, 1 << 20, 1 << 16, 64, p, dtype, None)
+                                            1, None, scale, p, 1 << 20, 1 << 16, 64, p, rest, dtype, None)
 
     def bwd(Tq=8, Tk=8, work=1 << 30, dq=p):
         return L.walsh_window_attention_bwd(p, 1 << 20, 1 << 16, 64, p, p, 1 << 20, 1 << 16, 64, p, 1 << 20, 1 << 16, 64,
-                                            p, 1 << 20, 1 << 16, 64, p, 1, 2, 1, Tq, Tk, 64, 4, 1, None, 0.1, dq, p, p,
+                                            p, 1 << 20, 1 << 16, 64, p, None, 1, 2, 1, Tq, Tk, 64, 4, 1, None, 0.1, dq, p, p,
                                             1, p, work, None)
     for kw, rc in ((dict(H=3, G=2), -1), (dict(Tq=(1 << 24) + 1), -1), (dict(D=24), -2), (dict(st=60), -2),
-                   (dict(st=1 << 23), -2), (dict(q=p + 8), -2), (dict(scale=0.0), -1), (dict(dtype=5), -2),
+                   (dict(st=1 << 23), -2), (dict(q=p + 8), -2), (dict(rest=p + 8), -2), (dict(scale=0.0), -1), (dict(dtype=5), -2),
                    (dict(B=1 << 14, H=1 << 10, Tq=128), -2), (dict(B=1 << 60, H=1 << 30), -2),
                    (dict(B=4, H=32, Tq=1 << 24, Tk=1 << 24), -2)):
         assert fwd(**kw) == rc, kw

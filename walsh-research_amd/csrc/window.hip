@@ -42,6 +42,7 @@ struct WinArgs {
     const int *lengths;   // [B] or null
     void *o;
     float *lse;           // [B, H, Tq]
+    void *rest;           // [B, H, Tq, D] or null (bf16): what rounding took from o
     WinTensor sq, skv, so;
     int B, H, G, Tq, Tk, W, S;
     float sl2;            // scale * log2(e)
@@ -80,7 +81,7 @@ __device__ __forceinline__ int win_kind(const WinArgs &a, int k0, int n, int pa,
 // Of 32 consecutive keys from k0 the ones that position p sees, and of 32
 // consecutive positions from p0 the ones that see key j, as bits; and scores
 // by such bits: row 8 (r / 4) + 4 hi + r % 4 of a result is bit 8 (r / 4) + r % 4
-// of bits >> 4 hi.  (Two instructions a score; comparing positions took eight.)
+// of bits >> 4 hi.  (Three instructions a score; comparing positions took eight.)
 __device__ __forceinline__ uint32_t bits_below(int n) { return (uint32_t)((1ull << max(0, min(n, 32))) - 1); }
 __device__ __forceinline__ uint32_t win_keys(const WinArgs &a, int p, int k0) {
     const int n = p - k0 + 1, W = a.W > 0 ? a.W : 1 << 29;
@@ -96,6 +97,20 @@ __device__ __forceinline__ void win_hide(f32x16 &s, uint32_t seen, int hi) {
     for (int r = 0; r < 16; ++r) {
         const uint32_t all = (uint32_t)((int)(hidden << (31 - 8 * (r >> 2) - (r & 3))) >> 31);   // the bit, 32 times
         s[r] = __uint_as_float((all & 0xff800000u) | (~all & __float_as_uint(s[r])));
+    }
+}
+
+// Four values of an output row, zeros where the row sees nothing, and what
+// their rounding took from them.
+template <typename T> __device__ __forceinline__ void win_store(const WinArgs &a, T *o, int64_t dense, f32x4 v, bool live) {
+    v = live ? v : f32x4{0.f, 0.f, 0.f, 0.f};
+    store4(o, v);
+    if constexpr (sizeof(T) == 2) {
+        if (a.rest) {
+            const uint32_t u0 = pack_bf16x2(v.x, v.y), u1 = pack_bf16x2(v.z, v.w);
+            store4((T *)a.rest + dense, v - f32x4{__uint_as_float(u0 << 16), __uint_as_float(u0 & 0xffff0000u),
+                                                  __uint_as_float(u1 << 16), __uint_as_float(u1 & 0xffff0000u)});
+        }
     }
 }
 
@@ -233,7 +248,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             const int d = 32 * c + 8 * t + 4 * hi;
             if (D % 32 && d >= D) continue;
             const f32x4 v = f32x4{acc[c][4 * t], acc[c][4 * t + 1], acc[c][4 * t + 2], acc[c][4 * t + 3]} * inv;
-            store4(op + d, live ? v : f32x4{0.f, 0.f, 0.f, 0.f});
+            win_store(a, op + d, (((int64_t)b * a.H + h) * a.Tq + qi) * D + d, v, live);
         }
     if (a.lse && hi == 0)
         a.lse[((int64_t)b * a.H + h) * a.Tq + qi] = live ? (m * a.sl2 + log2f(l)) * (1.f / kLog2e) : -INFINITY;
@@ -350,8 +365,8 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             v += load4((const float *)(smem + w * WinSplitCfg<T, D>::WAVE) + r * D + d) * f;
             ll += stat[w][1][r] * f;
         }
-        store4((T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)q * a.so.st + d,
-               live ? v * (1.f / ll) : f32x4{0.f, 0.f, 0.f, 0.f});
+        win_store(a, (T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)q * a.so.st + d,
+                  (((int64_t)b * a.H + h) * a.Tq + q) * D + d, v * (1.f / ll), live);
         if (a.lse && d == 0)
             a.lse[((int64_t)b * a.H + h) * a.Tq + q] = live ? (mm * a.sl2 + log2f(ll)) * (1.f / kLog2e) : -INFINITY;
     }
@@ -359,10 +374,13 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 
 // ---------------------------------------------------------------- backward: queries
 // dQ of 32 queries per wavefront, over the keys they see; also the rows' lse
-// and Delta as the keys' kernel reads them.  Delta is formed from the stored,
-// rounded output.  Tiles and bounds as in the forward, three products where
+// and Delta as the keys' kernel reads them.  Delta is formed from the output and
+// what its rounding to bf16 took: the rounded one alone shifts a row's dS all
+// to one side, and leaves dQ and dK 2.5 to 2.65e-3 off instead of 2.4e-3 (one
+// rounding of the results alone: 1.66e-3), for 4% less time.  Tiles and bounds as in the forward, three products where
 // that has two: 32 heads on 8 of 128, 2 x 4,096 padded tokens, window 1,024,
-// 16 first tokens, bf16: 199 us (the forward 151).
+// 16 first tokens, bf16: 205 us (the forward 151, with
+// what rounding took 170).
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
@@ -391,6 +409,11 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             qf[kk] = load_frag(qp + 16 * kk + 8 * hi);
             gf[kk] = load_frag(gp + 16 * kk + 8 * hi);
             delta += dot(gf[kk], load_frag(op + 16 * kk + 8 * hi));
+        }
+        if (sizeof(T) == 2 && a.rest) {
+            const T *rp = (const T *)a.rest + (((int64_t)b * a.H + h) * a.Tq + qc) * D;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) delta += dot(gf[kk], load_frag(rp + 16 * kk + 8 * hi));
         }
         delta = half_sum(delta);
     }
@@ -737,19 +760,21 @@ WALSH_EXPORT int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t
                                             const void *v, int64_t kv_sb, int64_t kv_sh, int64_t kv_st, int64_t B,
                                             int64_t H, int64_t G, int64_t Tq, int64_t Tk, int64_t D, int64_t window,
                                             int64_t sinks, const int *lengths, float scale, void *o, int64_t o_sb,
-                                            int64_t o_sh, int64_t o_st, float *lse, int dtype, void *stream) {
+                                            int64_t o_sh, int64_t o_st, float *lse, void *rest, int dtype,
+                                            void *stream) {
     const char *fn = "walsh_window_attention_fwd";
     WinArgs a{};
     a.scale = scale;
     int rc = win_check(fn, a, B, H, G, Tq, Tk, D, dtype);
     if (rc) return rc;
     if (B == 0 || Tq == 0) return WALSH_OK;
-    a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.o = o, a.lse = lse;
+    a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.o = o, a.lse = lse, a.rest = dtype == WALSH_BF16 ? rest : nullptr;
     a.sq = {q_sb, q_sh, q_st}, a.skv = {kv_sb, kv_sh, kv_st}, a.so = {o_sb, o_sh, o_st};
     rc = win_check_tensor(fn, "q", q, a.sq, B, H, Tq, D);
     if (!rc && Tk) rc = win_check_tensor(fn, "k", k, a.skv, B, G, Tk, D);
     if (!rc && Tk) rc = win_check_tensor(fn, "v", v, a.skv, B, G, Tk, D);
     if (!rc) rc = win_check_tensor(fn, "o", o, a.so, B, H, Tq, D);
+    if (!rc && (uintptr_t)rest % 16) rc = set_error(WALSH_ENOTSUP, "%s: rest must be 16-byte aligned", fn);
     if (rc) return rc;
     a.B = (int)B, a.H = (int)H, a.G = (int)G, a.Tq = (int)Tq, a.Tk = (int)Tk;
     a.W = window > 0 && window < Tk ? (int)window : 0;
@@ -792,8 +817,8 @@ WALSH_EXPORT int64_t walsh_window_attention_bwd_workspace_bytes(int64_t B, int64
 WALSH_EXPORT int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k,
                                             const void *v, int64_t kv_sb, int64_t kv_sh, int64_t kv_st, const void *o,
                                             int64_t o_sb, int64_t o_sh, int64_t o_st, const void *go, int64_t go_sb,
-                                            int64_t go_sh, int64_t go_st, const float *lse, int64_t B, int64_t H,
-                                            int64_t G, int64_t Tq, int64_t Tk, int64_t D, int64_t window, int64_t sinks,
+                                            int64_t go_sh, int64_t go_st, const float *lse, const void *rest, int64_t B,
+                                            int64_t H, int64_t G, int64_t Tq, int64_t Tk, int64_t D, int64_t window, int64_t sinks,
                                             const int *lengths, float scale, void *dq, void *dk, void *dv, int dtype,
                                             void *work, int64_t work_bytes, void *stream) {
     const char *fn = "walsh_window_attention_bwd";
@@ -804,7 +829,7 @@ WALSH_EXPORT int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t
     if (B == 0) return WALSH_OK;
     if (Tq == 0 || Tk == 0) return set_error(WALSH_EINVAL, "%s: no queries or no keys: the gradients are zeros", fn);
     a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.o = const_cast<void *>(o), a.lse = const_cast<float *>(lse);
-    a.go = go, a.dq = dq, a.dk = dk, a.dv = dv;
+    a.go = go, a.dq = dq, a.dk = dk, a.dv = dv, a.rest = dtype == WALSH_BF16 ? const_cast<void *>(rest) : nullptr;
     a.sq = {q_sb, q_sh, q_st}, a.skv = {kv_sb, kv_sh, kv_st}, a.so = {o_sb, o_sh, o_st}, a.sgo = {go_sb, go_sh, go_st};
     rc = win_check_tensor(fn, "q", q, a.sq, B, H, Tq, D);
     if (!rc) rc = win_check_tensor(fn, "k", k, a.skv, B, G, Tk, D);
@@ -813,8 +838,8 @@ WALSH_EXPORT int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t
     if (!rc) rc = win_check_tensor(fn, "go", go, a.sgo, B, H, Tq, D);
     if (rc) return rc;
     if (!lse || !dq || !dk || !dv || !work) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
-    if ((uintptr_t)dq % 16 || (uintptr_t)dk % 16 || (uintptr_t)dv % 16 || (uintptr_t)work % 16)
-        return set_error(WALSH_ENOTSUP, "%s: the gradients and the workspace must be 16-byte aligned", fn);
+    if ((uintptr_t)rest % 16 || (uintptr_t)dq % 16 || (uintptr_t)dk % 16 || (uintptr_t)dv % 16 || (uintptr_t)work % 16)
+        return set_error(WALSH_ENOTSUP, "%s: rest, the gradients and the workspace must be 16-byte aligned", fn);
     a.B = (int)B, a.H = (int)H, a.G = (int)G, a.Tq = (int)Tq, a.Tk = (int)Tk;
     a.W = window > 0 && window < Tk ? (int)window : 0;
     a.S = sinks < 0 ? 0 : (int)(sinks < Tk ? sinks : Tk);

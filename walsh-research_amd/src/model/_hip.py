@@ -83,10 +83,10 @@ SIGNATURES = {
     "walsh_prefill_attention": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                      ctypes.c_float, _P, _I64, _I64, _I64, _I, _P]),
     "walsh_window_attention_fwd": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
-                                        _I64, _I64, _I64, _P, _F, _P, _I64, _I64, _I64, _P, _I, _P]),
+                                        _I64, _I64, _I64, _P, _F, _P, _I64, _I64, _I64, _P, _P, _I, _P]),
     "walsh_window_attention_bwd_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I]),
     "walsh_window_attention_bwd": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64,
-                                        _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _F, _P, _P,
+                                        _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _F, _P, _P,
                                         _P, _I, _P, _I64, _P]),
     "walsh_paged_decode_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I]),
     "walsh_paged_decode_attention": (_I, [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P,

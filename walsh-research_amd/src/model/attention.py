@@ -21,8 +21,8 @@ class WindowAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, lengths, scale):
-        o, lse = kernels.window_attention(q, k, v, window, sinks, lengths, scale, need_lse=True)
-        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        o, lse, rest = kernels.window_attention(q, k, v, window, sinks, lengths, scale, need_rest=True)
+        ctx.save_for_backward(q, k, v, o, lse, lengths, rest)
         ctx.args = (window, sinks, scale)
         return o
 
@@ -31,9 +31,9 @@ class WindowAttentionFunction(torch.autograd.Function):
     def backward(ctx, go):
         if not first_order(go):
             raise RuntimeError("window_attention: its gradient takes one plain tensor (no batched or transformed ones)")
-        q, k, v, o, lse, lengths = ctx.saved_tensors
+        q, k, v, o, lse, lengths, rest = ctx.saved_tensors
         window, sinks, scale = ctx.args
-        grads = kernels.window_attention_bwd(q, k, v, o, lse, go, window, sinks, lengths, scale)
+        grads = kernels.window_attention_bwd(q, k, v, o, lse, go, window, sinks, lengths, scale, rest)
         return tuple(g if n else None for g, n in zip(grads, ctx.needs_input_grad)) + (None,) * 4
 
 

@@ -920,11 +920,14 @@ def _check_window_attention(fn, q, k, v, lengths):
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
-                     lengths: torch.Tensor = None, scale: float = None, need_lse: bool = False):
+                     lengths: torch.Tensor = None, scale: float = None, need_lse: bool = False,
+                     need_rest: bool = False):
     """Causal attention over the last ``window`` keys and the first ``sinks``
     ones: q [B, H, Tq, D], k / v [B, G, Tk, D] (G dividing H) -> contiguous
     [B, H, Tq, D], with ``need_lse`` also the rows' float32 log sum of
-    exponentials [B, H, Tq].  The queries are the last Tq of Tk positions;
+    exponentials [B, H, Tq], with ``need_rest`` (after lse) what rounding to
+    bf16 took from the output, in its shape (None in float32): both are for
+    window_attention_bwd.  The queries are the last Tq of Tk positions;
     ``window`` <= 0 is no window; ``lengths`` (int32 [B], on the device) are
     the keys that each sequence has of Tk.  Rows that see no key are zeros
     (lse -inf).  Values of keys within the lengths have to be finite, also
@@ -939,26 +942,32 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     scale = D ** -0.5 if scale is None else float(scale)
     lengths = None if lengths is None else lengths.contiguous()
     o = torch.empty(B, H, Tq, D, device=q.device, dtype=q.dtype)
-    lse = torch.empty(B, H, Tq, device=q.device, dtype=torch.float32) if need_lse else None
+    lse = torch.empty(B, H, Tq, device=q.device, dtype=torch.float32) if need_lse or need_rest else None
+    rest = torch.empty_like(o) if need_rest and q.dtype == torch.bfloat16 else None
     span = min(Tk, window + sinks) if window > 0 else Tk
     _hip.call_on(q.get_device(), "walsh_window_attention_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
                  *k.stride()[:3], B, H, G, Tq, Tk, D, int(window), int(sinks), _hip.ptr(lengths), scale, o.data_ptr(),
-                 *o.stride()[:3], _hip.ptr(lse), _hip.dtype_code(q.dtype),
+                 *o.stride()[:3], _hip.ptr(lse), _hip.ptr(rest), _hip.dtype_code(q.dtype),
                  kernel="window_fwd_kernel", nbytes=2 * B * D * (H * Tq + G * Tk) * q.element_size(),
                  flops=4 * B * H * Tq * span * D)
-    return (o, lse) if need_lse else o
+    return (o, lse, rest) if need_rest else (o, lse) if need_lse else o
 
 
 def window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                          go: torch.Tensor, window: int, sinks: int = 0, lengths: torch.Tensor = None,
-                         scale: float = None):
+                         scale: float = None, rest: torch.Tensor = None):
     """(dq, dk, dv) of window_attention for the gradient ``go`` of its output:
-    contiguous, in the tensors' dtype.  The same call gives the same bits."""
+    contiguous, in the tensors' dtype.  ``rest`` is what the forward gave with
+    ``need_rest``; without it bf16 gradients are a little less exact.  The same
+    call gives the same bits."""
     _check_window_attention("window_attention_bwd", q, k, v, lengths)
     assert go.shape == o.shape == q.shape and lse.shape == q.shape[:3], "window_attention_bwd: o, go as q, lse [B, H, Tq]"
     if go.dtype != q.dtype or o.dtype != q.dtype or lse.dtype != torch.float32:
         raise TypeError(f"window_attention_bwd: o, go in {q.dtype} and lse in float32")
-    _hip.same_device("window_attention_bwd", q, o, lse, go)
+    if rest is not None:
+        assert rest.shape == q.shape and rest.dtype == q.dtype, "window_attention_bwd: rest as o"
+        rest = rest.contiguous()
+    _hip.same_device("window_attention_bwd", q, o, lse, go, rest)
     q, k, v, o, go = (_attn_rows(t) for t in (q, k, v, o, go))
     if v.stride() != k.stride():
         k, v = k.contiguous(), v.contiguous()
@@ -976,7 +985,7 @@ def window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     ws = torch.empty(nws, device=q.device, dtype=torch.uint8)
     span = min(Tk, window + sinks) if window > 0 else Tk
     _hip.call_on(q.get_device(), "walsh_window_attention_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
-                 *k.stride()[:3], o.data_ptr(), *o.stride()[:3], go.data_ptr(), *go.stride()[:3], lse.data_ptr(), B, H, G,
+                 *k.stride()[:3], o.data_ptr(), *o.stride()[:3], go.data_ptr(), *go.stride()[:3], lse.data_ptr(), _hip.ptr(rest), B, H, G,
                  Tq, Tk, D, int(window), int(sinks), _hip.ptr(lengths), scale, dq.data_ptr(), dk.data_ptr(),
                  dv.data_ptr(), dt, ws.data_ptr(), nws, kernel="window_bwd_kernels",
                  nbytes=4 * B * D * (H * Tq + G * Tk) * q.element_size(), flops=14 * B * H * Tq * span * D)
