@@ -377,10 +377,10 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // and Delta as the keys' kernel reads them.  Delta is formed from the output and
 // what its rounding to bf16 took: the rounded one alone shifts a row's dS all
 // to one side, and leaves dQ and dK 2.5 to 2.65e-3 off instead of 2.4e-3 (one
-// rounding of the results alone: 1.66e-3), for 4% less time.  Tiles and bounds as in the forward, three products where
-// that has two: 32 heads on 8 of 128, 2 x 4,096 padded tokens, window 1,024,
-// 16 first tokens, bf16: 205 us (the forward 151, with
-// what rounding took 170).
+// rounding of the results alone: 1.66e-3), for 4% less time.  Tiles and bounds
+// as in the forward, three products where that has two: 32 heads on 8 of 128,
+// 2 x 4,096 padded tokens, window 1,024, 16 first tokens, bf16: 205 us (the
+// forward 151, with what rounding took 170).
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
