@@ -112,6 +112,30 @@ def test_paged_decode_of_infinite_scores_is_no_number(H, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("H,G,D,lengths,parts", [
+    # parts (float32, bf16) of a table as long: joined by 80 and 144 threads' worth of head_dim 16, by 96, 160 and 224
+    # of head_dim 32, by whole wavefronts
+    (2, 2, 16, [9000, 200], (18, 18)), (4, 1, 16, [17000], (34, 34)), (3, 1, 32, [2500, 64], (10, 5)),
+    (2, 2, 32, [4900], (20, 10)), (6, 1, 32, [6700, 3000], (27, 14)), (2, 1, 32, [9900, 513], (39, 20)),
+    (2, 1, 64, [2600], (21, 11)), (1, 1, 128, [2600], (21, 21)),
+])
+def test_paged_decode_joins_scores_of_one_sign(H, G, D, lengths, parts, sign, dtype):
+    """Every logit below -120 or above 120: a maximum of the parts that any
+    other number enters leaves no weight at all, or infinite ones."""
+    from src.model import _hip
+    page, B = 64, len(lengths)
+    q, kp, vp, table, n = make(B, H, G, D, page, lengths, dtype, D + len(lengths))
+    table = table[:, :-1]                          # exactly as many pages as the longest sequence has
+    reach = (130.0 / D ** 0.5) ** 0.5
+    q, kp = (reach * 1.01 + 0.02 * q.float()).to(dtype), (sign * reach * 1.01 + 0.02 * kp.float()).to(dtype)
+    got = _hip.lib().walsh_paged_decode_workspace_bytes(B, H, G, table.shape[1], page, D, 0, 0, _hip.dtype_code(dtype))
+    assert got == B * H * parts[dtype == torch.bfloat16] * (D + 2) * 4
+    check(decode(q, kp, vp, table, n), q, kp, vp, table, n, 0, 0)
+
+
+@pytest.mark.gpu
 def test_paged_decode_takes_a_dense_cache_as_one_page_per_sequence():
     """[B, H, Lmax, D] storage of any length is B pages; the result equals the
     dense decode attention's up to the order of sums."""

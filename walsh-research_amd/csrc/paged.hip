@@ -391,7 +391,7 @@ template <int D, int R> __global__ __launch_bounds__(64 * kPgWaves) void paged_d
 }
 
 // The chunks' parts of one (sequence, query head) joined: blockDim.x / D groups
-// of D threads take every so many parts each.  Latency of the launch and of
+// of D threads (whole wavefronts) take every so many parts each.  Latency of the launch and of
 // two dependent loads: 3.8 us for 32 rows of 16 parts, 8 for 128 of 128.
 template <typename T, int D> __global__ __launch_bounds__(1024) void paged_decode_join_kernel(PgArgs a) {
     __shared__ float num_l[1024], den_l[1024 / D], max_l[16];
@@ -407,7 +407,7 @@ template <typename T, int D> __global__ __launch_bounds__(1024) void paged_decod
     for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
     if ((tid & 63) == 0) max_l[tid >> 6] = mm;
     __syncthreads();
-    for (int w = 0; w < ((int)blockDim.x + 63) / 64; ++w) mm = fmaxf(mm, max_l[w]);
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) mm = fmaxf(mm, max_l[w]);
     float num = 0.f, den = 0.f;
 #pragma unroll 8
     for (int s = grp; s < ns; s += groups) {
@@ -574,10 +574,10 @@ WALSH_EXPORT int walsh_paged_decode_attention(const void *q, int64_t q_sb, int64
         }
         if (sizeof(T) == 2 || R > 4)
             launch(paged_decode_kernel<T, DD>, grid, threads, (uint32_t)PgCfg<T, DD>::LDS, s, a);
-        // about four parts per group of threads, a wavefront at least
-        int64_t groups = ceil_div(ns, 4);
+        // about four parts per group of threads, whole wavefronts (the maximum goes over all 64 lanes)
+        constexpr int64_t wave = DD < 64 ? 64 / DD : 1;
+        int64_t groups = ceil_div(ceil_div(ns, 4), wave) * wave;
         if (groups > 1024 / DD) groups = 1024 / DD;
-        if (groups * DD < 64) groups = 64 / DD;
         if (ns > 1)
             launch(paged_decode_join_kernel<T, DD>, dim3((unsigned)(B * H)), dim3((unsigned)(groups * DD)), 0, s, a);
     });
