@@ -510,7 +510,8 @@ int walsh_paged_kv_write(const void *k, const void *v, int64_t sb, int64_t st, i
  *   top_k    the k largest logits stay (of equal ones the lowest indexes);
  *            k <= 0 or >= V: all
  *   top_p    of these, in descending order, a token stays while the weight
- *            before it is below top_p of their sum; >= 1: all
+ *            before it is below top_p of their sum; >= 1 (or no number): all,
+ *            <= 0: the first alone
  *   min_p    of these, those with w >= min_p stay
  *   out      the first index whose running sum of what stays, in index order,
  *            exceeds u times the whole sum

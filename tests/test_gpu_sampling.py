@@ -141,6 +141,26 @@ def test_sample_more_asked_for_than_there_are_numbers(V):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1, 300, 20000, 60000])
+def test_sample_top_p_of_nothing_and_less_keeps_the_first(V, dtype):
+    """A top_p at or below 0, for every row or for some of them, leaves the
+    largest logit alone; one that is no number leaves all."""
+    z, u = rows(6, V, dtype, V + 1)
+    first = torch.from_numpy(np.array([np.argmax(r) for r in z.double().numpy()]))
+    each = torch.tensor([-0.5, 0.9, 0.0, -1.0, -float("inf"), float("nan")])
+    for k in (0, 1, 40, V):
+        for m in (0.0, 0.05):
+            for p in (0.0, -1e-30, -0.5, -1.0, -3.0, -float("inf")):
+                assert torch.equal(run(z, u, 0.8, k, p, m), first), (k, m, p)
+            got = run(z, u, 0.8, k, each, m)
+            assert torch.equal(got[[0, 2, 3, 4]], first[[0, 2, 3, 4]]), (k, m)
+            assert torch.equal(got[[1]], run(z, u, 0.8, k, 0.9, m)[[1]])
+            assert torch.equal(got[[5]], run(z, u, 0.8, k, 1.0, m)[[5]])
+            check(z[:5], u[:5], 0.8, k, each[:5], m, got[:5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_sample_masks_of_the_lowest_value_at_any_temperature(dtype):
     """Logits masked with the type's lowest value have no weight, at
     temperatures where their distance passes float32, too."""

@@ -2,7 +2,7 @@
 //     z_i = l_i / T,   w_i = exp(z_i - max z)
 //   top-k   the k largest l (of equal ones the lowest indexes first)
 //   top-p   of these, in the same order, a token stays while the weight before
-//           it is below p of their sum (the first always stays)
+//           it is below p of their sum (the first always stays, p <= 0: alone)
 //   min-p   of these, w_i >= min_p
 //   draw    the first index whose running sum of remaining weights, in index
 //           order, exceeds u times their sum
@@ -431,7 +431,8 @@ template <typename T, int NPT> __global__ __launch_bounds__(kSmThreads) void sam
         }
     }
     const float temp = a.temperature ? a.temperature[b] : a.temperature0;
-    const float top_p = a.top_p ? a.top_p[b] : a.top_p0, min_p = a.min_p ? a.min_p[b] : a.min_p0;
+    const float share = a.top_p ? a.top_p[b] : a.top_p0, min_p = a.min_p ? a.min_p[b] : a.min_p0;
+    const float top_p = share < 0.f ? 0.f : share;                  // (what is no number keeps all)
     const int top_k = a.top_k ? a.top_k[b] : a.top_k0;
     const float u = a.u[b];
     for (int i = tid; i < kSmBins; i += kSmThreads) sh.count[i] = 0, sh.mass[i] = 0;

@@ -1090,7 +1090,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     """Tokens [B] (int64) of logits [B, V] that the uniform numbers u [B]
     (float32, in [0, 1)) pick: of the ``top_k`` largest (<= 0: all; of equal
     ones the lowest indexes), those in descending order before which less than
-    ``top_p`` of the weight lies (>= 1: all), of these the ones with at least
+    ``top_p`` of the weight lies (>= 1: all, <= 0: the first alone), of these the ones with at least
     ``min_p`` of the largest probability; the first token, in index order,
     whose running probability exceeds u.  ``temperature`` <= 0 takes the
     largest logit.  Each setting is a number or a tensor [B] (float32, top_k
