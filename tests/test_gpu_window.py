@@ -342,3 +342,111 @@ def test_window_attention_refusals_on_the_gpu():
     o = window_attention(qr, k, k, 4)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(o, (qr,), torch.ones(2, *o.shape, device="cuda"), is_grads_batched=True)
+
+
+# What a kernel call would hide from those who look at each operation: dual
+# numbers, traces, transforms and dispatch modes take the plain operations.
+
+def _small(dtype, seed=21):
+    q, k, v, go = make(2, 4, 2, 20, 26, 16, dtype, seed, "bhtd")
+    return q, k, v, go, (7, 2, torch.tensor([26, 13], dtype=torch.int32, device="cuda"))
+
+
+def _jvp_f64(q, k, v, args, t):
+    """The oracle's derivative along the tangents t: the sum of its gradients
+    against them, an output's unit direction at a time, by differences."""
+    x = [a.double().cpu().numpy() for a in (q, k, v)]
+    t = [a.double().cpu().numpy() for a in t]
+    f = lambda e: oatt.window_attention_f64(*(a + e * b for a, b in zip(x, t)), args[0], args[1],  # noqa: E731
+                                            args[2].cpu().numpy())["o"]
+    h = 1e-4
+    return (8 * (f(h) - f(-h)) - (f(2 * h) - f(-2 * h))) / (12 * h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("grad", [False, True])
+def test_window_attention_in_forward_mode(grad, dtype):
+    """A dual number's tangent arrives, whether or not a gradient is asked for
+    as well.  float32 sums of 26 keys and 16 elements: a score is off by 2^-24
+    times 16 |q| |k| / 4, a few 1e-6 of it, and the tangent's terms by as much
+    relatively; bf16 adds one rounding of the result."""
+    import torch.autograd.forward_ad as fw
+    from src.model.attention import window_attention
+    q, k, v, _, args = _small(dtype)
+    t = [torch.randn_like(a) for a in (q, k, v)]
+    want = _jvp_f64(q, k, v, args, t)
+    with fw.dual_level():
+        x = [fw.make_dual(a.requires_grad_(grad), b) for a, b in zip((q, k, v), t)]
+        o, do = fw.unpack_dual(window_attention(*x, *args))
+    assert do is not None and do.dtype == dtype
+    got = do.detach().double().cpu().numpy()
+    assert (np.abs(got - want) <= HALF[dtype] * np.abs(want) + 2e-4).all() and np.abs(want).max() > 1
+    with torch.no_grad():
+        plain = window_attention(q, k, v, *args)
+    assert (o.detach().float() - plain.float()).abs().max() <= (0.05 if dtype == torch.bfloat16 else 1e-5)
+
+
+@pytest.mark.gpu
+def test_window_attention_traced():
+    """A trace computes the operator of the inputs that it is given."""
+    from src.model.attention import window_attention
+    q, k, v, _, args = _small(torch.float32)
+    traced = torch.jit.trace(lambda *x: window_attention(*x, *args), (q, k, v), check_trace=False)
+    for seed in (1, 2):
+        x = _small(torch.float32, seed)[:3]
+        want = window_attention(*x, *args)
+        assert (traced(*x) - want).abs().max() <= 1e-5 and want.abs().max() > 0.1
+
+
+@pytest.mark.gpu
+def test_window_attention_under_transforms():
+    """torch.func's grad, jvp and vmap, against the kernels' results."""
+    from src.model.attention import window_attention
+    q, k, v, go, args = _small(torch.float32)
+    x = [a.clone().requires_grad_(True) for a in (q, k, v)]
+    want = torch.autograd.grad(window_attention(*x, *args), x, go)
+    got = torch.func.grad(lambda *x: (window_attention(*x, *args) * go).sum(), argnums=(0, 1, 2))(q, k, v)
+    assert all((a - b).abs().max() <= 1e-4 for a, b in zip(got, want))
+    _, do = torch.func.jvp(lambda q: window_attention(q, k, v, *args), (q,), (go,))
+    assert np.abs(do.double().cpu().numpy() - _jvp_f64(q, k, v, args, [go, 0 * k, 0 * v])).max() <= 2e-4
+    many = torch.stack([q, go, q + go])
+    got = torch.func.vmap(lambda q: window_attention(q, k, v, *args))(many)
+    for a, b in zip(got, many):
+        assert (a - window_attention(b, k, v, *args)).abs().max() <= 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("whole", [False, True])
+def test_window_attention_under_a_dispatch_mode(whole):
+    """A mode that counts operations sees products (over the backward alone,
+    or both), and the results are the kernels'."""
+    from torch.utils.flop_counter import FlopCounterMode
+    from src.model.attention import window_attention
+    q, k, v, go, args = _small(torch.float32)
+    x = [a.requires_grad_(True) for a in (q, k, v)]
+    want = torch.autograd.grad(window_attention(*x, *args), x, go)
+    o = None if whole else window_attention(*x, *args)
+    with FlopCounterMode(display=False) as count:
+        if whole:
+            o = window_attention(*x, *args)
+            assert count.get_total_flops() > 0
+        got = torch.autograd.grad(o, x, go)
+    assert count.get_total_flops() > 0
+    assert all((a - b).abs().max() <= 1e-4 for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_windowed_attention_layer_in_forward_mode():
+    """A layer's single token over a dense cache, too."""
+    import torch.autograd.forward_ad as fw
+    from src.model import WalshConfig
+    from src.model.chassis import CausalSelfAttention
+    layer = CausalSelfAttention(WalshConfig(n_layer=1, n_head=8, n_embd=256, algebra="hadamard", head_mixing=False,
+                                            attn_window=8, attn_sinks=1)).cuda().eval()
+    g = torch.Generator().manual_seed(3)
+    q, k, v, t = (torch.randn(2, 8, n, 32, generator=g).cuda() for n in (1, 30, 30, 1))
+    want = _jvp_f64(q, k, v, (8, 1, torch.full((2,), 30)), [t, 0 * k, 0 * v])
+    with torch.no_grad(), fw.dual_level():
+        do = fw.unpack_dual(layer._windowed(fw.make_dual(q, t), k, v, 0, True)).tangent
+    assert np.abs(do.double().cpu().numpy() - want).max() <= 2e-4 and np.abs(want).max() > 0.1

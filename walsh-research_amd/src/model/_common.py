@@ -89,6 +89,16 @@ def plain_eager() -> bool:
             and torch.utils._python_dispatch._get_current_dispatch_mode() is None)
 
 
+TENSOR_TYPES = (torch.Tensor, torch.nn.Parameter)
+
+
+def plain_tensor(t: torch.Tensor) -> bool:
+    """A tensor or parameter itself: no subclass, batched or transformed one."""
+    f = torch._C._functorch
+    return (type(t) in TENSOR_TYPES and not f.is_legacy_batchedtensor(t)
+            and not f.is_functorch_wrapped_tensor(t))
+
+
 def first_order(gy: torch.Tensor) -> bool:
     """Whether a backward may run kernels on the gradient ``gy``: it is not
     differentiated itself, and neither a transform (batched gradients, a

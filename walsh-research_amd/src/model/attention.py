@@ -5,6 +5,7 @@ The reference's attention is causal over everything (chassis.py:441-478) and
 its cache one dense tensor (:262-330); here a query may see the last
 ``window`` keys and the first ``sinks`` ones, and the cache may lie in pages.
 """
+import math
 import numbers
 from typing import List, Sequence, Union
 
@@ -12,7 +13,33 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import kernels
-from ._common import first_order
+from ._common import TENSOR_TYPES, first_order, plain_eager, plain_tensor
+
+
+def window_attention_plain(q, k, v, window, sinks=0, lengths=None, scale=None):
+    """window_attention from torch's operations, in float32 and rounded once:
+    for forward-mode derivatives, transforms, traces and modes, which have to
+    see each operation.  As in the kernels, what lies in rows without a key and
+    past the lengths reaches nothing, gradients included."""
+    B, H, Tq, D = q.shape
+    G, Tk = k.shape[1], k.shape[2]
+    scale = D ** -0.5 if scale is None else float(scale)
+    p = torch.arange(Tk - Tq, Tk, device=q.device)
+    j = torch.arange(Tk, device=q.device)
+    n = lengths[:, None] if lengths is not None else torch.full((1, 1), int(Tk), device=q.device)
+    live = (p >= 0) & (p < n)
+    sees = j <= p[:, None]
+    if window > 0:
+        sees = sees & ((j > p[:, None] - window) | (j < sinks))
+    sees = (sees | ~live[:, :, None])[:, None, None]      # a row without a key: any weights, and no output
+    live, there = live[:, None, :, None], (j < n)[:, None, :, None]
+    # no autocast: bf16 batched products with a transposed operand have faulted the GPU
+    with torch.autocast(q.device.type, enabled=False):
+        qf = torch.where(live, q.float(), 0.).reshape(B, G, H // G, Tq, D)
+        kf, vf = (torch.where(there, t.float(), 0.)[:, :, None] for t in (k, v))
+        w = torch.softmax((torch.matmul(qf, kf.transpose(3, 4)) * scale).masked_fill(~sees, -math.inf), -1)
+        o = torch.matmul(w, vf).reshape(B, H, Tq, D)
+        return torch.where(live, o, 0.).to(q.dtype)
 
 
 class WindowAttentionFunction(torch.autograd.Function):
@@ -29,11 +56,17 @@ class WindowAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        if not first_order(go):
-            raise RuntimeError("window_attention: its gradient takes one plain tensor (no batched or transformed ones)")
         q, k, v, o, lse, lengths, rest = ctx.saved_tensors
         window, sinks, scale = ctx.args
-        grads = kernels.window_attention_bwd(q, k, v, o, lse, go, window, sinks, lengths, scale, rest)
+        if first_order(go):
+            grads = kernels.window_attention_bwd(q, k, v, o, lse, go, window, sinks, lengths, scale, rest)
+        elif plain_tensor(go):
+            # a mode, trace or forward derivative looks at the backward's operations
+            with torch.enable_grad():
+                x = [t.detach().requires_grad_(True) for t in (q, k, v)]
+                grads = torch.autograd.grad(window_attention_plain(*x, window, sinks, lengths, scale), x, go)
+        else:
+            raise RuntimeError("window_attention: its gradient takes one plain tensor (no batched or transformed ones)")
         return tuple(g if n else None for g, n in zip(grads, ctx.needs_input_grad)) + (None,) * 4
 
 
@@ -42,7 +75,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     """softmax(scale q k^T + mask) v with the mask of kernels.window_attention
     (key j <= query position p, and j > p - window or j < sinks): q
     [B, H, Tq, D], k / v [B, G, Tk, D] -> [B, H, Tq, D], differentiable in
-    q, k and v."""
+    q, k and v: once backward on the kernels; forward-mode derivatives,
+    torch.func's transforms, traces and dispatch modes take
+    window_attention_plain, whose [Tq, Tk] weights lie in memory."""
+    if not (type(q) in TENSOR_TYPES and type(k) in TENSOR_TYPES and type(v) in TENSOR_TYPES and plain_eager()):
+        kernels.check_window_attention("window_attention", q, k, v, lengths, scale)
+        return window_attention_plain(q, k, v, window, sinks, lengths, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return WindowAttentionFunction.apply(q, k, v, window, sinks, lengths, scale)
     return kernels.window_attention(q, k, v, window, sinks, lengths, scale)

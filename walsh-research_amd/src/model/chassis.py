@@ -347,7 +347,7 @@ class CausalSelfAttention(nn.Module):
         for head sizes that they do not take."""
         T, total = q.size(2), k.size(2)
         if drop == 0 and kernels.window_attention_supported(q):
-            if T == 1 and dense_cache and not (torch.is_grad_enabled() and q.requires_grad):
+            if T == 1 and dense_cache and not (torch.is_grad_enabled() and q.requires_grad) and plain_eager():
                 # one row over the cache, read in place as one page per
                 # sequence: split over its length
                 table = torch.arange(q.size(0), device=q.device, dtype=torch.int32)[:, None]

@@ -902,7 +902,7 @@ def _attn_rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _check_window_attention(fn, q, k, v, lengths):
+def check_window_attention(fn, q, k, v, lengths, scale=None):
     _hip.require_device(q, "query")
     assert q.dim() == 4 and k.dim() == 4 and k.shape == v.shape, f"{fn}: q [B, H, Tq, D], k and v [B, G, Tk, D]"
     B, H, Tq, D = q.shape
@@ -917,6 +917,9 @@ def _check_window_attention(fn, q, k, v, lengths):
         assert lengths.shape == (B,), f"{fn}: lengths [B]"
         if lengths.dtype != torch.int32:
             raise TypeError(f"{fn}: lengths are int32, got {lengths.dtype}")
+    _hip.dtype_code(q.dtype)
+    if scale is not None and not 0.0 < scale <= 1e6:
+        raise _hip.WalshHipError(f"{fn}: the scale must be positive and at most 1e6")
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
@@ -933,7 +936,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     (lse -inf).  Values of keys within the lengths have to be finite, also
     where the mask hides them from some rows.  Not differentiable by itself:
     src.model.attention.window_attention is."""
-    _check_window_attention("window_attention", q, k, v, lengths)
+    check_window_attention("window_attention", q, k, v, lengths)
     q, k, v = _attn_rows(q), _attn_rows(k), _attn_rows(v)
     if v.stride() != k.stride():
         k, v = k.contiguous(), v.contiguous()
@@ -960,7 +963,7 @@ def window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     contiguous, in the tensors' dtype.  ``rest`` is what the forward gave with
     ``need_rest``; without it bf16 gradients are a little less exact.  The same
     call gives the same bits."""
-    _check_window_attention("window_attention_bwd", q, k, v, lengths)
+    check_window_attention("window_attention_bwd", q, k, v, lengths)
     assert go.shape == o.shape == q.shape and lse.shape == q.shape[:3], "window_attention_bwd: o, go as q, lse [B, H, Tq]"
     if go.dtype != q.dtype or o.dtype != q.dtype or lse.dtype != torch.float32:
         raise TypeError(f"window_attention_bwd: o, go in {q.dtype} and lse in float32")
