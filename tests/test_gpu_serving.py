@@ -306,3 +306,33 @@ def test_generate_takes_lengths_as_a_tensor_and_no_other_cache():
     assert torch.equal(got, want)
     with pytest.raises(TypeError, match="PagedKVCache"):
         model.generate(idx, 3, kv_cache=object())
+
+
+def test_windowed_single_token_keeps_the_gradients_of_its_keys(monkeypatch):
+    """Keys and values that are trained while the queries are frozen: a single
+    token over a dense cache gives them their gradients."""
+    from src.model import KVCache, kernels
+    layer = make(C=256, n_head=8, attn_window=8, attn_sinks=1).layers[0].attention
+    for p in layer.wq.parameters():
+        p.requires_grad_(False)
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(2, 13, 256, generator=g).cuda()
+    # rotary angle 0 throughout: cos 1, sin 0
+    freqs = torch.polar(torch.ones(13, 16), torch.zeros(13, 16)).cuda()
+
+    def step():
+        kv = KVCache(1, 64, 8, 32, torch.device("cuda"), dtype=torch.float32, batch=2)
+        with torch.no_grad():
+            layer(x[:, :12], freqs[:12], kv)
+            kv.increment(12)
+        layer.zero_grad()
+        layer(x[:, 12:], freqs[12:], kv).square().sum().backward()
+        return {n: p.grad for n, p in layer.named_parameters() if n.startswith(("wk", "wv")) and p.grad is not None}
+    own = step()
+    monkeypatch.setattr(kernels, "window_attention_supported", lambda q: False)
+    with sdpa_kernel(SDPBackend.MATH):
+        ref = step()
+    assert ref and own.keys() == ref.keys()
+    for n in ref:
+        print(n, rel(own[n], ref[n]), flush=True)
+        assert rel(own[n], ref[n]) <= 1e-4 or ref[n].norm() < 1e-6

@@ -341,13 +341,13 @@ class CausalSelfAttention(nn.Module):
             q, k = apply_rotary_emb(q, k, freqs_cis)
         return q, k, v, False
 
-    def _windowed(self, q, k, v, drop, dense_cache):
+    def _windowed(self, q, k, v, drop, dense_cache, tracked=False):
         """Attention of the last T of the keys' positions over a window and
         the first tokens: on the HIP kernels, or masked SDPA for dropout and
         for head sizes that they do not take."""
         T, total = q.size(2), k.size(2)
         if drop == 0 and kernels.window_attention_supported(q):
-            if T == 1 and dense_cache and not (torch.is_grad_enabled() and q.requires_grad) and plain_eager():
+            if T == 1 and dense_cache and not tracked and plain_eager():
                 # one row over the cache, read in place as one page per
                 # sequence: split over its length
                 table = torch.arange(q.size(0), device=q.device, dtype=torch.int32)[:, None]
@@ -393,7 +393,7 @@ class CausalSelfAttention(nn.Module):
             if paged and T == 1:
                 y = kv_cache.attend(layer_idx, q, self.window, self.sinks)
             elif 0 < self.window < k.size(2):
-                y = self._windowed(q, k, v, drop, kv_cache is not None and not paged)
+                y = self._windowed(q, k, v, drop, kv_cache is not None and not paged, tracked)
             elif past > 0 and T == 1:
                 # one new position attends to every cached one: no mask needed;
                 # the split-K decode kernel reads the cache in place
