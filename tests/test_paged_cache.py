@@ -70,3 +70,26 @@ def test_refusals():
         c.write(0, k, k)
     with pytest.raises(AssertionError):
         c.write(0, k[:2], k[:2])
+
+
+def test_dual_numbers_and_traces_are_refused():
+    """Kernels that see values alone would drop a tangent without a word, and
+    leave nothing in a trace."""
+    import torch.autograd.forward_ad as fw
+    c = make()
+    c.reserve(1)
+    k = torch.ones(3, 1, 2, 16, dtype=torch.bfloat16)
+    q = torch.ones(3, 2, 1, 16, dtype=torch.bfloat16)
+    with fw.dual_level():
+        for args in ((fw.make_dual(k, k), k), (k, fw.make_dual(k, k))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                c.write(0, *args)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            c.attend(0, fw.make_dual(q, q))
+        # a level alone is no reason: these get to the kernels, which want a GPU
+        with pytest.raises(RuntimeError, match="GPU"):
+            c.write(0, k, k)
+        with pytest.raises(RuntimeError, match="GPU"):
+            c.attend(0, q)
+    with pytest.raises(RuntimeError, match="traces"):
+        torch.jit.trace(lambda q: c.attend(0, q), (q,), check_trace=False)

@@ -99,6 +99,12 @@ def plain_tensor(t: torch.Tensor) -> bool:
             and not f.is_functorch_wrapped_tensor(t))
 
 
+def carries_tangent(t: torch.Tensor) -> bool:
+    """Whether t is a dual number of forward-mode differentiation."""
+    ad = torch.autograd.forward_ad
+    return ad._current_level >= 0 and ad.unpack_dual(t).tangent is not None
+
+
 def first_order(gy: torch.Tensor) -> bool:
     """Whether a backward may run kernels on the gradient ``gy``: it is not
     differentiated itself, and neither a transform (batched gradients, a

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import kernels
-from ._common import TENSOR_TYPES, first_order, plain_eager, plain_tensor
+from ._common import TENSOR_TYPES, carries_tangent, first_order, plain_eager, plain_tensor
 
 
 def window_attention_plain(q, k, v, window, sinks=0, lengths=None, scale=None):
@@ -93,6 +93,12 @@ def window_mask(Tq: int, Tk: int, window: int, sinks: int, device) -> torch.Tens
     return (j <= p) & ((j > p - window) | (j < sinks))
 
 
+def _plain_values(*tensors) -> None:
+    """The cache's kernels see values alone: what would be lost is refused."""
+    if torch.jit.is_tracing() or any(carries_tangent(t) for t in tensors):
+        raise RuntimeError("PagedKVCache: no forward-mode derivatives and no traces")
+
+
 class PagedKVCache:
     """Per-layer keys and values of ``batch`` sequences of their own lengths,
     in pages of ``page_size`` tokens that a sequence takes as it grows and
@@ -106,7 +112,8 @@ class PagedKVCache:
 
     T == 1 takes sequences of any lengths; T > 1 (prompts, padded on the right
     to T) needs those that keep some to stand at one length.  ``counts`` 0
-    leaves a sequence as it is.  The tensors that the kernels read
+    leaves a sequence as it is.  A cache holds values alone: gradients,
+    forward-mode derivatives and traces through it are refused.  The tensors that the kernels read
     (``page_table`` [batch, pages], ``lengths``, ``counts``, ``totals``
     [batch], int32) keep their addresses, so a captured forward of T == 1 can
     be replayed between ``reserve(1)`` and ``increment()``."""
@@ -201,6 +208,7 @@ class PagedKVCache:
         assert k.shape[0] == self.batch, f"{k.shape[0]} rows for a cache of {self.batch} sequences"
         if max(self._counts) == 0 or max(self._counts) > k.shape[1]:
             raise RuntimeError(f"PagedKVCache: a forward of {k.shape[1]} tokens with {max(self._counts)} reserved")
+        _plain_values(k, v)
         kp, vp = self.k_pages[layer_idx], self.v_pages[layer_idx]
         kernels.paged_kv_write(k.detach().to(kp.dtype), v.detach().to(vp.dtype), kp, vp, self.page_table, self.lengths,
                                self.counts)
@@ -208,6 +216,7 @@ class PagedKVCache:
     def attend(self, layer_idx: int, q: torch.Tensor, window: int = 0, sinks: int = 0) -> torch.Tensor:
         """Attention of q [batch, heads, 1, head_dim], the sequences' newest
         tokens, over the cache with what was written for them."""
+        _plain_values(q)
         kp = self.k_pages[layer_idx]
         return kernels.paged_decode_attention(q.detach().to(kp.dtype), kp, self.v_pages[layer_idx], self.page_table,
                                               self.totals, window, sinks)
