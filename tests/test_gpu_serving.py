@@ -336,3 +336,25 @@ def test_windowed_single_token_keeps_the_gradients_of_its_keys(monkeypatch):
     for n in ref:
         print(n, rel(own[n], ref[n]), flush=True)
         assert rel(own[n], ref[n]) <= 1e-4 or ref[n].norm() < 1e-6
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(attn_window=16, attn_sinks=2)])
+def test_padding_past_the_rotary_table(kw):
+    """Parts and prompts padded past the model's 128 rotary positions, whose
+    tokens that count lie within them."""
+    model = make(**kw)
+    idx = tokens(2, 160)
+    kv = paged(model, 2)
+    with torch.no_grad():
+        kv.reserve([110, 110])
+        model(idx[:, :110], kv_cache=kv)
+        kv.increment()
+        kv.reserve([10, 18])
+        lg, _ = model(idx[:, 110:140], kv_cache=kv)
+        kv.increment()
+        for b, n in ((0, 120), (1, 128)):
+            compare(model, idx[b:b + 1, :n], lg[b:b + 1], torch.float32, f"{kw} row {b}")
+    lens = [100, 50]
+    want = model.generate(idx[:, :100], 4, temperature=0.0, kv_cache=paged(model, 2), lengths=lens)
+    got = model.generate(idx[:, :150], 4, temperature=0.0, kv_cache=paged(model, 2), lengths=lens)
+    assert torch.equal(got[:, 150:], want[:, 100:])

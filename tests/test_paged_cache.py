@@ -93,3 +93,17 @@ def test_dual_numbers_and_traces_are_refused():
             c.attend(0, q)
     with pytest.raises(RuntimeError, match="traces"):
         torch.jit.trace(lambda q: c.attend(0, q), (q,), check_trace=False)
+
+
+def test_rotary_rows_of_padding_past_the_table():
+    """A padded part may end past the rotary table as long as the tokens that
+    count do not: their rows are theirs, the padding's are any."""
+    from src.model.chassis import cache_freqs
+    table = torch.arange(128)[:, None].expand(128, 4)
+    c = make(n_pages=24, max_seq_len=128)
+    c.reserve([110, 110, 3])
+    c.increment()
+    c.reserve([10, 18, 0])
+    for T, n in ((18, 18), (19, 18), (30, 18), (300, 18)):
+        rows = cache_freqs(table, T, 0, c)
+        assert rows.shape == (T, 4) and rows[:n, 0].tolist() == list(range(110, 110 + n))

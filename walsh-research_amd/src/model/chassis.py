@@ -189,13 +189,17 @@ class KVCache:
 def cache_freqs(freqs_cis, T, start_pos, kv_cache):
     """Rotary rows of a forward: positions start_pos .. start_pos + T - 1, or
     where a paged cache stands: one position per sequence for a single token,
-    the sequences' common one for several."""
+    the sequences' common one for several, whose padding may run past the last
+    (it takes any row: it is not kept)."""
     if not isinstance(kv_cache, PagedKVCache):
         return freqs_cis[start_pos:start_pos + T]
     if kv_cache.max_seq_len > freqs_cis.shape[0]:
         raise ValueError(f"paged cache of {kv_cache.max_seq_len} positions for {freqs_cis.shape[0]} rotary rows")
     if T > 1:
-        return freqs_cis[kv_cache.cached_len:kv_cache.cached_len + T]
+        past, rows = kv_cache.cached_len, freqs_cis.shape[0]
+        if past + T <= rows:
+            return freqs_cis[past:past + T]
+        return freqs_cis.index_select(0, torch.arange(past, past + T, device=freqs_cis.device).clamp_max(rows - 1))
     return freqs_cis.index_select(0, kv_cache.lengths.clamp(0, freqs_cis.shape[0] - 1))
 
 
