@@ -358,3 +358,23 @@ def test_padding_past_the_rotary_table(kw):
     want = model.generate(idx[:, :100], 4, temperature=0.0, kv_cache=paged(model, 2), lengths=lens)
     got = model.generate(idx[:, :150], 4, temperature=0.0, kv_cache=paged(model, 2), lengths=lens)
     assert torch.equal(got[:, 150:], want[:, 100:])
+
+
+def test_generate_takes_settings_per_row():
+    """Each of the sampling's settings as a tensor with one value per row."""
+    from src.model import kernels
+    model = make(n_layer=1)
+    idx = tokens(3, 9)
+    settings = dict(temperature=torch.tensor([0.7, 1.0, 1.3]).cuda(), top_p=torch.tensor([0.9, 1.0, 0.5]).cuda(),
+                    min_p=torch.tensor([0.0, 0.02, 0.01]).cuda())
+    for k in (torch.tensor([0, 3, 40], dtype=torch.int32).cuda(), 0, None):
+        torch.manual_seed(7)
+        w = idx
+        with torch.no_grad():
+            for _ in range(4):
+                t = kernels.sample(model(w)[0][:, -1], torch.rand(3, device="cuda"), top_k=0 if k is None else k, **settings)
+                w = torch.cat([w, t[:, None]], 1)
+        torch.manual_seed(7)
+        assert torch.equal(model.generate(idx, 4, top_k=k, **settings), w)
+        torch.manual_seed(7)
+        assert torch.equal(model.generate(idx, 4, top_k=k, kv_cache=paged(model, 3), **settings), w)

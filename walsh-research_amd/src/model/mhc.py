@@ -536,7 +536,8 @@ class mHCWalsh(nn.Module):
 
         Without the last four arguments the reference's loop (mhc.py:754-772):
         no cache, torch.multinomial.  ``top_p`` or ``min_p`` draws each token
-        with kernels.sample (its filters) from torch's uniform numbers.
+        with kernels.sample (its filters; settings are numbers or tensors with
+        a value per row) from torch's uniform numbers.
         ``kv_cache``, an empty PagedKVCache for B sequences of at least T +
         max_new_tokens positions, keeps the keys and values; the prompts may
         then be padded on the right to T, ``lengths`` (B whole numbers) of
@@ -579,8 +580,9 @@ class mHCWalsh(nn.Module):
                 kv_cache.reserve(1)
                 logits, _ = self(idx[:, -1:], kv_cache=kv_cache)
                 kv_cache.increment()
-            token = kernels.sample(logits[:, -1, :], torch.rand(idx.size(0), device=idx.device), temperature, top_k or 0,
-                                   1.0 if top_p is None else top_p, 0.0 if min_p is None else min_p)
+            token = kernels.sample(logits[:, -1, :], torch.rand(idx.size(0), device=idx.device), temperature,
+                                   0 if top_k is None else top_k, 1.0 if top_p is None else top_p,
+                                   0.0 if min_p is None else min_p)
             token.clamp_(min=0)     # a row of logits that are no numbers has no token: an index that is one
             idx = torch.cat((idx, token[:, None]), dim=1)
         return idx
