@@ -378,3 +378,19 @@ def test_generate_takes_settings_per_row():
         assert torch.equal(model.generate(idx, 4, top_k=k, **settings), w)
         torch.manual_seed(7)
         assert torch.equal(model.generate(idx, 4, top_k=k, kv_cache=paged(model, 3), **settings), w)
+
+
+def test_generate_whatever_the_default_dtype():
+    """The drawn numbers are float32, which the sampling takes, also where
+    new tensors are something else by default."""
+    model = make(n_layer=1)
+    idx = tokens(2, 6)
+    torch.manual_seed(1)
+    want = model.generate(idx, 3, top_p=0.9)
+    try:
+        torch.set_default_dtype(torch.float64)
+        torch.manual_seed(1)
+        got = model.generate(idx, 3, top_p=0.9)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert torch.equal(got, want)

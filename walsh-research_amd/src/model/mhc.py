@@ -580,9 +580,9 @@ class mHCWalsh(nn.Module):
                 kv_cache.reserve(1)
                 logits, _ = self(idx[:, -1:], kv_cache=kv_cache)
                 kv_cache.increment()
-            token = kernels.sample(logits[:, -1, :], torch.rand(idx.size(0), device=idx.device), temperature,
-                                   0 if top_k is None else top_k, 1.0 if top_p is None else top_p,
-                                   0.0 if min_p is None else min_p)
+            u = torch.rand(idx.size(0), device=idx.device, dtype=torch.float32)
+            token = kernels.sample(logits[:, -1, :], u, temperature, 0 if top_k is None else top_k,
+                                   1.0 if top_p is None else top_p, 0.0 if min_p is None else min_p)
             token.clamp_(min=0)     # a row of logits that are no numbers has no token: an index that is one
             idx = torch.cat((idx, token[:, None]), dim=1)
         return idx
