@@ -394,3 +394,32 @@ def test_generate_whatever_the_default_dtype():
     finally:
         torch.set_default_dtype(torch.float32)
     assert torch.equal(got, want)
+
+
+def test_generate_refuses_before_it_draws():
+    """A pool that would run out of pages on the way, and a cache of another
+    batch, are refused with nothing drawn and nothing taken; a pool that is
+    just large enough serves to the end."""
+    model = make(n_layer=1)
+    idx = tokens(2, 20)
+    # 20 + 13 - 1 = 32 and 4 + 12 = 16 positions of pages of 16: 3 pages; one token more needs 5
+    lens, steps = [20, 4], 13
+    kv = paged(model, 2, pages=3)
+    state = torch.cuda.get_rng_state()
+    for n in (steps + 1, 100):
+        with pytest.raises(RuntimeError, match="pages"):
+            model.generate(idx, n, kv_cache=kv, lengths=lens)
+    for other in (1, 3):
+        kv2 = paged(model, other, pages=40)
+        for ln in (None, lens):
+            with pytest.raises(ValueError, match="sequences"):
+                model.generate(idx, 2, kv_cache=kv2, lengths=ln)
+        assert kv2.free_pages == 40 and not kv2.counts.any()
+    assert torch.equal(torch.cuda.get_rng_state(), state) and kv.free_pages == 3 and kv.seq_lens == [0, 0]
+    got = model.generate(idx, steps, temperature=0.0, kv_cache=kv, lengths=lens)
+    assert torch.equal(got, model.generate(idx, steps, temperature=0.0, kv_cache=paged(model, 2), lengths=lens))
+    assert kv.free_pages == 0
+    # pages that a sequence holds already count as its own
+    kv.reset()
+    kv.reserve([17, 1])
+    assert torch.equal(model.generate(idx, steps, temperature=0.0, kv_cache=kv, lengths=lens), got)

@@ -149,6 +149,14 @@ class PagedKVCache:
             raise ValueError(f"several tokens at once need sequences of one length, got {sorted(at)}")
         return at.pop() if at else 0
 
+    def require_pages(self, ends: Sequence[int]) -> List[int]:
+        """Pages that each sequence still lacks to be ``ends`` long; raises
+        where the pool has fewer."""
+        more = [max(0, -(-e // self.page_size) - len(p)) for e, p in zip(ends, self._pages)]
+        if sum(more) > len(self._free):
+            raise RuntimeError(f"PagedKVCache: {sum(more)} pages needed, {len(self._free)} free")
+        return more
+
     def reserve(self, counts: Union[int, Sequence[int]]) -> None:
         """Room for the next ``counts`` tokens (one number, or one per
         sequence) of the coming forward; nothing is taken if any does not
@@ -159,9 +167,7 @@ class PagedKVCache:
         ends = [n + c for n, c in zip(self.seq_lens, counts)]
         if max(ends) > self.max_seq_len:
             raise ValueError(f"PagedKVCache: {max(ends)} tokens of at most {self.max_seq_len}")
-        more = [max(0, -(-e // self.page_size) - len(p)) for e, p in zip(ends, self._pages)]
-        if sum(more) > len(self._free):
-            raise RuntimeError(f"PagedKVCache: {sum(more)} pages needed, {len(self._free)} free")
+        more = self.require_pages(ends)
         if any(more):
             for pages, n in zip(self._pages, more):
                 pages.extend(self._free.pop() for _ in range(n))

@@ -564,11 +564,15 @@ class mHCWalsh(nn.Module):
         if kv_cache is not None:
             if not isinstance(kv_cache, PagedKVCache):
                 raise TypeError("generate: kv_cache is a PagedKVCache")
+            if kv_cache.batch != idx.size(0):
+                raise ValueError(f"generate: {idx.size(0)} prompts for a kv_cache of {kv_cache.batch} sequences")
             if any(kv_cache.seq_lens):
                 raise ValueError("generate: the kv_cache is not empty")
             if max(lengths or [idx.size(1)]) + max_new_tokens - 1 > kv_cache.max_seq_len:
                 raise ValueError(f"generate: {max_new_tokens} tokens behind {idx.size(1)} of at most "
                                  f"{kv_cache.max_seq_len} positions")
+            if max_new_tokens > 0:   # to the end, or not at all
+                kv_cache.require_pages([n + max_new_tokens - 1 for n in lengths or [idx.size(1)] * idx.size(0)])
         for step in range(max_new_tokens):
             if kv_cache is None:
                 logits, _ = self(idx[:, -self.config.block_size:])
