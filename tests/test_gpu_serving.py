@@ -423,3 +423,31 @@ def test_generate_refuses_before_it_draws():
     kv.reset()
     kv.reserve([17, 1])
     assert torch.equal(model.generate(idx, steps, temperature=0.0, kv_cache=kv, lengths=lens), got)
+
+
+def test_paged_single_token_refuses_dropout():
+    """The kernel drops nothing: in training mode with dropout the step raises
+    instead of leaving it out."""
+    model = make(n_layer=1, dropout=0.5).train()
+    kv = paged(model, 2)
+    with torch.no_grad():
+        kv.reserve(1)
+        with pytest.raises(RuntimeError, match="dropout"):
+            model(tokens(2, 1), kv_cache=kv)
+        kv.reset()
+        kv.reserve(1)
+        assert model.eval()(tokens(2, 1), kv_cache=kv)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_windowed_model_with_dropout_trains(dtype):
+    """Dropout takes the masked attention of the library: it runs, its result
+    is random in training and the kernels' in evaluation."""
+    model = make(n_layer=1, dropout=0.3, attn_window=8, attn_sinks=2).train()
+    idx, tgt = tokens(2, 40), tokens(2, 40, 2)
+    with torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+        a, loss = model(idx, targets=tgt)
+        loss.backward()
+        b, _ = model(idx, targets=tgt)
+        assert not torch.equal(a, b)
+    assert all(p.grad.isfinite().all() for p in model.parameters() if p.grad is not None)

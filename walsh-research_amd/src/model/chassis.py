@@ -395,6 +395,8 @@ class CausalSelfAttention(nn.Module):
         drop = self.dropout if self.training else 0
         with _attention_backends(tracked and q.is_cuda and q.dtype != torch.float32):
             if paged and T == 1:
+                if drop:
+                    raise RuntimeError("a single token over a paged cache takes no dropout: model.eval() first")
                 y = kv_cache.attend(layer_idx, q, self.window, self.sinks)
             elif 0 < self.window < k.size(2):
                 y = self._windowed(q, k, v, drop, kv_cache is not None and not paged, tracked)
