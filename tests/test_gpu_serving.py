@@ -451,3 +451,24 @@ def test_windowed_model_with_dropout_trains(dtype):
         b, _ = model(idx, targets=tgt)
         assert not torch.equal(a, b)
     assert all(p.grad.isfinite().all() for p in model.parameters() if p.grad is not None)
+
+
+def test_launch_timing_names_the_kernels_that_ran():
+    """Labels are the kernels that the library picked, with the operations of
+    the pairs that the mask leaves."""
+    from src.model import _hip, kernels
+    z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+
+    def ran(f):
+        with _hip.LaunchTimer() as lt:
+            f()
+        (name, d), = lt.summary().items()
+        return name, d["flops"]
+    few, many = z(1, 2, 100, 16), z(64, 32, 100, 16)
+    assert ran(lambda: kernels.window_attention(few, few, few, 0)) == ("window_fwd_split_kernel", 4 * 2 * 16 * 5050)
+    assert ran(lambda: kernels.window_attention(many, many, many, 10, 2)) == \
+        ("window_fwd_kernel", 4 * 64 * 32 * 16 * (55 + 90 * 10 + 2 * 90 - 1))
+    table, n = z(1, 1).int(), z(1).int() + 64
+    for H, name in ((2, "paged_decode_rows_kernel"), (8, "paged_decode_kernel")):
+        pages = z(1, 1, 64, 16)
+        assert ran(lambda: kernels.paged_decode_attention(z(1, H, 1, 16), pages, pages, table, n))[0] == name

@@ -78,3 +78,13 @@ def test_paged_decode_is_window_attention_of_the_last_row():
             v = np.stack([vp[table[b, j // page], :, j % page] for j in range(n[b])], 1)[None]
             want = oatt.window_attention_f64(q[b][None, :, None], k, v, W, S)["o"][0, :, 0]
             assert np.allclose(o[b], want, atol=1e-14)
+
+
+def test_visible_pairs_by_the_mask():
+    from src.model.kernels import visible_pairs
+    for Tk in (0, 1, 2, 9, 16):
+        for Tq in (0, 1, 5, 9, 16, 20):
+            for W in (-1, 0, 1, 3, 9, 15, 16, 30):
+                for S in (-2, 0, 1, 4, 9, 20):
+                    want = int(oatt.window_mask(Tq, Tk, W, max(S, 0)).sum())
+                    assert visible_pairs(Tq, Tk, W, S) == want, (Tq, Tk, W, S)

@@ -886,6 +886,19 @@ def _workspace(name: str, device: int, *sizes) -> int:
     return _hip.on_device(device, getattr(_hip.lib(), name), *sizes)
 
 
+@functools.lru_cache(maxsize=1024)
+def visible_pairs(Tq: int, Tk: int, window: int, sinks: int) -> int:
+    """(query, key) pairs of a windowed causal mask, the queries the last Tq
+    of Tk positions (no lengths)."""
+    window, sinks = (window, max(sinks, 0)) if 0 < window < Tk else (Tk, 0)
+
+    def upto(n):   # of the queries at positions below n
+        far = max(n - window, 0)   # queries whose window has left the first position
+        s, near = min(sinks, far), n - far
+        return near * (near + 1) // 2 + far * window + s * far - s * (s - 1) // 2
+    return upto(Tk) - upto(max(Tk - Tq, 0))
+
+
 def window_attention_supported(q: torch.Tensor) -> bool:
     """Whether window_attention takes a query of this device, type and head size."""
     return q.is_cuda and q.dtype in (torch.float32, torch.bfloat16) and q.shape[-1] in ATTENTION_HEAD_DIMS
@@ -947,12 +960,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     o = torch.empty(B, H, Tq, D, device=q.device, dtype=q.dtype)
     lse = torch.empty(B, H, Tq, device=q.device, dtype=torch.float32) if need_lse or need_rest else None
     rest = torch.empty_like(o) if need_rest and q.dtype == torch.bfloat16 else None
-    span = min(Tk, window + sinks) if window > 0 else Tk
     _hip.call_on(q.get_device(), "walsh_window_attention_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
                  *k.stride()[:3], B, H, G, Tq, Tk, D, int(window), int(sinks), _hip.ptr(lengths), scale, o.data_ptr(),
                  *o.stride()[:3], _hip.ptr(lse), _hip.ptr(rest), _hip.dtype_code(q.dtype),
-                 kernel="window_fwd_kernel", nbytes=2 * B * D * (H * Tq + G * Tk) * q.element_size(),
-                 flops=4 * B * H * Tq * span * D)
+                 kernel="*", nbytes=2 * B * D * (H * Tq + G * Tk) * q.element_size(),
+                 flops=4 * B * H * D * visible_pairs(Tq, Tk, int(window), int(sinks)))
     return (o, lse, rest) if need_rest else (o, lse) if need_lse else o
 
 
@@ -986,12 +998,12 @@ def window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     nws = _workspace("walsh_window_attention_bwd_workspace_bytes", q.get_device(), B, H, G, Tq, Tk, D, int(window),
                      int(sinks), dt)
     ws = torch.empty(nws, device=q.device, dtype=torch.uint8)
-    span = min(Tk, window + sinks) if window > 0 else Tk
     _hip.call_on(q.get_device(), "walsh_window_attention_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), v.data_ptr(),
                  *k.stride()[:3], o.data_ptr(), *o.stride()[:3], go.data_ptr(), *go.stride()[:3], lse.data_ptr(), _hip.ptr(rest), B, H, G,
                  Tq, Tk, D, int(window), int(sinks), _hip.ptr(lengths), scale, dq.data_ptr(), dk.data_ptr(),
                  dv.data_ptr(), dt, ws.data_ptr(), nws, kernel="window_bwd_kernels",
-                 nbytes=4 * B * D * (H * Tq + G * Tk) * q.element_size(), flops=14 * B * H * Tq * span * D)
+                 nbytes=4 * B * D * (H * Tq + G * Tk) * q.element_size(),
+                 flops=14 * B * H * D * visible_pairs(Tq, Tk, int(window), int(sinks)))
     return dq, dk, dv
 
 
@@ -1043,7 +1055,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     _hip.call_on(q.get_device(), "walsh_paged_decode_attention", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(),
                  v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.shape[0], page, page_table.data_ptr(),
                  page_table.stride(0), N, lengths.data_ptr(), B, H, G, D, int(window), int(sinks), scale, o.data_ptr(),
-                 o.stride(0), o.stride(1), dt, _hip.ptr(ws), nws, kernel="paged_decode_kernel",
+                 o.stride(0), o.stride(1), dt, _hip.ptr(ws), nws, kernel="*",
                  nbytes=2 * B * G * span * D * q.element_size(), flops=4 * B * H * span * D)
     return o
 
