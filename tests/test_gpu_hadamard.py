@@ -262,6 +262,41 @@ def _layer(K, in_o, out_o, g, scale=0.1):
             (scale * torch.randn(32, out_o, generator=g)).cuda())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M", [1, 17, 180, 300, 2100])
+def test_hadamard_padded_groups_are_zeros_whatever_memory_held(K, M, dtype, monkeypatch):
+    """The slots [out_o, roundup(out_o, 4)) of a padded result are written, in
+    every kernel that the shapes reach: the next layer multiplies them by zero
+    weights, which NaN left in memory would survive.  Also the input gradient
+    of a padded layer."""
+    def poisoned(*size, **kw):
+        t = empty(*size, **kw)
+        return t.fill_(float("nan")) if t.is_floating_point() else t
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", poisoned)
+    monkeypatch.setattr(torch, "empty_like", lambda t, **kw: poisoned(t.shape, dtype=t.dtype, device=t.device))
+    g = torch.Generator().manual_seed(M)
+    for in_o, out_o in ((8, 5), (16, 43), (20, 3), (24, 50), (32, 86), (33, 101), (43, 18), (64, 171), (86, 32), (100, 127),
+                        (128, 69), (150, 66), (40, 131)):
+        gs = (out_o + 3) // 4 * 4
+        kw, alpha, beta = _layer(K, in_o, out_o, g)
+        x = torch.randn(M, 32 * in_o, generator=g).to(dtype).cuda()
+        y = K.hadamard_linear(x, in_o, out_o, kw, alpha, beta).view(M, 32, out_o)
+        for gsy in (gs, gs + 4):
+            z = K.hadamard_linear(x, in_o, out_o, kw, alpha, beta, gsy=gsy).view(M, 32, gsy)
+            assert (z[..., out_o:gs] == 0).all(), (in_o, out_o, gsy, "pads")
+            assert torch.allclose(z[..., :out_o].float(), y.float(), rtol=0, atol=2.0 ** -7 * float(y.float().abs().max()))
+        if in_o <= 24:
+            h = K.hadamard_swiglu(x, in_o, out_o, (kw, alpha, beta), (kw, alpha, beta)).view(M, 32, gs)
+            assert (h[..., out_o:] == 0).all() and h.isfinite().all(), (in_o, out_o, "swiglu pads")
+        kwt = _prepare(K, torch.randint(-1, 2, (32, in_o, out_o), generator=g).numpy().astype(np.int8))
+        xp = torch.zeros(M, 32, (in_o + 3) // 4 * 4, dtype=dtype, device="cuda")
+        xp[..., :in_o] = x.view(M, 32, in_o)
+        gx = K.hadamard_linear_bwd(xp.view(M, -1), x.new_ones(M, 32 * out_o), in_o, out_o, kw, kwt, alpha, beta,
+                                   need=(True, False, False, False), gsx=xp.shape[2])[0].view(xp.shape)
+        assert (gx[..., in_o:] == 0).all() and gx.isfinite().all(), (in_o, out_o, "gradient pads")
+
+
 @pytest.mark.parametrize("in_o,out_o,M", [(24, 136, 2048), (64, 172, 17), (64, 172, 1489), (64, 172, 1490),
                                           (32, 256, 1040), (80, 132, 4096), (84, 132, 300),
                                           (32, 16, 16385), (32, 16, 32768), (32, 16, 32769), (48, 16, 27264),

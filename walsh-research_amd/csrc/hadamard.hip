@@ -1592,7 +1592,8 @@ __global__ __launch_bounds__(kWideThreads, 1) void hadamard_split3_kernel(HadArg
     for (int g = 0; g < 32; ++g) v[g] = pp[g * 256];
     fht32<float>(v);
     const __amdgpu_buffer_rsrc_t yr = make_rsrc(a.y, (uint32_t)((int64_t)a.M * a.ldy * 2));
-    const uint32_t voff = ok ? (uint32_t)((int64_t)orow * a.ldy * 2) + (uint32_t)o * 2 : kOOB;
+    const bool store = orow < a.M && o < a.out_o + a.pad;           // (beta is 0 past out_o)
+    const uint32_t voff = store ? (uint32_t)((int64_t)orow * a.ldy * 2) + (uint32_t)o * 2 : kOOB;
     const uint32_t hstride = (uint32_t)(GS ? GS : a.gsy) * 2;
     const f32x2 cs = cs_ok ? f32x2{__uint_as_float(csr.x), __uint_as_float(csr.y)} : f32x2{1.f, 0.f};
 #pragma unroll
@@ -1762,7 +1763,8 @@ __global__ __launch_bounds__(kThreads, (BF16MMA && KC1) ? 2 : 1) void hadamard_s
             voff[0] = (row_ok && o0 < g.out_o) ? yoff + (uint32_t)o0 * esz : kOOB;
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) voff[j] = (row_ok && o0 + j < g.out_o) ? yoff + (uint32_t)(o0 + j) * esz : kOOB;
+            for (int j = 0; j < 4; ++j)
+                voff[j] = (row_ok && o0 + j < g.out_o + g.pad) ? yoff + (uint32_t)(o0 + j) * esz : kOOB;
         }
         // beta and the stashed gate four groups at a time (reads of a batch
         // in flight together)
@@ -2560,8 +2562,9 @@ WALSH_EXPORT int walsh_hadamard_linear_ex_fwd(const void *x, int64_t ldx, int64_
     if (rc) return rc;
     if (!kweight || !alpha || !beta) return set_error(WALSH_EINVAL, "%s: null weight pointer", fn);
     if (M == 0) return WALSH_OK;
-    return hadamard_launch(fn, had_args(x, ldx, gsx, in_o, out_o, kweight, alpha, beta, y, ldy, gsy), nullptr, M,
-                           dtype == WALSH_BF16, (hipStream_t)stream);
+    HadArgs a = had_args(x, ldx, gsx, in_o, out_o, kweight, alpha, beta, y, ldy, gsy);
+    a.pad = pad_slots(out_o, gsy);
+    return hadamard_launch(fn, a, nullptr, M, dtype == WALSH_BF16, (hipStream_t)stream);
 }
 
 WALSH_EXPORT int walsh_hadamard_linear_fwd(const void *x, int64_t ldx, int64_t M, int64_t in_o, int64_t out_o,
@@ -2727,7 +2730,8 @@ WALSH_EXPORT int walsh_hadamard_swiglu_fwd(const void *x, int64_t ldx, int64_t g
     if (!kw_gate || !alpha_gate || !beta_gate || !kw_up || !alpha_up || !beta_up)
         return set_error(WALSH_EINVAL, "%s: null weight pointer", fn);
     if (M == 0) return WALSH_OK;
-    const HadArgs ga = had_args(x, ldx, gsx, in_o, hid_o, kw_gate, alpha_gate, beta_gate, h, ldh, gsh);
+    HadArgs ga = had_args(x, ldx, gsx, in_o, hid_o, kw_gate, alpha_gate, beta_gate, h, ldh, gsh);
+    ga.pad = pad_slots(hid_o, gsh);
     const HadArgs ua = had_args(x, ldx, gsx, in_o, hid_o, kw_up, alpha_up, beta_up, h, ldh, gsh);
     return hadamard_launch(fn, ga, &ua, M, dtype == WALSH_BF16, (hipStream_t)stream);
 }

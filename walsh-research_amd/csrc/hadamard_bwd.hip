@@ -762,6 +762,7 @@ WALSH_EXPORT int walsh_hadamard_linear_ex_bwd(const void *x, int64_t ldx, int64_
         j.a.x = gc; j.a.ldx = ldg; j.a.in_o = (int)out_o; j.a.out_o = (int)in_o; j.a.Nt = Kc; j.a.Kc = Nt;
         j.a.gsx = (int)gsy; j.a.gsy = (int)gsx; j.a.kw = kweight_t; j.a.alpha = beta; j.a.beta = alpha;
         j.a.beta_h = (int)in_o; j.a.y = gxc; j.a.ldy = gx ? ldgx : 0;
+        j.a.pad = pad_slots(in_o, gsx);
         j.ra = BwdRed{xc, ldx, (int)gsx, pa + ia * 32 * Ap, p.Sa, p.tpa};
         j.nA = need_a ? (pair ? p.Sa * Kc : (int)ceil_div((int64_t)p.Sa * Kc, kWaves)) : 0;
         // the layer on x without beta or store, aux = gy (dbeta)

@@ -71,7 +71,15 @@ struct HadArgs {
     // non-temporal output stores (whole-row variant): outputs far larger
     // than the caches, which a later kernel would read from HBM anyway
     int nt_store;
+    // slots past out_o of every group that stores fill with zeros (up to the
+    // next multiple of 4, where the group stride leaves room)
+    int pad;
 };
+// That number for rows of n values in groups of stride gs.
+inline int pad_slots(int64_t n, int64_t gs) {
+    const int64_t end = (n + 3) / 4 * 4;
+    return (int)((end < gs ? end : gs) - n);
+}
 
 // A kernel reads its arguments with scalar loads placed where each field is
 // first used, and in a latency-bound launch (decode sizes) every such load
@@ -84,7 +92,7 @@ __device__ __forceinline__ HadArgs load_args(const HadArgs &src) {
     asm volatile("" : "+s"(a.x), "+s"(a.ldx), "+s"(a.M), "+s"(a.in_o), "+s"(a.out_o), "+s"(a.Nt), "+s"(a.Kc),
                  "+s"(a.gsx), "+s"(a.gsy), "+s"(a.kw), "+s"(a.kw3), "+s"(a.alpha), "+s"(a.beta), "+s"(a.beta_h));
     asm volatile("" : "+s"(a.y), "+s"(a.ldy), "+s"(a.tpb), "+s"(a.bstride), "+s"(a.xspan), "+s"(a.rope),
-                 "+s"(a.rope_T), "+s"(a.rope_D), "+s"(a.rope_row0), "+s"(a.wave_tiles), "+s"(a.nt_store));
+                 "+s"(a.rope_T), "+s"(a.rope_D), "+s"(a.rope_row0), "+s"(a.wave_tiles), "+s"(a.nt_store), "+s"(a.pad));
     return a;
 }
 
@@ -268,10 +276,11 @@ __device__ __forceinline__ void transform_store(const HadArgs &a, f32x4 (&acc)[3
     } else {
         uint32_t voff[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) voff[j] = (row_ok && o0 + j < a.out_o) ? row_off + (uint32_t)(o0 + j) * esz : kOOB;
+        for (int j = 0; j < 4; ++j)
+            voff[j] = (row_ok && o0 + j < a.out_o + a.pad) ? row_off + (uint32_t)(o0 + j) * esz : kOOB;
 #pragma unroll
         for (int h = 0; h < 32; ++h) {
-            const f32x4 r = acc[h] * bl[h];
+            const f32x4 r = acc[h] * bl[h];             // (beta is 0 past out_o)
 #pragma unroll
             for (int j = 0; j < 4; ++j) Buf4<T>::store1(r[j], yr, voff[j], (uint32_t)h * hstride);
             if ((h & 7) == 7) __builtin_amdgcn_sched_barrier(0);
