@@ -472,3 +472,28 @@ def test_launch_timing_names_the_kernels_that_ran():
     for H, name in ((2, "paged_decode_rows_kernel"), (8, "paged_decode_kernel")):
         pages = z(1, 1, 64, 16)
         assert ran(lambda: kernels.paged_decode_attention(z(1, H, 1, 16), pages, pages, table, n))[0] == name
+
+
+@pytest.mark.parametrize("cls,kw", [("mHCWalsh", dict(attn_window=16, attn_sinks=2)),
+                                    ("Walsh", dict(C=1024, n_head=16, attn_window=24, attn_sinks=1, head_mixing=False))])
+def test_windowed_model_trains_under_bf16_autocast(cls, kw, monkeypatch):
+    """Logits and gradients of a training step on the kernels are as near to
+    the float32 step as those of masked attention in bf16."""
+    from src.model import kernels
+    model = make(cls=cls, **kw).train()
+    idx, tgt = tokens(3, 60), tokens(3, 60, 2)
+
+    def step(bf16):
+        model.zero_grad()
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=bf16):
+            logits, loss = model(idx, targets=tgt)
+            loss.backward()
+        return logits.detach(), torch.cat([p.grad.reshape(-1) for p in model.parameters() if p.grad is not None])
+    own = step(True)
+    monkeypatch.setattr(kernels, "window_attention_supported", lambda q: False)
+    lib = step(True)
+    with sdpa_kernel(SDPBackend.MATH):
+        ref = step(False)
+    for n, a, b, r in zip(("logits", "gradients"), own, lib, ref):
+        print(f"{cls} {n}: {rel(a, r):.2e}, masked attention in bf16 {rel(b, r):.2e}")
+        assert rel(a, r) <= max(1e-2, 1.25 * rel(b, r))
