@@ -331,3 +331,22 @@ def test_paged_refusals():
     with pytest.raises(TypeError, match="counts"):
         k = torch.zeros(2, 1, 2, 64, device="cuda").bfloat16()
         kernels.paged_kv_write(k, k, kp, vp, table, n, n.long())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,G,D,page,lengths,W,S", [
+    (2, 2, 128, 16, [1, 17, 300], 0, 0), (8, 2, 64, 32, [129, 64, 513], 0, 0), (6, 1, 32, 16, [700, 31], 0, 0),
+    (40, 1, 64, 64, [200, 65], 0, 0), (4, 4, 128, 64, [3000], 100, 5), (16, 2, 32, 64, [5000, 64], 0, 0)])
+def test_paged_decode_rounds_bf16_results_once(H, G, D, page, lengths, W, S):
+    """From head_dim 32 on the weights go into the product with v in two bf16
+    parts, 2^-8 of 2^-8 off: what is left is the one rounding of the output,
+    and the float32 sums of the tests above."""
+    q, kp, vp, table, n = make(len(lengths), H, G, D, page, lengths, torch.bfloat16, D + H)
+    o = decode(q, kp, vp, table, n, W, S)
+    want, a = oatt.paged_decode_f64(q[:, :, 0].double().numpy(), kp.double().numpy(), vp.double().numpy(), table.numpy(),
+                                    n.numpy(), W, S)
+    reach = float((q.double().abs().amax((0, 1, 2)) * kp.double().nan_to_num().abs().amax((0, 1, 2))).sum()) * D ** -0.5
+    rho = 2.0 ** -24 * (2 * D * reach + int(n.max()) + 64)
+    err, tol = np.abs(o[:, :, 0].double().numpy() - want), 2.0 ** -8 * np.abs(want) + (2.0 ** -16 + 2 * rho) * a
+    print(f"worst error / bound {(err / np.maximum(tol, 1e-30)).max():.3f}", flush=True)
+    assert (err <= tol).all()

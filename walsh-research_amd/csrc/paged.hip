@@ -23,9 +23,13 @@
 // the vector units up to R = 4 (paged_decode_rows_kernel), and reaches 2 to 3
 // TB/s by products above.
 //
-// Scores, maxima, sums and accumulators are float32; bf16 weights are rounded
-// to bf16 for the product with V (relative 2^-9, as the values' own rounding),
-// the sum takes them unrounded.
+// Scores, maxima, sums and accumulators are float32.  bf16 weights go into the
+// product with V in two bf16 parts, so that the output's own rounding is the
+// only one left (relative error 1.66e-3; 2.2e-3 with weights rounded to bf16,
+// off by up to 2^-8 each): the matrix cores have the time for it (64 sequences
+// of up to 4,096, 32 heads of 128: 390 us both ways, of 64, 32 sequences: 108
+// and 109, of 32: 102 and 106).  Not so heads of 16, whose vector work is the
+// bound (54 us with one part, 68 with two): they round the weights once.
 #include "tiles.h"
 
 namespace walsh {
@@ -131,6 +135,7 @@ __device__ __forceinline__ void pg_join(const PgArgs &a, int b, int h0, int head
 template <typename T, int D> struct PgCfg {
     // 32-key sub-blocks of a wavefront's step: 8 KB of K (bf16) whatever D
     static constexpr int NB = sizeof(T) == 2 ? (D == 128 ? 1 : D == 64 ? 2 : 4) : (D >= 64 ? 1 : D == 32 ? 2 : 4);
+    static constexpr bool TWO = sizeof(T) == 2 && D >= 32;   // bf16 weights in two parts
     static constexpr int VBYTES = NB * Tile<T, D, 32>::BYTES;
     // two V buffers per wavefront; at the end 32 rows of D float32
     static constexpr int WAVE = 2 * VBYTES > 32 * D * 4 ? 2 * VBYTES : 32 * D * 4;
@@ -140,6 +145,7 @@ template <typename T, int D> struct PgCfg {
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void paged_decode_kernel(PgArgs a) {
     constexpr int NB = PgCfg<T, D>::NB, KB = 32 * NB, NK = D / 16, ND = (D + 31) / 32;
+    constexpr bool TWO = PgCfg<T, D>::TWO;
     typedef Tile<T, D, 32> L;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ int pages[kPgEntries];
@@ -236,10 +242,15 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
             for (int r = 0; r < 16; ++r) l += w[r];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                Frag<T> pf;
+                Frag<T> pf, rest;
                 pack(pf, w + 8 * t);
+                if constexpr (TWO) pack_rest(rest, w + 8 * t, pf);
 #pragma unroll
-                for (int c = 0; c < ND; ++c) mma(acc[c], L::col(vt + u * L::BYTES, 16 * t, c, lane), pf);
+                for (int c = 0; c < ND; ++c) {
+                    const Frag<T> vc = L::col(vt + u * L::BYTES, 16 * t, c, lane);
+                    mma(acc[c], vc, pf);
+                    if constexpr (TWO) mma(acc[c], vc, rest);
+                }
             }
         }
     }
