@@ -497,3 +497,31 @@ def test_windowed_model_trains_under_bf16_autocast(cls, kw, monkeypatch):
     for n, a, b, r in zip(("logits", "gradients"), own, lib, ref):
         print(f"{cls} {n}: {rel(a, r):.2e}, masked attention in bf16 {rel(b, r):.2e}")
         assert rel(a, r) <= max(1e-2, 1.25 * rel(b, r))
+
+
+@pytest.mark.parametrize("cls", ["mHCWalsh", "Walsh"])
+def test_padding_need_not_be_tokens(cls):
+    """Prompts padded with -1 and with numbers past the vocabulary, and an idle
+    sequence's place, give what padding with a token gives."""
+    model = make(n_layer=1, cls=cls)
+    idx = tokens(3, 20)
+    lens = [20, 4, 11]
+    pad = torch.arange(20, device="cuda") >= torch.tensor(lens, device="cuda")[:, None]
+    outs = []
+    for fill in (0, -1, 2 ** 33):
+        kv = paged(model, 3)
+        with torch.no_grad():
+            kv.reserve(lens)
+            a, _ = model(idx.masked_fill(pad, fill), kv_cache=kv)
+            kv.increment()
+            kv.reserve([1, 0, 1])
+            last = idx[:, :1].clone()
+            last[1] = fill
+            b, _ = model(last, kv_cache=kv)
+            kv.increment()
+        outs.append((a, b[[0, 2]]))
+        if cls == "mHCWalsh":
+            new = model.generate(idx.masked_fill(pad, fill), 3, temperature=0.0, kv_cache=paged(model, 3), lengths=lens)
+            outs[-1] += (new[:, 20:],)
+    for other in outs[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(outs[0], other))

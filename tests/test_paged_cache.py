@@ -107,3 +107,21 @@ def test_rotary_rows_of_padding_past_the_table():
     for T, n in ((18, 18), (19, 18), (30, 18), (300, 18)):
         rows = cache_freqs(table, T, 0, c)
         assert rows.shape == (T, 4) and rows[:n, 0].tolist() == list(range(110, 110 + n))
+
+
+def test_tokens_that_do_not_count_are_replaced():
+    """Padding and idle sequences may hold any number: the embedding sees
+    token 0 there, and the tokens that count as they are."""
+    from src.model.chassis import counted_tokens
+    c = make()
+    far = 2 ** 40
+    c.reserve([3, 0, 4])
+    idx = torch.tensor([[5, 6, 7, -1, far], [-1, -1, -1, -1, -1], [1, 2, 3, 4, -100]])
+    assert counted_tokens(idx, c).tolist() == [[5, 6, 7, 0, 0], [0] * 5, [1, 2, 3, 4, 0]]
+    assert counted_tokens(idx[:, :3].int(), c).tolist() == [[5, 6, 7], [0] * 3, [1, 2, 3]]
+    c.increment()
+    c.reserve([1, 0, 1])
+    assert counted_tokens(torch.tensor([[9], [far], [8]]), c).tolist() == [[9], [0], [8]]
+    for other in (None, object()):
+        assert counted_tokens(idx, other) is idx
+    assert counted_tokens(idx[:2], c).tolist() == idx[:2].tolist()   # another batch: the cache's own check says so

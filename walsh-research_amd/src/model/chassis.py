@@ -203,6 +203,16 @@ def cache_freqs(freqs_cis, T, start_pos, kv_cache):
     return freqs_cis.index_select(0, kv_cache.lengths.clamp(0, freqs_cis.shape[0] - 1))
 
 
+def counted_tokens(idx, kv_cache):
+    """idx [B, T] with token 0 in the places that a paged cache does not count:
+    what a padded prompt or an idle sequence holds there need not be a token."""
+    if not isinstance(kv_cache, PagedKVCache) or idx.shape[0] != kv_cache.batch:
+        return idx
+    if idx.shape[1] == 1:
+        return idx * kv_cache.counts[:, None].clamp_max(1)
+    return idx * (torch.arange(idx.shape[1], device=idx.device) < kv_cache.counts[:, None])
+
+
 def last_rows(h, kv_cache):
     """[B, 1, C]: the last token of every row of h [B, T, C] (of a padded
     prompt going into a paged cache: the last that counts)."""
@@ -533,7 +543,7 @@ class Walsh(nn.Module):
     def forward(self, idx, targets=None, kv_cache: Optional[KVCache] = None, start_pos: int = 0,
                 return_hidden: bool = False):
         B, T = idx.shape
-        h = self.tok_embeddings(idx)
+        h = self.tok_embeddings(counted_tokens(idx, kv_cache))
         freqs_cis = cache_freqs(self.freqs_cis, T, start_pos, kv_cache)
         for layer_idx, layer in enumerate(self.layers):
             if self.training and torch.is_grad_enabled():

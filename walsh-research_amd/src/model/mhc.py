@@ -458,9 +458,9 @@ class mHCWalsh(nn.Module):
             torch.nn.init.normal_(module.weight, mean=0.0, std=0.02)
 
     def forward(self, idx, targets=None, kv_cache=None, start_pos=0, return_hidden=False):
-        from .chassis import cache_freqs, last_rows
+        from .chassis import cache_freqs, counted_tokens, last_rows
         B, T = idx.shape
-        h = self.tok_embeddings(idx)
+        h = self.tok_embeddings(counted_tokens(idx, kv_cache))
         h = cached_linear(self.stream_proj, h, self._casts["proj"])
         dt = act_dtype(h)
         h = h.to(dt).view(B, T, self.n_streams, self.config.n_embd)
