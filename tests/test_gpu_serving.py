@@ -525,3 +525,18 @@ def test_padding_need_not_be_tokens(cls):
             outs[-1] += (new[:, 20:],)
     for other in outs[1:]:
         assert all(torch.equal(x, y) for x, y in zip(outs[0], other))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_logits_of_the_last_token_as_before(bf16):
+    """Without a paged cache each model forms its last logits from the rows it
+    always did: bitwise, where the library's product goes by their strides (a
+    weight without gradients, or autocast's copy of one)."""
+    kw = dict(n_layer=1, C=512, vocab_size=50257, algebra="octonion", n_head=16)
+    idx = tokens(8, 60)
+    for cls, rows in (("Walsh", lambda h: h[:, [-1], :]), ("mHCWalsh", lambda h: h[:, -1:, :])):
+        model = make(cls=cls, **kw).requires_grad_(False)
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16, enabled=bf16):
+            logits, _, h = model(idx, return_hidden=True)
+            w = model.output.weight.bfloat16() if bf16 else model.output.weight
+            assert torch.equal(logits, torch.nn.functional.linear(rows(h), w)), cls

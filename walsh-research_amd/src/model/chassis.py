@@ -556,7 +556,8 @@ class Walsh(nn.Module):
             logits = cached_linear(self.output, h, self._output_cast)
             loss = F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1))
         else:
-            logits = cached_linear(self.output, last_rows(h, kv_cache), self._output_cast)
+            h_last = last_rows(h, kv_cache) if isinstance(kv_cache, PagedKVCache) else h[:, [-1], :]
+            logits = cached_linear(self.output, h_last, self._output_cast)
             loss = None
         if return_hidden:
             return logits, loss, h
