@@ -82,11 +82,16 @@ def cached_linear(mod: torch.nn.Linear, x: torch.Tensor, cache: WeightCache) -> 
     return torch.nn.functional.linear(x, cast[0], cast[1] if len(cast) > 1 else None)
 
 
+# (bound once: a call asks these each time)
+_forward_ad = torch.autograd.forward_ad
+_transforms_active, _is_tracing = torch._C._are_functorch_transforms_active, torch.jit.is_tracing
+_is_compiling, _dispatch_mode = torch.compiler.is_compiling, torch.utils._python_dispatch._get_current_dispatch_mode
+
+
 def plain_eager() -> bool:
     """No transform, trace or dispatch mode that has to see each operation."""
-    return (torch.autograd.forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active()
-            and not torch.jit.is_tracing() and not torch.compiler.is_compiling()
-            and torch.utils._python_dispatch._get_current_dispatch_mode() is None)
+    return (_forward_ad._current_level < 0 and not _transforms_active() and not _is_tracing() and not _is_compiling()
+            and _dispatch_mode() is None)
 
 
 TENSOR_TYPES = (torch.Tensor, torch.nn.Parameter)
@@ -101,8 +106,7 @@ def plain_tensor(t: torch.Tensor) -> bool:
 
 def carries_tangent(t: torch.Tensor) -> bool:
     """Whether t is a dual number of forward-mode differentiation."""
-    ad = torch.autograd.forward_ad
-    return ad._current_level >= 0 and ad.unpack_dual(t).tangent is not None
+    return _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None
 
 
 def first_order(gy: torch.Tensor) -> bool:
