@@ -294,8 +294,9 @@ int walsh_hadamard_linear_bwd(const void *x, int64_t ldx, const void *gy, int64_
  *   strides of walsh_hadamard_linear_ex_fwd: x and gx rows hold group g at
  *   g*gsx (gsx >= in_o), gy rows at g*gsy (gsy >= out_o); gx slots in
  *   [in_o, roundup(in_o, 4)) are written as zeros (slots past that are not
- *   written), pad slots of x and gy are not read.  The backward of the
- *   group-padded SwiGLU hidden layout. */
+ *   written); slots [in_o, roundup(in_o, 4)) of x and [out_o, roundup(out_o, 4))
+ *   of gy must hold finite values (they meet zero weights), those past them are
+ *   not read.  The backward of the group-padded SwiGLU hidden layout. */
 int walsh_hadamard_linear_ex_bwd(const void *x, int64_t ldx, int64_t gsx, const void *gy, int64_t ldg, int64_t gsy,
                                  int64_t M, int64_t in_o, int64_t out_o, const uint8_t *kweight,
                                  const uint8_t *kweight_t, const float *alpha, const float *beta, const float *latent,
@@ -473,7 +474,7 @@ int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_
  * (src/model/chassis.py:262-330).  Row j of sequence b is row j % page of page
  * table[b*table_sb + j / page] (int32); k_pages and v_pages hold n_pages pages
  * [G][page][D], element (p, g, r, d) at p*sp + g*sg + r*sr + d of both.  page is
- * a power of two from 16, or any size where pages_per_seq is 1; n_pages,
+ * a power of two from 16, or any size where pages_per_seq is 1;
  * strides multiples of 8, bases 16-byte aligned; pages_per_seq * page <= 2^30;
  * B <= 65535, B * H < 2^22.
  *
@@ -483,7 +484,8 @@ int walsh_window_attention_bwd(const void *q, int64_t q_sb, int64_t q_sh, int64_
  *   the last `window` rows and the first `sinks` ones (window <= 0: all).
  *   o = softmax(scale q k^T) v; zeros for a length of 0.  A length past the
  *   table, or a page number outside the pool among the rows seen, gives NaN
- *   for that sequence and reads nothing outside.  Chunks of the rows are
+ *   for that sequence and reads nothing outside.  bf16 weights enter the product
+ *   with v in two bf16 parts (D >= 32) or rounded once (16).  Chunks of the rows are
  *   joined from the workspace (walsh_paged_decode_workspace_bytes, 0 where one
  *   chunk holds them all).
  * walsh_paged_kv_write: k and v [B][T][G][D] (strides sb, st, sg of both) into

@@ -26,9 +26,13 @@
 //
 // Roundings.  Scores, maxima, sums, lse, Delta and all accumulators are
 // float32.  bf16 tensors have their weights P and dS rounded to bf16 for the
-// second products (the matrix cores' operand type; relative 2^-9 each, the
+// second products (the matrix cores' operand type; off by up to 2^-8 each, the
 // size of the inputs' own rounding); the sum of weights that normalises a row
-// takes them unrounded, and dQ at D <= 32 dS in two parts.
+// takes them unrounded, and dQ at D <= 32 dS in two parts.  Relative errors are
+// 2.2e-3 for o and 2.3 to 2.4e-3 for the gradients, where the rounding of the
+// results alone leaves 1.6 to 1.7e-3.  Two parts everywhere reach those, for
+// 23 to 34% more time of the forward and 18 to 32% of the backward (2 x 32
+// heads of 128, 4,096 tokens, window 1,024: 185 us and 228, 547 and 680).
 #include "tiles.h"
 
 namespace walsh {
@@ -128,13 +132,19 @@ __device__ __forceinline__ int xcd_item(int n) {
 // 32 keys that none of a wavefront's queries sees are passed over, and only
 // those seen in part are masked.  Bound by the matrix products and the
 // softmax's vector instructions, which two wavefronts per SIMD overlap in part:
-// 2 x 32 heads of 128, 8,192 tokens, window 1,024, bf16: 340 us, 760 TFLOP/s of
-// what is visible (a large product reaches 1,210).  Of 362 us without the
-// loads' present order, 51 went without the softmax, 54 without the tiles'
-// loads.  256 queries on a tile took 394 us, 64 queries per wavefront (each
+// 2 x 32 heads of 128, 8,192 tokens, window 1,024, bf16: 350 to 390 us alone
+// (from one card to another) and 480 in a row, at the clock that the card holds
+// then: 740 to 660 and 540 TFLOP/s of what is visible (a large product reaches
+// 1,210).  A block's scores, softmax and second products depend on each other,
+// and blocks follow one another strictly: the branch around the rescaling ends
+// the compiler's schedule.  Of 362 us without the loads' present order, 51 went
+// without the softmax, 54 without the tiles' loads.  256 queries on a tile took 394 us, 64 queries per wavefront (each
 // LDS operand used twice, at twice the accumulators) 680, three to four tiles
 // on their way 440.  Heads of 16: 28 us for 8 x 32 heads, 1,024 tokens, window
-// 256, the exponentials and masks of short products.
+// 256, the exponentials and masks of short products.  float32,
+// of which the matrix cores do an eighth of bf16's (154 TFLOP/s in a large
+// product): heads of 128, 64, 32 and 16 reach 103, 99, 82 and 43 TFLOP/s (2 x 32
+// heads of 64, 4,096 tokens, window 1,024: 608 us).
 constexpr int kWinWaves = 4;
 constexpr int kWinQ = 32 * kWinWaves;   // queries (or keys, dK and dV) per workgroup
 template <typename T, int D> struct WinCfg {
@@ -379,8 +389,8 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // to one side, and leaves dQ and dK 2.5 to 2.65e-3 off instead of 2.4e-3 (one
 // rounding of the results alone: 1.66e-3), for 4% less time.  Tiles and bounds
 // as in the forward, three products where that has two: 32 heads on 8 of 128,
-// 2 x 4,096 padded tokens, window 1,024, 16 first tokens, bf16: 205 us (the
-// forward 151, with what rounding took 170).
+// 2 x 4,096 padded tokens, window 1,024, 16 first tokens, bf16: 205 to 228 us
+// from one card to another (the forward 151, with what rounding took 170 to 188).
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
@@ -465,8 +475,10 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
                 pack(f, ds + 8 * t);
                 if constexpr (sizeof(T) == 2 && ND == 1) {
                     // one product a block: dS goes in two parts, its rounding
-                    // with it (relative error of dQ at D = 16, its own
-                    // rounding in it: 2.6e-3 without, 1.8e-3 so)
+                    // with it (relative error of dQ, its own rounding in it, 8
+                    // x 32 heads of 16 and 2 x 32 of 32, 1,024 tokens, window
+                    // 256: 2.48 and 2.43e-3 without, 1.74 and 1.72e-3 so; the
+                    // backward's kernels 81 and 39 us, 90 and 40 so)
                     const Frag<T> k0c = L::col_from(kc, 32 * j + 16 * t, 0);
                     Frag<T> rest;
                     pack_rest(rest, ds + 8 * t, f);
@@ -505,9 +517,12 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // are summed in a fixed order; an unsplit block is stored at once.  Keys stay
 // in registers and queries pass by, so shared heads' gradients need no sum
 // afterwards.  Four products, and registers for no more than one of the score
-// tiles at a time: 273 us for the case above (loads in two bursts, as in the
+// tiles at a time: 273 to 311 us for the case above (loads in two bursts, as in the
 // other kernels, took 12% more).  float32 at D = 64 runs two wavefronts per SIMD
-// (332 us for 32 heads on 8, 2,048 tokens, causal; 368 with one).
+// (332 us for 32 heads on 8, 2,048 tokens, causal; 368 with one).  The whole
+// backward in float32 takes 2.0 ms for 2 x 32 heads of 64, 4,096 tokens, window
+// 1,024, and 4.4 of 128: 74 and 68 TFLOP/s of the five products it cannot do
+// without, 104 and 96 of the seven that the two kernels form.
 template <typename T, int D> struct WinBwdCfg {
     static constexpr int KL = D == 128 && sizeof(T) == 2 ? 2 : 0;     // K operands kept in LDS
     static constexpr int QC = D == 128 && sizeof(T) == 4 ? 32 : 64;   // rows of a tile
