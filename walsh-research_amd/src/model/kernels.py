@@ -1035,7 +1035,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     rows and sees the last ``window`` (<= 0: all) and the first ``sinks`` of
     them -> [B, H, 1, D] in q.dtype, zeros for a length of 0, NaN where a
     length or a page number lies outside the table or the pool (they are on
-    the device: nothing outside is read)."""
+    the device: nothing outside is read).  Has no derivatives."""
     _hip.require_device(q, "query")
     assert q.dim() == 4 and q.shape[2] == 1, "paged_decode_attention: q [B, H, 1, D]"
     B, H, _, D = q.shape
