@@ -450,3 +450,31 @@ def test_windowed_attention_layer_in_forward_mode():
     with torch.no_grad(), fw.dual_level():
         do = fw.unpack_dual(layer._windowed(fw.make_dual(q, t), k, v, 0, True)).tangent
     assert np.abs(do.double().cpu().numpy() - want).max() <= 2e-4 and np.abs(want).max() > 0.1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,G,T,D,W,S,lengths", [(4, 2, 300, 16, 0, 0, None), (4, 2, 300, 32, 70, 3, [300, 129]),
+                                                 (4, 4, 513, 64, 0, 0, [513, 33]), (2, 1, 513, 64, 100, 40, None),
+                                                 (4, 2, 300, 128, 0, 0, [300, 1]), (4, 2, 700, 128, 65, 1, [700, 290])])
+def test_window_attention_query_gradients_of_keys_with_an_offset(H, G, T, D, W, S, lengths):
+    """A vector added to all keys moves all of a row's scores alike and
+    changes no gradient of q, whose weights dS sum to nothing: roundings that
+    leave a rest of the sum would be multiplied by it.  The keys are multiples
+    of 2^-5 within 1, so that 4 plus a key is a bf16 number: both calls have
+    the same exact result, and their errors, of roundings of the same sizes,
+    differ by less than 2."""
+    from src.model.attention import window_attention
+    q, k, v, go = make(2, H, G, T, T, D, torch.bfloat16, D + T, "bhtd")
+    k = (torch.rand(k.shape, generator=torch.Generator().manual_seed(T)).mul(64).floor().sub(32) / 32).bfloat16().cuda()
+    far = (k.float() + 4).bfloat16()
+    assert torch.equal(far.float() - 4, k.float())
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    want = oatt.window_attention_f64(*(t.double().cpu().numpy() for t in (q, k, v)), W, S, lengths,
+                                     go=go.double().cpu().numpy())["dq"]
+    err = []
+    for keys in (k, far):
+        x = q.clone().requires_grad_(True)
+        (dq,) = torch.autograd.grad(window_attention(x, keys, v, W, S, ln), (x,), go)
+        err.append(np.linalg.norm(dq.double().cpu().numpy() - want) / np.linalg.norm(want))
+    print(f"relative error {err[0]:.2e}, with the offset {err[1]:.2e}", flush=True)
+    assert err[1] <= 2 * err[0] and err[0] <= 2.0 ** -8

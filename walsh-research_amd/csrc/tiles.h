@@ -67,6 +67,17 @@ __device__ __forceinline__ float dot(const Frag<uint16_t> &a, const Frag<uint16_
     return s;
 }
 
+// c and the sum of an operand's elements (two to an instruction).
+__device__ __forceinline__ float add_all(float c, const Frag<uint16_t> &f) {
+    const u32x4 u = __builtin_bit_cast(u32x4, f.v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t pair = u[i];               // (of an element itself the cast takes the first)
+        c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, 0x3f803f80u), c, false);
+    }
+    return c;
+}
+
 // A value that is the same in every lane, as a scalar: quotients and loads
 // leave such values in vector registers, and their users with them.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }

@@ -391,6 +391,14 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // as in the forward, three products where that has two: 32 heads on 8 of 128,
 // 2 x 4,096 padded tokens, window 1,024, 16 first tokens, bf16: 205 to 228 us
 // from one card to another (the forward 151, with what rounding took 170 to 188).
+//
+// A row's dS sum to 0, so a vector common to its keys cancels from dQ.  Rounded
+// to bf16, and with a Delta that is, they leave a rest of the sum, which such a
+// vector multiplies (keys within 1 of it, 4 in every element: dQ 1.5e-2 off).
+// The rest is summed as the products took dS and goes back, with its sign
+// turned, in even parts to keys at the end of the row's range: 2.4e-3, as
+// without a common vector, for 1 to 2.5% of the backward's time at D >= 64 and
+// 5 to 6% below.
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
@@ -445,6 +453,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     uint32_t ka[NK], kc = L::col_base(smem, lane);
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) ka[kk] = L::row_base(smem, n, hi) ^ L::row_step(kk);
+    float sum = 0.f;                              // of the row's dS as the products took them
     if (ch.n > 0) fetch_k(0), fetch_v(0);
     for (int i = 0; i < ch.n; ++i) {
         tiles_ready();
@@ -473,6 +482,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             for (int t = 0; t < 2; ++t) {
                 Frag<T> f;
                 pack(f, ds + 8 * t);
+                if constexpr (sizeof(T) == 2) sum = add_all(sum, f);
                 if constexpr (sizeof(T) == 2 && ND == 1) {
                     // one product a block: dS goes in two parts, its rounding
                     // with it (relative error of dQ, its own rounding in it, 8
@@ -482,6 +492,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
                     const Frag<T> k0c = L::col_from(kc, 32 * j + 16 * t, 0);
                     Frag<T> rest;
                     pack_rest(rest, ds + 8 * t, f);
+                    sum = add_all(sum, rest);
                     mma(acc[0], k0c, f);
                     mma(acc[0], k0c, rest);
                 } else {
@@ -494,6 +505,22 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
         kc += other;
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) ka[kk] += other;
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (ch.n > 0) {
+            // what is left of the sum goes, with its sign turned, to the first
+            // 32 keys of the last tile (rows past the length are zeros there)
+            const int k0 = ch.at(ch.n - 1) * KC;
+            const float each = -half_sum(sum) / (float)min(32, len - k0);
+            const float w[8] = {each, each, each, each, each, each, each, each};
+            const uint32_t last = L::col_base(smem + ((ch.n - 1) & 1) * 2 * L::BYTES, lane);
+            Frag<T> f;
+            pack(f, w);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int c = 0; c < ND; ++c) mma(acc[c], L::col_from(last, 16 * t, c), f);
+        }
     }
     if (qi >= a.Tq) return;
     T *dq = (T *)a.dq + (((int64_t)b * a.H + h) * a.Tq + qi) * D;
