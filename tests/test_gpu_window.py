@@ -478,3 +478,29 @@ def test_window_attention_query_gradients_of_keys_with_an_offset(H, G, T, D, W, 
         err.append(np.linalg.norm(dq.double().cpu().numpy() - want) / np.linalg.norm(want))
     print(f"relative error {err[0]:.2e}, with the offset {err[1]:.2e}", flush=True)
     assert err[1] <= 2 * err[0] and err[0] <= 2.0 ** -8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,G,T,D,W,S", [(2, 4, 2, 300, 16, 64, 2), (2, 4, 2, 300, 32, 0, 0), (2, 4, 4, 300, 64, 0, 0),
+                                           (2, 2, 1, 513, 128, 100, 2), (2, 8, 4, 40, 128, 4, 2), (3, 32, 8, 300, 64, 70, 0)])
+def test_window_attention_gradients_of_values_with_an_offset(B, H, G, T, D, W, S):
+    """A vector added to all values moves every output alike, and with it
+    Delta and each go v^T: dS, dQ and dK do not change.  They would by what
+    the output's weights, rounded and not normalised as rounded, have too much
+    or too little.  Values are multiples of 2^-5 within 1, 4 plus them bf16
+    numbers; the roundings left are of the same sizes, so errors differ by less
+    than 2."""
+    from src.model.attention import window_attention
+    q, k, v, go = make(B, H, G, T, T, D, torch.bfloat16, D + T, "bhtd")
+    v = (torch.rand(v.shape, generator=torch.Generator().manual_seed(T)).mul(64).floor().sub(32) / 32).bfloat16().cuda()
+    far = (v.float() + 4).bfloat16()
+    go = (go.float() + 1).bfloat16()
+    assert torch.equal(far.float() - 4, v.float())
+    r = oatt.window_attention_f64(*(t.double().cpu().numpy() for t in (q, k, v)), W, S, go=go.double().cpu().numpy())
+    err = []
+    for values in (v, far):
+        x = [t.clone().requires_grad_(True) for t in (q, k)]
+        grads = torch.autograd.grad(window_attention(*x, values, W, S), x, go)
+        err.append([np.linalg.norm(t.double().cpu().numpy() - r[n]) / np.linalg.norm(r[n]) for n, t in zip(("dq", "dk"), grads)])
+    print(f"relative errors {err[0]}, with the offset {err[1]}", flush=True)
+    assert all(b <= 2 * a and a <= 2.0 ** -7 for a, b in zip(*err))

@@ -27,8 +27,14 @@
 // Roundings.  Scores, maxima, sums, lse, Delta and all accumulators are
 // float32.  bf16 tensors have their weights P and dS rounded to bf16 for the
 // second products (the matrix cores' operand type; off by up to 2^-8 each, the
-// size of the inputs' own rounding); the sum of weights that normalises a row
-// takes them unrounded, and dQ at D <= 32 dS in two parts.  Relative errors are
+// size of the inputs' own rounding), and dQ at D <= 32 takes dS in two parts.
+// A row is normalised by the sum of its rounded weights, lse by that of the
+// unrounded ones: o is then a mean of the values, and a vector common to them
+// passes through unchanged.  (Normalised by the unrounded sum it came out
+// (1 + 2^-9 or so) times as large, which Delta carried into dS: values within 1
+// of 4 in every element, and a gradient of o with a mean of 1, had dQ 1.0 to
+// 3.6e-2 and dK 0.5 to 3.7e-2 off.  It costs 2 to 6% of the forward where lse is
+// asked for, nothing measurable where it is not.)  Relative errors are
 // 2.2e-3 for o and 2.3 to 2.4e-3 for the gradients, where the rounding of the
 // results alone leaves 1.6 to 1.7e-3.  Two parts everywhere reach those, for
 // 23 to 34% more time of the forward and 18 to 32% of the backward (2 x 32
@@ -153,8 +159,9 @@ template <typename T, int D> struct WinCfg {
     static constexpr int ND = (D + 31) / 32;                          // 32-wide blocks of D
 };
 
-template <typename T, int D>
+template <typename T, int D, bool LSE>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_fwd_kernel(WinArgs a) {
+    constexpr bool EXACT = LSE || sizeof(T) == 4, ROUNDED = sizeof(T) == 2;   // sums of the weights in use
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
     typedef Tile<T, D, KC> L;
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -181,7 +188,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     f32x16 acc[ND];
 #pragma unroll
     for (int c = 0; c < ND; ++c) acc[c] = f32x16{};
-    float m = kNoScore, l = 0.f;
+    float m = kNoScore, l = 0.f, lr = 0.f;        // lr: of the weights as the products take them
 
     const T *kb = (const T *)a.k + b * a.skv.sb + g * a.skv.sh, *vb = (const T *)a.v + b * a.skv.sb + g * a.skv.sh;
     const Chunks ch = wlo <= whi ? win_chunks<KC>(a, wlo, whi) : Chunks{0, 0, 0};
@@ -221,23 +228,28 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
                 const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f((m - mn) * a.sl2);
                 m = mn;
                 l *= al;
+                lr *= al;
 #pragma unroll
                 for (int c = 0; c < ND; ++c) acc[c] *= al;
             }
             const float mo = -m * a.sl2;
-            float w[16], l0 = 0.f, l1 = 0.f;
+            float w[16];
+            [[maybe_unused]] float l0 = 0.f, l1 = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.sl2, mo));
+            if constexpr (EXACT) {
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                l0 += w[r];
-                l1 += w[r + 1];
+                for (int r = 0; r < 16; r += 2) {
+                    l0 += w[r];
+                    l1 += w[r + 1];
+                }
+                l += l0 + l1;
             }
-            l += l0 + l1;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 Frag<T> pf;
                 pack(pf, w + 8 * t);
+                if constexpr (ROUNDED) lr = add_all(lr, pf);
 #pragma unroll
                 for (int c = 0; c < ND; ++c) mma(acc[c], L::col_from(va, 32 * j + 16 * t, c), pf);
             }
@@ -248,8 +260,9 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
         for (int kk = 0; kk < NK; ++kk) ka[kk] += other;
     }
     l = half_sum(l);
+    lr = ROUNDED ? half_sum(lr) : l;
     if (qi >= a.Tq) return;
-    const float inv = 1.f / l;                    // (no row that sees a key has none but infinite scores' l = 0)
+    const float inv = 1.f / lr;                   // (no row that sees a key has none but infinite scores' sum 0)
     T *op = (T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)qi * a.so.st;
 #pragma unroll
     for (int c = 0; c < ND; ++c)
@@ -260,7 +273,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             const f32x4 v = f32x4{acc[c][4 * t], acc[c][4 * t + 1], acc[c][4 * t + 2], acc[c][4 * t + 3]} * inv;
             win_store(a, op + d, (((int64_t)b * a.H + h) * a.Tq + qi) * D + d, v, live);
         }
-    if (a.lse && hi == 0)
+    if (LSE && hi == 0)
         a.lse[((int64_t)b * a.H + h) * a.Tq + qi] = live ? (m * a.sl2 + log2f(l)) * (1.f / kLog2e) : -INFINITY;
 }
 
@@ -280,7 +293,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     constexpr int NK = D / 16, ND = (D + 31) / 32;
     typedef Tile<T, D, 32> L;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ float stat[kWinWaves][2][32];
+    __shared__ float stat[kWinWaves][3][32];      // maximum, both sums
     const int nqt = (a.Tq + 31) / 32;
     const int id = xcd_item(nqt * a.H * a.B);
     if (id < 0) return;
@@ -300,7 +313,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
     f32x16 acc[ND];
 #pragma unroll
     for (int c = 0; c < ND; ++c) acc[c] = f32x16{};
-    float m = kNoScore, l = 0.f;
+    float m = kNoScore, l = 0.f, lr = 0.f;
     const T *kb = (const T *)a.k + b * a.skv.sb + g * a.skv.sh, *vb = (const T *)a.v + b * a.skv.sb + g * a.skv.sh;
     const Chunks ch = pa <= pb ? win_chunks<32>(a, pa, pb) : Chunks{0, 0, 0};
     unsigned char *vl = smem + wave * WinSplitCfg<T, D>::WAVE;
@@ -329,6 +342,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f((m - mn) * a.sl2);
             m = mn;
             l *= al;
+            lr *= al;
 #pragma unroll
             for (int c = 0; c < ND; ++c) acc[c] *= al;
         }
@@ -343,12 +357,14 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
         for (int t = 0; t < 2; ++t) {
             Frag<T> pf;
             pack(pf, w + 8 * t);
+            if constexpr (sizeof(T) == 2) lr = add_all(lr, pf);
 #pragma unroll
             for (int c = 0; c < ND; ++c) mma(acc[c], L::col(vl + buf * WinSplitCfg<T, D>::VB, 16 * t, c, lane), pf);
         }
     }
     l = half_sum(l);
-    // the wavefronts' parts: o = sum_w acc_w e^(m_w - m) / sum_w l_w e^(m_w - m)
+    lr = sizeof(T) == 2 ? half_sum(lr) : l;
+    // the wavefronts' parts: o = sum_w acc_w e^(m_w - m) / sum_w lr_w e^(m_w - m)
     wait_loads();
     float *av = (float *)vl;   // [32 queries][D] of this wavefront (its V is used up)
 #pragma unroll
@@ -359,13 +375,13 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             if (D % 32 && d >= D) continue;
             store4(av + n * D + d, f32x4{acc[c][4 * t], acc[c][4 * t + 1], acc[c][4 * t + 2], acc[c][4 * t + 3]});
         }
-    if (hi == 0) stat[wave][0][n] = m, stat[wave][1][n] = l;
+    if (hi == 0) stat[wave][0][n] = m, stat[wave][1][n] = l, stat[wave][2][n] = lr;
     __syncthreads();
     for (int e = threadIdx.x; e < 32 * (D / 4); e += 64 * kWinWaves) {
         const int r = e / (D / 4), d = e % (D / 4) * 4, q = qt * 32 + r, pos = q + off;
         if (q >= a.Tq) break;
         const bool live = pos >= 0 && pos < len;
-        float mm = stat[0][0][r], ll = 0.f;
+        float mm = stat[0][0][r], ll = 0.f, lt = 0.f;
 #pragma unroll
         for (int w = 1; w < kWinWaves; ++w) mm = fmaxf(mm, stat[w][0][r]);
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -374,9 +390,10 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             const float f = __builtin_amdgcn_exp2f((stat[w][0][r] - mm) * a.sl2);
             v += load4((const float *)(smem + w * WinSplitCfg<T, D>::WAVE) + r * D + d) * f;
             ll += stat[w][1][r] * f;
+            lt += stat[w][2][r] * f;
         }
         win_store(a, (T *)a.o + b * a.so.sb + h * a.so.sh + (int64_t)q * a.so.st + d,
-                  (((int64_t)b * a.H + h) * a.Tq + q) * D + d, v * (1.f / ll), live);
+                  (((int64_t)b * a.H + h) * a.Tq + q) * D + d, v * (1.f / lt), live);
         if (a.lse && d == 0)
             a.lse[((int64_t)b * a.H + h) * a.Tq + q] = live ? (mm * a.sl2 + log2f(ll)) * (1.f / kLog2e) : -INFINITY;
     }
@@ -832,7 +849,8 @@ WALSH_EXPORT int walsh_window_attention_fwd(const void *q, int64_t q_sb, int64_t
             launch(window_fwd_split_kernel<T, DD>, dim3((unsigned)(ceil_div(n32, 8) * 8)), dim3(64 * kWinWaves),
                    (uint32_t)(kWinWaves * WinSplitCfg<T, DD>::WAVE), (hipStream_t)stream, a);
         else
-            launch(window_fwd_kernel<T, DD>, dim3((unsigned)(ceil_div(n, 8) * 8)), dim3(64 * kWinWaves),
+            launch(a.lse ? window_fwd_kernel<T, DD, true> : window_fwd_kernel<T, DD, false>,
+                   dim3((unsigned)(ceil_div(n, 8) * 8)), dim3(64 * kWinWaves),
                    (uint32_t)(4 * Tile<T, DD, WinCfg<T, DD>::KC>::BYTES), (hipStream_t)stream, a);
     });
     return check_hip(hipGetLastError(), fn);
