@@ -504,3 +504,20 @@ def test_window_attention_gradients_of_values_with_an_offset(B, H, G, T, D, W, S
         err.append([np.linalg.norm(t.double().cpu().numpy() - r[n]) / np.linalg.norm(r[n]) for n, t in zip(("dq", "dk"), grads)])
     print(f"relative errors {err[0]}, with the offset {err[1]}", flush=True)
     assert all(b <= 2 * a and a <= 2.0 ** -7 for a, b in zip(*err))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,G,T,D,W", [(4, 4, 300, 16, 64), (4, 4, 142, 32, 17), (4, 2, 513, 128, 100)])
+def test_window_attention_query_gradients_of_large_scores_in_float32(H, G, T, D, W):
+    """Queries and keys with an offset of twelve times their spread: scores
+    near 36 sqrt(D), whose float32 steps move each weight by some 1e-6
+    relatively.  That error enters dQ, dK and dV alike, term by term; the keys'
+    offset multiplies it in dQ unless a row's dS sum to nothing."""
+    from src.model.attention import window_attention
+    q, k, v, go = make(2, H, G, T, T, D, torch.float32, D + T, "bhtd")
+    x = [t.mul_(0.25).add_(3).requires_grad_(True) for t in (q, k)] + [v.requires_grad_(True)]
+    grads = torch.autograd.grad(window_attention(*x, W, 2), x, go)
+    r = oatt.window_attention_f64(*(t.detach().double().cpu().numpy() for t in x), W, 2, go=go.double().cpu().numpy())
+    err = [np.linalg.norm(t.double().cpu().numpy() - r[n]) / np.linalg.norm(r[n]) for n, t in zip(("dq", "dk", "dv"), grads)]
+    print("relative errors", err, flush=True)
+    assert err[0] <= 1.6 * max(err[1:])

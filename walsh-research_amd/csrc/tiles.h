@@ -78,6 +78,10 @@ __device__ __forceinline__ float add_all(float c, const Frag<uint16_t> &f) {
     return c;
 }
 
+__device__ __forceinline__ float add_all(float c, const Frag<float> &f) {
+    return c + (((f.v[0] + f.v[1]) + (f.v[2] + f.v[3])) + ((f.v[4] + f.v[5]) + (f.v[6] + f.v[7])));
+}
+
 // A value that is the same in every lane, as a scalar: quotients and loads
 // leave such values in vector registers, and their users with them.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }

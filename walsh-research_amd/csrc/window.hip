@@ -415,7 +415,9 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // The rest is summed as the products took dS and goes back, with its sign
 // turned, in even parts to keys at the end of the row's range: 2.4e-3, as
 // without a common vector, for 1 to 2.5% of the backward's time at D >= 64 and
-// 5 to 6% below.
+// 5 to 6% below.  In float32 the same holds of the steps of large scores (keys
+// and queries at 3, spread by 0.25: dQ 7 to 32e-6 off, 3 to 17e-6 so, as dK and
+// dV), for 1 to 2%.
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) void window_bwd_q_kernel(WinArgs a) {
     constexpr int KC = WinCfg<T, D>::KC, NK = WinCfg<T, D>::NK, ND = WinCfg<T, D>::ND, NJ = KC / 32;
@@ -499,7 +501,7 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
             for (int t = 0; t < 2; ++t) {
                 Frag<T> f;
                 pack(f, ds + 8 * t);
-                if constexpr (sizeof(T) == 2) sum = add_all(sum, f);
+                sum = add_all(sum, f);
                 if constexpr (sizeof(T) == 2 && ND == 1) {
                     // one product a block: dS goes in two parts, its rounding
                     // with it (relative error of dQ, its own rounding in it, 8
@@ -523,21 +525,19 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) ka[kk] += other;
     }
-    if constexpr (sizeof(T) == 2) {
-        if (ch.n > 0) {
-            // what is left of the sum goes, with its sign turned, to the first
-            // 32 keys of the last tile (rows past the length are zeros there)
-            const int k0 = ch.at(ch.n - 1) * KC;
-            const float each = -half_sum(sum) / (float)min(32, len - k0);
-            const float w[8] = {each, each, each, each, each, each, each, each};
-            const uint32_t last = L::col_base(smem + ((ch.n - 1) & 1) * 2 * L::BYTES, lane);
-            Frag<T> f;
-            pack(f, w);
+    if (ch.n > 0) {
+        // what is left of the sum goes, with its sign turned, to the first 32
+        // keys of the last tile (rows past the length are zeros there)
+        const int k0 = ch.at(ch.n - 1) * KC;
+        const float each = -half_sum(sum) / (float)min(32, len - k0);
+        const float w[8] = {each, each, each, each, each, each, each, each};
+        const uint32_t last = L::col_base(smem + ((ch.n - 1) & 1) * 2 * L::BYTES, lane);
+        Frag<T> f;
+        pack(f, w);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int c = 0; c < ND; ++c) mma(acc[c], L::col_from(last, 16 * t, c), f);
-        }
+            for (int c = 0; c < ND; ++c) mma(acc[c], L::col_from(last, 16 * t, c), f);
     }
     if (qi >= a.Tq) return;
     T *dq = (T *)a.dq + (((int64_t)b * a.H + h) * a.Tq + qi) * D;
