@@ -350,3 +350,17 @@ def test_paged_decode_rounds_bf16_results_once(H, G, D, page, lengths, W, S):
     err, tol = np.abs(o[:, :, 0].double().numpy() - want), 2.0 ** -8 * np.abs(want) + (2.0 ** -16 + 2 * rho) * a
     print(f"worst error / bound {(err / np.maximum(tol, 1e-30)).max():.3f}", flush=True)
     assert (err <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,n", [(1, 1), (1, 40), (4, 40), (4, 700), (2, 3000)])
+def test_paged_decode_of_equal_values_is_that_value(H, n):
+    """A mean of equal values is the value, whatever the weights' roundings:
+    at head_dim 16, where bf16 weights are rounded, their sum is taken as
+    rounded.  The sums are float32: 2^-24 times the number of terms, far below
+    half a step of bf16."""
+    q, kp, vp, table, lens = make(1, H, 1, 16, 16, [n], torch.bfloat16, n)
+    row = torch.randn(16, generator=torch.Generator().manual_seed(n)).bfloat16()
+    vp[:] = row
+    o = decode(q, kp, vp, table, lens)
+    assert torch.equal(o, row.expand_as(o))

@@ -29,7 +29,8 @@
 // off by up to 2^-8 each): the matrix cores have the time for it (64 sequences
 // of up to 4,096, 32 heads of 128: 390 us both ways, of 64, 32 sequences: 108
 // and 109, of 32: 102 and 106).  Not so heads of 16, whose vector work is the
-// bound (54 us with one part, 68 with two): they round the weights once.
+// bound (54 us with one part, 68 with two): they round the weights once, and
+// their sum takes them as rounded, as in the whole-sequence kernel.
 #include "tiles.h"
 
 namespace walsh {
@@ -238,13 +239,16 @@ __global__ __launch_bounds__(64 * kPgWaves, sizeof(T) == 4 && D == 128 ? 1 : 2) 
             float w[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(fmaf(sc[u][r], a.sl2, mo));
+            if constexpr (sizeof(T) == 4 || TWO) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) l += w[r];
+                for (int r = 0; r < 16; ++r) l += w[r];
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 Frag<T> pf, rest;
                 pack(pf, w + 8 * t);
                 if constexpr (TWO) pack_rest(rest, w + 8 * t, pf);
+                else if constexpr (sizeof(T) == 2) l = add_all(l, pf);
 #pragma unroll
                 for (int c = 0; c < ND; ++c) {
                     const Frag<T> vc = L::col(vt + u * L::BYTES, 16 * t, c, lane);
