@@ -146,7 +146,7 @@ __device__ __forceinline__ int xcd_item(int n) {
 // the compiler's schedule.  Of 362 us without the loads' present order, 51 went
 // without the softmax, 54 without the tiles' loads.  256 queries on a tile took 394 us, 64 queries per wavefront (each
 // LDS operand used twice, at twice the accumulators) 680, three to four tiles
-// on their way 440.  Heads of 16: 28 us for 8 x 32 heads, 1,024 tokens, window
+// on their way 440.  Heads of 16: 28 to 31 us for 8 x 32 heads, 1,024 tokens, window
 // 256, the exponentials and masks of short products.  float32,
 // of which the matrix cores do an eighth of bf16's (154 TFLOP/s in a large
 // product): heads of 128, 64, 32 and 16 reach 103, 99, 82 and 43 TFLOP/s (2 x 32
@@ -406,8 +406,9 @@ __global__ __launch_bounds__(64 * kWinWaves, sizeof(T) == 4 && D == 128 ? 1 : 2)
 // to one side, and leaves dQ and dK 2.5 to 2.65e-3 off instead of 2.4e-3 (one
 // rounding of the results alone: 1.66e-3), for 4% less time.  Tiles and bounds
 // as in the forward, three products where that has two: 32 heads on 8 of 128,
-// 2 x 4,096 padded tokens, window 1,024, 16 first tokens, bf16: 205 to 228 us
-// from one card to another (the forward 151, with what rounding took 170 to 188).
+// 2 x 4,096 padded tokens, window 1,024, 16 first tokens, bf16: 205 to 231 us
+// from one card to another (the forward 151, with lse and what rounding took 170
+// to 190).
 //
 // A row's dS sum to 0, so a vector common to its keys cancels from dQ.  Rounded
 // to bf16, and with a Delta that is, they leave a rest of the sum, which such a
