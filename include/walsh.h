@@ -445,8 +445,9 @@ int walsh_prefill_attention(const void *q, int64_t q_sb, int64_t q_sh, int64_t q
  * 0 < scale <= 1e6; B * H * ceil(max(Tq, Tk) / 128) < 2^24 - 7.  Scores,
  * softmax and sums in float32 (a visible q k^T below -1e30 has no weight);
  * bf16 rounds the weights (and their gradients) to bf16 for the products with
- * v (k and q).  k and v within the lengths must be finite: what the mask hides
- * from a row enters its sums with a weight of 0.
+ * v (k and q); o is divided by the sum of the rounded weights, lse is that of
+ * the unrounded ones.  k and v within the lengths must be finite: what the mask
+ * hides from a row enters its sums with a weight of 0.
  *
  * walsh_window_attention_fwd: lse [B, H, Tq] or null; rest, bf16, dense
  *   [B, H, Tq, D] or null, takes what rounding took from o.
