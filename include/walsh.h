@@ -872,6 +872,67 @@ int64_t walsh_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int walsh_linear_wgrad(const void *g, const void *x, int64_t M, int64_t N, int64_t K, float *dw, void *work,
                    int64_t work_bytes, void *stream);
 
+/* ------------------------------------------------------------------ tokens' probabilities
+ * walsh_token_logprobs_fwd: of every row of logits l [N][V] (row stride ld):
+ *     L = log(sum exp l);  logprob = l[token] - L;  entropy = -sum p log p, p = exp(l - L)
+ *     top [N][n], top_index [N][n]: the n largest l in descending order (of
+ *       equal ones the lowest indexes first), as l - L, and their indexes
+ *   in float32.  A negative token marks a row that is not counted: it is not
+ *   read; logprob and entropy are 0, top -inf and top_index -1.  A token of V
+ *   or more has logprob NaN.  -inf has probability 0; a row of nothing else
+ *   has logprob -inf everywhere and entropy 0.  NaN or +inf in a row make its
+ *   numbers NaN (as top_index NaN counts as -inf).  n up to 64 and V; with n 0
+ *   top and top_index may be null.  stats float [N][4], 16-byte aligned, or
+ *   null: what walsh_token_logprobs_bwd takes.
+ * walsh_token_logprobs_bwd: dlogits [N][V] (row stride ldd, the logits' dtype)
+ *   for the gradients g_logprob [N], g_entropy [N] and g_top [N][n] (each may
+ *   be null) of the outputs, with the forward's tokens, top_index and stats:
+ *     dl_i = [i = token] g_logprob + sum_j [i = top_index_j] g_top_j - p_i (G + g_entropy (log p_i + entropy)),
+ *     G = g_logprob + sum_j g_top_j
+ *   Rows that are not counted and rows of -inf get zeros; rows whose token is
+ *   V or more NaN.  dlogits may not alias logits.
+ *   N below 2^23, V below 2^30. */
+int walsh_token_logprobs_fwd(const void *logits, int64_t ld, int64_t N, int64_t V, const int64_t *tokens, int64_t n,
+                             float *logprob, float *entropy, float *top, int64_t *top_index, float *stats, int dtype,
+                             void *stream);
+int walsh_token_logprobs_bwd(const void *logits, int64_t ld, int64_t N, int64_t V, const int64_t *tokens, int64_t n,
+                             const int64_t *top_index, const float *stats, const float *g_logprob, const float *g_entropy,
+                             const float *g_top, void *dlogits, int64_t ldd, int dtype, void *stream);
+
+/* ------------------------------------------------------------------ dropout, embedding
+ * Dropout keeps element (row r, column c) of a matrix where 16 random bits are
+ *   at least `drop` (0 to 65536) and multiplies it by 65536 / (65536 - drop).
+ *   The bits are those of the counter-based generator of Salmon, Moraes, Dror
+ *   and Shaw (SC 2011), four words of 32 bits and ten rounds: key *seed (64
+ *   bits, on the device: a captured launch takes what it holds when replayed),
+ *   counter (c / 8, r, 0, rng_stream), column c in half c % 2 of word
+ *   (c % 8) / 2.  They are the same in every call with one seed and
+ *   rng_stream (0 to 2^32 - 1), so a backward needs no mask.  seed may be null
+ *   where drop is 0.
+ * walsh_dropout: y = dropout(x) (+ residual), rows of C with strides ldx, ldr,
+ *   ldy.  ydtype is float32 where x or the residual is, except that without a
+ *   residual float32 x may give bf16 y: dx = dropout(dy).  What is dropped is
+ *   0 whatever x holds.  y may be x or the residual itself.
+ * walsh_embedding_fwd: y[r] = dropout(scale weight[tokens[r]]), N rows of C;
+ *   rows of NaN for tokens outside 0 .. V - 1.
+ * walsh_embedding_bwd: dw[v] = scale times the sum, over the r with tokens[r] =
+ *   v, of dropout(gy)[r], every row of dw [V][C] written; tokens outside and
+ *   padding_idx (negative: none) add to none.  The sums are float32 in a fixed
+ *   order (deterministic).  Needs work of
+ *   walsh_embedding_bwd_workspace_bytes(N, V, C) bytes, 16-byte aligned.
+ * Each takes fewer than 2^31 - 65536 blocks of 8 columns (a row's last may be
+ *   part of one), rows at any alignment of their elements. */
+int walsh_dropout(const void *x, int64_t ldx, int xdtype, const void *residual, int64_t ldr, int rdtype, int64_t M,
+                  int64_t C, int drop, const int64_t *seed, int64_t rng_stream, void *y, int64_t ldy, int ydtype,
+                  void *stream);
+int walsh_embedding_fwd(const int64_t *tokens, int64_t N, const void *weight, int64_t ldw, int64_t V, int64_t C,
+                        float scale, int drop, const int64_t *seed, int64_t rng_stream, void *y, int64_t ldy,
+                        int wdtype, int ydtype, void *stream);
+int64_t walsh_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t C);
+int walsh_embedding_bwd(const int64_t *tokens, int64_t N, const void *gy, int64_t ldg, int64_t V, int64_t C, float scale,
+                        int64_t padding_idx, int drop, const int64_t *seed, int64_t rng_stream, void *dw, int64_t ldw,
+                        int gdtype, int wdtype, void *work, int64_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

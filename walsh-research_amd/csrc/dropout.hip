@@ -1,0 +1,91 @@
+// Dropout whose mask is never stored:
+//     y = x 65536 / (65536 - drop)  where the element's 16 random bits (rows8.h)
+//     are at least `drop`, else 0;  + residual
+// The gradient of x is the same function of the output's gradient without a
+// residual, its bits computed again.  What is dropped is 0 whatever x holds.
+#include "rows8.h"
+
+namespace walsh {
+
+struct DropoutArgs {
+    const void *x, *residual;
+    void *y;
+    int64_t ldx, ldr, ldy;
+    int C;
+    Blocks g;
+    Drop d;
+    float f;
+};
+
+// TR void: no residual.  U: blocks of a lane, loaded before the first is used.
+template <typename TX, typename TR, typename TY, int U>
+__global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
+    const uint32_t first = blockIdx.x * (256u * U);
+    const DropBits bits(a.d);
+    BlockAt at[U];
+    float v[U][8], r[U][8];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        at[j] = block_at(a.g, first, 256u * j + threadIdx.x);
+        if (at[j].row < a.g.rows) {
+            const int64_t row = at[j].row;
+            const int c = 8 * (int)at[j].col;
+            load8((const TX *)a.x + row * a.ldx + c, a.C - c, v[j]);
+            if constexpr (!__is_same(TR, void)) load8((const TR *)a.residual + row * a.ldr + c, a.C - c, r[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        if (at[j].row < a.g.rows) {
+            bits.apply(v[j], at[j].row, at[j].col);
+            const int c = 8 * (int)at[j].col;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[j][i] *= a.f;
+                if constexpr (!__is_same(TR, void)) v[j][i] += r[j][i];
+            }
+            store8((TY *)a.y + at[j].row * a.ldy + c, a.C - c, v[j]);
+        }
+    }
+}
+
+}  // namespace walsh
+
+using namespace walsh;
+
+WALSH_EXPORT int walsh_dropout(const void *x, int64_t ldx, int xdtype, const void *residual, int64_t ldr, int rdtype,
+                               int64_t M, int64_t C, int drop, const int64_t *seed, int64_t rng_stream, void *y,
+                               int64_t ldy, int ydtype, void *stream) {
+    const char *fn = "walsh_dropout";
+    if (M < 0 || C < 0 || C > 0x7fffffff - 8 || M > 0x7fffffff || M * ceil_div(C, 8) > kMaxBlocks)
+        return set_error(WALSH_ENOTSUP, "%s: M=%lld rows of C=%lld pass %lld blocks of 8", fn, (long long)M, (long long)C,
+                         (long long)kMaxBlocks);
+    if (drop < 0 || drop > 65536 || rng_stream < 0 || rng_stream > 0xffffffffll)
+        return set_error(WALSH_EINVAL, "%s: drop %d (0 to 65536), stream %lld (32 bits)", fn, drop, (long long)rng_stream);
+    for (int dt : {xdtype, ydtype, residual ? rdtype : ydtype})
+        if (dt != WALSH_F32 && dt != WALSH_BF16) return set_error(WALSH_ENOTSUP, "%s: dtype %d", fn, dt);
+    if (M == 0 || C == 0) return WALSH_OK;
+    if (!x || !y || (drop && !seed)) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
+    if (M > 1 && (ldx < C || ldy < C || (residual && ldr < C)))
+        return set_error(WALSH_EINVAL, "%s: rows of %lld overlap", fn, (long long)C);
+    constexpr int U = 2;
+    const DropoutArgs a{x, residual, y, ldx, ldr, ldy, (int)C, make_blocks(M, C),
+                        Drop{(const uint64_t *)seed, (uint32_t)rng_stream, (uint32_t)drop}, (float)kept_factor(drop)};
+    const dim3 G((unsigned)ceil_div(M * a.g.per_row, 256 * U)), N(256);
+    const hipStream_t s = (hipStream_t)stream;
+    const bool xb = xdtype == WALSH_BF16, rb = rdtype == WALSH_BF16, yb = ydtype == WALSH_BF16;
+    if (!residual) {
+        if (xb && yb) launch(dropout_kernel<uint16_t, void, uint16_t, U>, G, N, 0, s, a);
+        else if (!xb && yb) launch(dropout_kernel<float, void, uint16_t, U>, G, N, 0, s, a);
+        else if (!xb) launch(dropout_kernel<float, void, float, U>, G, N, 0, s, a);
+        else return set_error(WALSH_ENOTSUP, "%s: float32 from bf16", fn);
+    } else if (yb != (xb && rb)) {
+        return set_error(WALSH_ENOTSUP, "%s: the output has the wider type of x and the residual", fn);
+    } else {
+        if (xb && rb) launch(dropout_kernel<uint16_t, uint16_t, uint16_t, U>, G, N, 0, s, a);
+        else if (xb) launch(dropout_kernel<uint16_t, float, float, U>, G, N, 0, s, a);
+        else if (rb) launch(dropout_kernel<float, uint16_t, float, U>, G, N, 0, s, a);
+        else launch(dropout_kernel<float, float, float, U>, G, N, 0, s, a);
+    }
+    return check_hip(hipGetLastError(), fn);
+}

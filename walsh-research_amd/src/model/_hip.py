@@ -94,6 +94,12 @@ SIGNATURES = {
     "walsh_paged_kv_write": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64,
                                   _I64, _P, _I64, _I64, _P, _P, _I, _P]),
     "walsh_sample": (_I, [_P, _I64, _I64, _I64, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _I, _P]),
+    "walsh_token_logprobs_fwd": (_I, [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P, _I, _P]),
+    "walsh_token_logprobs_bwd": (_I, [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I, _P]),
+    "walsh_dropout": (_I, [_P, _I64, _I, _P, _I64, _I, _I64, _I64, _I, _P, _I64, _P, _I64, _I, _P]),
+    "walsh_embedding_fwd": (_I, [_P, _I64, _P, _I64, _I64, _I64, _F, _I, _P, _I64, _P, _I64, _I, _I, _P]),
+    "walsh_embedding_bwd_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "walsh_embedding_bwd": (_I, [_P, _I64, _P, _I64, _I64, _I64, _F, _I64, _I, _P, _I64, _P, _I64, _I, _I, _P, _I64, _P]),
     "walsh_linear_wgrad_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "walsh_linear_wgrad": (_I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "walsh_rmsnorm_fwd": (_I, [_P, _P, _I64, _I64, ctypes.c_float, _P, _P, _P]),

@@ -1136,6 +1136,211 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     return out
 
 
+# ------------------------------------------------------------------ tokens' probabilities
+
+MAX_TOP_LOGPROBS = 64
+
+
+def check_token_logprobs(fn, logits, tokens, top_n):
+    _hip.require_device(logits, "logits")
+    assert logits.dim() > 0 and logits.shape[-1] > 0 and tokens.shape == logits.shape[:-1], \
+        f"{fn}: logits [..., V] and tokens [...], got {tuple(logits.shape)} and {tuple(tokens.shape)}"
+    if tokens.dtype != torch.int64:
+        raise TypeError(f"{fn}: tokens are int64, got {tokens.dtype}")
+    _hip.dtype_code(logits.dtype)
+    if not 0 <= top_n <= min(MAX_TOP_LOGPROBS, logits.shape[-1]):
+        raise ValueError(f"{fn}: {top_n} alternatives of {logits.shape[-1]} tokens (up to {MAX_TOP_LOGPROBS})")
+    _hip.same_device(fn, logits, tokens)
+
+
+def _separate_rows(t: torch.Tensor):
+    """(tensor, rows, row stride) of t [..., C] with rows that do not overlap."""
+    t, rows, ld = _rows_view(t, t.shape[-1])
+    if rows > 1 and ld < t.shape[-1]:
+        t = t.contiguous()
+        ld = t.shape[-1]
+    return t, rows, ld
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0, need_stats: bool = False):
+    """Of logits [..., V] and tokens [...] (int64): the tokens' log
+    probabilities, the rows' entropies (both [...]), and the ``top_n`` (up to
+    64 and V) largest log probabilities in descending order with their tokens
+    ([..., top_n], of equal ones the lowest tokens first), float32 and int64.
+    A negative token marks a row that is not counted: zeros, and -inf and -1
+    as alternatives.  A token of V or more has NaN.  Logits of -inf have
+    probability 0 (a row of nothing else: log probabilities of -inf, entropy
+    0); NaN and +inf make their row NaN.  With ``need_stats`` also what
+    token_logprobs_bwd takes.  Not differentiable by itself:
+    src.model.token_logprobs is."""
+    check_token_logprobs("token_logprobs", logits, tokens, top_n)
+    V, dev = logits.shape[-1], logits.device
+    rows, N, ld = _separate_rows(logits)
+    tokens = tokens.contiguous()
+    logprob = torch.empty(tokens.shape, device=dev, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    top = torch.empty(tokens.shape + (top_n,), device=dev, dtype=torch.float32)
+    index = torch.empty(tokens.shape + (top_n,), device=dev, dtype=torch.int64)
+    stats = torch.empty(N, 4, device=dev, dtype=torch.float32) if need_stats else None
+    _hip.call_on(logits.get_device(), "walsh_token_logprobs_fwd", rows.data_ptr(), ld, N, V, tokens.data_ptr(), top_n,
+                 logprob.data_ptr(), entropy.data_ptr(), top.data_ptr(), index.data_ptr(), _hip.ptr(stats),
+                 _hip.dtype_code(logits.dtype), kernel="*", nbytes=N * V * logits.element_size(), flops=6 * N * V)
+    return (logprob, entropy, top, index, stats) if need_stats else (logprob, entropy, top, index)
+
+
+def token_logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor, top_index: torch.Tensor, stats: torch.Tensor,
+                       g_logprob: torch.Tensor = None, g_entropy: torch.Tensor = None, g_top: torch.Tensor = None):
+    """The gradient of the logits (contiguous, in their dtype), for gradients
+    of token_logprobs's outputs (float32, None: zeros) and its index and stats."""
+    n = top_index.shape[-1]
+    check_token_logprobs("token_logprobs_bwd", logits, tokens, n)
+    for g, shape in ((g_logprob, tokens.shape), (g_entropy, tokens.shape), (g_top, top_index.shape)):
+        assert g is None or g.shape == shape and g.dtype == torch.float32, "token_logprobs_bwd: gradients as the outputs"
+    assert top_index.shape[:-1] == tokens.shape and top_index.dtype == torch.int64, "token_logprobs_bwd: index [..., n]"
+    rows, N, ld = _separate_rows(logits)
+    assert stats.shape == (N, 4) and stats.dtype == torch.float32, "token_logprobs_bwd: stats [rows, 4]"
+    _hip.same_device("token_logprobs_bwd", logits, top_index, stats, g_logprob, g_entropy, g_top)
+    # (held until the launch: a copy must not be freed before it)
+    tokens, top_index, stats = tokens.contiguous(), top_index.contiguous(), _rows16(stats)
+    g = [None if t is None else t.contiguous() for t in (g_logprob, g_entropy, g_top)]
+    V = logits.shape[-1]
+    out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    _hip.call_on(logits.get_device(), "walsh_token_logprobs_bwd", rows.data_ptr(), ld, N, V, tokens.data_ptr(), n,
+                 top_index.data_ptr(), stats.data_ptr(), *map(_hip.ptr, g), out.data_ptr(), V,
+                 _hip.dtype_code(logits.dtype), kernel="logprobs_bwd_kernel", nbytes=2 * N * V * logits.element_size(),
+                 flops=6 * N * V)
+    return out
+
+
+# ------------------------------------------------------------------ dropout, embedding
+
+def drop_threshold(fn, p: float) -> int:
+    """Of the 65536 values of an element's random bits those that drop it."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{fn}: probability {p} (0 to 1)")
+    return int(round(p * 65536))
+
+
+def check_seed(fn, like, seed, stream, drop):
+    if not 0 <= stream < 1 << 32:
+        raise ValueError(f"{fn}: stream {stream} (0 to 2^32 - 1)")
+    if seed is None:
+        if drop:
+            raise ValueError(f"{fn}: dropout needs a seed")
+        return
+    if not isinstance(seed, torch.Tensor) or seed.dtype != torch.int64:
+        raise TypeError(f"{fn}: the seed is an int64 tensor of one element on the device")
+    assert seed.numel() == 1, f"{fn}: a seed of {seed.numel()} elements"
+    _hip.same_device(fn, like, seed)
+
+
+def check_dropout(fn, x, p, seed, stream, residual=None):
+    _hip.require_device(x, "input")
+    _hip.dtype_code(x.dtype)
+    assert x.dim() > 0, f"{fn}: rows [..., C]"
+    if residual is not None:
+        assert residual.shape == x.shape, f"{fn}: residual {tuple(residual.shape)} for {tuple(x.shape)}"
+        _hip.dtype_code(residual.dtype)
+        _hip.same_device(fn, x, residual)
+    drop = drop_threshold(fn, p)
+    check_seed(fn, x, seed, stream, drop)
+    return drop
+
+
+def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, stream: int = 0, residual: torch.Tensor = None,
+            out_dtype: torch.dtype = None) -> torch.Tensor:
+    """Dropout of x [..., C], and ``residual`` of its shape added, as a new
+    contiguous tensor in the wider of their types (without a residual
+    ``out_dtype`` may be bf16 for float32 x).  An element is kept where 16 bits
+    of a generator are at least round(65536 p), and multiplied by 65536 / (65536
+    - that).  The bits depend on the seed (int64 tensor of one element on the
+    device, read when the kernel runs), ``stream`` (0 to 2^32 - 1), the
+    element's row (of those that all leading dimensions make) and column: the
+    same call again gives the gradient's mask."""
+    drop = check_dropout("dropout", x, p, seed, stream, residual)
+    C = x.shape[-1]
+    if out_dtype is None:
+        out_dtype = x.dtype if residual is None or residual.dtype == x.dtype else torch.float32
+    y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
+    if x.numel() == 0:
+        return y
+    rows, M, ldx = _separate_rows(x)
+    res, _, ldr = (None, 0, 0) if residual is None else _separate_rows(residual)
+    xt, yt = _hip.dtype_code(x.dtype), _hip.dtype_code(out_dtype)
+    rt = yt if residual is None else _hip.dtype_code(residual.dtype)
+    esz = x.element_size() + y.element_size() + (0 if residual is None else residual.element_size())
+    _hip.call_on(x.get_device(), "walsh_dropout", rows.data_ptr(), ldx, xt, _hip.ptr(res), ldr, rt, M, C, drop, _hip.ptr(seed),
+                 stream, y.data_ptr(), C, yt, kernel="dropout_kernel", nbytes=M * C * esz, flops=3 * M * C)
+    return y
+
+
+def check_embedding(fn, tokens, weight, p, seed, stream, out_dtype, padding_idx=None):
+    _hip.require_device(weight, "weight")
+    assert weight.dim() == 2 and weight.shape[0] > 0, f"{fn}: weight [V, C]"
+    if tokens.dtype != torch.int64:
+        raise TypeError(f"{fn}: tokens are int64, got {tokens.dtype}")
+    _hip.dtype_code(weight.dtype)
+    _hip.dtype_code(out_dtype)
+    _hip.same_device(fn, weight, tokens)
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"{fn}: padding_idx {padding_idx} of {weight.shape[0]} tokens")
+    drop = drop_threshold(fn, p)
+    check_seed(fn, weight, seed, stream, drop)
+    return drop
+
+
+def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, out_dtype: torch.dtype = None,
+              p: float = 0.0, seed: torch.Tensor = None, stream: int = 0) -> torch.Tensor:
+    """dropout(scale weight[tokens]): tokens [...] (int64) of weight [V, C] ->
+    [..., C] in ``out_dtype`` (None: the weight's), formed in float32 and
+    rounded once; ``p``, ``seed`` and ``stream`` as in ``dropout``, a token a
+    row.  Rows of NaN for tokens outside 0 .. V - 1."""
+    out_dtype = weight.dtype if out_dtype is None else out_dtype
+    drop = check_embedding("embedding", tokens, weight, p, seed, stream, out_dtype)
+    V, C = weight.shape
+    N = tokens.numel()
+    y = torch.empty(tokens.shape + (C,), device=weight.device, dtype=out_dtype)
+    if y.numel() == 0:
+        return y
+    tokens = tokens.contiguous()
+    rows, _, ldw = _separate_rows(weight)
+    _hip.call_on(weight.get_device(), "walsh_embedding_fwd", tokens.data_ptr(), N, rows.data_ptr(), ldw, V, C, float(scale),
+                 drop, _hip.ptr(seed), stream, y.data_ptr(), C, _hip.dtype_code(weight.dtype), _hip.dtype_code(out_dtype),
+                 kernel="embed_kernel", nbytes=N * C * (weight.element_size() + y.element_size()), flops=N * C)
+    return y
+
+
+def embedding_bwd(tokens: torch.Tensor, gy: torch.Tensor, V: int, scale: float = 1.0, dtype: torch.dtype = None,
+                  padding_idx: int = None, p: float = 0.0, seed: torch.Tensor = None, stream: int = 0) -> torch.Tensor:
+    """The gradient [V, C] of ``embedding``'s weight (``dtype``: its type,
+    None: gy's) for the gradient gy [..., C] of its output: a token's rows are
+    added in their order in float32, so equal calls give equal bits.  Tokens
+    outside 0 .. V - 1 and ``padding_idx`` add to none."""
+    dtype = gy.dtype if dtype is None else dtype
+    _hip.require_device(gy, "gradient")
+    assert V > 0 and gy.dim() > 0 and gy.shape[:-1] == tokens.shape, \
+        f"embedding_bwd: tokens [...] and gy [..., C], got {tuple(tokens.shape)} and {tuple(gy.shape)}"
+    if tokens.dtype != torch.int64:
+        raise TypeError(f"embedding_bwd: tokens are int64, got {tokens.dtype}")
+    gt, wt = _hip.dtype_code(gy.dtype), _hip.dtype_code(dtype)
+    _hip.same_device("embedding_bwd", gy, tokens)
+    drop = drop_threshold("embedding_bwd", p)
+    check_seed("embedding_bwd", gy, seed, stream, drop)
+    C, N = gy.shape[-1], tokens.numel()
+    dw = torch.empty(V, C, device=gy.device, dtype=dtype)
+    if C == 0:
+        return dw
+    tokens = tokens.contiguous()
+    rows, _, ldg = _separate_rows(gy)
+    nws = _workspace("walsh_embedding_bwd_workspace_bytes", gy.get_device(), N, V, C)
+    ws = torch.empty(nws, device=gy.device, dtype=torch.uint8)
+    _hip.call_on(gy.get_device(), "walsh_embedding_bwd", tokens.data_ptr(), N, rows.data_ptr(), ldg, V, C, float(scale),
+                 -1 if padding_idx is None else padding_idx, drop, _hip.ptr(seed), stream, dw.data_ptr(), C, gt, wt,
+                 ws.data_ptr(), nws, kernel="embed_bwd_kernels",
+                 nbytes=N * C * gy.element_size() + V * C * dw.element_size(), flops=2 * N * C)
+    return dw
+
+
 # ------------------------------------------------------------------ channel modulation
 
 def _groups(x: torch.Tensor) -> torch.Tensor:
