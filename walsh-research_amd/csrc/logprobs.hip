@@ -19,6 +19,8 @@
 // at their tokens again.  Those go to a list in LDS and are ranked there by
 // value and index.  Where there are too many (thousands of equal ones) or a
 // group has none, the row is walked once for every alternative instead.
+#include <type_traits>
+
 #include "rows8.h"
 
 namespace walsh {
@@ -38,11 +40,40 @@ struct LogprobArgs {
     f32x4 *stats;                      // (m, S, H, 0) of every row, or null
 };
 
-// Sums over tokens relative to a maximum m, in powers of two: s = sum w,
-// e = sum w log2 w for w = 2^((l - m) log2(e)).
+// Sums over tokens, in powers of two: s = sum w, e = sum w log2 w for
+// w = 2^(l log2(e) - r), with r the rounded product of a maximum m.  What its
+// rounding leaves out is a factor common to all (taken back at the end), so a
+// weight costs one multiply-add besides the exponential.  Lanes begin below
+// every usual logit; a row where that, or an infinity or NaN, spoils the sums
+// shows in them (`usual`) and is walked again with the distances l - m
+// themselves (LpExact).
 struct LpSums {
-    float m, s, e;
+    float m, r, s, e;
+    __device__ __forceinline__ LpSums() : m(-1e30f), r(-1e30f * kLog2e), s(0.f), e(0.f) {}
+    __device__ __forceinline__ LpSums(f32x4 v) : m(v.x), r(v.x * kLog2e), s(v.y), e(v.z) {}
     // a larger maximum: at most 2^1000 below, where nothing is left of s
+    __device__ __forceinline__ void move(float to) {
+        const float rt = to * kLog2e, d = fmaxf(r - rt, -1000.f), c = __builtin_amdgcn_exp2f(d);
+        e = c * (e + d * s);
+        s *= c;
+        m = to, r = rt;
+    }
+    __device__ __forceinline__ void add(float x) {
+        const float t = fmaf(x, kLog2e, -r), w = __builtin_amdgcn_exp2f(t);
+        s += w;
+        e = fmaf(w, fmaxf(t, -1000.f), e);         // (0 times -inf)
+    }
+    __device__ __forceinline__ bool usual() const { return m < 2e38f && s > 0.f && s < INFINITY && fabsf(e) < INFINITY; }
+};
+struct LpExact {
+    float m, s, e;
+    __device__ __forceinline__ LpExact(float m_, float s_, float e_) : m(m_), s(s_), e(e_) {}
+    __device__ __forceinline__ LpExact(f32x4 v) : m(v.x), s(v.y), e(v.z) {}
+    // the sums of q relative to m itself: r off by d makes w 2^d times as large
+    __device__ __forceinline__ explicit LpExact(const LpSums &q) : m(q.m) {
+        const float d = fmaf(q.m, kLog2e, -q.r), c = __builtin_amdgcn_exp2f(-d);
+        s = c * q.s, e = c * (q.e - d * q.s);
+    }
     __device__ __forceinline__ void move(float to) {
         const float d = fmaxf((m - to) * kLog2e, -1000.f), c = __builtin_amdgcn_exp2f(d);
         e = c * (e + d * s);
@@ -52,9 +83,32 @@ struct LpSums {
     __device__ __forceinline__ void add(float x) {
         const float t = (x - m) * kLog2e, w = __builtin_amdgcn_exp2f(t);
         s += w;
-        e = fmaf(w, fmaxf(t, -1000.f), e);         // (0 times -inf)
+        e = fmaf(w, fmaxf(t, -1000.f), e);
     }
 };
+
+// Over the lanes of a wavefront (ROWS 4) or of its first 16 (ROWS 1), in a
+// fixed order; the result in every lane.
+template <int CTRL, int MASK> __device__ __forceinline__ float lp_dpp(float none, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, MASK, 0xf, false));
+}
+template <int ROWS, typename F> __device__ __forceinline__ float lp_reduce(float v, float none, F f) {
+    v = f(v, lp_dpp<0x111, 0xf>(none, v));         // 1, 2, 4, 8 lanes to the left in the row of 16
+    v = f(v, lp_dpp<0x112, 0xf>(none, v));
+    v = f(v, lp_dpp<0x114, 0xf>(none, v));
+    v = f(v, lp_dpp<0x118, 0xf>(none, v));
+    if (ROWS > 1) {
+        v = f(v, lp_dpp<0x142, 0xa>(none, v));     // the row before's last lane, the second row's last
+        v = f(v, lp_dpp<0x143, 0xc>(none, v));
+    }
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16 * ROWS - 1));
+}
+template <int ROWS> __device__ __forceinline__ float lp_max(float v) {
+    return lp_reduce<ROWS>(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int ROWS> __device__ __forceinline__ float lp_sum(float v) {
+    return lp_reduce<ROWS>(v, 0.f, [](float a, float b) { return a + b; });
+}
 
 // Tokens in order of preference: larger values first, then lower indexes.
 __device__ __forceinline__ uint64_t lp_key(float x, int i) {
@@ -69,16 +123,33 @@ __device__ __forceinline__ uint64_t lp_xor(uint64_t v, int o) {
     return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, o);
 }
 
-template <int NT> struct LpShared {
+template <int NT, bool TOP> struct LpShared {
     f32x4 part[NT / 64];
-    float group[NT / 64][64];
-    uint64_t list[kLpList], best[NT / 64];
+    float group[TOP ? NT / 64 : 1][64];
+    uint64_t list[TOP ? kLpList : 1], best[NT / 64];
     int n;
 };
 
-template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
+// The lanes' sums joined: over the wavefront, through LDS, over the wavefronts.
+template <int NT, typename Q, typename S> __device__ __forceinline__ Q lp_join(S &sh, Q q, int lane, int wave) {
+    constexpr int W = NT / 64;
+    q.move(lp_max<4>(q.m));
+    q.s = lp_sum<4>(q.s), q.e = lp_sum<4>(q.e);
+    if (lane == 0) sh.part[wave] = f32x4{q.m, q.s, q.e, 0.f};
+    __syncthreads();
+    const f32x4 v = sh.part[lane & (W - 1)];
+    q = Q(v);
+    if (lane >= W) q.s = q.e = 0.f;
+    q.move(lp_max<1>(q.m));
+    q.s = lp_sum<1>(q.s), q.e = lp_sum<1>(q.e);
+    return q;
+}
+
+// STEPS: blocks of 8 tokens that a lane holds in registers, all of its row's
+// (V <= 8 NT STEPS + 7); or 0: it walks them, U at a time.
+template <typename T, int NT, int STEPS, bool TOP> __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
     constexpr int W = NT / 64, U = 4;
-    __shared__ LpShared<NT> sh;
+    __shared__ LpShared<NT, TOP> sh;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t t = a.tokens[row];
@@ -90,62 +161,88 @@ template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void lo
         if (TOP && tid < a.n) a.top[row * a.n + tid] = -INFINITY, a.top_index[row * a.n + tid] = -1;
         return;
     }
+    // Blocks begin at a multiple of 4 bytes: of rows that begin between two
+    // (bf16, odd strides) 16-byte loads reach 4.7 TB/s, else 5.7.  What is left
+    // at both ends of the row goes to a lane each, as token `last`.
     const T *p = (const T *)a.logits + row * a.ld;
-    const int blocks = a.V / 8, rest = a.V & 7;
-    // each(f): f(first index, values), 8 at a time
-    LpSums q{kLpLowest, 0.f, 0.f};
-    for (int b0 = tid; b0 < blocks; b0 += NT * U) {
-        Raw8<T> r[U];
-        float x[U][8], top = kLpLowest;
+    const int lead = (uintptr_t)p & 3 ? 1 : 0;
+    const int blocks = (a.V - lead) / 8, rest = (a.V - lead) & 7;
+    const T *body = p + lead;
+    const int last = tid < rest ? lead + 8 * blocks + tid : 0;
+    LpSums q;
+    Raw8<T> held[STEPS ? STEPS : 1];
+    float end = tid < rest + lead ? Act<T>::load(p + last) : -INFINITY;
+    auto take = [&](const auto &r, auto n) {       // the sums of n blocks
+        float x[decltype(n)::value][8], top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            r[j].fill(-INFINITY);
-            if (b0 + j * NT < blocks) r[j].load(p + 8 * (b0 + j * NT));
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
+        for (int j = 0; j < n; ++j) {
             r[j].unpack(x[j]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, x[j][i]);
         }
         if (top > q.m) q.move(top);
 #pragma unroll
-        for (int j = 0; j < U; ++j)
+        for (int j = 0; j < n; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) q.add(x[j][i]);
-    }
-    const int last = 8 * blocks + tid;             // the row's last tokens, one to a lane
-    if (tid < rest) {
-        const float x = Act<T>::load(p + last);
-        if (x > q.m) q.move(x);
-        q.add(x);
+    };
+    if constexpr (STEPS > 0) {
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+            held[j].fill(-INFINITY);
+            if (tid + j * NT < blocks) held[j].load(body + 8 * (tid + j * NT));
+        }
+        float top = end;
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+            float x[8];
+            held[j].unpack(x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
+        }
+        if (top > q.m) q.move(top);
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+            float x[8];
+            held[j].unpack(x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q.add(x[i]);
+        }
+        q.add(end);
+    } else {
+        int b = tid;
+        for (; b + (U - 1) * NT < blocks; b += NT * U) {
+            Raw8<T> r[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) r[j].load(body + 8 * (int64_t)(b + j * NT));
+            take(r, std::integral_constant<int, U>{});
+        }
+        for (; b < blocks; b += NT) {
+            Raw8<T> r[1];
+            r[0].load(body + 8 * (int64_t)b);
+            take(r, std::integral_constant<int, 1>{});
+        }
+        if (end > q.m) q.move(end);
+        q.add(end);
     }
     const float own = q.m;
-    // the wavefront's, then the row's
-    float m = own;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    q.move(m);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) q.s += __shfl_xor(q.s, o), q.e += __shfl_xor(q.e, o);
-    if (lane == 0) sh.part[wave] = f32x4{q.m, q.s, q.e, 0.f};
     if constexpr (TOP) {
         sh.group[wave][lane] = own;
         if (tid == 0) sh.n = 0;
     }
-    __syncthreads();
-    LpSums all{sh.part[0].x, sh.part[0].y, sh.part[0].z};
-#pragma unroll
-    for (int w = 1; w < W; ++w) m = fmaxf(m, sh.part[w].x);
-    m = fmaxf(m, all.m);
-    all.move(m);
-#pragma unroll
-    for (int w = 1; w < W; ++w) {
-        LpSums o{sh.part[w].x, sh.part[w].y, sh.part[w].z};
-        o.move(m);
-        all.s += o.s, all.e += o.e;
+    q = lp_join<NT>(sh, q, lane, wave);
+    LpExact all(q);
+    if (!q.usual()) {
+        all = LpExact(kLpLowest, 0.f, 0.f);
+        for (int i = tid; i < a.V; i += NT) {
+            const float x = Act<T>::load(p + i);
+            if (x > all.m) all.move(x);
+            all.add(x);
+        }
+        __syncthreads();
+        all = lp_join<NT>(sh, all, lane, wave);
     }
-    const float logs = __builtin_amdgcn_logf(all.s) * kLn2;
+    const float m = all.m, logs = __builtin_amdgcn_logf(all.s) * kLn2;
     const bool nothing = all.s == 0.f;             // (not where it is NaN)
     auto logprob = [&](float x) { return nothing ? -INFINITY : (x - m) - logs; };
     if (tid == 0) {
@@ -170,23 +267,35 @@ template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void lo
     }
     const uint64_t nth = __ballot(rank == a.n - 1);
     const float bound = __shfl(g, (int)__ffsll((long long)nth) - 1);
-    if (bound > kLpLowest) {
-        auto put = [&](float x, int i) {
-            if (x >= bound) {
-                const int at = atomicAdd(&sh.n, 1);
-                if (at < kLpList) sh.list[at] = lp_key(x, i);
-            }
+    if (bound > -1e30f) {
+        auto put = [&](const Raw8<T> &r, int b) {
+            float x[8];
+            r.unpack(x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (x[i] >= bound) {
+                    const int at = atomicAdd(&sh.n, 1);
+                    if (at < kLpList) sh.list[at] = lp_key(x[i], lead + 8 * b + i);
+                }
         };
         if (own >= bound) {
-            for (int b = tid; b < blocks; b += NT) {
-                Raw8<T> r;
-                float x[8];
-                r.load(p + 8 * b);
-                r.unpack(x);
+            if constexpr (STEPS > 0) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) put(x[i], 8 * b + i);
+                for (int j = 0; j < STEPS; ++j) put(held[j], tid + j * NT);
+            } else {
+                for (int b = tid; b < blocks; b += NT * U) {
+                    Raw8<T> r[U];
+#pragma unroll
+                    for (int j = 0; j < U; ++j) r[j].load(body + 8 * (int64_t)min(b + j * NT, blocks - 1));
+#pragma unroll
+                    for (int j = 0; j < U; ++j)
+                        if (b + j * NT < blocks) put(r[j], b + j * NT);
+                }
             }
-            if (tid < rest) put(Act<T>::load(p + last), last);
+            if (end >= bound) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < kLpList) sh.list[at] = lp_key(end, last);
+            }
         }
         __syncthreads();
         const int count = sh.n;
@@ -289,6 +398,19 @@ template <typename T> __global__ __launch_bounds__(256) void logprobs_bwd_kernel
     Act<T>::store(d + i, add + grad(Act<T>::load(p + i)));
 }
 
+template <typename T> static void logprobs_launch(const LogprobArgs &a, int64_t N, hipStream_t s) {
+    auto go = [&](auto kernel, int nt) { launch(kernel, dim3((unsigned)N), dim3(nt), 0, s, a); };
+    const int steps = (int)ceil_div(a.V / 8, 1024);
+    if (a.n) {
+        if (steps <= 2) go(logprobs_kernel<T, 1024, 2, true>, 1024);
+        else if (steps <= 4) go(logprobs_kernel<T, 1024, 4, true>, 1024);
+        else if (steps <= 7) go(logprobs_kernel<T, 1024, 7, true>, 1024);
+        else go(logprobs_kernel<T, 1024, 0, true>, 1024);
+    } else {
+        go(logprobs_kernel<T, 256, 0, false>, 256);
+    }
+}
+
 static int logprobs_check(const char *fn, int64_t N, int64_t V, int64_t n, int64_t ld, int dtype) {
     if (N < 0 || N > 0x7fffff || V < 1 || V > 0x7fffffff / 2 || n < 0 || n > kLpTop || n > V)
         return set_error(WALSH_EINVAL, "%s: N=%lld rows (below 2^23) of V=%lld, %lld alternatives (up to 64 and V)", fn,
@@ -313,14 +435,8 @@ WALSH_EXPORT int walsh_token_logprobs_fwd(const void *logits, int64_t ld, int64_
         return set_error(WALSH_EINVAL, "%s: null pointer", fn);
     if ((uintptr_t)stats % 16) return set_error(WALSH_EINVAL, "%s: stats 16-byte aligned", fn);
     const LogprobArgs a{logits, tokens, ld, (int)V, (int)n, logprob, entropy, top, top_index, (f32x4 *)stats};
-    auto go = [&](auto kernel, int nt) { launch(kernel, dim3((unsigned)N), dim3(nt), 0, (hipStream_t)stream, a); };
-    if (dtype == WALSH_BF16) {
-        if (n) go(logprobs_kernel<uint16_t, 1024, true>, 1024);
-        else go(logprobs_kernel<uint16_t, 256, false>, 256);
-    } else {
-        if (n) go(logprobs_kernel<float, 1024, true>, 1024);
-        else go(logprobs_kernel<float, 256, false>, 256);
-    }
+    if (dtype == WALSH_BF16) logprobs_launch<uint16_t>(a, N, (hipStream_t)stream);
+    else logprobs_launch<float>(a, N, (hipStream_t)stream);
     return check_hip(hipGetLastError(), fn);
 }
 
