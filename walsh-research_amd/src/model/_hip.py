@@ -282,12 +282,14 @@ def stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_DTYPE_CODES = {torch.float32: WALSH_F32, torch.bfloat16: WALSH_BF16}
+
+
 def dtype_code(dt: torch.dtype) -> int:
-    if dt == torch.float32:
-        return WALSH_F32
-    if dt == torch.bfloat16:
-        return WALSH_BF16
-    raise TypeError(f"activation dtype {dt} is not supported (float32 or bfloat16)")
+    code = _DTYPE_CODES.get(dt)
+    if code is None:
+        raise TypeError(f"activation dtype {dt} is not supported (float32 or bfloat16)")
+    return code
 
 
 _cu = {}

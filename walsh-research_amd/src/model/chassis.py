@@ -24,6 +24,7 @@ from .octonion import OctonionHeadMixerFused, OctonionTernaryLinear
 from . import kernels
 from ._common import WeightCache, act_dtype, cached_linear, first_order, plain_eager
 from .attention import PagedKVCache, window_attention, window_mask
+from .tokens import drop_output, embed_tokens, score, step_seed
 
 _HADAMARD_AVAILABLE = True
 _HADAMARD_HEAD_MIXER_AVAILABLE = True
@@ -31,7 +32,7 @@ _HADAMARD_HEAD_MIXER_AVAILABLE = True
 
 @dataclass
 class WalshConfig:
-    """chassis.py:33-51 (its fields and defaults unchanged, two added)."""
+    """chassis.py:33-51 (its fields and defaults unchanged, five added)."""
     block_size: int = 256
     vocab_size: int = 65
     n_layer: int = 6
@@ -51,6 +52,11 @@ class WalshConfig:
     # positions and the first attn_sinks ones (0: over all of them)
     attn_window: int = 0
     attn_sinks: int = 0
+    # nor of these: a factor of the tokens' rows, and the dropout of training
+    # on those rows and on what each layer adds to the residual stream
+    embed_scale: float = 1.0
+    embed_dropout: float = 0.0
+    resid_dropout: float = 0.0
 
 
 def get_linear_layer(config: WalshConfig):
@@ -499,6 +505,7 @@ class LlamaBlock(nn.Module):
         self.attention_norm = RMSNorm(config.n_embd)
         self.attention = CausalSelfAttention(config)
         self.ffn_norm = RMSNorm(config.n_embd)
+        self.resid_dropout = getattr(config, 'resid_dropout', 0.0)
         if getattr(config, 'use_moe', False):
             from .moe import HadamardMoE
             self.feed_forward = HadamardMoE(
@@ -510,10 +517,11 @@ class LlamaBlock(nn.Module):
         else:
             self.feed_forward = SwiGLUMLP(config)
 
-    def forward(self, x, freqs_cis, kv_cache: Optional[KVCache] = None, layer_idx: int = 0):
-        dt = act_dtype(x)
-        h = x + self.attention(self.attention_norm(x).to(dt), freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx)
-        return h + self.feed_forward(self.ffn_norm(h).to(dt))
+    def forward(self, x, freqs_cis, kv_cache: Optional[KVCache] = None, layer_idx: int = 0, seed=None):
+        dt, p = act_dtype(x), self.resid_dropout
+        y = self.attention(self.attention_norm(x).to(dt), freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx)
+        h = drop_output(y, p, seed, layer_idx, 0, x)
+        return drop_output(self.feed_forward(self.ffn_norm(h).to(dt)), p, seed, layer_idx, 1, h)
 
 
 class Walsh(nn.Module):
@@ -543,14 +551,17 @@ class Walsh(nn.Module):
     def forward(self, idx, targets=None, kv_cache: Optional[KVCache] = None, start_pos: int = 0,
                 return_hidden: bool = False):
         B, T = idx.shape
-        h = self.tok_embeddings(counted_tokens(idx, kv_cache))
+        seed = step_seed(self, idx)
+        h = embed_tokens(self, counted_tokens(idx, kv_cache), seed)
         freqs_cis = cache_freqs(self.freqs_cis, T, start_pos, kv_cache)
         for layer_idx, layer in enumerate(self.layers):
             if self.training and torch.is_grad_enabled():
                 # every layer checkpointed in training (chassis.py:570-572)
-                h = torch.utils.checkpoint.checkpoint(layer, h, freqs_cis, use_reentrant=False)
+                at = {} if seed is None else {"layer_idx": layer_idx, "seed": seed}
+                h = torch.utils.checkpoint.checkpoint(layer, h, freqs_cis, use_reentrant=False, **at)
             else:
-                h = layer(h, freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx)
+                at = {} if seed is None else {"seed": seed}
+                h = layer(h, freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx, **at)
         h = self.norm(h)
         if targets is not None:
             logits = cached_linear(self.output, h, self._output_cast)
@@ -562,3 +573,12 @@ class Walsh(nn.Module):
         if return_hidden:
             return logits, loss, h
         return logits, loss
+
+    def all_logits(self, idx):
+        """Logits of every position of idx [B, T]."""
+        _, _, h = self(idx, return_hidden=True)
+        return cached_linear(self.output, h, self._output_cast)
+
+    def score(self, idx, lengths=None, top_n=0):
+        """Token probabilities of given texts (tokens.score)."""
+        return score(self, idx, lengths, top_n)

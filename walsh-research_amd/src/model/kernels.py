@@ -1142,23 +1142,28 @@ MAX_TOP_LOGPROBS = 64
 
 
 def check_token_logprobs(fn, logits, tokens, top_n):
+    """The checks of a call; its logits' dtype code."""
     _hip.require_device(logits, "logits")
-    assert logits.dim() > 0 and logits.shape[-1] > 0 and tokens.shape == logits.shape[:-1], \
-        f"{fn}: logits [..., V] and tokens [...], got {tuple(logits.shape)} and {tuple(tokens.shape)}"
+    shape = logits.shape
+    assert len(shape) > 0 and shape[-1] > 0 and tokens.shape == shape[:-1], \
+        f"{fn}: logits [..., V] and tokens [...], got {tuple(shape)} and {tuple(tokens.shape)}"
     if tokens.dtype != torch.int64:
         raise TypeError(f"{fn}: tokens are int64, got {tokens.dtype}")
-    _hip.dtype_code(logits.dtype)
-    if not 0 <= top_n <= min(MAX_TOP_LOGPROBS, logits.shape[-1]):
-        raise ValueError(f"{fn}: {top_n} alternatives of {logits.shape[-1]} tokens (up to {MAX_TOP_LOGPROBS})")
+    if not 0 <= top_n <= MAX_TOP_LOGPROBS or top_n > shape[-1]:
+        raise ValueError(f"{fn}: {top_n} alternatives of {shape[-1]} tokens (up to {MAX_TOP_LOGPROBS})")
     _hip.same_device(fn, logits, tokens)
+    return _hip.dtype_code(logits.dtype)
 
 
 def _separate_rows(t: torch.Tensor):
-    """(tensor, rows, row stride) of t [..., C] with rows that do not overlap."""
-    t, rows, ld = _rows_view(t, t.shape[-1])
-    if rows > 1 and ld < t.shape[-1]:
+    """(tensor, rows, row stride) of t [..., C], C > 0, with rows that do not overlap."""
+    C = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // C, C
+    t, rows, ld = _rows_view(t, C)
+    if rows > 1 and ld < C:
         t = t.contiguous()
-        ld = t.shape[-1]
+        ld = C
     return t, rows, ld
 
 
@@ -1173,18 +1178,18 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0, n
     0); NaN and +inf make their row NaN.  With ``need_stats`` also what
     token_logprobs_bwd takes.  Not differentiable by itself:
     src.model.token_logprobs is."""
-    check_token_logprobs("token_logprobs", logits, tokens, top_n)
-    V, dev = logits.shape[-1], logits.device
+    dt = check_token_logprobs("token_logprobs", logits, tokens, top_n)
+    dev, shape, V = logits.device, tokens.shape, logits.shape[-1]
     rows, N, ld = _separate_rows(logits)
     tokens = tokens.contiguous()
-    logprob = torch.empty(tokens.shape, device=dev, dtype=torch.float32)
+    logprob = torch.empty(shape, device=dev, dtype=torch.float32)
     entropy = torch.empty_like(logprob)
-    top = torch.empty(tokens.shape + (top_n,), device=dev, dtype=torch.float32)
-    index = torch.empty(tokens.shape + (top_n,), device=dev, dtype=torch.int64)
+    wide = (*shape, top_n)
+    top, index = torch.empty(wide, device=dev, dtype=torch.float32), torch.empty(wide, device=dev, dtype=torch.int64)
     stats = torch.empty(N, 4, device=dev, dtype=torch.float32) if need_stats else None
     _hip.call_on(logits.get_device(), "walsh_token_logprobs_fwd", rows.data_ptr(), ld, N, V, tokens.data_ptr(), top_n,
-                 logprob.data_ptr(), entropy.data_ptr(), top.data_ptr(), index.data_ptr(), _hip.ptr(stats),
-                 _hip.dtype_code(logits.dtype), kernel="*", nbytes=N * V * logits.element_size(), flops=6 * N * V)
+                 logprob.data_ptr(), entropy.data_ptr(), top.data_ptr(), index.data_ptr(), _hip.ptr(stats), dt,
+                 kernel="logprobs_kernel", nbytes=(4 - 2 * dt) * N * V, flops=6 * N * V)
     return (logprob, entropy, top, index, stats) if need_stats else (logprob, entropy, top, index)
 
 
@@ -1235,16 +1240,17 @@ def check_seed(fn, like, seed, stream, drop):
 
 
 def check_dropout(fn, x, p, seed, stream, residual=None):
+    """The checks of a call; (drop threshold, x's and the residual's dtype codes)."""
     _hip.require_device(x, "input")
-    _hip.dtype_code(x.dtype)
+    xt = rt = _hip.dtype_code(x.dtype)
     assert x.dim() > 0, f"{fn}: rows [..., C]"
     if residual is not None:
         assert residual.shape == x.shape, f"{fn}: residual {tuple(residual.shape)} for {tuple(x.shape)}"
-        _hip.dtype_code(residual.dtype)
+        rt = _hip.dtype_code(residual.dtype)
         _hip.same_device(fn, x, residual)
     drop = drop_threshold(fn, p)
     check_seed(fn, x, seed, stream, drop)
-    return drop
+    return drop, xt, rt
 
 
 def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, stream: int = 0, residual: torch.Tensor = None,
@@ -1257,36 +1263,35 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, stream: int = 0, resi
     device, read when the kernel runs), ``stream`` (0 to 2^32 - 1), the
     element's row (of those that all leading dimensions make) and column: the
     same call again gives the gradient's mask."""
-    drop = check_dropout("dropout", x, p, seed, stream, residual)
-    C = x.shape[-1]
+    drop, xt, rt = check_dropout("dropout", x, p, seed, stream, residual)
     if out_dtype is None:
-        out_dtype = x.dtype if residual is None or residual.dtype == x.dtype else torch.float32
+        out_dtype = x.dtype if xt == rt else torch.float32
     y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
-    if x.numel() == 0:
+    n = x.numel()
+    if n == 0:
         return y
+    C, yt = x.shape[-1], _hip.dtype_code(out_dtype)
     rows, M, ldx = _separate_rows(x)
     res, _, ldr = (None, 0, 0) if residual is None else _separate_rows(residual)
-    xt, yt = _hip.dtype_code(x.dtype), _hip.dtype_code(out_dtype)
-    rt = yt if residual is None else _hip.dtype_code(residual.dtype)
-    esz = x.element_size() + y.element_size() + (0 if residual is None else residual.element_size())
     _hip.call_on(x.get_device(), "walsh_dropout", rows.data_ptr(), ldx, xt, _hip.ptr(res), ldr, rt, M, C, drop, _hip.ptr(seed),
-                 stream, y.data_ptr(), C, yt, kernel="dropout_kernel", nbytes=M * C * esz, flops=3 * M * C)
+                 stream, y.data_ptr(), C, yt, kernel="dropout_kernel",
+                 nbytes=n * (8 - 2 * xt - 2 * yt + (0 if res is None else 4 - 2 * rt)), flops=3 * n)
     return y
 
 
 def check_embedding(fn, tokens, weight, p, seed, stream, out_dtype, padding_idx=None):
+    """The checks of a call; (drop threshold, weight's and output's dtype codes)."""
     _hip.require_device(weight, "weight")
     assert weight.dim() == 2 and weight.shape[0] > 0, f"{fn}: weight [V, C]"
     if tokens.dtype != torch.int64:
         raise TypeError(f"{fn}: tokens are int64, got {tokens.dtype}")
-    _hip.dtype_code(weight.dtype)
-    _hip.dtype_code(out_dtype)
+    wt, ot = _hip.dtype_code(weight.dtype), _hip.dtype_code(out_dtype)
     _hip.same_device(fn, weight, tokens)
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"{fn}: padding_idx {padding_idx} of {weight.shape[0]} tokens")
     drop = drop_threshold(fn, p)
     check_seed(fn, weight, seed, stream, drop)
-    return drop
+    return drop, wt, ot
 
 
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, out_dtype: torch.dtype = None,
@@ -1296,17 +1301,17 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, ou
     rounded once; ``p``, ``seed`` and ``stream`` as in ``dropout``, a token a
     row.  Rows of NaN for tokens outside 0 .. V - 1."""
     out_dtype = weight.dtype if out_dtype is None else out_dtype
-    drop = check_embedding("embedding", tokens, weight, p, seed, stream, out_dtype)
+    drop, wt, ot = check_embedding("embedding", tokens, weight, p, seed, stream, out_dtype)
     V, C = weight.shape
     N = tokens.numel()
-    y = torch.empty(tokens.shape + (C,), device=weight.device, dtype=out_dtype)
-    if y.numel() == 0:
+    y = torch.empty((*tokens.shape, C), device=weight.device, dtype=out_dtype)
+    if N == 0 or C == 0:
         return y
     tokens = tokens.contiguous()
     rows, _, ldw = _separate_rows(weight)
     _hip.call_on(weight.get_device(), "walsh_embedding_fwd", tokens.data_ptr(), N, rows.data_ptr(), ldw, V, C, float(scale),
-                 drop, _hip.ptr(seed), stream, y.data_ptr(), C, _hip.dtype_code(weight.dtype), _hip.dtype_code(out_dtype),
-                 kernel="embed_kernel", nbytes=N * C * (weight.element_size() + y.element_size()), flops=N * C)
+                 drop, _hip.ptr(seed), stream, y.data_ptr(), C, wt, ot, kernel="embed_kernel",
+                 nbytes=N * C * (8 - 2 * wt - 2 * ot), flops=N * C)
     return y
 
 

@@ -15,6 +15,7 @@ import torch.nn.functional as F
 from . import kernels
 from .attention import PagedKVCache
 from .linear import FewRowsLinear
+from .tokens import drop_output, embed_tokens, score, stack_steps, step_seed, token_logprobs
 from ._common import WeightCache, act_dtype, cached_linear, invalidate_weight_caches
 
 _MAX_STREAMS = 4
@@ -375,6 +376,7 @@ class mHCLlamaBlock(nn.Module):
         else:
             self.feed_forward = SwiGLUMLP(config)
         self._moe = getattr(config, 'use_moe', False)
+        self.resid_dropout = getattr(config, 'resid_dropout', 0.0)
         self.use_channel_mod = getattr(config, 'use_channel_mod', False)
         if self.use_channel_mod:
             from .moe import HadamardChannelModulation
@@ -384,10 +386,10 @@ class mHCLlamaBlock(nn.Module):
         self.attn_stream = mHCResidualStream(config.n_embd, n_streams)
         self.ffn_stream = mHCResidualStream(config.n_embd, n_streams)
 
-    def forward(self, x, freqs_cis, kv_cache=None, layer_idx=0):
-        return materialize(self.forward_deferred(x, freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx))
+    def forward(self, x, freqs_cis, kv_cache=None, layer_idx=0, seed=None):
+        return materialize(self.forward_deferred(x, freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx, seed=seed))
 
-    def forward_deferred(self, x, freqs_cis, kv_cache=None, layer_idx=0):
+    def forward_deferred(self, x, freqs_cis, kv_cache=None, layer_idx=0, seed=None):
         """forward() for x a tensor or a PendingUpdate; the FFN stream's
         update may come back pending (applied by the next block's first
         mapping kernel)."""
@@ -395,17 +397,19 @@ class mHCLlamaBlock(nn.Module):
         # ffn_stream(x, feed_forward(ffn_norm(.))) (mhc.py:507-534), with each
         # RMSNorm fused into its stream's mapping kernel and each stream
         # update fused into the next stream's mapping kernel
+        def drop(y, which):
+            return drop_output(y, self.resid_dropout, seed, layer_idx, which)
         x = self.attn_stream.forward_normed(
             x, self.attention_norm,
-            lambda v: self.attention(v, freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx), defer=True)
+            lambda v: drop(self.attention(v, freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx), 0), defer=True)
         ff = self.feed_forward
         defer = not self.use_channel_mod
         if self._moe:
             # the stream update rounds the FFN output to the stream dtype
             # (autocast matmul, mhc.py:374-377), so produce it in that dtype
-            x = self.ffn_stream.forward_normed(x, self.ffn_norm, lambda v: ff(v, out_dtype=v.dtype), defer=defer)
+            x = self.ffn_stream.forward_normed(x, self.ffn_norm, lambda v: drop(ff(v, out_dtype=v.dtype), 1), defer=defer)
         else:
-            x = self.ffn_stream.forward_normed(x, self.ffn_norm, ff, defer=defer)
+            x = self.ffn_stream.forward_normed(x, self.ffn_norm, lambda v: drop(ff(v), 1), defer=defer)
         if self.use_channel_mod:
             # x + channel_mod(norm(x)) on the [B*n, T, C] view of the
             # contiguous [B, T, n, C] streams (mhc.py:528-532): a "group" of T
@@ -460,7 +464,9 @@ class mHCWalsh(nn.Module):
     def forward(self, idx, targets=None, kv_cache=None, start_pos=0, return_hidden=False):
         from .chassis import cache_freqs, counted_tokens, last_rows
         B, T = idx.shape
-        h = self.tok_embeddings(counted_tokens(idx, kv_cache))
+        seed = step_seed(self, idx)
+        seeded = {} if seed is None else {"seed": seed}
+        h = embed_tokens(self, counted_tokens(idx, kv_cache), seed)
         h = cached_linear(self.stream_proj, h, self._casts["proj"])
         dt = act_dtype(h)
         h = h.to(dt).view(B, T, self.n_streams, self.config.n_embd)
@@ -472,9 +478,9 @@ class mHCWalsh(nn.Module):
                 # layer's forward is recomputed in the backward; it takes and
                 # returns plain tensors (no pending stream update crosses it)
                 h = torch.utils.checkpoint.checkpoint(layer.forward, materialize(h), freqs_cis, kv_cache, layer_idx,
-                                                      use_reentrant=False)
+                                                      use_reentrant=False, **seeded)
             else:
-                h = layer.forward_deferred(h, freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx)
+                h = layer.forward_deferred(h, freqs_cis, kv_cache=kv_cache, layer_idx=layer_idx, **seeded)
         h = materialize(h)
         h_flat = h.reshape(B, T, self.n_streams * self.config.n_embd)
         h_out = self.norm(cached_linear(self.stream_merge, h_flat, self._casts["merge"]))
@@ -487,6 +493,15 @@ class mHCWalsh(nn.Module):
         if return_hidden:
             return logits, loss, h_out
         return logits, loss
+
+    def all_logits(self, idx):
+        """Logits of every position of idx [B, T]."""
+        _, _, h = self(idx, return_hidden=True)
+        return cached_linear(self.output, h, self._casts["output"])
+
+    def score(self, idx, lengths=None, top_n=0):
+        """Token probabilities of given texts (tokens.score)."""
+        return score(self, idx, lengths, top_n)
 
     def invalidate_weight_caches(self) -> None:
         """Rebuild the ternary codes and kernel layouts on the next forward:
@@ -531,10 +546,13 @@ class mHCWalsh(nn.Module):
 
     @torch.no_grad()
     def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None, top_p=None, min_p=None, kv_cache=None,
-                 lengths=None):
-        """``idx`` [B, T] with ``max_new_tokens`` sampled tokens behind it.
+                 lengths=None, logprobs=None):
+        """``idx`` [B, T] with ``max_new_tokens`` sampled tokens behind it; with
+        ``logprobs``, a number of alternatives, also the new tokens'
+        TokenLogprobs [B, max_new_tokens]: under the model's softmax itself,
+        before temperature and filters.
 
-        Without the last four arguments the reference's loop (mhc.py:754-772):
+        Without ``top_p`` to ``lengths`` the reference's loop (mhc.py:754-772):
         no cache, torch.multinomial.  ``top_p`` or ``min_p`` draws each token
         with kernels.sample (its filters; settings are numbers or tensors with
         a value per row) from torch's uniform numbers.
@@ -542,19 +560,31 @@ class mHCWalsh(nn.Module):
         max_new_tokens positions, keeps the keys and values; the prompts may
         then be padded on the right to T, ``lengths`` (B whole numbers) of
         them each."""
+        probs_of = []
+
+        def note(logits, token):
+            if logprobs is not None:
+                probs_of.append(token_logprobs(logits, token, logprobs))
+
+        def result(idx):
+            return idx if logprobs is None else (idx, stack_steps(probs_of, idx, logprobs))
+        if logprobs is not None and not 0 <= logprobs <= min(kernels.MAX_TOP_LOGPROBS, self.config.vocab_size):
+            raise ValueError(f"generate: logprobs {logprobs} (0 to {kernels.MAX_TOP_LOGPROBS} alternatives, or None)")
         if top_p is None and min_p is None and kv_cache is None:
             if lengths is not None:
                 raise ValueError("generate: prompts of unequal lengths need a kv_cache")
             for _ in range(max_new_tokens):
                 idx_cond = idx if idx.size(1) <= self.config.block_size else idx[:, -self.config.block_size:]
-                logits, _ = self(idx_cond)
-                logits = logits[:, -1, :].float() / temperature
+                raw, _ = self(idx_cond)
+                logits = raw[:, -1, :].float() / temperature
                 if top_k is not None and top_k > 0:
                     v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
                     logits[logits < v[:, [-1]]] = -float('Inf')
                 probs = F.softmax(logits, dim=-1)
-                idx = torch.cat((idx, torch.multinomial(probs, num_samples=1)), dim=1)
-            return idx
+                token = torch.multinomial(probs, num_samples=1)
+                note(raw[:, -1, :], token[:, 0])
+                idx = torch.cat((idx, token), dim=1)
+            return result(idx)
         if kv_cache is None and lengths is not None:
             raise ValueError("generate: prompts of unequal lengths need a kv_cache")
         if lengths is not None:
@@ -588,5 +618,6 @@ class mHCWalsh(nn.Module):
             token = kernels.sample(logits[:, -1, :], u, temperature, 0 if top_k is None else top_k,
                                    1.0 if top_p is None else top_p, 0.0 if min_p is None else min_p)
             token.clamp_(min=0)     # a row of logits that are no numbers has no token: an index that is one
+            note(logits[:, -1, :], token)
             idx = torch.cat((idx, token[:, None]), dim=1)
-        return idx
+        return result(idx)

@@ -15,12 +15,21 @@ from . import kernels
 from ._common import TENSOR_TYPES, first_order, plain_eager
 
 
-def _plain_types(*tensors) -> bool:
-    return plain_eager() and all(t is None or type(t) in TENSOR_TYPES for t in tensors)
+def _kernel_tensors(*tensors) -> bool:
+    """Whether a call may run kernels: tensors themselves (or None), and no
+    transform, trace or mode that has to see each operation."""
+    for t in tensors:
+        if t is not None and type(t) not in TENSOR_TYPES:
+            return False
+    return plain_eager()
 
 
 def _tracked(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ------------------------------------------------------------------ probabilities
@@ -117,11 +126,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0) -
     their log probabilities (kernels.token_logprobs says what odd rows give).
     Differentiable in the logits through all three.  A row whose token is
     negative is not counted: zeros, and no gradient."""
-    if not _plain_types(logits, tokens):
+    if not _kernel_tensors(logits, tokens):
         kernels.check_token_logprobs("token_logprobs", logits, tokens, top_n)
         return token_logprobs_plain(logits, tokens, top_n)
     if _tracked(logits):
-        kernels.check_token_logprobs("token_logprobs", logits, tokens, top_n)
         return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, top_n))
     return TokenLogprobs(*kernels.token_logprobs(logits, tokens, top_n))
 
@@ -205,11 +213,10 @@ def counter_dropout(x: torch.Tensor, p: float, seed: torch.Tensor, stream: int =
     give the same mask.  Probabilities are in steps of 2^-16.  The seed is read
     when the kernels run, so a captured step takes what it holds at each
     replay; it must hold the same in the forward and its backward."""
-    if not _plain_types(x, residual, seed):
+    if not _kernel_tensors(x, residual, seed):
         kernels.check_dropout("counter_dropout", x, p, seed, stream, residual)
         return counter_dropout_plain(x, p, seed, stream, residual)
     if _tracked(x, residual):
-        kernels.check_dropout("counter_dropout", x, p, seed, stream, residual)
         return CounterDropoutFunction.apply(x, residual, p, seed, stream)
     return kernels.dropout(x, p, seed, stream, residual)
 
@@ -269,11 +276,69 @@ def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1
     once.  Differentiable in the weight; a token's gradients are added in their
     order in float32, so equal calls give equal bits.  Tokens outside
     0 .. V - 1 give rows of NaN and no gradient, and ``padding_idx`` none."""
-    plain = not _plain_types(tokens, weight, seed)
-    if plain or padding_idx is not None or _tracked(weight):
+    plain = not _kernel_tensors(tokens, weight, seed)
+    if plain or padding_idx is not None:
         kernels.check_embedding("token_embedding", tokens, weight, p, seed, stream, out_dtype or weight.dtype, padding_idx)
     if plain:
         return token_embedding_plain(tokens, weight, scale, padding_idx, out_dtype, p, seed, stream)
     if _tracked(weight):
         return TokenEmbeddingFunction.apply(weight, tokens, scale, padding_idx, out_dtype, p, seed, stream)
     return kernels.embedding(tokens, weight, scale, out_dtype, p, seed, stream)
+
+
+# ------------------------------------------------------------------ in a model
+
+def embed_tokens(model, tokens: torch.Tensor, seed: torch.Tensor = None) -> torch.Tensor:
+    """A model's token rows: its embedding as it is, or with its config's scale
+    and (given a seed) dropout."""
+    scale = getattr(model.config, "embed_scale", 1.0)
+    p = getattr(model.config, "embed_dropout", 0.0) if seed is not None else 0.0
+    if scale == 1.0 and p == 0.0:
+        return model.tok_embeddings(tokens)
+    return token_embedding(tokens, model.tok_embeddings.weight, scale, p=p, seed=seed)
+
+
+def step_seed(model, tokens: torch.Tensor):
+    """The seed of one forward of a model that trains with dropout of its
+    tokens' rows or its layers' outputs, else None."""
+    c = model.config
+    if model.training and (getattr(c, "embed_dropout", 0.0) > 0 or getattr(c, "resid_dropout", 0.0) > 0):
+        return fresh_seed(tokens.device)
+    return None
+
+
+def drop_output(y: torch.Tensor, p: float, seed, layer_idx: int, which: int, residual: torch.Tensor = None) -> torch.Tensor:
+    """Output ``which`` (0 attention, 1 feed-forward) of a layer with dropout,
+    where the step has a seed, onto the residual stream if there is one.  Stream
+    0 is the tokens' rows'."""
+    if seed is None or p == 0.0:
+        return y if residual is None else residual + y
+    return counter_dropout(y, p, seed, 1 + 2 * layer_idx + which, residual)
+
+
+def stack_steps(steps, idx: torch.Tensor, top_n: int) -> TokenLogprobs:
+    """The TokenLogprobs [B, steps] of a loop's steps, each [B]."""
+    if not steps:
+        none = torch.empty(idx.shape[0], 0, device=idx.device)
+        wide = none.new_empty(idx.shape[0], 0, top_n)
+        return TokenLogprobs(none, none.clone(), wide, wide.long())
+    return TokenLogprobs(*(torch.stack(parts, 1) for parts in zip(*steps)))
+
+
+def score(model, idx: torch.Tensor, lengths=None, top_n: int = 0) -> TokenLogprobs:
+    """The log probabilities of the tokens idx[:, 1:] of idx [B, T], each under
+    the model's softmax behind those before it, with entropies and ``top_n``
+    alternatives: [B, T - 1].  ``lengths`` (B whole numbers) are the tokens
+    that each text has, padded on the right with anything: what lies past them
+    is not counted.  Differentiable where autograd is on."""
+    if idx.dim() != 2 or idx.shape[1] < 2:
+        raise ValueError(f"score: texts [B, T] of at least two tokens, got {tuple(idx.shape)}")
+    tokens = idx[:, 1:]
+    if lengths is not None:
+        n = torch.as_tensor(lengths, device=idx.device, dtype=torch.int64)
+        if n.shape != idx.shape[:1]:
+            raise ValueError(f"score: lengths {tuple(n.shape)} of texts {tuple(idx.shape)}")
+        there = torch.arange(idx.shape[1], device=idx.device) < n[:, None]
+        idx = torch.where(there, idx, 0)
+        tokens = torch.where(there[:, 1:], tokens, -1)
+    return token_logprobs(model.all_logits(idx[:, :-1]), tokens, top_n)
