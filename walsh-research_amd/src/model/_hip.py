@@ -262,14 +262,23 @@ def on_device(index: int, fn, *args):
         return fn(*args)
 
 
+# (bound once: every launch asks these)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def call_on(index: int, name: str, *args, **kw) -> None:
     """``call`` with the current stream of device ``index`` as the last
     argument, on whichever device is current."""
-    if index == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index), **kw)
+    if index == _current_device():
+        if _timer is None and _lib is not None:
+            rc = getattr(_lib, name)(*args, _raw_stream(index))
+            if rc:
+                check(rc, name)
+        else:
+            call(name, *args, _raw_stream(index), **kw)
     else:
         with torch.cuda.device(index):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(index), **kw)
+            call(name, *args, _raw_stream(index), **kw)
 
 
 def require_device(t: torch.Tensor, what: str = "tensor") -> None:

@@ -1198,22 +1198,24 @@ def token_logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor, top_index: to
     """The gradient of the logits (contiguous, in their dtype), for gradients
     of token_logprobs's outputs (float32, None: zeros) and its index and stats."""
     n = top_index.shape[-1]
-    check_token_logprobs("token_logprobs_bwd", logits, tokens, n)
-    for g, shape in ((g_logprob, tokens.shape), (g_entropy, tokens.shape), (g_top, top_index.shape)):
+    dt = check_token_logprobs("token_logprobs_bwd", logits, tokens, n)
+    shape = tokens.shape
+    for g in (g_logprob, g_entropy):
         assert g is None or g.shape == shape and g.dtype == torch.float32, "token_logprobs_bwd: gradients as the outputs"
-    assert top_index.shape[:-1] == tokens.shape and top_index.dtype == torch.int64, "token_logprobs_bwd: index [..., n]"
+    assert g_top is None or g_top.shape == top_index.shape and g_top.dtype == torch.float32, \
+        "token_logprobs_bwd: gradients as the outputs"
+    assert top_index.shape[:-1] == shape and top_index.dtype == torch.int64, "token_logprobs_bwd: index [..., n]"
     rows, N, ld = _separate_rows(logits)
     assert stats.shape == (N, 4) and stats.dtype == torch.float32, "token_logprobs_bwd: stats [rows, 4]"
     _hip.same_device("token_logprobs_bwd", logits, top_index, stats, g_logprob, g_entropy, g_top)
     # (held until the launch: a copy must not be freed before it)
     tokens, top_index, stats = tokens.contiguous(), top_index.contiguous(), _rows16(stats)
-    g = [None if t is None else t.contiguous() for t in (g_logprob, g_entropy, g_top)]
+    g0, g1, g2 = (None if t is None else t.contiguous() for t in (g_logprob, g_entropy, g_top))
     V = logits.shape[-1]
     out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
     _hip.call_on(logits.get_device(), "walsh_token_logprobs_bwd", rows.data_ptr(), ld, N, V, tokens.data_ptr(), n,
-                 top_index.data_ptr(), stats.data_ptr(), *map(_hip.ptr, g), out.data_ptr(), V,
-                 _hip.dtype_code(logits.dtype), kernel="logprobs_bwd_kernel", nbytes=2 * N * V * logits.element_size(),
-                 flops=6 * N * V)
+                 top_index.data_ptr(), stats.data_ptr(), _hip.ptr(g0), _hip.ptr(g1), _hip.ptr(g2), out.data_ptr(), V, dt,
+                 kernel="logprobs_bwd_kernel", nbytes=(8 - 4 * dt) * N * V, flops=6 * N * V)
     return out
 
 
@@ -1263,7 +1265,11 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, stream: int = 0, resi
     device, read when the kernel runs), ``stream`` (0 to 2^32 - 1), the
     element's row (of those that all leading dimensions make) and column: the
     same call again gives the gradient's mask."""
-    drop, xt, rt = check_dropout("dropout", x, p, seed, stream, residual)
+    return dropout_run(x, *check_dropout("dropout", x, p, seed, stream, residual), seed, stream, residual, out_dtype)
+
+
+def dropout_run(x, drop, xt, rt, seed, stream, residual=None, out_dtype=None):
+    """``dropout`` of arguments that are known to be right."""
     if out_dtype is None:
         out_dtype = x.dtype if xt == rt else torch.float32
     y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
@@ -1331,18 +1337,24 @@ def embedding_bwd(tokens: torch.Tensor, gy: torch.Tensor, V: int, scale: float =
     _hip.same_device("embedding_bwd", gy, tokens)
     drop = drop_threshold("embedding_bwd", p)
     check_seed("embedding_bwd", gy, seed, stream, drop)
+    return embedding_bwd_run(tokens, gy, V, scale, dtype, padding_idx, drop, gt, wt, seed, stream)
+
+
+def embedding_bwd_run(tokens, gy, V, scale, dtype, padding_idx, drop, gt, wt, seed, stream):
+    """``embedding_bwd`` of arguments that are known to be right."""
     C, N = gy.shape[-1], tokens.numel()
     dw = torch.empty(V, C, device=gy.device, dtype=dtype)
     if C == 0:
         return dw
     tokens = tokens.contiguous()
     rows, _, ldg = _separate_rows(gy)
-    nws = _workspace("walsh_embedding_bwd_workspace_bytes", gy.get_device(), N, V, C)
+    index = gy.get_device()
+    nws = _workspace("walsh_embedding_bwd_workspace_bytes", index, N, V, C)
     ws = torch.empty(nws, device=gy.device, dtype=torch.uint8)
-    _hip.call_on(gy.get_device(), "walsh_embedding_bwd", tokens.data_ptr(), N, rows.data_ptr(), ldg, V, C, float(scale),
+    _hip.call_on(index, "walsh_embedding_bwd", tokens.data_ptr(), N, rows.data_ptr(), ldg, V, C, float(scale),
                  -1 if padding_idx is None else padding_idx, drop, _hip.ptr(seed), stream, dw.data_ptr(), C, gt, wt,
-                 ws.data_ptr(), nws, kernel="embed_bwd_kernels",
-                 nbytes=N * C * gy.element_size() + V * C * dw.element_size(), flops=2 * N * C)
+                 ws.data_ptr(), nws, kernel="embed_bwd_kernels", nbytes=N * C * (4 - 2 * gt) + V * C * (4 - 2 * wt),
+                 flops=2 * N * C)
     return dw
 
 

@@ -13,6 +13,7 @@ from torch.nn import functional as F
 
 from . import kernels
 from ._common import TENSOR_TYPES, first_order, plain_eager
+from ._hip import dtype_code
 
 
 def _kernel_tensors(*tensors) -> bool:
@@ -184,18 +185,20 @@ class CounterDropoutFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, p, seed, stream):
+        drop, xt, rt = kernels.check_dropout("counter_dropout", x, p, seed, stream, residual)
         ctx.save_for_backward(seed)
-        ctx.args = (p, stream, x.dtype, None if residual is None else residual.dtype)
-        return kernels.dropout(x, p, seed, stream, residual)
+        ctx.args = (p, drop, stream, x.dtype, None if residual is None else residual.dtype)
+        return kernels.dropout_run(x, drop, xt, rt, seed, stream, residual)
 
     @staticmethod
     def backward(ctx, gy):
         seed, = ctx.saved_tensors
-        p, stream, dtype, rdtype = ctx.args
+        p, drop, stream, dtype, rdtype = ctx.args
         gx = gr = None
         if ctx.needs_input_grad[0]:
             if first_order(gy):
-                gx = kernels.dropout(gy, p, seed, stream, out_dtype=dtype)
+                gt = dtype_code(gy.dtype)
+                gx = kernels.dropout_run(gy, drop, gt, gt, seed, stream, None, dtype)
             else:
                 gx = counter_dropout_plain(gy.float(), p, seed, stream).to(dtype)
         if ctx.needs_input_grad[1]:
@@ -248,17 +251,18 @@ class TokenEmbeddingFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, tokens, scale, padding_idx, out_dtype, p, seed, stream):
         ctx.save_for_backward(tokens, seed)
-        ctx.args = (weight.shape[0], scale, padding_idx, weight.dtype, p, stream)
+        ctx.args = (weight.shape[0], scale, padding_idx, weight.dtype, kernels.drop_threshold("token_embedding", p), stream)
         return kernels.embedding(tokens, weight, scale, out_dtype, p, seed, stream)
 
     @staticmethod
     def backward(ctx, gy):
         tokens, seed = ctx.saved_tensors
-        V, scale, padding_idx, dtype, p, stream = ctx.args
+        V, scale, padding_idx, dtype, drop, stream = ctx.args
         if first_order(gy):
-            gw = kernels.embedding_bwd(tokens, gy, V, scale, dtype, padding_idx, p, seed, stream)
+            gw = kernels.embedding_bwd_run(tokens, gy, V, scale, dtype, padding_idx, drop, dtype_code(gy.dtype),
+                                           dtype_code(dtype), seed, stream)
         else:
-            g = _drop_plain(gy, kernels.drop_threshold("token_embedding", p), seed, stream, scale)
+            g = _drop_plain(gy, drop, seed, stream, scale)
             skip = (tokens < 0) | (tokens >= V)
             if padding_idx is not None:
                 skip = skip | (tokens == padding_idx)
