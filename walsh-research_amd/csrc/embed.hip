@@ -7,13 +7,19 @@
 // calls give equal bits.  Three kernels:
 //   sort   a workgroup takes a range of up to 256 tokens and walks all N: it
 //          counts those below its range, which is where its part of the sorted
-//          order begins (no workgroup waits for another), and those in it by
-//          token; a second walk puts them in place.
-//   rows   a lane takes 8 columns of a row of dW and adds its tokens' rows, up
-//          to 32 of them; rows without tokens are zeros.  Longer rows are cut
-//          where the sorted order is, every 32 places (more past 32,768
-//          tokens), and their pieces summed into a workspace.
-//   join   adds the pieces of each long row, in order.
+//          order begins (no workgroup waits for another), and lists those in
+//          it, to count and place them.  What every workgroup repeats, ten
+//          instructions for 64 tokens, costs less than a launch would: 5.9 us for
+//          8,192 tokens, 8.3 for 16,384, 19 for 65,536, 4 of them the launch.
+//   rows   zeros where a token does not occur; else the sum of its tokens' rows,
+//          a lane 8 columns, up to 32 of them.  Longer rows are cut where the
+//          sorted order is, every 32 places (more past 32,768 tokens), and their
+//          pieces summed into a workspace.
+//   join   adds the pieces of each long row, in a fixed order.
+// Bound by memory: 50,257 x 4,096 bf16 from 16,384 rows (546 MB) take 111 us for
+// the rows, 4.9 TB/s, x 512 float32 from 8,192 (120 MB) 22 us, of 128 and 33 in
+// all; a character model's 65 x 768 from 16,384 rows 25 us, all of it latency.
+// The lookup of 16,384 x 4,096 takes 41 us, of 64 rows 2.9.
 #include <type_traits>
 
 #include "rows8.h"

@@ -11,14 +11,26 @@
 //
 // One workgroup per row, one pass over it: every lane keeps a running maximum
 // and sums relative to it, in float32, moved when a step of its values brings a
-// larger one; lanes and wavefronts are joined at the end.
+// larger one; lanes and wavefronts are joined at the end.  Four wavefronts take
+// a row; sixteen where rows of more than 8,192 tokens are no more than CUs, so
+// that a row is not left to a quarter of its CU (50,257 tokens: one row 5.8 us
+// instead of 6.0, with 5 alternatives 9.3, 256 rows 7.1 instead of 7.6; at 512
+// rows sixteen take 18.2, four 12.8).  A row over several workgroups would need
+// a second launch, of 4 us.
 //
 // Alternatives: the lanes' maxima, taken together over the wavefronts, are the
-// largest of 64 groups of tokens.  The n-th largest of them is a bound that at
-// least n tokens reach, and few more: only lanes whose own maximum does look
-// at their tokens again.  Those go to a list in LDS and are ranked there by
-// value and index.  Where there are too many (thousands of equal ones) or a
-// group has none, the row is walked once for every alternative instead.
+// largest of 256 groups of tokens.  A search by their bits finds a bound that
+// at least n of them reach and few more, so at least n tokens do; lanes whose
+// own maximum does read again those of their steps whose maximum does.  Those
+// tokens go to a list in LDS and are ranked there by value and index.  Where
+// there are too many (thousands of equal ones) or a group has none, the row is
+// walked once for every alternative instead.
+//
+// Bound by memory: 8,192 rows of 50,257 bf16 logits take 141 us (5.8 TB/s), with
+// 5 and 20 alternatives 166 and 187, with float32 logits 269 (6.1), 275, 283.
+// Of 10 instructions a token the exponential takes the time of four.  Their
+// gradient, 823 MB read and as many written, takes 291 us (5.7 TB/s), in
+// float32 641 (5.1, the rate of a copy).
 #include <type_traits>
 
 #include "rows8.h"
@@ -110,11 +122,12 @@ template <int ROWS> __device__ __forceinline__ float lp_sum(float v) {
     return lp_reduce<ROWS>(v, 0.f, [](float a, float b) { return a + b; });
 }
 
-// Tokens in order of preference: larger values first, then lower indexes.
-__device__ __forceinline__ uint64_t lp_key(float x, int i) {
+// Tokens in order of preference: larger values first (NaN as -inf), then lower indexes.
+__device__ __forceinline__ uint32_t lp_order(float x) {
     const uint32_t b = __float_as_uint(fmaxf(x, -INFINITY) + 0.f);
-    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~i;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ uint64_t lp_key(float x, int i) { return (uint64_t)lp_order(x) << 32 | (uint32_t)~i; }
 __device__ __forceinline__ float lp_value(uint64_t key) {
     const uint32_t b = (uint32_t)(key >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
@@ -123,8 +136,11 @@ __device__ __forceinline__ uint64_t lp_xor(uint64_t v, int o) {
     return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, o);
 }
 
+constexpr int kLpU = 4;                // blocks of 8 tokens that a lane takes in a step
+constexpr int kLpSlots = 16;           // of the steps' maxima
 template <int NT, bool TOP> struct LpShared {
     f32x4 part[NT / 64];
+    float step[TOP ? kLpSlots : 1][NT];            // a lane's largest of steps i, i + kLpSlots ...
     float group[TOP ? NT / 64 : 1][64];
     uint64_t list[TOP ? kLpList : 1], best[NT / 64];
     int n;
@@ -145,10 +161,8 @@ template <int NT, typename Q, typename S> __device__ __forceinline__ Q lp_join(S
     return q;
 }
 
-// STEPS: blocks of 8 tokens that a lane holds in registers, all of its row's
-// (V <= 8 NT STEPS + 7); or 0: it walks them, U at a time.
-template <typename T, int NT, int STEPS, bool TOP> __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
-    constexpr int W = NT / 64, U = 4;
+template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
+    constexpr int W = NT / 64, U = kLpU;
     __shared__ LpShared<NT, TOP> sh;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -170,9 +184,21 @@ template <typename T, int NT, int STEPS, bool TOP> __global__ __launch_bounds__(
     const T *body = p + lead;
     const int last = tid < rest ? lead + 8 * blocks + tid : 0;
     LpSums q;
-    Raw8<T> held[STEPS ? STEPS : 1];
-    float end = tid < rest + lead ? Act<T>::load(p + last) : -INFINITY;
-    auto take = [&](const auto &r, auto n) {       // the sums of n blocks
+    const float end = tid < rest + lead ? Act<T>::load(p + last) : -INFINITY;
+    // up to U blocks of the lane's step from block b on; what there is not is -inf
+    auto load = [&](Raw8<T> (&r)[U], int b) {
+        if (b + (U - 1) * NT < blocks) {
+#pragma unroll
+            for (int j = 0; j < U; ++j) r[j].load(body + 8 * (int64_t)(b + j * NT));
+        } else {
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                r[j].fill(-INFINITY);
+                if (b + j * NT < blocks) r[j].load(body + 8 * (int64_t)(b + j * NT));
+            }
+        }
+    };
+    auto take = [&](const auto &r, auto n) {       // the sums of n blocks; their maximum
         float x[decltype(n)::value][8], top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < n; ++j) {
@@ -185,46 +211,30 @@ template <typename T, int NT, int STEPS, bool TOP> __global__ __launch_bounds__(
         for (int j = 0; j < n; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) q.add(x[j][i]);
+        return top;
     };
-    if constexpr (STEPS > 0) {
+    if constexpr (TOP) {
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-            held[j].fill(-INFINITY);
-            if (tid + j * NT < blocks) held[j].load(body + 8 * (tid + j * NT));
-        }
-        float top = end;
-#pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-            float x[8];
-            held[j].unpack(x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
-        }
-        if (top > q.m) q.move(top);
-#pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-            float x[8];
-            held[j].unpack(x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q.add(x[i]);
-        }
-        q.add(end);
-    } else {
-        int b = tid;
-        for (; b + (U - 1) * NT < blocks; b += NT * U) {
-            Raw8<T> r[U];
-#pragma unroll
-            for (int j = 0; j < U; ++j) r[j].load(body + 8 * (int64_t)(b + j * NT));
-            take(r, std::integral_constant<int, U>{});
-        }
-        for (; b < blocks; b += NT) {
-            Raw8<T> r[1];
-            r[0].load(body + 8 * (int64_t)b);
-            take(r, std::integral_constant<int, 1>{});
-        }
-        if (end > q.m) q.move(end);
-        q.add(end);
+        for (int i = 0; i < kLpSlots; ++i) sh.step[i][tid] = -INFINITY;
     }
+    int step = 0;
+    for (int b = tid; b < blocks; b += NT * U, ++step) {
+        float top;
+        Raw8<T> r[U];
+        if (b + NT < blocks) {
+            load(r, b);
+            top = take(r, std::integral_constant<int, U>{});
+        } else {
+            r[0].load(body + 8 * (int64_t)b);
+            top = take(r, std::integral_constant<int, 1>{});
+        }
+        if constexpr (TOP) {
+            float &slot = sh.step[step % kLpSlots][tid];
+            slot = step < kLpSlots ? top : fmaxf(slot, top);
+        }
+    }
+    if (end > q.m) q.move(end);
+    q.add(end);
     const float own = q.m;
     if constexpr (TOP) {
         sh.group[wave][lane] = own;
@@ -255,47 +265,50 @@ template <typename T, int NT, int STEPS, bool TOP> __global__ __launch_bounds__(
 
     float *top = a.top + row * a.n;
     int64_t *index = a.top_index + row * a.n;
-    // the n-th largest of the groups' maxima
-    float g = sh.group[0][lane];
+    // a bound that at least n of the groups' maxima reach, and few more
+    constexpr int K = 4, PER = W / K;
+    uint32_t key[K];
+    float least = INFINITY, most = -INFINITY;
 #pragma unroll
-    for (int w = 1; w < W; ++w) g = fmaxf(g, sh.group[w][lane]);
-    int rank = 0;
+    for (int k = 0; k < K; ++k) {
+        float g = sh.group[k * PER][lane];
 #pragma unroll
-    for (int j = 0; j < 64; ++j) {
-        const float o = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), j));
-        rank += o > g || (o == g && j < lane);
+        for (int w = 1; w < PER; ++w) g = fmaxf(g, sh.group[k * PER + w][lane]);
+        key[k] = lp_order(g);
+        least = fminf(least, g), most = fmaxf(most, g);
     }
-    const uint64_t nth = __ballot(rank == a.n - 1);
-    const float bound = __shfl(g, (int)__ffsll((long long)nth) - 1);
-    if (bound > -1e30f) {
-        auto put = [&](const Raw8<T> &r, int b) {
-            float x[8];
-            r.unpack(x);
+    uint32_t lo = lp_order(-lp_max<4>(-least)), hi = lp_order(lp_max<4>(most)) + 1;
+    for (int reach = 64 * K; reach > a.n + a.n / 4 + 2 && hi - lo > 1;) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        int c = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (x[i] >= bound) {
-                    const int at = atomicAdd(&sh.n, 1);
-                    if (at < kLpList) sh.list[at] = lp_key(x[i], lead + 8 * b + i);
-                }
+        for (int k = 0; k < K; ++k) c += __popcll(__ballot(key[k] >= mid));
+        if (c >= a.n) lo = mid, reach = c;
+        else hi = mid;
+    }
+    const float bound = lp_value((uint64_t)lo << 32);
+    if (bound > -1e30f) {
+        auto put = [&](float x, int i) {
+            if (x >= bound) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < kLpList) sh.list[at] = lp_key(x, i);
+            }
         };
         if (own >= bound) {
-            if constexpr (STEPS > 0) {
+            step = 0;
+            for (int b = tid; b < blocks; b += NT * U, ++step) {
+                if (sh.step[step % kLpSlots][tid] < bound) continue;
+                Raw8<T> r[U];
+                load(r, b);
 #pragma unroll
-                for (int j = 0; j < STEPS; ++j) put(held[j], tid + j * NT);
-            } else {
-                for (int b = tid; b < blocks; b += NT * U) {
-                    Raw8<T> r[U];
+                for (int j = 0; j < U; ++j) {
+                    float x[8];
+                    r[j].unpack(x);
 #pragma unroll
-                    for (int j = 0; j < U; ++j) r[j].load(body + 8 * (int64_t)min(b + j * NT, blocks - 1));
-#pragma unroll
-                    for (int j = 0; j < U; ++j)
-                        if (b + j * NT < blocks) put(r[j], b + j * NT);
+                    for (int i = 0; i < 8; ++i) put(x[i], lead + 8 * (b + j * NT) + i);
                 }
             }
-            if (end >= bound) {
-                const int at = atomicAdd(&sh.n, 1);
-                if (at < kLpList) sh.list[at] = lp_key(end, last);
-            }
+            put(end, last);
         }
         __syncthreads();
         const int count = sh.n;
@@ -400,14 +413,13 @@ template <typename T> __global__ __launch_bounds__(256) void logprobs_bwd_kernel
 
 template <typename T> static void logprobs_launch(const LogprobArgs &a, int64_t N, hipStream_t s) {
     auto go = [&](auto kernel, int nt) { launch(kernel, dim3((unsigned)N), dim3(nt), 0, s, a); };
-    const int steps = (int)ceil_div(a.V / 8, 1024);
-    if (a.n) {
-        if (steps <= 2) go(logprobs_kernel<T, 1024, 2, true>, 1024);
-        else if (steps <= 4) go(logprobs_kernel<T, 1024, 4, true>, 1024);
-        else if (steps <= 7) go(logprobs_kernel<T, 1024, 7, true>, 1024);
-        else go(logprobs_kernel<T, 1024, 0, true>, 1024);
+    // four wavefronts to a row, or sixteen where there are few long ones
+    if (N <= device_info().cu_count && a.V > 8192) {
+        if (a.n) go(logprobs_kernel<T, 1024, true>, 1024);
+        else go(logprobs_kernel<T, 1024, false>, 1024);
     } else {
-        go(logprobs_kernel<T, 256, 0, false>, 256);
+        if (a.n) go(logprobs_kernel<T, 256, true>, 256);
+        else go(logprobs_kernel<T, 256, false>, 256);
     }
 }
 
