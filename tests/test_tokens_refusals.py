@@ -94,10 +94,10 @@ def test_nothing_to_do(L):
 
 
 def test_workspace_bytes(L):
-    """Row starts, sorted places and two partial rows for every 32 tokens."""
+    """Row starts, sorted places and their tokens, two partial rows for every chunk."""
     f = L.walsh_embedding_bwd_workspace_bytes
     for N, V, C in ((1, 1, 1), (33, 5, 7), (8192, 50257, 512)):
-        least = 4 * (V + 1) + 4 * N
+        least = 4 * (V + 1) + 8 * N
         assert least <= f(N, V, C) and f(N, V, C) % 4 == 0
         assert f(N, V, C) >= f(N - 1, V, C)
     assert f(-1, 5, 5) == 0 and f(5, 0, 5) == 0

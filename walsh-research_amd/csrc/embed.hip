@@ -13,12 +13,12 @@
 //          8,192 tokens, 8.3 for 16,384, 19 for 65,536, 4 of them the launch.
 //   rows   zeros where a token does not occur; else the sum of its tokens' rows,
 //          a lane 8 columns, up to 32 of them.  Longer rows are cut where the
-//          sorted order is, every 32 places (more past 32,768 tokens), and their
-//          pieces summed into a workspace.
+//          sorted order is, every 32 places (embed_most), and their pieces summed
+//          into a workspace.
 //   join   adds the pieces of each long row, in a fixed order.
 // Bound by memory: 50,257 x 4,096 bf16 from 16,384 rows (546 MB) take 111 us for
 // the rows, 4.9 TB/s, x 512 float32 from 8,192 (120 MB) 22 us, of 128 and 33 in
-// all; a character model's 65 x 768 from 16,384 rows 25 us, all of it latency.
+// all; a character model's 65 x 768 from 16,384 rows 22 us, all of it latency.
 // The lookup of 16,384 x 4,096 takes 41 us, of 64 rows 2.9.
 #include <type_traits>
 
@@ -409,13 +409,17 @@ template <typename TW> __global__ __launch_bounds__(256) void embed_join_kernel(
     store8((TW *)a.dw + t * a.ldw + c, a.C - c, acc);
 }
 
-// Places of a chunk: 32, or as many as leave 1,024 pieces of the longest row.
-static int64_t embed_most(int64_t N) {
-    int64_t most = 32;
+// Places of a chunk: fewer than 32 where that leaves too few lanes for the chip
+// (16,384 x 768 in chunks of 16 instead of 32: 30 us instead of 34 in all, 4,096 x
+// 384 in 8 17 instead of 26; 16,384 x 4,096 in 8 133 instead of 126), more
+// where the longest row would have more than 1,024 pieces.
+static int64_t embed_most(int64_t N, int64_t C) {
+    int64_t most = 8;
+    while (most < 32 && N * ceil_div(C, 8) > most * 131072) most *= 2;
     while (most * 1024 < N) most *= 2;
     return most;
 }
-static int64_t embed_chunks(int64_t N) { return ceil_div(N, embed_most(N)); }
+static int64_t embed_chunks(int64_t N, int64_t C) { return ceil_div(N, embed_most(N, C)); }
 // start, order, token, parts: each from a multiple of 16 bytes on
 static int64_t embed_start_bytes(int64_t V) { return ceil_div(4 * (V + 1), 16) * 16; }
 static int64_t embed_order_bytes(int64_t N) { return ceil_div(4 * N, 16) * 16; }
@@ -471,7 +475,7 @@ WALSH_EXPORT int walsh_embedding_fwd(const int64_t *tokens, int64_t N, const voi
 
 WALSH_EXPORT int64_t walsh_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t C) {
     if (N < 0 || V < 1 || C < 0) return 0;
-    return embed_start_bytes(V) + 2 * embed_order_bytes(N) + 2 * embed_chunks(N) * C * 4;
+    return embed_start_bytes(V) + 2 * embed_order_bytes(N) + 2 * embed_chunks(N, C) * C * 4;
 }
 
 WALSH_EXPORT int walsh_embedding_bwd(const int64_t *tokens, int64_t N, const void *gy, int64_t ldg, int64_t V, int64_t C,
@@ -482,7 +486,7 @@ WALSH_EXPORT int walsh_embedding_bwd(const int64_t *tokens, int64_t N, const voi
     int rc = embed_check(fn, N, V, C, drop, seed, rng_stream, gdtype, wdtype);
     if (rc) return rc;
     if (C == 0) return WALSH_OK;
-    const Blocks rows = make_blocks(V, C), chunks = make_blocks(embed_chunks(N), C);
+    const Blocks rows = make_blocks(V, C), chunks = make_blocks(embed_chunks(N, C), C);
     if (V * (int64_t)rows.per_row > kMaxBlocks)
         return set_error(WALSH_ENOTSUP, "%s: V=%lld rows of C=%lld", fn, (long long)V, (long long)C);
     if ((N && (!tokens || !gy)) || !dw || !work) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
@@ -505,10 +509,10 @@ WALSH_EXPORT int walsh_embedding_bwd(const int64_t *tokens, int64_t N, const voi
     constexpr int U = 1, F = 4;
     const uint32_t head_groups = (uint32_t)ceil_div(N * rows.per_row, 256 * U);
     const uint32_t rest_groups = (uint32_t)ceil_div(V * rows.per_row, 256 * F);
-    // (up to 32 tokens no row is long)
-    const uint32_t chunk_groups = N > embed_most(N) ? (uint32_t)ceil_div((int64_t)chunks.rows * chunks.per_row, 256) : 0;
+    const int64_t most = embed_most(N, C);         // (up to so many tokens no row is long)
+    const uint32_t chunk_groups = N > most ? (uint32_t)ceil_div((int64_t)chunks.rows * chunks.per_row, 256) : 0;
     const EmbedBwd a{start, order, token, gy, dw, parts, V, ldg, ldw,
-                     (int)(padding_idx >= 0 && padding_idx < V ? padding_idx : -1), (int)C, (int)embed_most(N), rows, make_blocks(N, C),
+                     (int)(padding_idx >= 0 && padding_idx < V ? padding_idx : -1), (int)C, (int)most, rows, make_blocks(N, C),
                      chunks, chunk_groups, head_groups, Drop{(const uint64_t *)seed, (uint32_t)rng_stream, (uint32_t)drop},
                      (float)((double)scale * kept_factor(drop))};
     embed_types(gdtype, wdtype, drop, [&](auto g, auto w, auto d) {
