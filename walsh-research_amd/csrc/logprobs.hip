@@ -463,7 +463,7 @@ WALSH_EXPORT int walsh_token_logprobs_bwd(const void *logits, int64_t ld, int64_
     if (!logits || !tokens || !stats || !dlogits || (n && !top_index)) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
     if ((uintptr_t)stats % 16) return set_error(WALSH_EINVAL, "%s: stats 16-byte aligned", fn);
     const int64_t blocks = V / 8, parts = blocks ? ceil_div(blocks, 1024) : 1, per = ceil_div(blocks, parts);
-    if (N * parts > kMaxBlocks / 256)
+    if (N * parts > 0xffffffffll / 256)
         return set_error(WALSH_ENOTSUP, "%s: N=%lld rows of V=%lld", fn, (long long)N, (long long)V);
     const LogprobBwd a{logits, tokens, top_index, (const f32x4 *)stats, g_logprob, g_entropy, n ? g_top : nullptr, dlogits,
                        ld, ldd, (int)V, (int)n, (int)parts, (int)per};
