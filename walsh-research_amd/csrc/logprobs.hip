@@ -26,11 +26,11 @@
 // there are too many (thousands of equal ones) or a group has none, the row is
 // walked once for every alternative instead.
 //
-// Bound by memory: 8,192 rows of 50,257 bf16 logits take 141 us (5.8 TB/s), with
-// 5 and 20 alternatives 166 and 187, with float32 logits 269 (6.1), 275, 283.
+// Bound by memory: 8,192 rows of 50,257 bf16 logits take 129 us (6.4 TB/s), with
+// 5 and 20 alternatives 166 and 187, with float32 logits 257 (6.4), 275, 283.
 // Of 10 instructions a token the exponential takes the time of four.  Their
-// gradient, 823 MB read and as many written, takes 291 us (5.7 TB/s), in
-// float32 641 (5.1, the rate of a copy).
+// gradient, 823 MB read and as many written, takes 292 us (5.6 TB/s), in
+// float32 582 (5.7, where a copy reaches 5.1).
 #include <type_traits>
 
 #include "rows8.h"
@@ -41,6 +41,48 @@ constexpr int kLpTop = 64;             // most alternatives
 constexpr int kLpList = 1024;
 constexpr float kLpLowest = -3.402823466e38f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// Bytes that the memory side's cache holds.  What is read or written once and
+// is more than that is streamed past the caches: 823 MB of bf16 logits are read
+// in 129 us instead of 142, and with a gradient to come, whose kernel finds the
+// last of them there, forward and gradient take 414 us instead of 446 (float32
+// 828, 896), with the product that reads the gradient 987 instead of 996.  A
+// gradient that fits beside its logits is better left there (8,192 x 4,096: 42
+// us, streamed 44), one that does not is streamed (2,048 rows: 97 us, not 109).
+constexpr int64_t kLpCache = 256 << 20;
+
+// 16 bytes of logits, at any element alignment.  STREAM: not kept in caches.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+template <typename T> struct LpBlock {
+    static constexpr int E = 16 / sizeof(T);
+    u32x4 a;
+    template <bool STREAM> __device__ __forceinline__ void load(const T *p) {
+        if (STREAM) a = __builtin_nontemporal_load((const u32x4_any *)p);
+        else a = *(const u32x4_any *)p;
+    }
+    template <bool STREAM> __device__ __forceinline__ void store(T *p) const {
+        if (STREAM) __builtin_nontemporal_store(a, (u32x4_any *)p);
+        else *(u32x4_any *)p = a;
+    }
+    __device__ __forceinline__ void unpack(float (&v)[E]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (E == 8) v[2 * i] = __uint_as_float(a[i] << 16), v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+            else v[i] = __uint_as_float(a[i]);
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&v)[E]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (E == 8) a[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+            else a[i] = __float_as_uint(v[i]);
+        }
+    }
+    __device__ __forceinline__ void fill(float v) {
+        const uint32_t w = E == 8 ? pack_bf16x2(v, v) : __float_as_uint(v);
+        a = u32x4{w, w, w, w};
+    }
+};
 
 struct LogprobArgs {
     const void *logits;
@@ -136,7 +178,6 @@ __device__ __forceinline__ uint64_t lp_xor(uint64_t v, int o) {
     return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, o);
 }
 
-constexpr int kLpU = 4;                // blocks of 8 tokens that a lane takes in a step
 constexpr int kLpSlots = 16;           // of the steps' maxima
 template <int NT, bool TOP> struct LpShared {
     f32x4 part[NT / 64];
@@ -161,8 +202,9 @@ template <int NT, typename Q, typename S> __device__ __forceinline__ Q lp_join(S
     return q;
 }
 
-template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
-    constexpr int W = NT / 64, U = kLpU;
+// A lane takes U blocks of E tokens in a step.
+template <typename T, int NT, bool TOP, bool STREAM> __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
+    constexpr int W = NT / 64, E = LpBlock<T>::E, U = 32 / E;
     __shared__ LpShared<NT, TOP> sh;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -180,37 +222,37 @@ template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void lo
     // at both ends of the row goes to a lane each, as token `last`.
     const T *p = (const T *)a.logits + row * a.ld;
     const int lead = (uintptr_t)p & 3 ? 1 : 0;
-    const int blocks = (a.V - lead) / 8, rest = (a.V - lead) & 7;
+    const int blocks = (a.V - lead) / E, rest = (a.V - lead) % E;
     const T *body = p + lead;
-    const int last = tid < rest ? lead + 8 * blocks + tid : 0;
+    const int last = tid < rest ? lead + E * blocks + tid : 0;
     LpSums q;
     const float end = tid < rest + lead ? Act<T>::load(p + last) : -INFINITY;
     // up to U blocks of the lane's step from block b on; what there is not is -inf
-    auto load = [&](Raw8<T> (&r)[U], int b) {
+    auto load = [&](LpBlock<T> (&r)[U], int b) {
         if (b + (U - 1) * NT < blocks) {
 #pragma unroll
-            for (int j = 0; j < U; ++j) r[j].load(body + 8 * (int64_t)(b + j * NT));
+            for (int j = 0; j < U; ++j) r[j].template load<STREAM>(body + E * (int64_t)(b + j * NT));
         } else {
 #pragma unroll
             for (int j = 0; j < U; ++j) {
                 r[j].fill(-INFINITY);
-                if (b + j * NT < blocks) r[j].load(body + 8 * (int64_t)(b + j * NT));
+                if (b + j * NT < blocks) r[j].template load<STREAM>(body + E * (int64_t)(b + j * NT));
             }
         }
     };
     auto take = [&](const auto &r, auto n) {       // the sums of n blocks; their maximum
-        float x[decltype(n)::value][8], top = -INFINITY;
+        float x[decltype(n)::value][E], top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < n; ++j) {
             r[j].unpack(x[j]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, x[j][i]);
+            for (int i = 0; i < E; ++i) top = fmaxf(top, x[j][i]);
         }
         if (top > q.m) q.move(top);
 #pragma unroll
         for (int j = 0; j < n; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q.add(x[j][i]);
+            for (int i = 0; i < E; ++i) q.add(x[j][i]);
         return top;
     };
     if constexpr (TOP) {
@@ -220,12 +262,12 @@ template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void lo
     int step = 0;
     for (int b = tid; b < blocks; b += NT * U, ++step) {
         float top;
-        Raw8<T> r[U];
+        LpBlock<T> r[U];
         if (b + NT < blocks) {
             load(r, b);
             top = take(r, std::integral_constant<int, U>{});
         } else {
-            r[0].load(body + 8 * (int64_t)b);
+            r[0].template load<STREAM>(body + E * (int64_t)b);
             top = take(r, std::integral_constant<int, 1>{});
         }
         if constexpr (TOP) {
@@ -298,14 +340,14 @@ template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void lo
             step = 0;
             for (int b = tid; b < blocks; b += NT * U, ++step) {
                 if (sh.step[step % kLpSlots][tid] < bound) continue;
-                Raw8<T> r[U];
+                LpBlock<T> r[U];
                 load(r, b);
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
-                    float x[8];
+                    float x[E];
                     r[j].unpack(x);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) put(x[i], lead + 8 * (b + j * NT) + i);
+                    for (int i = 0; i < E; ++i) put(x[i], lead + E * (b + j * NT) + i);
                 }
             }
             put(end, last);
@@ -352,25 +394,27 @@ struct LogprobBwd {
     const float *g_logprob, *g_entropy, *g_top;    // [N], [N], [N][n], or null
     void *dlogits;
     int64_t ld, ldd;
-    int V, n, parts, per;              // parts of a row, blocks of 8 in each
+    int V, n, parts, per;              // parts of a row, blocks of 16 bytes in each
 };
 
 // A workgroup writes a part of a row by the formula without its first two
 // terms, then the tokens that have one of them again, whole.
-template <typename T> __global__ __launch_bounds__(256) void logprobs_bwd_kernel(LogprobBwd a) {
+// SL, SS: loads and stores are streamed.
+template <typename T, bool SL, bool SS> __global__ __launch_bounds__(256) void logprobs_bwd_kernel(LogprobBwd a) {
+    constexpr int E = LpBlock<T>::E;
     const int64_t row = blockIdx.x / (uint32_t)a.parts;
     const int part = blockIdx.x % (uint32_t)a.parts, tid = threadIdx.x, lane = tid & 63;
-    const int blocks = a.V / 8, b1 = min(blocks, (part + 1) * a.per);
-    const int rest = part == a.parts - 1 ? a.V & 7 : 0, last = 8 * blocks + tid;
+    const int blocks = a.V / E, b1 = min(blocks, (part + 1) * a.per);
+    const int rest = part == a.parts - 1 ? a.V % E : 0, last = E * blocks + tid;
     const T *p = (const T *)a.logits + row * a.ld;
     T *d = (T *)a.dlogits + row * a.ldd;
     const int64_t t = a.tokens[row];
     const f32x4 st = a.stats[row];
     const float m = st.x, S = st.y, h = st.z;
     if (t < 0 || S == 0.f) {
-        Raw8<T> z;
+        LpBlock<T> z;
         z.fill(0.f);
-        for (int b = part * a.per + tid; b < b1; b += 256) z.store(d + 8 * b);
+        for (int b = part * a.per + tid; b < b1; b += 256) z.template store<SS>(d + E * b);
         if (tid < rest) Act<T>::store(d + last, 0.f);
         return;
     }
@@ -385,21 +429,21 @@ template <typename T> __global__ __launch_bounds__(256) void logprobs_bwd_kernel
         return -w * (G + gh * (fmaxf(t, -1000.f) + hs));
     };
     for (int b = part * a.per + tid; b < b1; b += 256) {
-        Raw8<T> r;
-        float x[8];
-        r.load(p + 8 * b);
+        LpBlock<T> r;
+        float x[E];
+        r.template load<SL>(p + E * b);
         r.unpack(x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = grad(x[i]);
+        for (int i = 0; i < E; ++i) x[i] = grad(x[i]);
         r.pack(x);
-        r.store(d + 8 * b);
+        r.template store<SS>(d + E * b);
     }
     if (tid < rest) Act<T>::store(d + last, grad(Act<T>::load(p + last)));
     __syncthreads();
     // the token's lane is n, the alternatives' 0 .. n - 1
     if (tid > a.n) return;
     const int64_t i = tid < a.n ? a.top_index[row * a.n + tid] : t;
-    const int64_t from = 8 * (int64_t)part * a.per, to = part == a.parts - 1 ? a.V : 8 * (int64_t)b1;
+    const int64_t from = E * (int64_t)part * a.per, to = part == a.parts - 1 ? a.V : E * (int64_t)b1;
     if (i < from || i >= to) return;
     float add = tid < a.n ? (a.g_top ? a.g_top[row * a.n + tid] : 0.f) : g;
     if (tid < a.n) {
@@ -415,11 +459,14 @@ template <typename T> static void logprobs_launch(const LogprobArgs &a, int64_t 
     auto go = [&](auto kernel, int nt) { launch(kernel, dim3((unsigned)N), dim3(nt), 0, s, a); };
     // four wavefronts to a row, or sixteen where there are few long ones
     if (N <= device_info().cu_count && a.V > 8192) {
-        if (a.n) go(logprobs_kernel<T, 1024, true>, 1024);
-        else go(logprobs_kernel<T, 1024, false>, 1024);
+        if (a.n) go(logprobs_kernel<T, 1024, true, false>, 1024);
+        else go(logprobs_kernel<T, 1024, false, false>, 1024);
+    } else if (a.n) {                              // (reads some of them again)
+        go(logprobs_kernel<T, 256, true, false>, 256);
+    } else if (!a.stats && N * a.V * (int64_t)sizeof(T) > kLpCache) {
+        go(logprobs_kernel<T, 256, false, true>, 256);
     } else {
-        if (a.n) go(logprobs_kernel<T, 256, true>, 256);
-        else go(logprobs_kernel<T, 256, false>, 256);
+        go(logprobs_kernel<T, 256, false, false>, 256);
     }
 }
 
@@ -462,13 +509,20 @@ WALSH_EXPORT int walsh_token_logprobs_bwd(const void *logits, int64_t ld, int64_
     if (N == 0) return WALSH_OK;
     if (!logits || !tokens || !stats || !dlogits || (n && !top_index)) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
     if ((uintptr_t)stats % 16) return set_error(WALSH_EINVAL, "%s: stats 16-byte aligned", fn);
-    const int64_t blocks = V / 8, parts = blocks ? ceil_div(blocks, 1024) : 1, per = ceil_div(blocks, parts);
+    const int64_t blocks = V / (dtype == WALSH_BF16 ? 8 : 4), parts = blocks ? ceil_div(blocks, 1024) : 1, per = ceil_div(blocks, parts);
     if (N * parts > 0xffffffffll / 256)
         return set_error(WALSH_ENOTSUP, "%s: N=%lld rows of V=%lld", fn, (long long)N, (long long)V);
     const LogprobBwd a{logits, tokens, top_index, (const f32x4 *)stats, g_logprob, g_entropy, n ? g_top : nullptr, dlogits,
                        ld, ldd, (int)V, (int)n, (int)parts, (int)per};
-    const dim3 G((unsigned)(N * parts)), B(256);
-    if (dtype == WALSH_BF16) launch(logprobs_bwd_kernel<uint16_t>, G, B, 0, (hipStream_t)stream, a);
-    else launch(logprobs_bwd_kernel<float>, G, B, 0, (hipStream_t)stream, a);
+    auto go = [&](auto kernel) { launch(kernel, dim3((unsigned)(N * parts)), dim3(256), 0, (hipStream_t)stream, a); };
+    auto pick = [&](auto t) {
+        using T = decltype(t);
+        const int64_t bytes = N * V * (int64_t)sizeof(T);
+        if (bytes > kLpCache) go(logprobs_bwd_kernel<T, true, true>);
+        else if (2 * bytes > kLpCache) go(logprobs_bwd_kernel<T, false, true>);
+        else go(logprobs_bwd_kernel<T, false, false>);
+    };
+    if (dtype == WALSH_BF16) pick(uint16_t{});
+    else pick(float{});
     return check_hip(hipGetLastError(), fn);
 }
