@@ -16,10 +16,10 @@
 //          sorted order is, every 32 places (embed_most), and their pieces summed
 //          into a workspace.
 //   join   adds the pieces of each long row, in a fixed order.
-// Bound by memory: 50,257 x 4,096 bf16 from 16,384 rows (546 MB) take 111 us for
-// the rows, 4.9 TB/s, x 512 float32 from 8,192 (120 MB) 22 us, of 128 and 33 in
+// Bound by memory: 50,257 x 4,096 bf16 from 16,384 rows (546 MB) take 91 us for
+// the rows, 6.0 TB/s, x 512 float32 from 8,192 (120 MB) 18 us, of 107 and 28 in
 // all; a character model's 65 x 768 from 16,384 rows 22 us, all of it latency.
-// The lookup of 16,384 x 4,096 takes 41 us, of 64 rows 2.9.
+// The lookup of 16,384 x 4,096 takes 34 us, of 64 rows 2.9.
 #include <type_traits>
 
 #include "rows8.h"
@@ -39,6 +39,8 @@ struct EmbedArgs {
     float f;
 };
 
+// Stores of bf16 are streamed, as in dropout (lookup and gradient of 16,384 x
+// 4,096 one after the other 142 us instead of 160).
 template <typename TW, typename TY, bool DROP, int U>
 __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs a) {
     const uint32_t first = blockIdx.x * (256u * U);
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs a) {
             if (DROP && (uint64_t)t[j] < (uint64_t)a.V) bits.apply(v[j], at[j].row, at[j].col);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[j][i] *= a.f;
-            store8((TY *)a.y + at[j].row * a.ldy + c, a.C - c, v[j]);
+            store8<true>((TY *)a.y + at[j].row * a.ldy + c, a.C - c, v[j]);
         }
     }
 }
@@ -239,7 +241,7 @@ struct EmbedBwd {
     int64_t V, ldg, ldw;
     int pad;                           // a row that stays zeros (-1: none)
     int C, most;                       // most: tokens of a row that one lane adds, places of a chunk
-    Blocks rows, places, chunks;       // rows of dW, places of the sorted order, chunks of those
+    Blocks rows, places, chunks;       // rows of dW (16 bytes), places of the sorted order, chunks of those
     uint32_t chunk_groups, head_groups;
     Drop d;
     float f;
@@ -266,7 +268,7 @@ __device__ __forceinline__ void embed_add(const EmbedBwd &a, const DropBits &bit
         if (a.C - c >= 8) {
             Raw8<TG> raw[U];
 #pragma unroll
-            for (int j = 0; j < U; ++j) raw[j].load(g + now[j] * a.ldg);
+            for (int j = 0; j < U; ++j) raw[j].template load<false>(g + now[j] * a.ldg);
 #pragma unroll
             for (int j = 0; j < U; ++j) r[j] = a.order[min(k + U + j, e - 1)];
 #pragma unroll
@@ -294,8 +296,12 @@ __device__ __forceinline__ void embed_add(const EmbedBwd &a, const DropBits &bit
 //   chunks  the pieces of long rows
 //   heads   the rows of tokens that occur, at the first place of each in the
 //           sorted order: U blocks of a lane, their first tokens' rows loaded together
-//   rest    zeros in the rows of those that do not: F blocks of a lane
-template <typename TG, typename TW, bool DROP, int U, int F> __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedBwd a) {
+//   rest    zeros in the rows of those that do not: F blocks of 16 bytes of a lane
+// SS: stores are streamed, of a gradient that the caches do not hold (50,257 x
+// 4,096 bf16: 107 us instead of 129 in all, x 2,048 float32 100 instead of 132;
+// with a pass over the gradient and the weights behind it 378 and 376 instead of
+// 390 and 399).
+template <typename TG, typename TW, bool DROP, int U, int F, bool SS> __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedBwd a) {
     const DropBits bits(a.d);
     const int all = a.start[a.V];
     if (blockIdx.x < a.chunk_groups) {
@@ -350,12 +356,12 @@ template <typename TG, typename TW, bool DROP, int U, int F> __global__ __launch
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[j][i] *= a.f;
-            store8((TW *)a.dw + t[j] * a.ldw + c, a.C - c, v[j]);
+            store8<SS>((TW *)a.dw + t[j] * a.ldw + c, a.C - c, v[j]);
         }
     } else {
+        constexpr int E = 16 / sizeof(TW);
         BlockAt at[F];
         bool none[F];
-        const float zero[8] = {};
 #pragma unroll
         for (int j = 0; j < F; ++j) {
             at[j] = block_at(a.rows, (blockIdx.x - a.chunk_groups - a.head_groups) * (256u * F), 256u * j + threadIdx.x);
@@ -365,8 +371,14 @@ template <typename TG, typename TW, bool DROP, int U, int F> __global__ __launch
         }
 #pragma unroll
         for (int j = 0; j < F; ++j) {
-            const int c = 8 * (int)at[j].col;
-            if (none[j]) store8((TW *)a.dw + at[j].row * a.ldw + c, a.C - c, zero);
+            const int c = E * (int)at[j].col;
+            TW *p = (TW *)a.dw + at[j].row * a.ldw + c;
+            if (!none[j]) continue;
+            if (a.C - c >= E) {
+                store16<SS>(p, u32x4{0, 0, 0, 0});
+            } else {
+                for (int i = 0; i < a.C - c; ++i) p[i] = 0;
+            }
         }
     }
 }
@@ -486,7 +498,7 @@ WALSH_EXPORT int walsh_embedding_bwd(const int64_t *tokens, int64_t N, const voi
     int rc = embed_check(fn, N, V, C, drop, seed, rng_stream, gdtype, wdtype);
     if (rc) return rc;
     if (C == 0) return WALSH_OK;
-    const Blocks rows = make_blocks(V, C), chunks = make_blocks(embed_chunks(N, C), C);
+    const Blocks rows = make_blocks(V, wdtype == WALSH_BF16 ? C : 2 * C), chunks = make_blocks(embed_chunks(N, C), C);
     if (V * (int64_t)rows.per_row > kMaxBlocks)
         return set_error(WALSH_ENOTSUP, "%s: V=%lld rows of C=%lld", fn, (long long)V, (long long)C);
     if ((N && (!tokens || !gy)) || !dw || !work) return set_error(WALSH_EINVAL, "%s: null pointer", fn);
@@ -507,7 +519,7 @@ WALSH_EXPORT int walsh_embedding_bwd(const int64_t *tokens, int64_t N, const voi
     rc = check_hip(hipGetLastError(), fn);
     if (rc) return rc;
     constexpr int U = 1, F = 4;
-    const uint32_t head_groups = (uint32_t)ceil_div(N * rows.per_row, 256 * U);
+    const uint32_t head_groups = (uint32_t)ceil_div(N * chunks.per_row, 256 * U);
     const uint32_t rest_groups = (uint32_t)ceil_div(V * rows.per_row, 256 * F);
     const int64_t most = embed_most(N, C);         // (up to so many tokens no row is long)
     const uint32_t chunk_groups = N > most ? (uint32_t)ceil_div((int64_t)chunks.rows * chunks.per_row, 256) : 0;
@@ -516,8 +528,11 @@ WALSH_EXPORT int walsh_embedding_bwd(const int64_t *tokens, int64_t N, const voi
                      chunks, chunk_groups, head_groups, Drop{(const uint64_t *)seed, (uint32_t)rng_stream, (uint32_t)drop},
                      (float)((double)scale * kept_factor(drop))};
     embed_types(gdtype, wdtype, drop, [&](auto g, auto w, auto d) {
-        launch(embed_rows_kernel<decltype(g), decltype(w), decltype(d)::value, U, F>,
-               dim3(chunk_groups + head_groups + rest_groups), dim3(256), 0, s, a);
+        const dim3 G(chunk_groups + head_groups + rest_groups), B(256);
+        if (V * C * (int64_t)sizeof(w) >= kCacheBytes)
+            launch(embed_rows_kernel<decltype(g), decltype(w), decltype(d)::value, U, F, true>, G, B, 0, s, a);
+        else
+            launch(embed_rows_kernel<decltype(g), decltype(w), decltype(d)::value, U, F, false>, G, B, 0, s, a);
     });
     rc = check_hip(hipGetLastError(), fn);
     if (rc || !chunk_groups) return rc;

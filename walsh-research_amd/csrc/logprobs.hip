@@ -27,7 +27,7 @@
 // walked once for every alternative instead.
 //
 // Bound by memory: 8,192 rows of 50,257 bf16 logits take 129 us (6.4 TB/s), with
-// 5 and 20 alternatives 166 and 187, with float32 logits 257 (6.4), 275, 283.
+// 5 and 20 alternatives 152 and 172, with float32 logits 257 (6.4), 268, 303.
 // Of 10 instructions a token the exponential takes the time of four.  Their
 // gradient, 823 MB read and as many written, takes 292 us (5.6 TB/s), in
 // float32 582 (5.7, where a copy reaches 5.1).
@@ -42,27 +42,21 @@ constexpr int kLpList = 1024;
 constexpr float kLpLowest = -3.402823466e38f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// Bytes that the memory side's cache holds.  What is read or written once and
-// is more than that is streamed past the caches: 823 MB of bf16 logits are read
-// in 129 us instead of 142, and with a gradient to come, whose kernel finds the
-// last of them there, forward and gradient take 414 us instead of 446 (float32
-// 828, 896), with the product that reads the gradient 987 instead of 996.  A
-// gradient that fits beside its logits is better left there (8,192 x 4,096: 42
-// us, streamed 44), one that does not is streamed (2,048 rows: 97 us, not 109).
-constexpr int64_t kLpCache = 256 << 20;
-
-// 16 bytes of logits, at any element alignment.  STREAM: not kept in caches.
-typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+// 16 bytes of logits.  What is read or written once and is more than the caches
+// hold is streamed: 823 MB of bf16 logits are read in 129 us instead of 142, and
+// with a gradient to come, whose kernel finds the last of them there, forward
+// and gradient take 414 us instead of 446 (float32 828, 896), with the product
+// that reads the gradient 987 instead of 996.  A gradient that fits beside its
+// logits is better left there (8,192 x 4,096: 42 us, streamed 44), one that does
+// not is streamed (2,048 rows: 97 us, not 109).
 template <typename T> struct LpBlock {
     static constexpr int E = 16 / sizeof(T);
     u32x4 a;
     template <bool STREAM> __device__ __forceinline__ void load(const T *p) {
-        if (STREAM) a = __builtin_nontemporal_load((const u32x4_any *)p);
-        else a = *(const u32x4_any *)p;
+        a = load16<STREAM>(p);
     }
     template <bool STREAM> __device__ __forceinline__ void store(T *p) const {
-        if (STREAM) __builtin_nontemporal_store(a, (u32x4_any *)p);
-        else *(u32x4_any *)p = a;
+        store16<STREAM>(p, a);
     }
     __device__ __forceinline__ void unpack(float (&v)[E]) const {
 #pragma unroll
@@ -461,12 +455,12 @@ template <typename T> static void logprobs_launch(const LogprobArgs &a, int64_t 
     if (N <= device_info().cu_count && a.V > 8192) {
         if (a.n) go(logprobs_kernel<T, 1024, true, false>, 1024);
         else go(logprobs_kernel<T, 1024, false, false>, 1024);
-    } else if (a.n) {                              // (reads some of them again)
-        go(logprobs_kernel<T, 256, true, false>, 256);
-    } else if (!a.stats && N * a.V * (int64_t)sizeof(T) > kLpCache) {
-        go(logprobs_kernel<T, 256, false, true>, 256);
+    } else if (!a.stats && N * a.V * (int64_t)sizeof(T) > kCacheBytes) {
+        if (a.n) go(logprobs_kernel<T, 256, true, true>, 256);
+        else go(logprobs_kernel<T, 256, false, true>, 256);
     } else {
-        go(logprobs_kernel<T, 256, false, false>, 256);
+        if (a.n) go(logprobs_kernel<T, 256, true, false>, 256);
+        else go(logprobs_kernel<T, 256, false, false>, 256);
     }
 }
 
@@ -518,8 +512,8 @@ WALSH_EXPORT int walsh_token_logprobs_bwd(const void *logits, int64_t ld, int64_
     auto pick = [&](auto t) {
         using T = decltype(t);
         const int64_t bytes = N * V * (int64_t)sizeof(T);
-        if (bytes > kLpCache) go(logprobs_bwd_kernel<T, true, true>);
-        else if (2 * bytes > kLpCache) go(logprobs_bwd_kernel<T, false, true>);
+        if (bytes > kCacheBytes) go(logprobs_bwd_kernel<T, true, true>);
+        else if (2 * bytes > kCacheBytes) go(logprobs_bwd_kernel<T, false, true>);
         else go(logprobs_bwd_kernel<T, false, false>);
     };
     if (dtype == WALSH_BF16) pick(uint16_t{});

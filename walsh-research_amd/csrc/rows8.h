@@ -7,13 +7,29 @@
 namespace walsh {
 
 // ---------------------------------------------------------------- 8 values
-// As they lie in memory, at any element alignment (the hardware takes 16-byte
-// accesses at any address).
+// Bytes that the memory side's cache holds.
+constexpr int64_t kCacheBytes = 256 << 20;
+
+// 16 bytes at any element alignment (the hardware takes them at any address).
+// STREAM: past the caches, for what is touched once and is more than they hold.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+template <bool STREAM> __device__ __forceinline__ u32x4 load16(const void *p) {
+    if (STREAM) return __builtin_nontemporal_load((const u32x4_any *)p);
+    return *(const u32x4_any *)p;
+}
+template <bool STREAM> __device__ __forceinline__ void store16(void *p, u32x4 v) {
+    if (STREAM) __builtin_nontemporal_store(v, (u32x4_any *)p);
+    else *(u32x4_any *)p = v;
+}
+
+// Values as they lie in memory.  Of float32 a lane's 32 bytes are two accesses,
+// each half of what a line holds: streamed, lines go out in halves (a gradient
+// of 50,257 x 512 takes 49 us instead of 32), so they never are.
 template <typename T> struct Raw8;
 template <> struct Raw8<uint16_t> {
     u32x4 a;
-    __device__ __forceinline__ void load(const uint16_t *p) { __builtin_memcpy(&a, p, 16); }
-    __device__ __forceinline__ void store(uint16_t *p) const { __builtin_memcpy(p, &a, 16); }
+    template <bool STREAM> __device__ __forceinline__ void load(const uint16_t *p) { a = load16<STREAM>(p); }
+    template <bool STREAM> __device__ __forceinline__ void store(uint16_t *p) const { store16<STREAM>(p, a); }
     __device__ __forceinline__ void unpack(float (&v)[8]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -25,41 +41,36 @@ template <> struct Raw8<uint16_t> {
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
     }
-    __device__ __forceinline__ void fill(float v) {
-        const uint32_t w = pack_bf16x2(v, v);
-        a = u32x4{w, w, w, w};
-    }
 };
 template <> struct Raw8<float> {
-    f32x4 a, b;
-    __device__ __forceinline__ void load(const float *p) { __builtin_memcpy(&a, p, 16), __builtin_memcpy(&b, p + 4, 16); }
-    __device__ __forceinline__ void store(float *p) const { __builtin_memcpy(p, &a, 16), __builtin_memcpy(p + 4, &b, 16); }
+    u32x4 a, b;
+    template <bool> __device__ __forceinline__ void load(const float *p) { a = load16<false>(p), b = load16<false>(p + 4); }
+    template <bool> __device__ __forceinline__ void store(float *p) const { store16<false>(p, a), store16<false>(p + 4, b); }
     __device__ __forceinline__ void unpack(float (&v)[8]) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(a[i]), v[4 + i] = __uint_as_float(b[i]);
     }
     __device__ __forceinline__ void pack(const float (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = v[i], b[i] = v[4 + i];
+        for (int i = 0; i < 4; ++i) a[i] = __float_as_uint(v[i]), b[i] = __float_as_uint(v[4 + i]);
     }
-    __device__ __forceinline__ void fill(float v) { a = b = f32x4{v, v, v, v}; }
 };
 // The first n of 8 values, 0 behind them; and back.
-template <typename T> __device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) {
+template <bool STREAM = false, typename T> __device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) {
     if (n >= 8) {
         Raw8<T> r;
-        r.load(p);
+        r.template load<STREAM>(p);
         r.unpack(v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i < n ? Act<T>::load(p + i) : 0.f;
     }
 }
-template <typename T> __device__ __forceinline__ void store8(T *p, int n, const float (&v)[8]) {
+template <bool STREAM = false, typename T> __device__ __forceinline__ void store8(T *p, int n, const float (&v)[8]) {
     if (n >= 8) {
         Raw8<T> r;
         r.pack(v);
-        r.store(p);
+        r.template store<STREAM>(p);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
