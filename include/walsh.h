@@ -912,7 +912,7 @@ int walsh_token_logprobs_bwd(const void *logits, int64_t ld, int64_t N, int64_t 
  * walsh_dropout: y = dropout(x) (+ residual), rows of C with strides ldx, ldr,
  *   ldy.  ydtype is float32 where x or the residual is, except that without a
  *   residual float32 x may give bf16 y: dx = dropout(dy).  What is dropped is
- *   0 whatever x holds.  y may be x or the residual itself.
+ *   0 whatever x holds.  y may be x or the residual itself, in its layout and type.
  * walsh_embedding_fwd: y[r] = dropout(scale weight[tokens[r]]), N rows of C;
  *   rows of NaN for tokens outside 0 .. V - 1.
  * walsh_embedding_bwd: dw[v] = scale times the sum, over the r with tokens[r] =
@@ -921,7 +921,8 @@ int walsh_token_logprobs_bwd(const void *logits, int64_t ld, int64_t N, int64_t 
  *   order (deterministic).  Needs work of
  *   walsh_embedding_bwd_workspace_bytes(N, V, C) bytes, 16-byte aligned.
  * Each takes fewer than 2^31 - 65536 blocks of 8 columns (a row's last may be
- *   part of one), rows at any alignment of their elements. */
+ *   part of one; of dw in float32 blocks of 4), the embedding fewer than 2^28
+ *   tokens, rows at any alignment of their elements. */
 int walsh_dropout(const void *x, int64_t ldx, int xdtype, const void *residual, int64_t ldr, int rdtype, int64_t M,
                   int64_t C, int drop, const int64_t *seed, int64_t rng_stream, void *y, int64_t ldy, int ydtype,
                   void *stream);

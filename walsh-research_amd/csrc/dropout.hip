@@ -5,8 +5,8 @@
 // residual, its bits computed again.  What is dropped is 0 whatever x holds.
 //
 // A lane takes two blocks of 8 columns, whose loads go out together.  Bound by
-// memory: 8,192 x 4,096 bf16 with a residual (201 MB) 36 us, its gradient (134)
-// 26 us; the bits are 20 multiply-adds of 64 bits for 8 elements, 15
+// memory: 8,192 x 4,096 bf16 with a residual (201 MB) 32 us, its gradient (134)
+// 23 us; the bits are 19 multiply-adds of 64 bits for 8 elements, 13
 // instructions' time an element where a bf16 copy leaves 31.
 #include <type_traits>
 

@@ -18,7 +18,7 @@
 //   join   adds the pieces of each long row, in a fixed order.
 // Bound by memory: 50,257 x 4,096 bf16 from 16,384 rows (546 MB) take 91 us for
 // the rows, 6.0 TB/s, x 512 float32 from 8,192 (120 MB) 18 us, of 107 and 28 in
-// all; a character model's 65 x 768 from 16,384 rows 22 us, all of it latency.
+// all; a character model's 65 x 768 from 16,384 rows 21 us, all of it latency.
 // The lookup of 16,384 x 4,096 takes 34 us, of 64 rows 2.9.
 #include <type_traits>
 

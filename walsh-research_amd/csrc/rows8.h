@@ -117,6 +117,9 @@ struct Drop {
     const uint64_t *seed;
     uint32_t stream, drop;             // dropped where the 16 bits are below `drop` (0: nothing is)
 };
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+    return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);             // (written out it is two instructions)
+}
 struct DropBits {
     uint32_t k0, k1, stream, drop;
     __device__ __forceinline__ explicit DropBits(const Drop &d) : k0(0), k1(0), stream(d.stream), drop(d.drop) {
@@ -131,8 +134,8 @@ struct DropBits {
 #pragma unroll
         for (int i = 0; i < 10; ++i) {
             const uint64_t p = (uint64_t)c0 * 0xD2511F53u, q = (uint64_t)c2 * 0xCD9E8D57u;
-            c0 = (uint32_t)(q >> 32) ^ c1 ^ a, c1 = (uint32_t)q;
-            c2 = (uint32_t)(p >> 32) ^ c3 ^ b, c3 = (uint32_t)p;
+            c0 = xor3((uint32_t)(q >> 32), c1, a), c1 = (uint32_t)q;
+            c2 = xor3((uint32_t)(p >> 32), c3, b), c3 = (uint32_t)p;
             a += 0x9E3779B9u, b += 0xBB67AE85u;
         }
         const uint32_t w[4] = {c0, c1, c2, c3};
