@@ -120,6 +120,31 @@ def test_equal_and_ordered(V, dtype):
         check(z, t, n, run(z, t, n), V)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [100, 4099, 50257])
+def test_few_tokens_allowed(V, dtype):
+    """Rows that a grammar has masked, by -inf and by the type's lowest value:
+    fewer tokens left than alternatives are asked for, or all left side by side;
+    and values that no usual logit has below them."""
+    g = torch.Generator().manual_seed(V)
+    low = torch.finfo(dtype).min
+    z = torch.full((9, V), -INF)
+    z[:, torch.randperm(V, generator=g)[:3]] = torch.tensor([1.0, -2.0, 1.0])
+    z[1][z[1] == -INF] = low
+    z[2, :90] = torch.randn(90, generator=g)
+    z[3, V - 64:] = torch.randn(64, generator=g)
+    z[4, 10:14] = torch.tensor([-1e35, -2e35, -1e35, -1e30])
+    z[5, 20:80] = low
+    z[6] = -INF
+    z[6, V // 2] = 0.0
+    z[7, ::2] = -1e30
+    z[8, 1::3] = NAN
+    z = z.to(dtype)
+    t = z.float().nan_to_num(-INF).argmax(-1)
+    for n in (1, 3, 4, 20, 64):
+        check(z, t, n, run(z, t, n), V)
+
+
 def test_layouts():
     """Rows of a wider matrix, at odd addresses, transposed, expanded, with
     several leading dimensions; tokens and outputs keep theirs."""

@@ -23,8 +23,8 @@
 // at least n of them reach and few more, so at least n tokens do; lanes whose
 // own maximum does read again those of their steps whose maximum does.  Those
 // tokens go to a list in LDS and are ranked there by value and index.  Where
-// there are too many (thousands of equal ones) or a group has none, the row is
-// walked once for every alternative instead.
+// there are too many (thousands of equal ones), or fewer are not masked than are
+// asked for, the row is walked once for each further value.
 //
 // Bound by memory: 8,192 rows of 50,257 bf16 logits take 129 us (6.4 TB/s), with
 // 5 and 20 alternatives 152 and 172, with float32 logits 257 (6.4), 268, 303.
@@ -168,16 +168,13 @@ __device__ __forceinline__ float lp_value(uint64_t key) {
     const uint32_t b = (uint32_t)(key >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
-__device__ __forceinline__ uint64_t lp_xor(uint64_t v, int o) {
-    return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, o);
-}
-
 constexpr int kLpSlots = 16;           // of the steps' maxima
 template <int NT, bool TOP> struct LpShared {
     f32x4 part[NT / 64];
     float step[TOP ? kLpSlots : 1][NT];            // a lane's largest of steps i, i + kLpSlots ...
     float group[TOP ? NT / 64 : 1][64];
-    uint64_t list[TOP ? kLpList : 1], best[NT / 64];
+    uint64_t list[TOP ? kLpList : 1];
+    uint32_t most[NT / 64], many[NT / 64], first[NT / 64];
     int n;
 };
 
@@ -322,61 +319,105 @@ template <typename T, int NT, bool TOP, bool STREAM> __global__ __launch_bounds_
         if (c >= a.n) lo = mid, reach = c;
         else hi = mid;
     }
+    // (what lies at -1e30 or below is taken from the whole row, further down)
+    lo = max(lo, lp_order(-1e30f) + 1);
     const float bound = lp_value((uint64_t)lo << 32);
-    if (bound > -1e30f) {
-        auto put = [&](float x, int i) {
-            if (x >= bound) {
-                const int at = atomicAdd(&sh.n, 1);
-                if (at < kLpList) sh.list[at] = lp_key(x, i);
-            }
-        };
-        if (own >= bound) {
-            step = 0;
-            for (int b = tid; b < blocks; b += NT * U, ++step) {
-                if (sh.step[step % kLpSlots][tid] < bound) continue;
-                LpBlock<T> r[U];
-                load(r, b);
-#pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    float x[E];
-                    r[j].unpack(x);
-#pragma unroll
-                    for (int i = 0; i < E; ++i) put(x[i], lead + E * (b + j * NT) + i);
-                }
-            }
-            put(end, last);
+    auto put = [&](float x, int i) {
+        if (x >= bound) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < kLpList) sh.list[at] = lp_key(x, i);
         }
-        __syncthreads();
-        const int count = sh.n;
-        if (count <= kLpList) {
-            for (int i = tid; i < count; i += NT) {
-                const uint64_t k = sh.list[i];
-                int before = 0;
-                for (int j = 0; j < count; ++j) before += sh.list[j] > k;
-                if (before < a.n) top[before] = logprob(lp_value(k)), index[before] = (int64_t)(uint32_t)~(uint32_t)k;
+    };
+    if (own >= bound) {
+        step = 0;
+        for (int b = tid; b < blocks; b += NT * U, ++step) {
+            if (sh.step[step % kLpSlots][tid] < bound) continue;
+            LpBlock<T> r[U];
+            load(r, b);
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                float x[E];
+                r[j].unpack(x);
+#pragma unroll
+                for (int i = 0; i < E; ++i) put(x[i], lead + E * (b + j * NT) + i);
             }
-            return;
         }
+        put(end, last);
     }
-    uint64_t prev = ~0ull;
-    for (int j = 0; j < a.n; ++j) {
-        uint64_t k = 0;
-        for (int i = tid; i < a.V; i += NT) {
-            const uint64_t c = lp_key(Act<T>::load(p + i), i);
-            if (c < prev && c > k) k = c;
+    __syncthreads();
+    int got = 0;
+    uint32_t below = 0xffffffffu;      // tokens of lower order are still to be looked at
+    if (sh.n <= kLpList) {
+        const int count = sh.n;
+        for (int i = tid; i < count; i += NT) {
+            const uint64_t k = sh.list[i];
+            int before = 0;
+            for (int j = 0; j < count; ++j) before += sh.list[j] > k;
+            if (before < a.n) top[before] = logprob(lp_value(k)), index[before] = (int64_t)(uint32_t)~(uint32_t)k;
         }
+        got = min(count, a.n), below = lo;
+    }
+    // too many for the list, or fewer than asked for: one value after the other,
+    // each with as many of its tokens as are wanted, the lowest first
+    while (got < a.n) {
+        uint32_t most = 0, n = 0, at = 0;          // the lane's largest, how many, the first
+        auto look = [&](float x, int i) {
+            const uint32_t k = lp_order(x);
+            if (k >= below || k < most) return;
+            n = k > most ? 1 : n + 1;
+            at = k > most ? i : min(at, (uint32_t)i);
+            most = k;
+        };
+        for (int b = tid; b < blocks; b += NT) {
+            LpBlock<T> r;
+            float x[E];
+            r.template load<STREAM>(body + E * (int64_t)b);
+            r.unpack(x);
+#pragma unroll
+            for (int i = 0; i < E; ++i) look(x[i], lead + E * b + i);
+        }
+        if (tid < rest + lead) look(end, last);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t c = lp_xor(k, o);
-            if (c > k) k = c;
+            const uint32_t k = (uint32_t)__shfl_xor((int)most, o), c = (uint32_t)__shfl_xor((int)n, o);
+            const uint32_t i = (uint32_t)__shfl_xor((int)at, o);
+            at = k > most ? i : k < most ? at : min(at, i);
+            n = k > most ? c : k < most ? n : n + c;
+            most = max(most, k);
         }
         __syncthreads();
-        if (lane == 0) sh.best[wave] = k;
+        if (lane == 0) sh.most[wave] = most, sh.many[wave] = n, sh.first[wave] = at;
         __syncthreads();
-        prev = sh.best[0];
-        for (int w = 1; w < W; ++w)
-            if (sh.best[w] > prev) prev = sh.best[w];
-        if (tid == 0) top[j] = logprob(lp_value(prev)), index[j] = (int64_t)(uint32_t)~(uint32_t)prev;
+        most = n = at = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const uint32_t k = sh.most[w];
+            at = k > most ? sh.first[w] : k < most ? at : min(at, sh.first[w]);
+            n = k > most ? sh.many[w] : k < most ? n : n + sh.many[w];
+            most = max(most, k);
+        }
+        if (!n) break;
+        const int want = min((int)n, a.n - got);
+        const float v = logprob(lp_value((uint64_t)most << 32));
+        if (want == 1) {
+            if (tid == 0) top[got] = v, index[got] = at;
+        } else {
+            for (int base = (int)at, found = 0; found < want && base < a.V; base += NT) {
+                const int i = base + tid;
+                const bool is = i < a.V && lp_order(Act<T>::load(p + i)) == most;
+                const uint64_t who = __ballot(is);
+                __syncthreads();
+                if (lane == 0) sh.many[wave] = (uint32_t)__popcll(who);
+                __syncthreads();
+                int before = found + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+                for (int w = 0; w < W; ++w) {
+                    if (w < wave) before += (int)sh.many[w];
+                    found += (int)sh.many[w];
+                }
+                if (is && before < want) top[got + before] = v, index[got + before] = i;
+            }
+        }
+        got += want, below = most;
     }
 }
 

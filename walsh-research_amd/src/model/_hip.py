@@ -263,7 +263,7 @@ def on_device(index: int, fn, *args):
 
 
 # (bound once: every launch asks these)
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_current_device, _raw_stream = (getattr(torch._C, n, None) for n in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 
 
 def call_on(index: int, name: str, *args, **kw) -> None:
