@@ -67,6 +67,27 @@ def test_ends_of_the_range():
     assert counter_dropout(x[:0], 0.5, s).shape == (0, 40) and counter_dropout(x[:, :0], 0.5, s).shape == (50, 0)
 
 
+@pytest.mark.parametrize("seed,stream", [(-5, 2 ** 32 - 1), (-(2 ** 63), 0), (2 ** 63 - 1, 1), (0, 0)])
+def test_every_seed_is_one(seed, stream):
+    from src.model import counter_dropout
+    y = counter_dropout(torch.ones(33, 50, device="cuda"), 0.5, seed_of(seed), stream)
+    assert np.array_equal((y != 0).cpu().numpy(), otok.kept(33, 50, 32768, seed % 2 ** 64, stream))
+
+
+def test_tensors_past_the_caches():
+    """bf16 rows of more than 256 MB, whose loads are streamed, at an odd width."""
+    from src.model import counter_dropout
+    M, C = 70003, 2001
+    g = torch.Generator("cuda").manual_seed(1)
+    x, r = (torch.empty(M, C, device="cuda", dtype=BF16).normal_(generator=g) for _ in range(2))
+    y = counter_dropout(x, 0.25, seed_of(6), 3, r)
+    for at in (0, 1, 35001, M - 2, M - 1):
+        keep = otok.kept(1, C, 16384, 6, 3, first=at)[0]
+        d = np.where(keep, x[at].double().cpu().numpy() * (65536 / 49152), 0)
+        want = d + r[at].double().cpu().numpy()
+        close(y[at], want, np.abs(d) + np.abs(want - d), BF16)
+
+
 def test_layouts():
     """Strided, transposed and expanded rows, odd addresses, several leading
     dimensions, one: the mask goes by row and column, not by address."""

@@ -174,6 +174,30 @@ def test_rows_past_2_31_elements():
     assert d[-1].eq(6).all() and not d[-3:-1].any() and not d[1::4096].any()
 
 
+@pytest.mark.parametrize("dtype,C", [(BF16, 2001), (F32, 1001), (BF16, 4096)])
+def test_gradients_past_the_caches(dtype, C):
+    """Weights of more than 256 MB, whose gradient is streamed, at odd widths:
+    rows that occur once, often and not at all."""
+    from src.model import kernels
+    V, N = 70001, 3000
+    g = torch.Generator().manual_seed(C)
+    t = torch.cat([torch.randint(V, (N - 700,), generator=g), torch.full((600,), V - 1), torch.arange(100)])
+    gy = torch.randn(N, C, generator=g).to(dtype)
+    d = kernels.embedding_bwd(t.cuda(), gy.cuda(), V, 0.5, padding_idx=7)
+    rows = torch.unique(t)
+    some = rows[torch.randperm(len(rows), generator=g)[:40]].tolist() + [V - 1, 7, 0, 99]
+    for v in some:
+        mine = gy[t == v].double() * 0.5
+        want, size = mine.sum(0), mine.abs().sum(0)
+        if v == 7:
+            want = size = torch.zeros(C, dtype=torch.float64)
+        bound = (len(mine) + 3) * 2.0 ** -24 * size + torch.finfo(dtype).eps / 2 * want.abs()
+        assert ((d[v].double().cpu() - want).abs() <= bound).all(), v
+    none = torch.ones(V, dtype=torch.bool)
+    none[rows] = False
+    assert not d[none.cuda()].any()
+
+
 def test_streams_and_graphs():
     """Captured with the seed and tokens in place and replayed with others; two
     backward passes on two streams have a workspace each."""

@@ -101,6 +101,32 @@ def test_training_agrees_with_the_torch_forms(kind, monkeypatch):
         assert (x - y).norm() <= 1e-3 * y.norm() + 1e-6
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(use_moe=True), dict(use_channel_mod=True), dict(algebra="octonion"),
+                                dict(attn_window=8, attn_sinks=2)])
+@pytest.mark.parametrize("kind", MODELS)
+def test_every_kind_of_layer_trains_with_dropout(kind, kw):
+    """Under bf16 autocast: finite losses and gradients that the same generator
+    state gives again."""
+    import src.model as S
+    torch.manual_seed(0)
+    cfg = S.WalshConfig(**{**dict(block_size=64, vocab_size=97, n_layer=2, n_head=8, n_embd=128, algebra="hadamard",
+                                  embed_dropout=0.1, resid_dropout=0.1, embed_scale=4.0), **kw})
+    m = getattr(S, kind)(cfg).cuda().train()
+    idx = texts(2, 24)
+
+    def step():
+        torch.manual_seed(4)
+        m.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", torch.bfloat16):
+            loss = m(idx, texts(2, 24, 2))[1] - m.score(idx).logprob.mean()
+        loss.backward()
+        return loss.detach(), [p.grad.clone() for p in m.parameters() if p.grad is not None]
+    (l0, g0), (l1, g1) = step(), step()
+    assert l0.isfinite() and torch.equal(l0, l1) and all(x.isfinite().all() for x in g0)
+    # (atomics of torch's own operations aside)
+    assert all((x - y).norm() <= 1e-2 * x.norm() + 1e-6 for x, y in zip(g0, g1))
+
+
 @pytest.mark.parametrize("kind", MODELS)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_score(kind, dtype):
@@ -149,6 +175,16 @@ def test_generate_with_probabilities():
         assert torch.allclose(r.logprob, want.logprob[:, 5:], atol=1e-3)
         assert torch.allclose(r.entropy, want.entropy[:, 5:], atol=1e-3)
         assert (r.logprob <= r.top_logprob[..., 0]).all()
+    # padded prompts: the same probabilities as each prompt alone
+    cache.reset()
+    torch.manual_seed(9)
+    padded = idx.clone()
+    padded[1, 4:] = 0
+    out, r = m.generate(padded, 3, temperature=0.0, top_p=0.9, kv_cache=cache, lengths=[6, 4], logprobs=2)
+    cache.reset()
+    with torch.no_grad():
+        alone = m.score(torch.cat([padded[1:, :4], out[1:, 6:]], 1), top_n=2)
+    assert torch.allclose(r.logprob[1], alone.logprob[0, 3:], atol=1e-3)
     out, r = m.generate(idx, 0, logprobs=3)
     assert torch.equal(out, idx) and r.top_logprob.shape == (2, 0, 3) and r.top_index.dtype == torch.int64
     for bad in (-1, 65):
