@@ -92,8 +92,10 @@ WALSH_EXPORT int walsh_dropout(const void *x, int64_t ldx, int xdtype, const voi
         using TX = decltype(x);
         using TR = std::conditional_t<std::is_same_v<decltype(r), char>, void, decltype(r)>;
         using TY = decltype(y);
-        if (xb && M * C * 2 >= kCacheBytes) launch(dropout_kernel<TX, TR, TY, U, true>, G, N, 0, s, a);
-        else launch(dropout_kernel<TX, TR, TY, U, false>, G, N, 0, s, a);
+        if constexpr (sizeof(TX) == 2) {
+            if (M * C * 2 >= kCacheBytes) return launch(dropout_kernel<TX, TR, TY, U, true>, G, N, 0, s, a);
+        }
+        launch(dropout_kernel<TX, TR, TY, U, false>, G, N, 0, s, a);
     };
     constexpr uint16_t b16 = 0;
     constexpr float f32 = 0;
