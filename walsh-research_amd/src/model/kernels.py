@@ -1182,10 +1182,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0, n
     dev, shape, V = logits.device, tokens.shape, logits.shape[-1]
     rows, N, ld = _separate_rows(logits)
     tokens = tokens.contiguous()
-    logprob = torch.empty(shape, device=dev, dtype=torch.float32)
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
     entropy = torch.empty_like(logprob)
-    wide = (*shape, top_n)
-    top, index = torch.empty(wide, device=dev, dtype=torch.float32), torch.empty(wide, device=dev, dtype=torch.int64)
+    top = torch.empty(*shape, top_n, device=dev, dtype=torch.float32)
+    index = torch.empty_like(top, dtype=torch.int64)
     stats = torch.empty(N, 4, device=dev, dtype=torch.float32) if need_stats else None
     _hip.call_on(logits.get_device(), "walsh_token_logprobs_fwd", rows.data_ptr(), ld, N, V, tokens.data_ptr(), top_n,
                  logprob.data_ptr(), entropy.data_ptr(), top.data_ptr(), index.data_ptr(), _hip.ptr(stats), dt,
@@ -1205,14 +1205,19 @@ def token_logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor, top_index: to
     assert g_top is None or g_top.shape == top_index.shape and g_top.dtype == torch.float32, \
         "token_logprobs_bwd: gradients as the outputs"
     assert top_index.shape[:-1] == shape and top_index.dtype == torch.int64, "token_logprobs_bwd: index [..., n]"
-    rows, N, ld = _separate_rows(logits)
-    assert stats.shape == (N, 4) and stats.dtype == torch.float32, "token_logprobs_bwd: stats [rows, 4]"
+    assert stats.shape == (tokens.numel(), 4) and stats.dtype == torch.float32, "token_logprobs_bwd: stats [rows, 4]"
     _hip.same_device("token_logprobs_bwd", logits, top_index, stats, g_logprob, g_entropy, g_top)
+    return token_logprobs_bwd_run(logits, dt, tokens, top_index, stats, g_logprob, g_entropy, g_top)
+
+
+def token_logprobs_bwd_run(logits, dt, tokens, top_index, stats, g_logprob, g_entropy, g_top):
+    """``token_logprobs_bwd`` of arguments that are known to be right."""
+    rows, N, ld = _separate_rows(logits)
+    V, n = logits.shape[-1], top_index.shape[-1]
     # (held until the launch: a copy must not be freed before it)
     tokens, top_index, stats = tokens.contiguous(), top_index.contiguous(), _rows16(stats)
     g0, g1, g2 = (None if t is None else t.contiguous() for t in (g_logprob, g_entropy, g_top))
-    V = logits.shape[-1]
-    out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     _hip.call_on(logits.get_device(), "walsh_token_logprobs_bwd", rows.data_ptr(), ld, N, V, tokens.data_ptr(), n,
                  top_index.data_ptr(), stats.data_ptr(), _hip.ptr(g0), _hip.ptr(g1), _hip.ptr(g2), out.data_ptr(), V, dt,
                  kernel="logprobs_bwd_kernel", nbytes=(8 - 4 * dt) * N * V, flops=6 * N * V)
@@ -1272,7 +1277,7 @@ def dropout_run(x, drop, xt, rt, seed, stream, residual=None, out_dtype=None):
     """``dropout`` of arguments that are known to be right."""
     if out_dtype is None:
         out_dtype = x.dtype if xt == rt else torch.float32
-    y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
+    y = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
     n = x.numel()
     if n == 0:
         return y
@@ -1310,7 +1315,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, ou
     drop, wt, ot = check_embedding("embedding", tokens, weight, p, seed, stream, out_dtype)
     V, C = weight.shape
     N = tokens.numel()
-    y = torch.empty((*tokens.shape, C), device=weight.device, dtype=out_dtype)
+    y = torch.empty(*tokens.shape, C, device=weight.device, dtype=out_dtype)
     if N == 0 or C == 0:
         return y
     tokens = tokens.contiguous()

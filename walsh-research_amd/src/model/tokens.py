@@ -12,7 +12,7 @@ import torch
 from torch.nn import functional as F
 
 from . import kernels
-from ._common import TENSOR_TYPES, first_order, plain_eager
+from ._common import TENSOR_TYPES, first_order, plain_eager, plain_tensor
 from ._hip import dtype_code
 
 
@@ -116,8 +116,9 @@ class TokenLogprobsFunction(torch.autograd.Function):
         grads = [g for g in (g_logprob, g_entropy, g_top) if g is not None]
         if not grads:
             return None, None, None
-        if all(first_order(g) for g in grads):
-            return kernels.token_logprobs_bwd(logits, tokens, index, stats, g_logprob, g_entropy, g_top), None, None
+        if first_order(grads[0]) and all(plain_tensor(g) for g in grads[1:]):
+            return kernels.token_logprobs_bwd_run(logits, dtype_code(logits.dtype), tokens, index, stats, g_logprob,
+                                                  g_entropy, g_top), None, None
         return _logprobs_grad_plain(logits, tokens, index, g_logprob, g_entropy, g_top), None, None
 
 
