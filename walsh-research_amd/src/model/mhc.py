@@ -495,7 +495,9 @@ class mHCWalsh(nn.Module):
         return logits, loss
 
     def all_logits(self, idx):
-        """Logits of every position of idx [B, T]."""
+        """Logits of every position of idx [B, T], of one forward: with channel
+        modulation each depends on the whole text (tokens.causal_logits are
+        those that do not)."""
         _, _, h = self(idx, return_hidden=True)
         return cached_linear(self.output, h, self._casts["output"])
 

@@ -330,12 +330,24 @@ def stack_steps(steps, idx: torch.Tensor, top_n: int) -> TokenLogprobs:
     return TokenLogprobs(*(torch.stack(parts, 1) for parts in zip(*steps)))
 
 
+def causal_logits(model, idx: torch.Tensor) -> torch.Tensor:
+    """Logits [B, T, V] of every position of idx [B, T], each from the tokens up
+    to it: of one forward, or where layers mix positions (channel modulation
+    takes means over all of a text's rows) of one for every beginning of the
+    texts."""
+    if any(getattr(layer, "use_channel_mod", False) for layer in model.layers):
+        return torch.cat([model(idx[:, :n])[0] for n in range(1, idx.shape[1] + 1)], 1)
+    return model.all_logits(idx)
+
+
 def score(model, idx: torch.Tensor, lengths=None, top_n: int = 0) -> TokenLogprobs:
     """The log probabilities of the tokens idx[:, 1:] of idx [B, T], each under
     the model's softmax behind those before it, with entropies and ``top_n``
     alternatives: [B, T - 1].  ``lengths`` (B whole numbers) are the tokens
     that each text has, padded on the right with anything: what lies past them
-    is not counted.  Differentiable where autograd is on."""
+    is not counted.  Differentiable where autograd is on.  One forward, or T - 1
+    of a model with channel modulation (causal_logits), whose training drops
+    other things in each."""
     if idx.dim() != 2 or idx.shape[1] < 2:
         raise ValueError(f"score: texts [B, T] of at least two tokens, got {tuple(idx.shape)}")
     tokens = idx[:, 1:]
@@ -346,4 +358,4 @@ def score(model, idx: torch.Tensor, lengths=None, top_n: int = 0) -> TokenLogpro
         there = torch.arange(idx.shape[1], device=idx.device) < n[:, None]
         idx = torch.where(there, idx, 0)
         tokens = torch.where(there[:, 1:], tokens, -1)
-    return token_logprobs(model.all_logits(idx[:, :-1]), tokens, top_n)
+    return token_logprobs(causal_logits(model, idx[:, :-1]), tokens, top_n)
