@@ -877,7 +877,8 @@ int walsh_linear_wgrad(const void *g, const void *x, int64_t M, int64_t N, int64
  *     L = log(sum exp l);  logprob = l[token] - L;  entropy = -sum p log p, p = exp(l - L)
  *     top [N][n], top_index [N][n]: the n largest l in descending order (of
  *       equal ones the lowest indexes first), as l - L, and their indexes
- *   in float32.  A negative token marks a row that is not counted: it is not
+ *   in float32; log probabilities are never above 0, entropies never below.
+ *   A negative token marks a row that is not counted: it is not
  *   read; logprob and entropy are 0, top -inf and top_index -1.  A token of V
  *   or more has logprob NaN.  -inf has probability 0; a row of nothing else
  *   has logprob -inf everywhere and entropy 0.  NaN or +inf in a row make its

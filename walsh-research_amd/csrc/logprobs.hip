@@ -285,11 +285,15 @@ template <typename T, int NT, bool TOP, bool STREAM> __global__ __launch_bounds_
         __syncthreads();
         all = lp_join<NT>(sh, all, lane, wave);
     }
-    const float m = all.m, logs = __builtin_amdgcn_logf(all.s) * kLn2;
     const bool nothing = all.s == 0.f;             // (not where it is NaN)
+    // the largest logit's own weight is 1: what rounding leaves below that would
+    // make log probabilities positive
+    if (all.s < 1.f && !nothing) all.s = 1.f;
+    const float m = all.m, logs = __builtin_amdgcn_logf(all.s) * kLn2;
     auto logprob = [&](float x) { return nothing ? -INFINITY : (x - m) - logs; };
     if (tid == 0) {
-        const float h = nothing ? 0.f : logs - all.e / all.s * kLn2;
+        const float sum = logs - all.e / all.s * kLn2;
+        const float h = nothing || sum < 0.f ? 0.f : sum;          // (NaN stays)
         a.logprob[row] = t < a.V ? logprob(Act<T>::load(p + t)) : NAN;
         a.entropy[row] = h;
         if (a.stats) a.stats[row] = f32x4{m, all.s, h, 0.f};
