@@ -416,7 +416,12 @@ class mHCLlamaBlock(nn.Module):
             # rows is that view's, as there, not one stream's.  The result
             # stays in the stream dtype.
             B, T, n, C = x.shape
-            x = self.channel_mod.fused_residual(x.contiguous().view(B * n, T, C), self.channel_mod_norm)
+            x = x.contiguous().view(B * n, T, C)
+            if seed is None or self.resid_dropout == 0.0:
+                x = self.channel_mod.fused_residual(x, self.channel_mod_norm)
+            else:
+                y = self.channel_mod(self.channel_mod_norm(x))
+                x = drop_output(y, self.resid_dropout, seed, layer_idx, 2, x).to(x.dtype)
             x = x.view(B, T, n, C)
         return x
 

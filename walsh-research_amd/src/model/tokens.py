@@ -313,12 +313,13 @@ def step_seed(model, tokens: torch.Tensor):
 
 
 def drop_output(y: torch.Tensor, p: float, seed, layer_idx: int, which: int, residual: torch.Tensor = None) -> torch.Tensor:
-    """Output ``which`` (0 attention, 1 feed-forward) of a layer with dropout,
-    where the step has a seed, onto the residual stream if there is one.  Stream
-    0 is the tokens' rows'."""
+    """Output ``which`` (0 attention, 1 feed-forward, 2 channel modulation) of a
+    layer with dropout, where the step has a seed, onto the residual stream if
+    there is one.  Stream 0 is the tokens' rows', channel modulation's are from
+    2^31 on."""
     if seed is None or p == 0.0:
         return y if residual is None else residual + y
-    return counter_dropout(y, p, seed, 1 + 2 * layer_idx + which, residual)
+    return counter_dropout(y, p, seed, (1 << 31) + layer_idx if which == 2 else 1 + 2 * layer_idx + which, residual)
 
 
 def stack_steps(steps, idx: torch.Tensor, top_n: int) -> TokenLogprobs:
