@@ -2,6 +2,7 @@
 channel modulation, hooks and layers of its own, weights of an earlier time."""
 import pytest
 import torch
+from torch import nn
 
 pytestmark = pytest.mark.gpu
 MODELS = ["Walsh", "mHCWalsh"]
@@ -69,3 +70,84 @@ def test_training_with_channel_modulation_repeats():
     assert torch.equal(l0, l1) and torch.equal(l0, l2)
     for x, y, z in zip(g0, g1, g2):
         assert torch.allclose(x, y, rtol=1e-4, atol=1e-5) and torch.allclose(x, z, rtol=1e-4, atol=1e-5)
+
+
+# ------------------------------------------------------------------ the embedding module
+
+class Shifted(nn.Embedding):
+    def forward(self, tokens):
+        return super().forward(tokens) + 1.0
+
+
+def changed(how, m):
+    """Changes what the model's embedding gives; its rows then."""
+    e, idx = m.tok_embeddings, texts()
+    if how == "forward hook":
+        e.register_forward_hook(lambda mod, args, out: out + 1.0)
+    elif how == "pre-hook":
+        e.register_forward_pre_hook(lambda mod, args: ((args[0] + 1) % 97,))
+    elif how == "global hook":
+        return nn.modules.module.register_module_forward_hook(
+            lambda mod, args, out: out + 1.0 if isinstance(mod, nn.Embedding) else None)
+    elif how == "subclass":
+        m.tok_embeddings = Shifted(97, 64).cuda()
+    elif how == "own forward":
+        e.forward = lambda tokens: nn.functional.embedding(tokens, e.weight) + 1.0
+    elif how == "max_norm":
+        e.max_norm = 0.05
+    return None
+
+
+CHANGES = ["forward hook", "pre-hook", "global hook", "subclass", "own forward", "max_norm"]
+
+
+@pytest.mark.parametrize("how", CHANGES)
+@pytest.mark.parametrize("kind", MODELS)
+def test_hooks_and_own_embeddings_are_run(kind, how):
+    """A factor (a power of two) and dropout of everything apply to what the
+    module gives, whatever it is: the same as rows that are that much larger."""
+    a, b = model(kind, embed_scale=8.0).eval(), model(kind).eval()
+    handles = [changed(how, m) for m in (a, b)]
+    if how == "subclass":
+        b.tok_embeddings.load_state_dict(a.tok_embeddings.state_dict())
+    hook = b.tok_embeddings.register_forward_hook(lambda mod, args, out: out * 8)
+    try:
+        with torch.no_grad():
+            if how == "global hook":
+                [h.remove() for h in handles[1:]]         # (there are two, and each is called for both)
+            ha, hb = a(texts(), return_hidden=True)[2], b(texts(), return_hidden=True)[2]
+            plain = model(kind, embed_scale=8.0).eval()(texts(), return_hidden=True)[2] if how != "global hook" else None
+        assert torch.equal(ha, hb)
+        assert plain is None or not torch.allclose(ha, plain, atol=1e-3)
+    finally:
+        hook.remove()
+        [h.remove() for h in handles if h is not None]
+
+
+def test_gradients_and_dropout_through_a_hook():
+    """A hook that changes nothing changes nothing: rows, masks and gradients."""
+    got = []
+    for hooked in (False, True):
+        m = model("mHCWalsh", embed_scale=2.0, embed_dropout=0.25).train()
+        calls = []
+        if hooked:
+            m.tok_embeddings.register_forward_hook(lambda *a: calls.append(1))
+        torch.manual_seed(4)
+        loss = m(texts(), texts(seed=2))[1]
+        loss.backward()
+        assert len(calls) == hooked
+        got.append((loss.detach(), m.tok_embeddings.weight.grad.clone()))
+    # (2 times 4 / 3 is one factor in the kernel, two here)
+    assert torch.allclose(got[0][0], got[1][0], rtol=1e-5)
+    assert (got[0][1] - got[1][1]).norm() <= 1e-4 * got[0][1].norm()
+
+
+def test_padding_row_learns_nothing():
+    """An embedding with a padding_idx keeps it with a factor."""
+    m = model("mHCWalsh", embed_scale=2.0).train()
+    m.tok_embeddings = nn.Embedding(97, 64, padding_idx=5).cuda()
+    idx = texts()
+    idx[:, ::3] = 5
+    m(idx, texts(seed=2))[1].backward()
+    g = m.tok_embeddings.weight.grad
+    assert not g[5].any() and g[idx[0, 1]].any()

@@ -293,14 +293,34 @@ def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1
 
 # ------------------------------------------------------------------ in a model
 
+_modules = torch.nn.modules.module
+
+
+def _plain_lookup(e) -> bool:
+    """Whether calling the module ``e`` looks rows up and does nothing else: an
+    nn.Embedding itself, without hooks, a forward of its own or options that
+    change its weights or their gradient's form."""
+    return (type(e) is torch.nn.Embedding and "forward" not in e.__dict__
+            and e.max_norm is None and not e.sparse and not e.scale_grad_by_freq
+            and not (e._forward_hooks or e._forward_pre_hooks or e._backward_hooks or e._backward_pre_hooks
+                     or _modules._global_forward_hooks or _modules._global_forward_pre_hooks
+                     or _modules._global_backward_hooks or _modules._global_backward_pre_hooks))
+
+
 def embed_tokens(model, tokens: torch.Tensor, seed: torch.Tensor = None) -> torch.Tensor:
     """A model's token rows: its embedding as it is, or with its config's scale
-    and (given a seed) dropout."""
+    and (given a seed) dropout, in one kernel where the module is a lookup and
+    no more, else on what the module gives."""
     scale = getattr(model.config, "embed_scale", 1.0)
     p = getattr(model.config, "embed_dropout", 0.0) if seed is not None else 0.0
+    e = model.tok_embeddings
     if scale == 1.0 and p == 0.0:
-        return model.tok_embeddings(tokens)
-    return token_embedding(tokens, model.tok_embeddings.weight, scale, p=p, seed=seed)
+        return e(tokens)
+    if _plain_lookup(e):
+        return token_embedding(tokens, e.weight, scale, e.padding_idx, p=p, seed=seed)
+    y = e(tokens)
+    rows = y.float() * scale
+    return (counter_dropout(rows, p, seed) if p else rows).to(y.dtype)
 
 
 def step_seed(model, tokens: torch.Tensor):
