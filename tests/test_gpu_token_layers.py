@@ -151,3 +151,17 @@ def test_padding_row_learns_nothing():
     m(idx, texts(seed=2))[1].backward()
     g = m.tok_embeddings.weight.grad
     assert not g[5].any() and g[idx[0, 1]].any()
+
+
+# ------------------------------------------------------------------ what a model is given
+
+@pytest.mark.parametrize("kind", MODELS)
+def test_tokens_of_32_bits(kind):
+    """A model takes the tokens that its embedding takes, with a factor too."""
+    for kw in (dict(), dict(embed_scale=2.0), dict(embed_scale=2.0, embed_dropout=0.5)):
+        m = model(kind, **kw).eval()
+        with torch.no_grad():
+            a, b = m(texts())[0], m(texts().int())[0]
+            assert torch.equal(a, b)
+            assert torch.equal(m.score(texts()).logprob, m.score(texts().int()).logprob)
+            assert torch.equal(m.score(texts(), [17, 4, 9]).logprob, m.score(texts().int(), [17, 4, 9]).logprob)

@@ -317,6 +317,8 @@ def embed_tokens(model, tokens: torch.Tensor, seed: torch.Tensor = None) -> torc
     if scale == 1.0 and p == 0.0:
         return e(tokens)
     if _plain_lookup(e):
+        if tokens.dtype == torch.int32:          # (an nn.Embedding takes both)
+            tokens = tokens.long()
         return token_embedding(tokens, e.weight, scale, e.padding_idx, p=p, seed=seed)
     y = e(tokens)
     rows = y.float() * scale
@@ -371,6 +373,8 @@ def score(model, idx: torch.Tensor, lengths=None, top_n: int = 0) -> TokenLogpro
     other things in each."""
     if idx.dim() != 2 or idx.shape[1] < 2:
         raise ValueError(f"score: texts [B, T] of at least two tokens, got {tuple(idx.shape)}")
+    if idx.dtype == torch.int32:                 # (models take both)
+        idx = idx.long()
     tokens = idx[:, 1:]
     if lengths is not None:
         n = torch.as_tensor(lengths, device=idx.device, dtype=torch.int64)
