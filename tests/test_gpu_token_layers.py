@@ -165,3 +165,12 @@ def test_tokens_of_32_bits(kind):
             assert torch.equal(a, b)
             assert torch.equal(m.score(texts()).logprob, m.score(texts().int()).logprob)
             assert torch.equal(m.score(texts(), [17, 4, 9]).logprob, m.score(texts().int(), [17, 4, 9]).logprob)
+
+
+@pytest.mark.parametrize("field", ["embed_dropout", "resid_dropout"])
+@pytest.mark.parametrize("p", [-0.1, 1.5, float("nan")])
+@pytest.mark.parametrize("kind", MODELS)
+def test_probabilities_that_are_none(kind, p, field):
+    m = model(kind, **{field: p})
+    with pytest.raises(ValueError, match="probability"):
+        m.train()(texts(), texts())

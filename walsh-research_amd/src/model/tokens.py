@@ -329,7 +329,7 @@ def step_seed(model, tokens: torch.Tensor):
     """The seed of one forward of a model that trains with dropout of its
     tokens' rows or its layers' outputs, else None."""
     c = model.config
-    if model.training and (getattr(c, "embed_dropout", 0.0) > 0 or getattr(c, "resid_dropout", 0.0) > 0):
+    if model.training and (getattr(c, "embed_dropout", 0.0) != 0 or getattr(c, "resid_dropout", 0.0) != 0):
         return fresh_seed(tokens.device)
     return None
 
