@@ -174,3 +174,13 @@ def test_probabilities_that_are_none(kind, p, field):
     m = model(kind, **{field: p})
     with pytest.raises(ValueError, match="probability"):
         m.train()(texts(), texts())
+
+
+@pytest.mark.parametrize("kind", MODELS)
+def test_layers_of_an_earlier_time(kind):
+    """Modules that were stored before there was a dropout of outputs."""
+    m = model(kind).train()
+    want = m(texts(), texts(seed=2))[1]
+    for layer in m.layers:
+        layer.__dict__.pop("resid_dropout", None)
+    assert torch.equal(m(texts(), texts(seed=2))[1], want)

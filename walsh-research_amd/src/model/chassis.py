@@ -499,6 +499,7 @@ class SwiGLUMLP(nn.Module):
 
 class LlamaBlock(nn.Module):
     """Pre-norm residual block (chassis.py:509-531)."""
+    resid_dropout = 0.0          # (also of blocks stored without one)
 
     def __init__(self, config):
         super().__init__()

@@ -356,6 +356,7 @@ def wrap_with_mhc(model_class, n_streams=4):
 
 class mHCLlamaBlock(nn.Module):
     """Llama block with mHC streams around attention and FFN (mhc.py:451-534)."""
+    resid_dropout = 0.0          # (also of blocks stored without one)
 
     def __init__(self, config, n_streams=4):
         super().__init__()
