@@ -184,3 +184,13 @@ def test_layers_of_an_earlier_time(kind):
     for layer in m.layers:
         layer.__dict__.pop("resid_dropout", None)
     assert torch.equal(m(texts(), texts(seed=2))[1], want)
+
+
+def test_no_new_tokens_have_float32_probabilities():
+    m = model("mHCWalsh").eval()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        _, r = m.generate(texts(), 0, logprobs=2)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(x.dtype == torch.float32 for x in r[:3]) and r.top_index.dtype == torch.int64

@@ -347,7 +347,7 @@ def drop_output(y: torch.Tensor, p: float, seed, layer_idx: int, which: int, res
 def stack_steps(steps, idx: torch.Tensor, top_n: int) -> TokenLogprobs:
     """The TokenLogprobs [B, steps] of a loop's steps, each [B]."""
     if not steps:
-        none = torch.empty(idx.shape[0], 0, device=idx.device)
+        none = torch.empty(idx.shape[0], 0, device=idx.device, dtype=torch.float32)
         wide = none.new_empty(idx.shape[0], 0, top_n)
         return TokenLogprobs(none, none.clone(), wide, wide.long())
     return TokenLogprobs(*(torch.stack(parts, 1) for parts in zip(*steps)))
