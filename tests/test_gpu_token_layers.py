@@ -194,3 +194,13 @@ def test_no_new_tokens_have_float32_probabilities():
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(x.dtype == torch.float32 for x in r[:3]) and r.top_index.dtype == torch.int64
+
+
+@pytest.mark.parametrize("kind", MODELS)
+def test_lengths_that_no_text_has(kind):
+    """As generate's: whole numbers from 1 to the width, one a text, on either side."""
+    m = model(kind).eval()
+    for bad in ([17, 0, 3], [17, -1, 3], [18, 3, 3], [3, 4], [17.0, 3.0, 3.0], [[17, 3, 3]]):
+        for lengths in (bad, torch.tensor(bad), torch.tensor(bad, device="cuda")):
+            with pytest.raises((ValueError, TypeError), match="lengths"):
+                m.score(texts(), lengths)

@@ -363,11 +363,27 @@ def causal_logits(model, idx: torch.Tensor) -> torch.Tensor:
     return model.all_logits(idx)
 
 
+def text_lengths(lengths, idx: torch.Tensor) -> torch.Tensor:
+    """Lengths of the texts idx [B, T] on their device: B whole numbers from 1 to
+    T.  (The host reads a device's, except where a transform or trace has to see each
+    operation.)"""
+    n = torch.as_tensor(lengths)
+    if n.numel() == 0:
+        n = n.long()
+    if n.shape != idx.shape[:1] or n.dtype == torch.bool or n.is_floating_point() or n.is_complex():
+        raise ValueError(f"score: lengths {tuple(n.shape)} ({n.dtype}) of texts {tuple(idx.shape)}")
+    if plain_eager():
+        values = n.tolist()
+        if values and (min(values) < 1 or max(values) > idx.shape[1]):
+            raise ValueError(f"score: lengths {values} of texts {tuple(idx.shape)}")
+    return n.to(device=idx.device, dtype=torch.int64)
+
+
 def score(model, idx: torch.Tensor, lengths=None, top_n: int = 0) -> TokenLogprobs:
     """The log probabilities of the tokens idx[:, 1:] of idx [B, T], each under
     the model's softmax behind those before it, with entropies and ``top_n``
-    alternatives: [B, T - 1].  ``lengths`` (B whole numbers) are the tokens
-    that each text has, padded on the right with anything: what lies past them
+    alternatives: [B, T - 1].  ``lengths`` (B whole numbers from 1 to T) are the
+    tokens that each text has, padded on the right with anything: what lies past them
     is not counted.  Differentiable where autograd is on.  One forward, or T - 1
     of a model with channel modulation (causal_logits), whose training drops
     other things in each."""
@@ -377,9 +393,7 @@ def score(model, idx: torch.Tensor, lengths=None, top_n: int = 0) -> TokenLogpro
         idx = idx.long()
     tokens = idx[:, 1:]
     if lengths is not None:
-        n = torch.as_tensor(lengths, device=idx.device, dtype=torch.int64)
-        if n.shape != idx.shape[:1]:
-            raise ValueError(f"score: lengths {tuple(n.shape)} of texts {tuple(idx.shape)}")
+        n = text_lengths(lengths, idx)
         there = torch.arange(idx.shape[1], device=idx.device) < n[:, None]
         idx = torch.where(there, idx, 0)
         tokens = torch.where(there[:, 1:], tokens, -1)
