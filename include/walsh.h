@@ -920,7 +920,8 @@ int walsh_token_logprobs_bwd(const void *logits, int64_t ld, int64_t N, int64_t 
  *   v, of dropout(gy)[r], every row of dw [V][C] written; tokens outside and
  *   padding_idx (negative: none) add to none.  The sums are float32 in a fixed
  *   order (deterministic).  Needs work of
- *   walsh_embedding_bwd_workspace_bytes(N, V, C) bytes, 16-byte aligned.
+ *   walsh_embedding_bwd_workspace_bytes(N, V, C) bytes, 16-byte aligned (0 for
+ *   sizes that are refused).
  * Each takes fewer than 2^31 - 65536 blocks of 8 columns (a row's last may be
  *   part of one; of dw in float32 blocks of 4), the embedding fewer than 2^28
  *   tokens, rows at any alignment of their elements. */

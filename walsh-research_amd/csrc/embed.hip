@@ -436,10 +436,15 @@ static int64_t embed_chunks(int64_t N, int64_t C) { return ceil_div(N, embed_mos
 static int64_t embed_start_bytes(int64_t V) { return ceil_div(4 * (V + 1), 16) * 16; }
 static int64_t embed_order_bytes(int64_t N) { return ceil_div(4 * N, 16) * 16; }
 
+// Sizes that a call takes.
+static bool embed_sizes(int64_t N, int64_t V, int64_t C) {
+    return N >= 0 && C >= 0 && V >= 1 && C <= 0x7fffffff - 8 && N < 1 << 28 && V <= 0x7fffffff - 2048 &&
+           N * ceil_div(C, 8) <= kMaxBlocks;
+}
+
 static int embed_check(const char *fn, int64_t N, int64_t V, int64_t C, int drop, const int64_t *seed, int64_t rng_stream,
                        int dt0, int dt1) {
-    if (N < 0 || C < 0 || V < 1 || C > 0x7fffffff - 8 || N >= 1 << 28 || V > 0x7fffffff - 2048 ||
-        N * ceil_div(C, 8) > kMaxBlocks)
+    if (!embed_sizes(N, V, C))
         return set_error(WALSH_ENOTSUP, "%s: N=%lld tokens, V=%lld rows of C=%lld", fn, (long long)N, (long long)V, (long long)C);
     if (drop < 0 || drop > 65536 || rng_stream < 0 || rng_stream > 0xffffffffll)
         return set_error(WALSH_EINVAL, "%s: drop %d (0 to 65536), stream %lld (32 bits)", fn, drop, (long long)rng_stream);
@@ -486,7 +491,7 @@ WALSH_EXPORT int walsh_embedding_fwd(const int64_t *tokens, int64_t N, const voi
 }
 
 WALSH_EXPORT int64_t walsh_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t C) {
-    if (N < 0 || V < 1 || C < 0) return 0;
+    if (!embed_sizes(N, V, C)) return 0;
     return embed_start_bytes(V) + 2 * embed_order_bytes(N) + 2 * embed_chunks(N, C) * C * 4;
 }
 
