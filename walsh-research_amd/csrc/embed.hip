@@ -3,23 +3,26 @@
 // with keep() the mask and factor of dropout (rows8.h).  A token outside the
 // vocabulary gives a row of NaN and adds to no gradient; nor does padding_idx.
 //
-// The gradient adds the rows of a token in their order, in float32, so equal
-// calls give equal bits.  Three kernels:
+// The gradient adds the rows of a token in float32 in a fixed order, which
+// depends on the call's tokens and sizes (where a long row is cut): equal calls
+// give equal bits.  Three kernels:
 //   sort   a workgroup takes a range of up to 256 tokens and walks all N: it
 //          counts those below its range, which is where its part of the sorted
 //          order begins (no workgroup waits for another), and lists those in
 //          it, to count and place them.  What every workgroup repeats, ten
-//          instructions for 64 tokens, costs less than a launch would: 5.9 us for
-//          8,192 tokens, 8.3 for 16,384, 19 for 65,536, 4 of them the launch.
+//          instructions for 64 tokens, costs less than a launch would: 6.5 us for
+//          8,192 tokens, 8.6 for 16,384, 20 for 65,536, 4 of them the launch.
+//          The range with the most tokens places them alone: with frequent
+//          tokens side by side in the vocabulary 11, 19 and 72 us.
 //   rows   zeros where a token does not occur; else the sum of its tokens' rows,
 //          a lane 8 columns, up to 32 of them.  Longer rows are cut where the
 //          sorted order is, every 32 places (embed_most), and their pieces summed
 //          into a workspace.
 //   join   adds the pieces of each long row, in a fixed order.
-// Bound by memory: 50,257 x 4,096 bf16 from 16,384 rows (546 MB) take 91 us for
-// the rows, 6.0 TB/s, x 512 float32 from 8,192 (120 MB) 18 us, of 107 and 28 in
+// Bound by memory: 50,257 x 4,096 bf16 from 16,384 rows (546 MB) take 93 us for
+// the rows, 5.9 TB/s, x 512 float32 from 8,192 (120 MB) 18 us, of 108 and 29 in
 // all; a character model's 65 x 768 from 16,384 rows 21 us, all of it latency.
-// The lookup of 16,384 x 4,096 takes 34 us, of 64 rows 2.9.
+// The lookup of 16,384 x 4,096 takes 32 us, of 64 rows 3.0.
 #include <type_traits>
 
 #include "rows8.h"

@@ -14,9 +14,11 @@
 // larger one; lanes and wavefronts are joined at the end.  Four wavefronts take
 // a row; sixteen where rows of more than 8,192 tokens are no more than CUs, so
 // that a row is not left to a quarter of its CU (50,257 tokens: one row 5.8 us
-// instead of 6.0, with 5 alternatives 9.3, 256 rows 7.1 instead of 7.6; at 512
-// rows sixteen take 18.2, four 12.8).  A row over several workgroups would need
-// a second launch, of 4 us.
+// instead of 6.0, with 5 alternatives 9 to 10, 256 rows 7.1 instead of 7.6; at
+// 512 rows sixteen take 18.2, four 12).  Rows are not split over workgroups, of
+// which the last to arrive could join the others' sums in the same launch: 64
+// float32 rows take 7.1 us, with 20 alternatives 12.8, where a copy of their
+// bytes would take 2.5.
 //
 // Alternatives: the lanes' maxima, taken together over the wavefronts, are the
 // largest of 256 groups of tokens.  A search by their bits finds a bound that
@@ -27,7 +29,8 @@
 // asked for, the row is walked once for each further value.
 //
 // Bound by memory: 8,192 rows of 50,257 bf16 logits take 129 us (6.4 TB/s), with
-// 5 and 20 alternatives 152 and 172, with float32 logits 257 (6.4), 268, 303.
+// 5 and 20 alternatives 152 to 175 and 172 to 186 by how many lie near them, with
+// float32 logits 257 (6.4), 269, 304.
 // Of 10 instructions a token the exponential takes the time of four.  Their
 // gradient, 823 MB read and as many written, takes 292 us (5.6 TB/s), in
 // float32 582 (5.7, where a copy reaches 5.1).

@@ -1330,7 +1330,8 @@ def embedding_bwd(tokens: torch.Tensor, gy: torch.Tensor, V: int, scale: float =
                   padding_idx: int = None, p: float = 0.0, seed: torch.Tensor = None, stream: int = 0) -> torch.Tensor:
     """The gradient [V, C] of ``embedding``'s weight (``dtype``: its type,
     None: gy's) for the gradient gy [..., C] of its output: a token's rows are
-    added in their order in float32, so equal calls give equal bits.  Tokens
+    added in float32 in a fixed order that depends on the call's tokens and
+    sizes, so equal calls give equal bits.  Tokens
     outside 0 .. V - 1 and ``padding_idx`` add to none."""
     dtype = gy.dtype if dtype is None else dtype
     _hip.require_device(gy, "gradient")

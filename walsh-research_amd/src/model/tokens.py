@@ -278,9 +278,9 @@ def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1
     """scale weight[tokens], with dropout of probability ``p`` (its ``seed`` and
     ``stream`` as in counter_dropout, a token a row): tokens [...] (int64),
     weight [V, C] -> [..., C] in ``out_dtype`` (None: the weight's), rounded
-    once.  Differentiable in the weight; a token's gradients are added in their
-    order in float32, so equal calls give equal bits.  Tokens outside
-    0 .. V - 1 give rows of NaN and no gradient, and ``padding_idx`` none."""
+    once.  Differentiable in the weight; a token's gradients are added in float32
+    in a fixed order that depends on the call's tokens and sizes, so equal calls
+    give equal bits.  Tokens outside 0 .. V - 1 give rows of NaN and no gradient, and ``padding_idx`` none."""
     plain = not _kernel_tensors(tokens, weight, seed)
     if plain or padding_idx is not None:
         kernels.check_embedding("token_embedding", tokens, weight, p, seed, stream, out_dtype or weight.dtype, padding_idx)
